@@ -23,14 +23,14 @@
 #include "triton_ext/tx_passes.h"
 
 #include "kernels.h"
+#include "launch_common.h"
 
 using namespace txk;
 
-namespace {
+static thread_local std::string g_last_error;
 
-thread_local std::string g_last_error;
+namespace txk {
 
-int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char *fmt, ...) {
   char buf[512];
   va_list ap;
@@ -40,13 +40,11 @@ int fail(int code, const char *fmt, ...) {
   g_last_error = buf;
   return code;
 }
+void clearError() { g_last_error.clear(); }
 
-#define TX_HIP_CHECK(expr)                                                     \
-  do {                                                                         \
-    hipError_t e_ = (expr);                                                    \
-    if (e_ != hipSuccess)                                                      \
-      return fail(TX_ERR_HIP, "%s failed: %s", #expr, hipGetErrorString(e_));  \
-  } while (0)
+} // namespace txk
+
+namespace {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

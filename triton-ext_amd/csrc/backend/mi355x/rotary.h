@@ -1,0 +1,253 @@
+// Rotary positions, and new tokens written into a paged cache.
+//
+// A pair (x1, x2) at position p with frequency f goes to (x1 c - x2 s, x2 c + x1 s),
+// c + i s = scale e^(i p f).  The angle's turn is taken in 64 bits (at a position of
+// 10^6 the product in fp32 is off by 0.06), sine and cosine of the reduced turn and
+// the rotation in fp32, and the result is rounded once.
+//
+// Every thread takes the same piece of a token's heads: `item` of one head is VEC
+// elements of each half of the rotated part (halves layout), VEC adjacent elements
+// (interleaved), or VEC elements past rot_dim, which are copied.  So it forms its
+// VEC (or VEC / 2) sines once and goes through the token's heads, every
+// head_lanes-th of them.  Bound by memory: 16-byte loads and stores.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "tile_common.h"
+
+namespace txk {
+
+struct RotaryArgs {
+  const void *x;
+  const void *pos;
+  const float *inv_freq;
+  void *out;
+  int64_t N, tokens; // tokens: Z * N
+  int64_t pos_sz, x_sz, x_sn, x_sh, o_sz, o_sn, o_sh;
+  int32_t H, head_dim, rot, items, head_lanes, pos64, inverse;
+  float scale;
+};
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void *q_out;
+  uint8_t *kc, *vc;
+  const int32_t *table, *kv_len, *cu_q;
+  const float *inv_freq, *k_scale, *v_scale;
+  int64_t T, pages, table_width, table_s;
+  int64_t q_st, q_sh, o_st, o_sh, k_st, k_sh, v_st, v_sh;
+  int64_t kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh;
+  int32_t B, Hq, Hkv, head_dim, rot, items, head_lanes, page_shift;
+  float scale;
+};
+
+__device__ __forceinline__ float elt_to_f32(float x) { return x; }
+__device__ __forceinline__ float elt_to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float elt_to_f32(__bf16 x) { return (float)x; }
+
+template <class T, int VEC> struct alignas(sizeof(T) * VEC) EltVec {
+  T v[VEC];
+};
+template <class T, int VEC>
+__device__ __forceinline__ void load_f32(const T *p, float (&f)[VEC]) {
+  const EltVec<T, VEC> r = *reinterpret_cast<const EltVec<T, VEC> *>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    f[i] = elt_to_f32(r.v[i]);
+}
+template <class T, int VEC>
+__device__ __forceinline__ void store_f32(T *p, const float (&f)[VEC]) {
+  EltVec<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    r.v[i] = (T)f[i];
+  *reinterpret_cast<EltVec<T, VEC> *>(p) = r;
+}
+
+// cos and sin of position * f, times scale.
+__device__ __forceinline__ void turn_of(double pos, float f, float scale, bool inverse, float &c,
+                                        float &s) {
+  double t = pos * (double)f * 0.15915494309189535; // turns
+  t -= rint(t);
+  float si, co;
+  sincospif(2.0f * (float)t, &si, &co);
+  c = co * scale;
+  s = (inverse ? -si : si) * scale;
+}
+
+// What one item of a head is: offsets of its one or two runs of VEC elements, and
+// the sines of its pairs.
+template <int VEC, bool INTER> struct RotaryItem {
+  static constexpr int P = INTER ? (VEC > 1 ? VEC / 2 : 1) : VEC;
+  int at, second; // second < 0: one run; interleaved VEC 1: the pair's other element
+  bool rotate;
+  float c[P], s[P];
+
+  __device__ __forceinline__ RotaryItem(int item, int rot, double pos, const float *inv_freq,
+                                        float scale, bool inverse) {
+    // pair items come first
+    const int step = INTER ? (VEC > 1 ? VEC : 2) : VEC;
+    const int pairs = INTER ? rot / step : rot / 2 / VEC;
+    rotate = item < pairs;
+    if (rotate) {
+      at = item * step;
+      second = INTER ? (VEC > 1 ? -1 : at + 1) : at + rot / 2;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        turn_of(pos, inv_freq[INTER ? at / 2 + i : at + i], scale, inverse, c[i], s[i]);
+    } else {
+      at = rot + (item - pairs) * VEC;
+      second = -1;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        c[i] = 1.f, s[i] = 0.f;
+    }
+  }
+  // Loads the item of one head and rotates it (or not): y1 goes to `at`, y2 to `second`.
+  template <class T>
+  __device__ __forceinline__ void apply(const T *head, bool rot_it, float (&y1)[VEC],
+                                        float (&y2)[VEC]) const {
+    load_f32<T, VEC>(head + at, y1);
+    if (second >= 0)
+      load_f32<T, VEC>(head + second, y2);
+    if (!rotate || !rot_it)
+      return;
+    if constexpr (INTER && VEC > 1) {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float a = y1[2 * i], b = y1[2 * i + 1];
+        y1[2 * i] = a * c[i] - b * s[i];
+        y1[2 * i + 1] = b * c[i] + a * s[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float a = y1[i], b = y2[i];
+        y1[i] = a * c[i] - b * s[i];
+        y2[i] = b * c[i] + a * s[i];
+      }
+    }
+  }
+};
+
+template <class T, int VEC, bool INTER>
+__global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs p) {
+  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int item = (int)(idx % p.items);
+  const int64_t rest = idx / p.items;
+  const int lane = (int)(rest % p.head_lanes);
+  const int64_t tok = rest / p.head_lanes;
+  if (tok >= p.tokens)
+    return;
+  const int64_t z = tok / p.N, n = tok % p.N;
+  const int64_t pi = z * p.pos_sz + n;
+  const double pos = p.pos64 ? (double)static_cast<const int64_t *>(p.pos)[pi]
+                             : (double)static_cast<const int32_t *>(p.pos)[pi];
+  const RotaryItem<VEC, INTER> it(item, p.rot, pos, p.inv_freq, p.scale, p.inverse);
+  const T *x = static_cast<const T *>(p.x) + z * p.x_sz + n * p.x_sn;
+  T *o = static_cast<T *>(p.out) + z * p.o_sz + n * p.o_sn;
+  for (int h = lane; h < p.H; h += p.head_lanes) {
+    float y1[VEC], y2[VEC];
+    it.template apply<T>(x + h * p.x_sh, true, y1, y2);
+    T *oh = o + h * p.o_sh;
+    store_f32<T, VEC>(oh + it.at, y1);
+    if (it.second >= 0)
+      store_f32<T, VEC>(oh + it.second, y2);
+  }
+}
+
+// The sequence of token t: the largest b with cu_q[b] <= t (cu_q ascends).
+__device__ __forceinline__ int sequence_of(const int32_t *cu_q, int B, int64_t t) {
+  int lo = 0, hi = B; // cu_q[lo] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (cu_q[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint8_t f32_to_e4m3(float x) {
+  // saturates at 448 (the conversion itself makes NaN past it); NaN stays NaN
+  x = x > 448.f ? 448.f : x < -448.f ? -448.f : x;
+  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff);
+}
+
+template <class T, class C, int VEC>
+__device__ __forceinline__ void store_cache(uint8_t *head, int at, const float (&y)[VEC],
+                                            float scale) {
+  if constexpr (std::is_same<C, uint8_t>::value) {
+    EltVec<uint8_t, VEC> r;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      r.v[i] = f32_to_e4m3(y[i] / scale);
+    *reinterpret_cast<EltVec<uint8_t, VEC> *>(head + at) = r;
+  } else {
+    store_f32<T, VEC>(reinterpret_cast<T *>(head) + at, y);
+  }
+}
+
+// C: T, or uint8_t for e4m3.  Heads in the order q, k, v.
+template <class T, class C, int VEC, bool INTER>
+__global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs p) {
+  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int item = (int)(idx % p.items);
+  const int64_t rest = idx / p.items;
+  const int lane = (int)(rest % p.head_lanes);
+  const int64_t t = rest / p.head_lanes;
+  if (t >= p.T)
+    return;
+  // Token t's sequence b, position and place in the cache (page < 0: none).
+  int b = (int)t;
+  int64_t pos = -1, page = -1;
+  bool mine = true;
+  if (p.cu_q) {
+    b = sequence_of(p.cu_q, p.B, t);
+    const int64_t first = p.cu_q[b], last = p.cu_q[b + 1];
+    mine = t >= first && t < last;
+    pos = p.kv_len[b] - last + t;
+  } else {
+    pos = (int64_t)p.kv_len[b] - 1;
+  }
+  const int64_t e = pos >> p.page_shift;
+  if (mine && pos >= 0 && e < p.table_width) {
+    page = p.table[b * p.table_s + e];
+    if (page >= p.pages)
+      page = -1;
+  }
+  const int64_t slot = pos & ((1 << p.page_shift) - 1);
+  const RotaryItem<VEC, INTER> it(item, p.rot, (double)pos, p.inv_freq, p.scale, false);
+  const int heads = p.Hq + 2 * p.Hkv;
+  for (int h = lane; h < heads; h += p.head_lanes) {
+    float y1[VEC], y2[VEC];
+    if (h < p.Hq) {
+      it.template apply<T>(static_cast<const T *>(p.q) + t * p.q_st + h * p.q_sh, mine, y1, y2);
+      T *o = static_cast<T *>(p.q_out) + t * p.o_st + h * p.o_sh;
+      store_f32<T, VEC>(o + it.at, y1);
+      if (it.second >= 0)
+        store_f32<T, VEC>(o + it.second, y2);
+      continue;
+    }
+    if (page < 0)
+      return; // (the heads after this one are k's and v's too)
+    const bool is_k = h < p.Hq + p.Hkv;
+    const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
+    const T *src = is_k ? static_cast<const T *>(p.k) + t * p.k_st + hk * p.k_sh
+                        : static_cast<const T *>(p.v) + t * p.v_st + hk * p.v_sh;
+    it.template apply<T>(src, is_k, y1, y2);
+    const float *sc = is_k ? p.k_scale : p.v_scale;
+    const float scale = sc ? sc[hk] : 1.f;
+    uint8_t *dst = is_k ? p.kc + (page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh) * sizeof(C)
+                        : p.vc + (page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh) * sizeof(C);
+    store_cache<T, C, VEC>(dst, it.at, y1, scale);
+    if (it.second >= 0)
+      store_cache<T, C, VEC>(dst, it.second, y2, scale);
+  }
+}
+
+} // namespace txk

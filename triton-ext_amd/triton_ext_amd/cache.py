@@ -1,0 +1,488 @@
+"""Rotary positions, a paged key/value cache and the attention that reads it, over torch
+device tensors (include/triton_ext/tx_cache.h).
+
+A cache is a pair of tensors [pages, page_size, Hkv, D] for k and v, in any order in
+memory with D contiguous (a permuted [pages, Hkv, page_size, D] does), its books int32
+tensors: page_table [S, W], kv_len [S] and refs [pages] (how many table entries hold a
+page).  Token j of sequence b lies in page page_table[b, j // page_size], slot
+j % page_size.  A decoding step is
+
+    page_table, kv_len, refs, missing = page_reserve(page_table, kv_len, refs, kv_len + 1, 16)
+    q = paged_append(k, v, k_cache, v_cache, page_table, kv_len, q=q, inv_freq=inv_freq)
+    o = paged_attention(q, k_cache, v_cache, page_table, kv_len, sm_scale=D ** -0.5)
+
+and a chunk of several new tokens a sequence the same with cu_q, their starts in q, k
+and v.  Nothing here reads device memory on the host: every call can be captured into
+a graph and replayed with other contents.
+"""
+import ctypes
+import math
+
+from . import capi
+from .dot import _current_stream, _tx_of, workspace_for
+
+_plans = {}
+
+
+def _plan(kind, desc_type, plan_type, key):
+    """The plan of a descriptor with these fields in order, kept by its fields."""
+    full = (kind,) + key
+    p = _plans.get(full)
+    if p is None:
+        p = plan_type()
+        capi.check(getattr(capi.load(), f"tx_{kind}_plan_create")(
+            ctypes.byref(desc_type(*key)), ctypes.byref(p)))
+        if len(_plans) >= 4096:  # a program of ever new sizes
+            _plans.clear()
+        _plans[full] = p
+    return p
+
+
+def _int32(t, name, dims):
+    import torch
+    if t.dtype != torch.int32 or t.dim() != dims:
+        raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s), got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _dense_last(t):
+    """t, or a copy, with its last dimension contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, context=4096,
+                       turns=(1.0, 32.0), device=None):
+    """The frequencies of `rot_dim` rotated dims, base^(-2 i / rot_dim), as an fp32 tensor
+    [rot_dim // 2], and the factor for cos and sin (`scale` of rotary and paged_append).
+
+    scaling, for contexts `factor` times as long as the `context` trained on: None;
+    "linear" (positions divided by factor); "ntk" (base times factor^(rot_dim /
+    (rot_dim - 2))); "yarn" (frequencies of fewer than turns[0] turns over the context
+    divided by factor, those of more than turns[1] kept, a line between, and a scale
+    of 0.1 ln(factor) + 1)."""
+    import torch
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim}: an even number of dims")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling {scaling!r}: None, 'linear', 'ntk' or 'yarn'")
+    if scaling is not None and not factor >= 1.0:
+        raise ValueError(f"factor {factor}: at least 1")
+    base = float(base)
+    if scaling == "ntk":
+        if rot_dim < 4:
+            raise ValueError("ntk scaling needs a rot_dim of 4 or more")
+        base *= factor ** (rot_dim / (rot_dim - 2))
+    f = base ** (-2.0 * torch.arange(rot_dim // 2, dtype=torch.float64) / rot_dim)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        lo, hi = turns
+        keep = ((context * f / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        f = f / factor * (1 - keep) + f * keep
+        scale = 0.1 * math.log(factor) + 1.0
+    return f.to(torch.float32).to(device), scale
+
+
+def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=False, out=None,
+           stream=None):
+    """Rotary positions: pair i of every head of x goes to (x1 c - x2 s, x2 c + x1 s) with
+    c = scale cos(position * inv_freq[i]), s = scale sin(..), the angle in 64 bits.
+
+    x [T, H, D] with positions [T], or [Z, H, N, D] (the layout of attention()) with
+    positions [N] or [Z, N]; fp16, bf16 or fp32, any strides with D contiguous;
+    positions int32 or int64; inv_freq fp32 [rot_dim / 2] (rotary_frequencies), rot_dim
+    <= D: the dims past it are copied.  The pairs are dims (i, i + rot_dim / 2), or
+    (2 i, 2 i + 1) when interleaved.  inverse: the transposed map, which takes the
+    gradient of the result to that of x.  out may be x itself."""
+    import torch
+    if x.dim() not in (3, 4):
+        raise ValueError(f"x must be [T, H, D] or [Z, H, N, D], got {tuple(x.shape)}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be an fp32 vector")
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"x: fp32, fp16 and bf16 are implemented, got {x.dtype}")
+    _same_device(x.device, positions=positions, inv_freq=inv_freq, out=out)
+    x = _dense_last(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+        raise ValueError("out must be as x, with its last dimension contiguous")
+    xs, os_ = x.stride(), out.stride()
+    if x.dim() == 3:
+        (N, H, D), Z = x.shape, 1
+        if positions.shape != (N,):
+            raise ValueError(f"positions must be [{N}], got {tuple(positions.shape)}")
+        st = (0, xs[0], xs[1], 0, os_[0], os_[1])
+        pos_sz = 0
+    else:
+        Z, H, N, D = x.shape
+        if positions.shape == (Z, N):
+            pos_sz = N
+        elif positions.shape == (N,):
+            pos_sz = 0
+        else:
+            raise ValueError(f"positions must be [{N}] or [{Z}, {N}], got {tuple(positions.shape)}")
+        st = (xs[0], xs[2], xs[1], os_[0], os_[2], os_[1])
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    p = _plan("rotary", capi.RotaryDesc, capi.RotaryPlan,
+              (Z, N, H, D, 2 * inv_freq.shape[0], _tx_of(x.dtype), int(bool(interleaved)),
+               int(bool(inverse)), 8 * positions.element_size(), float(scale), 0, pos_sz) + st)
+    if stream is None:
+        stream = _current_stream(x.device)
+    capi.check(capi.load().tx_rotary_launch(ctypes.byref(p), x.data_ptr(), positions.data_ptr(),
+                                            inv_freq.data_ptr(), out.data_ptr(), stream))
+    return out
+
+
+def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, dtype):
+    """What paged_append and paged_attention ask alike; the index arrays, contiguous."""
+    import torch
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must share one [pages, page_size, Hkv, D] shape and "
+                         f"type: {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if tuple(k_cache.shape[2:]) != (Hkv, D):
+        raise ValueError(f"the cache holds heads of {tuple(k_cache.shape[2:])}, not ({Hkv}, {D})")
+    if k_cache.dtype != dtype and k_cache.dtype != torch.float8_e4m3fn:
+        raise NotImplementedError(f"a cache of {k_cache.dtype} under {dtype}: the same type, or "
+                                  "float8_e4m3fn")
+    if D > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError("the caches' last dimension must be contiguous")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t is None:
+            continue
+        if k_cache.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"{name} is for float8_e4m3fn caches")
+        if t.dtype != torch.float32 or t.shape != (Hkv,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous fp32 [{Hkv}] tensor")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or (
+            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be an int32 [sequences, entries] tensor with contiguous "
+                         "rows")
+    kv_len = _int32(kv_len, "kv_len", 1)
+    B = kv_len.shape[0]
+    if page_table.shape[0] != B:
+        raise ValueError(f"page_table has {page_table.shape[0]} rows, kv_len {B}")
+    if cu_q is None:
+        if T != B:
+            raise ValueError(f"{T} new tokens of {B} sequences: give cu_q")
+    else:
+        cu_q = _int32(cu_q, "cu_q", 1)
+        if cu_q.shape[0] != B + 1:
+            raise ValueError(f"cu_q must be [{B + 1}], got {tuple(cu_q.shape)}")
+    return page_table, kv_len, cu_q
+
+
+def _tokens(t, name, heads, D, dtype, T):
+    """t [T, heads, D] with D contiguous."""
+    if t.dim() != 3 or tuple(t.shape) != (T, heads, D):
+        raise ValueError(f"{name} must be [{T}, {heads}, {D}], got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+    return _dense_last(t)
+
+
+def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=None, inv_freq=None,
+                 interleaved=False, scale=1.0, k_scale=None, v_scale=None, q_out=None,
+                 stream=None):
+    """New tokens into a paged cache: k, v [T, Hkv, D] go to the pages of their sequences,
+    k (and q [T, Hq, D], which is returned, in q_out if given) rotated at the token's
+    position first when inv_freq is given (see rotary for interleaved and scale).
+
+    kv_len [B] counts the new tokens too, cu_q [B + 1] says which rows are whose (None:
+    one token each): row cu_q[b] + i of sequence b's n is its token kv_len[b] - n + i.
+    The pages must be there (page_reserve); a token without one is not written.  fp16 or
+    bf16; a float8_e4m3fn cache holds k / k_scale[head] and v / v_scale[head] (fp32 [Hkv];
+    None: 1), saturated.  Rows of q from cu_q[B] on come back as they are."""
+    import torch
+    if k.dim() != 3:
+        raise ValueError(f"k must be [T, Hkv, D], got {tuple(k.shape)}")
+    T, Hkv, D = k.shape
+    dtype = k.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"k: fp16 and bf16 are implemented, got {dtype}")
+    k, v = _dense_last(k), _tokens(v, "v", Hkv, D, dtype, T)
+    page_table, kv_len, cu_q = _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale,
+                                             v_scale, T, Hkv, D, dtype)
+    _same_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                 kv_len=kv_len, cu_q=cu_q, q=q, inv_freq=inv_freq, k_scale=k_scale,
+                 v_scale=v_scale, q_out=q_out)
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+            raise ValueError("inv_freq must be an fp32 vector")
+        inv_freq = inv_freq.contiguous()
+        rot = 2 * inv_freq.shape[0]
+    Hq, q_st = 0, (0, 0, 0, 0)
+    if q is not None:
+        Hq = q.shape[1] if q.dim() == 3 else 0
+        q = _tokens(q, "q", Hq, D, dtype, T)
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != dtype or (D > 1 and q_out.stride(2) != 1):
+            raise ValueError("q_out must be as q, with its last dimension contiguous")
+        q_st = q.stride()[:2] + q_out.stride()[:2]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    p = _plan("paged_append", capi.PagedAppendDesc, capi.PagedAppendPlan,
+              (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D, rot,
+               k_cache.shape[1], _tx_of(dtype), _tx_of(k_cache.dtype), int(bool(interleaved)),
+               int(cu_q is not None), float(scale)) + q_st + k.stride()[:2] + v.stride()[:2]
+              + k_cache.stride()[:3] + v_cache.stride()[:3] + (page_table.stride(0),))
+    if stream is None:
+        stream = _current_stream(k.device)
+    capi.check(capi.load().tx_paged_append_launch(
+        ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
+        v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(inv_freq),
+        _ptr(k_scale), _ptr(v_scale), stream))
+    return q_out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_scale, causal=True,
+                    window=0, k_scale=None, v_scale=None, out=None, return_lse=False,
+                    workspace=None, stream=None):
+    """Attention of the new tokens q [T, Hq, D] over a paged cache that holds them already
+    (paged_append), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)).
+
+    The new token at position p attends to its sequence's tokens j < kv_len[b] that have
+    a page, j <= p if causal, j > p - window if window > 0; one that attends to nothing,
+    and rows from cu_q[B] on, get 0.  fp16 or bf16, the cache in q's type or float8_e4m3fn
+    (times k_scale, v_scale, fp32 [Hkv]), D a multiple of 8 (e4m3: 16) up to 256.  Returns
+    o [T, Hq, D], with return_lse also log2 of the sum of e^(score), fp32 [T, Hq] (-inf
+    where nothing is attended to).  cu_q as for paged_append."""
+    import torch
+    if q.dim() != 3:
+        raise ValueError(f"q must be [T, Hq, D], got {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    dtype = q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"q: fp16 and bf16 are implemented, got {dtype}")
+    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
+    page_table, kv_len, cu_q = _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale,
+                                             v_scale, T, Hkv, D, dtype)
+    _same_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, kv_len=kv_len,
+                 cu_q=cu_q, k_scale=k_scale, v_scale=v_scale, out=out)
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or s0 % 8 or s1 % 8 or q.data_ptr() % 16:
+        q = torch.empty((T, Hq, D), dtype=dtype, device=q.device).copy_(q)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError("out must be as q, with its last dimension contiguous")
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    p = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
+              (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D,
+               k_cache.shape[1], _tx_of(dtype), _tx_of(k_cache.dtype), int(bool(causal)),
+               int(window), int(cu_q is not None), float(sm_scale)) + q.stride()[:2]
+              + out.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
+              + (page_table.stride(0),))
+    if stream is None:
+        stream = _current_stream(q.device)
+    ws = workspace if workspace is not None else workspace_for(p, q.device, stream)
+    capi.check(capi.load().tx_paged_attn_launch(
+        ctypes.byref(p), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(k_scale), _ptr(v_scale),
+        out.data_ptr(), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
+        stream))
+    return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# Pages
+# ---------------------------------------------------------------------------
+
+def _page_bytes(t, name, P):
+    """(bytes from page to page, bytes of a page) of a cache tensor [P, ...] whose pages
+    are each one block of memory."""
+    if t.dim() < 2 or t.shape[0] != P:
+        raise ValueError(f"{name} must be [{P}, ...] pages, got {tuple(t.shape)}")
+    e, n = t.element_size(), 1
+    for size, st in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda x: x[1]):
+        if size != 1 and st != n:
+            raise ValueError(f"{name}: a page must be one block of memory (strides {t.stride()})")
+        n *= size
+    return t.stride(0) * e, n * e
+
+
+def _caches(d, caches, P, device):
+    if len(caches) > capi.PAGE_CACHES:
+        raise ValueError(f"{len(caches)} caches: at most {capi.PAGE_CACHES} a call")
+    ptrs = (ctypes.c_void_p * max(len(caches), 1))()
+    d.caches = len(caches)
+    for i, t in enumerate(caches):
+        if t.device != device:
+            raise ValueError(f"cache {i} is on {t.device}, not on {device}")
+        d.stride[i], d.bytes[i] = _page_bytes(t, f"cache {i}", P)
+        ptrs[i] = t.data_ptr()
+    return ptrs
+
+
+def _books(page_table, kv_len, refs):
+    page_table, refs = _int32(page_table, "page_table", 2), _int32(refs, "refs", 1)
+    if kv_len is not None:
+        kv_len = _int32(kv_len, "kv_len", 1)
+        if kv_len.shape[0] != page_table.shape[0]:
+            raise ValueError(f"page_table has {page_table.shape[0]} rows, kv_len "
+                             f"{kv_len.shape[0]}")
+    _same_device(page_table.device, kv_len=kv_len, refs=refs)
+    d = capi.PageDesc()
+    (d.S, d.W), d.P = page_table.shape, refs.shape[0]
+    d.page_size = 1
+    return d, page_table, kv_len, refs
+
+
+def _new_books(out, *like):
+    """The books to write: `out`, checked, or new ones."""
+    import torch
+    if out is None:
+        return tuple(torch.empty_like(t) for t in like)
+    if len(out) != len(like):
+        raise ValueError(f"out must be {len(like)} tensors")
+    for t, u in zip(out, like):
+        if t.shape != u.shape or t.dtype != u.dtype or t.device != u.device or not t.is_contiguous():
+            raise ValueError(f"out must be contiguous and as the books read: {tuple(t.shape)} "
+                             f"{t.dtype} for {tuple(u.shape)} {u.dtype}")
+    return tuple(out)
+
+
+_COUNTERS = 65536
+
+
+class _Need:
+    """What workspace_for asks of a plan: the scratch memory of a call on pages.  The first
+    64 KiB of a workspace are the arrival counters of other launches."""
+
+    def __init__(self, d):
+        n = ctypes.c_int64(0)
+        capi.check(capi.load().tx_page_workspace(ctypes.byref(d), ctypes.byref(n)))
+        self.workspace_bytes = _COUNTERS + n.value
+
+    def scratch(self, device, stream):
+        return workspace_for(self, device, stream).data_ptr() + _COUNTERS
+
+
+def page_copy(caches, src, dst, *, stream=None):
+    """Copies page src[i] of every cache [P, ...] to page dst[i] (int32 [n]).  Entries
+    outside [0, P) are skipped; no dst may be another dst, or a src but its own."""
+    caches = list(caches)
+    src, dst = _int32(src, "src", 1), _int32(dst, "dst", 1)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must be of one length")
+    if not caches:
+        return
+    d = capi.PageDesc()
+    d.P, d.n, d.page_size = caches[0].shape[0], src.shape[0], 1
+    _same_device(src.device, dst=dst)
+    ptrs = _caches(d, caches, d.P, src.device)
+    _Need(d)
+    if stream is None:
+        stream = _current_stream(src.device)
+    capi.check(capi.load().tx_page_copy(ctypes.byref(d), ptrs, src.data_ptr(), dst.data_ptr(),
+                                        stream))
+
+
+def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stream=None):
+    """Pages for sequences to grow to new_len [S] tokens (never less than kv_len, at most the
+    table's width): free pages (refs 0) in ascending order, for one sequence after
+    the other.  Returns page_table, kv_len, refs, and how many pages were missing (an
+    int32 scalar on the device; those entries are -1).  out: the three tensors to write,
+    which may be those read."""
+    import torch
+    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
+    new_len = _int32(new_len, "new_len", 1)
+    if new_len.shape != kv_len.shape:
+        raise ValueError("new_len must be as kv_len")
+    _same_device(refs.device, new_len=new_len)
+    d.page_size = page_size
+    t, n, r = _new_books(out, page_table, kv_len, refs)
+    missing = torch.empty((), dtype=torch.int32, device=refs.device)
+    need = _Need(d)
+    if stream is None:
+        stream = _current_stream(refs.device)
+    capi.check(capi.load().tx_page_reserve(
+        ctypes.byref(d), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        new_len.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(), missing.data_ptr(),
+        need.scratch(refs.device, stream), stream))
+    return t, n, r, missing
+
+
+def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stream=None):
+    """Sequences child[i] (empty rows, each named once) become copies of parent[i] that share
+    its pages; a last page that is not full is copied, in every cache [P, page_size, ...],
+    to a free one.  Returns page_table, kv_len, refs and the missing pages, as page_reserve."""
+    import torch
+    caches = list(caches)
+    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
+    parent, child = _int32(parent, "parent", 1), _int32(child, "child", 1)
+    if parent.shape != child.shape:
+        raise ValueError("parent and child must be of one length")
+    if not caches:
+        raise ValueError("page_fork needs the caches: the size of a page is theirs")
+    _same_device(refs.device, parent=parent, child=child)
+    d.n, d.page_size = parent.shape[0], caches[0].shape[1]
+    ptrs = _caches(d, caches, d.P, refs.device)
+    for i, c in enumerate(caches):
+        if c.shape[1] != d.page_size:
+            raise ValueError(f"cache {i} has pages of {c.shape[1]} tokens, cache 0 of {d.page_size}")
+    t, n, r = _new_books(out, page_table, kv_len, refs)
+    missing = torch.empty((), dtype=torch.int32, device=refs.device)
+    need = _Need(d)
+    if stream is None:
+        stream = _current_stream(refs.device)
+    capi.check(capi.load().tx_page_fork(
+        ctypes.byref(d), ptrs, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        parent.data_ptr(), child.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
+        missing.data_ptr(), need.scratch(refs.device, stream), stream))
+    return t, n, r, missing
+
+
+def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=None):
+    """Sequences with drop[s] (bool [S]) give their pages back and become empty.  Returns
+    page_table, kv_len, refs; out as for page_reserve."""
+    import torch
+    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
+    if drop.dtype not in (torch.bool, torch.uint8) or drop.shape != kv_len.shape:
+        raise ValueError("drop must be a bool tensor as long as kv_len")
+    drop = drop.contiguous()
+    _same_device(refs.device, drop=drop)
+    d.page_size = page_size
+    t, n, r = _new_books(out, page_table, kv_len, refs)
+    _Need(d)
+    if stream is None:
+        stream = _current_stream(refs.device)
+    capi.check(capi.load().tx_page_free(
+        ctypes.byref(d), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        drop.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(), stream))
+    return t, n, r
+
+
+def page_compact(caches, page_table, refs, *, out=None, stream=None):
+    """Moves the pages in use (refs > 0) together: with U of them, those from U on go, in
+    order, to the free ones below U, in every cache [P, ...] and in the books.  Returns
+    page_table, refs and how many were moved (an int32 scalar on the device)."""
+    import torch
+    caches = list(caches)
+    d, page_table, _, refs = _books(page_table, None, refs)
+    ptrs = _caches(d, caches, d.P, refs.device)
+    t, r = _new_books(out, page_table, refs)
+    moved = torch.empty((), dtype=torch.int32, device=refs.device)
+    need = _Need(d)
+    if stream is None:
+        stream = _current_stream(refs.device)
+    capi.check(capi.load().tx_page_compact(
+        ctypes.byref(d), ptrs, page_table.data_ptr(), refs.data_ptr(), t.data_ptr(), r.data_ptr(),
+        moved.data_ptr(), need.scratch(refs.device, stream), stream))
+    return t, r, moved

@@ -1,4 +1,4 @@
-"""ctypes mirror of include/triton_ext/{TritonExtPassInfra,tx_dot,tx_passes,tx_attn}.h."""
+"""ctypes mirror of include/triton_ext/{TritonExtPassInfra,tx_dot,tx_passes,tx_attn,tx_cache}.h."""
 import ctypes
 import os
 
@@ -74,6 +74,60 @@ class AttnPlan(ctypes.Structure):
                 ("block_threads", ctypes.c_int32), ("key_groups", ctypes.c_int32)]
 
 
+def _i64(names):
+    return [(n, ctypes.c_int64) for n in names.split()]
+
+
+def _i32(names):
+    return [(n, ctypes.c_int32) for n in names.split()]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = (_i64("Z N H") + _i32("head_dim rot_dim dtype interleaved inverse pos_bits")
+                + [("scale", ctypes.c_float)] + _i32("reserved")
+                + _i64("pos_sz x_sz x_sn x_sh o_sz o_sn o_sh"))
+
+
+class RotaryPlan(ctypes.Structure):
+    _fields_ = ([("desc", RotaryDesc), ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
+                + _i32("vec head_lanes grid_x block_threads"))
+
+
+class PagedAppendDesc(ctypes.Structure):
+    _fields_ = (_i64("T B pages table_width")
+                + _i32("Hq Hkv head_dim rot_dim page_size dtype cache_type interleaved ragged")
+                + [("scale", ctypes.c_float)]
+                + _i64("q_st q_sh o_st o_sh k_st k_sh v_st v_sh kc_sp kc_st kc_sh vc_sp vc_st "
+                       "vc_sh table_s"))
+
+
+class PagedAppendPlan(ctypes.Structure):
+    _fields_ = ([("desc", PagedAppendDesc), ("flops", ctypes.c_double),
+                 ("bytes", ctypes.c_double)] + _i32("vec head_lanes grid_x block_threads"))
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = (_i64("T B pages table_width")
+                + _i32("Hq Hkv head_dim page_size dtype cache_type causal window ragged")
+                + [("sm_scale", ctypes.c_float)]
+                + _i64("q_st q_sh o_st o_sh k_sp k_st k_sh v_sp v_st v_sh table_s"))
+
+
+class PagedAttnPlan(ctypes.Structure):
+    _fields_ = ([("desc", PagedAttnDesc)]
+                + _i32("variant rows slots units grid_x block_threads")
+                + _i64("workspace_bytes"))
+
+
+PAGE_CACHES = 128  # TX_PAGE_CACHES
+
+
+class PageDesc(ctypes.Structure):
+    _fields_ = (_i64("S W P n") + _i32("page_size caches")
+                + [("stride", ctypes.c_int64 * PAGE_CACHES),
+                   ("bytes", ctypes.c_int64 * PAGE_CACHES)])
+
+
 class LoopSplit(ctypes.Structure):
     _fields_ = [("split", ctypes.c_int32), ("first_value", ctypes.c_int32),
                 ("second_value", ctypes.c_int32), ("reserved", ctypes.c_int32),
@@ -102,7 +156,12 @@ EXPORTS = {
                               "tx_mi355x_peak_bw", "tx_arith_intensity", "tx_dot_operand_spans",
                               "tx_ring_reaches"],
     "libmi355x_dot.so": ["tx_dot_plan_create", "tx_dot_launch", "tx_dot_launch_noalloc",
-                         "tx_get_last_error", "tx_kernel_name", "tx_device_available"],
+                         "tx_get_last_error", "tx_kernel_name", "tx_device_available",
+                         "tx_rotary_plan_create", "tx_rotary_launch",
+                         "tx_paged_append_plan_create", "tx_paged_append_launch",
+                         "tx_paged_attn_plan_create", "tx_paged_attn_launch",
+                         "tx_page_workspace", "tx_page_copy", "tx_page_reserve", "tx_page_fork",
+                         "tx_page_free", "tx_page_compact"],
 }
 
 _libs = {}
@@ -161,6 +220,18 @@ def load(name="libmi355x_dot.so"):
         L.tx_kernel_name.restype = ctypes.c_char_p
         L.tx_attn_fwd_plan.argtypes = [ctypes.POINTER(AttnDesc), ctypes.POINTER(AttnPlan)]
         L.tx_attn_fwd_launch.argtypes = [ctypes.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp]
+        for f, desc, pl in (("rotary", RotaryDesc, RotaryPlan),
+                            ("paged_append", PagedAppendDesc, PagedAppendPlan),
+                            ("paged_attn", PagedAttnDesc, PagedAttnPlan)):
+            getattr(L, f"tx_{f}_plan_create").argtypes = [ctypes.POINTER(desc), ctypes.POINTER(pl)]
+        L.tx_rotary_launch.argtypes = [ctypes.POINTER(RotaryPlan)] + [vp] * 5
+        L.tx_paged_append_launch.argtypes = [ctypes.POINTER(PagedAppendPlan)] + [vp] * 13
+        L.tx_paged_attn_launch.argtypes = ([ctypes.POINTER(PagedAttnPlan)] + [vp] * 11
+                                           + [ctypes.c_size_t, vp])
+        pd = ctypes.POINTER(PageDesc)
+        L.tx_page_workspace.argtypes = [pd, ctypes.POINTER(i64)]
+        for f, n in (("copy", 4), ("reserve", 10), ("fork", 12), ("free", 8), ("compact", 8)):
+            getattr(L, f"tx_page_{f}").argtypes = [pd] + [vp] * n
     _libs[name] = L
     return L
 
