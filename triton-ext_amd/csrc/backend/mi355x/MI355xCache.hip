@@ -13,6 +13,12 @@
 
 using namespace txk;
 
+namespace txk {
+typedef void (*PagedAttnFn)(PagedAttnArgs);
+// [64, 96, 128, 256 dims][bf16][e4m3 cache] (kernels_paged_*.hip)
+extern const PagedAttnFn kPagedAttnSplit[4][2][2], kPagedAttnRows[4][2][2];
+} // namespace txk
+
 namespace {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -364,6 +370,28 @@ extern "C" TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, c
 // Attention over the cache
 // ---------------------------------------------------------------------------
 
+namespace {
+
+constexpr int64_t kAttnCounters = 65536; // the arrival counters that every workspace begins with
+
+// The dims that a head is computed in.
+int attnDims(int head_dim) {
+  return head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
+}
+// Keys of a block in the split form: tiles of 8 KiB (4: e4m3 heads of 64; 16: heads of 256).
+int splitBlock(int D, bool f8) { return f8 || D == 64 ? 64 : 32; }
+
+// Rows of a page that one buffer resource covers: as many as divide a page and the rows
+// that a wave loads, with 31-bit offsets.
+int runOf(int rows, int page_size, int64_t st, int64_t row_bytes) {
+  int run = std::min(rows, page_size);
+  while (run > 1 && ((run - 1) * st + row_bytes >= ((int64_t)1 << 31) || st >= ((int64_t)1 << 31)))
+    run /= 2;
+  return run;
+}
+
+} // namespace
+
 extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
                                                 tx_paged_attn_plan *plan) {
   clearError();
@@ -396,13 +424,31 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   if (d.k_sp % quantum || d.k_st % quantum || d.k_sh % quantum || d.v_sp % quantum ||
       d.v_st % quantum || d.v_sh % quantum)
     return fail(TX_ERR_INVALID, "cache strides must be multiples of 16 bytes");
+  if (d.T * (int64_t)(d.Hkv ? d.Hq / d.Hkv : 0) > INT32_MAX)
+    return fail(TX_ERR_UNSUPPORTED, "more than 2^31 rows of a kv head");
   std::memset(plan, 0, sizeof(*plan));
   plan->desc = d;
-  plan->variant = 0;
-  plan->rows = 1;
-  plan->units = (int32_t)d.T;
-  plan->grid_x = (int32_t)d.T;
   plan->block_threads = 256;
+  if (d.T == 0)
+    return TX_OK;
+  // Up to 32 rows a sequence of one kv head: units of 32, their keys shared out among waves
+  // (memory bounds both forms there); more: units of 128.
+  const int64_t G = d.Hq / d.Hkv;
+  plan->variant = d.T * G > 32 * d.B;
+  plan->rows = plan->variant ? 128 : 32;
+  const int D = attnDims(d.head_dim);
+  const bool f8 = d.cache_type == TX_F8E4M3;
+  const int per_cu = D > 128 ? 1 : 2;
+  // the most steps of work there can be (a step: the keys a workgroup takes at a time)
+  const int step = plan->variant ? 64 : 4 * splitBlock(D, f8);
+  const double units = (double)d.B + (double)d.T * G / plan->rows;
+  const double keys = (double)d.table_width * d.page_size;
+  const double steps = units * (keys / step + 1) * d.Hkv;
+  plan->units = (int32_t)std::min<double>(256 * per_cu, std::ceil(steps));
+  plan->grid_x = plan->units;
+  plan->slots = 2 * plan->units;
+  plan->workspace_bytes =
+      kAttnCounters + (int64_t)plan->slots * plan->rows * (D + 2) * (int64_t)sizeof(float);
   return TX_OK;
 }
 
@@ -443,24 +489,33 @@ extern "C" TX_API int tx_paged_attn_launch(const tx_paged_attn_plan *plan, const
   if (!tx_device_available())
     return fail(TX_ERR_NO_DEVICE, "no gfx950 device visible");
   PagedAttnArgs a;
+  const bool f8 = d.cache_type == TX_F8E4M3;
+  const int64_t ce = f8 ? 1 : 2;
+  const int D = attnDims(d.head_dim);
   a.q = q, a.o = o, a.lse = lse;
   a.kc = static_cast<const uint8_t *>(k_cache), a.vc = static_cast<const uint8_t *>(v_cache);
   a.table = page_table, a.kv_len = kv_len, a.cu_q = cu_q;
   a.k_scale = k_scale, a.v_scale = v_scale;
-  a.counters = nullptr, a.parts = nullptr;
-  a.T = d.T, a.pages = d.pages, a.table_width = d.table_width, a.table_s = d.table_s;
+  a.counters = static_cast<uint32_t *>(workspace);
+  a.parts = static_cast<uint8_t *>(workspace) + kAttnCounters;
+  a.table_width = d.table_width, a.table_s = d.table_s;
+  a.most = (int32_t)std::min<int64_t>(d.table_width * d.page_size, INT32_MAX - 127);
   a.q_st = d.q_st, a.q_sh = d.q_sh, a.o_st = d.o_st, a.o_sh = d.o_sh;
-  a.k_sp = d.k_sp, a.k_st = d.k_st, a.k_sh = d.k_sh;
-  a.v_sp = d.v_sp, a.v_st = d.v_st, a.v_sh = d.v_sh;
-  a.B = (int32_t)d.B, a.Hq = d.Hq, a.Hkv = d.Hkv, a.head_dim = d.head_dim;
-  a.page_shift = log2of(d.page_size), a.causal = d.causal, a.window = d.window;
+  a.k_sp = d.k_sp * ce, a.k_st = d.k_st * ce, a.k_sh = d.k_sh * ce;
+  a.v_sp = d.v_sp * ce, a.v_st = d.v_st * ce, a.v_sh = d.v_sh * ce;
+  a.pages = (uint32_t)d.pages, a.min_share = 1;
+  a.T = (int32_t)d.T, a.B = (int32_t)d.B, a.G = d.Hq / d.Hkv, a.Hq = d.Hq, a.Hkv = d.Hkv;
+  a.head_dim = d.head_dim, a.page_shift = log2of(d.page_size);
+  a.causal = d.causal, a.window = d.window;
+  const int wave_rows = plan->variant ? 16 : splitBlock(D, f8);
+  a.k_run = runOf(wave_rows, d.page_size, a.k_st, d.head_dim * ce);
+  a.v_run = runOf(wave_rows, d.page_size, a.v_st, d.head_dim * ce);
   a.qk_scale = d.sm_scale * 1.44269504f;
-  const bool f8 = d.cache_type == TX_F8E4M3;
-  auto fn = d.dtype == TX_F16 ? (f8 ? paged_attn_plain_kernel<_Float16, uint8_t>
-                                    : paged_attn_plain_kernel<_Float16, _Float16>)
-                              : (f8 ? paged_attn_plain_kernel<__bf16, uint8_t>
-                                    : paged_attn_plain_kernel<__bf16, __bf16>);
-  hipLaunchKernelGGL(fn, dim3(plan->grid_x, d.Hq), dim3(plan->block_threads), 0,
+  const PagedAttnFn fn =
+      (plan->variant ? kPagedAttnRows
+                     : kPagedAttnSplit)[D == 64 ? 0 : D == 96 ? 1 : D == 128 ? 2 : 3]
+                                       [d.dtype == TX_BF16][f8];
+  hipLaunchKernelGGL(fn, dim3(plan->grid_x), dim3(plan->block_threads), 0,
                      static_cast<hipStream_t>(stream), a);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;

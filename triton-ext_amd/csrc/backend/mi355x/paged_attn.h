@@ -1,7 +1,32 @@
-// Attention of new tokens over a paged cache (tx_cache.h), the plain way: one
-// workgroup per token and query head, 256 keys at a time.
+// Attention of new tokens over a paged cache (tx_cache.h).
+//
+// The G = Hq / Hkv query heads of one kv head read the same keys, so a sequence's new
+// tokens make n G rows of one (sequence, kv head): row r is token r / G, head r % G.  A
+// unit is a block of BM such rows; its keys are those between the first row's
+// first and the last row's last, BN at a time.  Per block, on 32 rows a wave:
+//   S^T = K . Q^T     32x32x16 MFMAs, A := K rows from LDS, B := Q rows, held in
+//                     registers: lane l holds row l%32 and keys 8 (r/4) + 4 (l/32) + r%4 of
+//                     each 32 of the block;
+//   softmax           running maximum and sum in fp32 (base 2);
+//   O^T += V^T . P^T  A := V columns by transposed LDS reads, B := P from the S^T
+//                     registers, rounded to q's type (the matrix cores' operand; the sum of
+//                     p is taken before that rounding).
+// e4m3 caches are widened to q's type (exactly) between LDS and the matrix cores.
+//
+// Pages: a load into LDS takes 1 KiB, whole rows of one page, through a buffer
+// resource made from the page's base by scalar instructions, so rows past the last
+// key and pages that are not there come as zeros and no lane forms an address.  A lane
+// holds each of 64 entries of the table row in turn.
+//
+// The lengths are known on the device only, and differ widely.  So the launch has one
+// workgroup per place on the chip, all blocks of all units (kv heads outermost) are
+// laid end to end, and each workgroup takes an equal run of them.  Parts of a unit go
+// to the workspace, and the last workgroup to arrive joins them in order (so the
+// result does not depend on which that is).
 #pragma once
 
+#include "attn_fwd.h"
+#include "decode_i8.h"
 #include "rotary.h"
 
 namespace txk {
@@ -13,96 +38,1136 @@ struct PagedAttnArgs {
   const float *k_scale, *v_scale;
   void *o;
   float *lse;
-  uint32_t *counters;
-  uint8_t *parts;
-  int64_t T, pages, table_width, table_s;
-  int64_t q_st, q_sh, o_st, o_sh, k_sp, k_st, k_sh, v_sp, v_st, v_sh;
-  int32_t B, Hq, Hkv, head_dim, page_shift, causal, window;
-  float qk_scale; // sm_scale / ln 2
+  uint32_t *counters; // [grid]
+  uint8_t *parts;     // [grid][2][A::PART]
+  int64_t table_width, table_s;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int64_t k_sp, k_st, k_sh, v_sp, v_st, v_sh; // bytes
+  uint32_t pages, min_share;
+  int32_t most; // keys that a table row has place for
+  int32_t T, B, G, Hq, Hkv, head_dim, page_shift, causal, window;
+  int32_t k_run, v_run; // rows of one resource
+  float qk_scale;       // sm_scale / ln 2
 };
 
-__device__ __forceinline__ float e4m3_to_f32(uint8_t x) {
-  return __builtin_amdgcn_cvt_f32_fp8(x, 0);
+// s_waitcnt that no memory access of the compiler's crosses.
+template <int N> __device__ __forceinline__ void paged_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-template <class T, class C> __device__ __forceinline__ float cache_f32(const uint8_t *row, int d) {
-  if constexpr (std::is_same<C, uint8_t>::value)
-    return e4m3_to_f32(row[d]);
-  else
-    return elt_to_f32(reinterpret_cast<const T *>(row)[d]);
+__device__ __forceinline__ void paged_lgkmcnt0() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ int lane_value(int v, int lane) {
+  return __builtin_amdgcn_readlane(v, lane);
 }
 
-template <class T, class C>
-__global__ void __launch_bounds__(256) paged_attn_plain_kernel(PagedAttnArgs p) {
-  __shared__ float qs[256], ps[256], red[4];
-  __shared__ int64_t pg[256];
-  const int tid = threadIdx.x, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
-  const int64_t t = blockIdx.x;
-  int b = (int)t;
-  int64_t pos, len = 0;
-  if (p.cu_q) {
-    b = sequence_of(p.cu_q, p.B, t);
-    const int64_t first = p.cu_q[b], last = p.cu_q[b + 1];
-    pos = (int64_t)p.kv_len[b] - last + t;
-    if (t >= first && t < last)
-      len = p.kv_len[b];
-  } else {
-    pos = (int64_t)p.kv_len[b] - 1;
-    len = p.kv_len[b];
+// ---------------------------------------------------------------------------
+// Fragments
+// ---------------------------------------------------------------------------
+
+// D: dims computed (heads of up to D); F8: the cache is e4m3; BN: keys of a block.
+// LDS rows have a power of two of bytes (96 dims in rows of 128); 16-byte chunk c of row r
+// lies at c ^ swizzle(r), so that the rows of one ds_read_b128 or transposed read fall on
+// different banks.
+template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
+  static constexpr int D = D_, BN = BN_;
+  static constexpr bool F8 = F8_;
+  static constexpr int ESZ = F8 ? 1 : 2;
+  static constexpr int ROW = (D == 96 ? 128 : D) * ESZ, TILE = BN * ROW, CPR = ROW / 16;
+  static constexpr int R = 1024 / ROW; // rows of a 1 KiB load
+  static constexpr uint32_t kOOB = 0x80000000u;
+  static_assert(D == 64 || D == 96 || D == 128 || D == 256, "head dims");
+  static_assert(BN == 32 || BN == 64, "blocks");
+  typedef AttnFwd<64, BF, 32, 64> X; // exchanges and MFMAs of the type
+  typedef typename X::elt elt;
+  typedef typename X::h8 h8;
+  typedef typename X::h4 h4;
+  typedef float f16v __attribute__((ext_vector_type(16)));
+  typedef elt h2 __attribute__((ext_vector_type(2)));
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+  __device__ __forceinline__ static int kswz(int r) {
+    return ROW == 64 ? (r >> 2) & 3 : ROW == 128 ? (r >> 1) & 7 : r & 15;
   }
-  int64_t lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
-  int64_t hi = p.causal && pos + 1 < len ? pos + 1 : len;
-  const int64_t most = p.table_width << p.page_shift;
-  hi = hi < most ? hi : most;
-  if (tid < p.head_dim)
-    qs[tid] = elt_to_f32(static_cast<const T *>(p.q)[t * p.q_st + h * p.q_sh + tid]) *
-              (p.k_scale ? p.k_scale[hk] : 1.f);
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int64_t j0 = lo; j0 < hi; j0 += 256) {
-    __syncthreads();
-    const int64_t j = j0 + tid;
-    int64_t page = -1;
-    if (j < hi)
-      page = p.table[b * p.table_s + (j >> p.page_shift)];
-    if (page >= p.pages)
-      page = -1;
-    float s = -INFINITY;
-    const int64_t slot = j & ((1 << p.page_shift) - 1);
-    if (page >= 0) {
-      const uint8_t *row = p.kc + (page * p.k_sp + slot * p.k_st + hk * p.k_sh) * sizeof(C);
-      s = 0.f;
-      for (int d = 0; d < p.head_dim; ++d)
-        s += qs[d] * cache_f32<T, C>(row, d);
-      s *= p.qk_scale;
+  // 16-bit: 4 rows x 64 bytes of a pass; e4m3: 8 rows (keys 0-3 and 8-11 of 16) x 32 bytes.
+  __device__ __forceinline__ static int vswz(int r) {
+    if constexpr (F8)
+      return ROW == 64    ? 2 * ((r >> 3) & 1)
+             : ROW == 128 ? 2 * (((r >> 1) & 1) | ((r >> 2) & 2))
+                          : 2 * ((r & 3) | ((r >> 1) & 4));
+    else
+      return ROW == 128 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+  }
+  // 8 e4m3 values to q's type, exact.
+  __device__ __forceinline__ static h8 widen(int lo, int hi) {
+    h8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int w = i < 2 ? lo : hi;
+      h2 t;
+      if constexpr (BF)
+        t = __builtin_bit_cast(h2, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+      else
+        t = __builtin_bit_cast(h2, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+      r[2 * i] = t[0], r[2 * i + 1] = t[1];
     }
-    float mx = s;
-    for (int d = 32; d; d /= 2)
-      mx = fmaxf(mx, __shfl_xor(mx, d));
-    if ((tid & 63) == 0)
-      red[tid >> 6] = mx;
+    return r;
+  }
+
+  // Lane offsets of the 1 KiB load `u` of a tile (row lane / CPR of it, at chunk position
+  // lane % CPR), from the row that the load's resource begins with (one of every `run`).
+  template <bool V>
+  __device__ __forceinline__ static uint32_t offset(int u, uint32_t st, int run, int row_bytes) {
+    const int lane = threadIdx.x & 63, row = R * u + lane / CPR, pos = lane % CPR;
+    const int c = pos ^ (V ? vswz(row) : kswz(row));
+    return 16 * c >= row_bytes ? kOOB : (uint32_t)(row & (run - 1)) * st + 16 * c;
+  }
+
+  // Per-lane LDS addresses of the fragment reads in a tile; the other fragments lie at
+  // constants from these.
+  //   K: key l%32, 16-byte chunk 2 c + l/32: dims 16 c + 8 (l/32) .. of MFMA c, or (e4m3) dims
+  //     32 c + 16 (l/32) .., 8 each of MFMAs 2 c and 2 c + 1;
+  //   V, dim block bd: the row and column that the lane gives a transposed read: 16-bit keys
+  //     4 (l/32) + (l%16)/4 (and 8 further); e4m3 keys 4 (l/32) + 0..3 and + 8..11 by (l%16)/2.
+  static constexpr int NK = F8 ? D / 32 : D / 16, NV = D / 32;
+  struct Bases {
+    uint32_t k[NK], v[NV];
+  };
+  __device__ __forceinline__ static void bases(uint32_t k_lds, uint32_t v_lds, Bases &bs) {
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5, L = lane & 15;
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+      bs.k[c] = k_lds + r * ROW + (((2 * c + g) ^ kswz(r)) << 4);
+#pragma unroll
+    for (int bd = 0; bd < NV; ++bd) {
+      const int d0 = 32 * bd + 16 * ((lane >> 4) & 1);
+      if constexpr (F8) {
+        const int j = L >> 1, key = 4 * g + (j & 3) + 8 * (j >> 2);
+        bs.v[bd] = v_lds + key * ROW + (((d0 >> 4) ^ vswz(key)) << 4) + 8 * (L & 1);
+      } else {
+        const int d = d0 + 4 * (L & 3), key = 4 * g + (L >> 2);
+        bs.v[bd] = v_lds + key * ROW + (((d >> 3) ^ vswz(key)) << 4) + (d & 7) * 2;
+      }
+    }
+  }
+
+  // Q rows as MFMA B operands in the order of K's dims.  scale < 0: the rows change their
+  // sign, scale 0: they are zero, so that scores are taken times |scale| (or 1) > 0.
+  struct QF {
+    h8 v[D / 16];
+  };
+  __device__ __forceinline__ static void load_q(const void *row, bool live, int head_dim,
+                                                float scale, QF &qf) {
+    const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const int d = F8 ? 32 * (c / 2) + 16 * g + 8 * (c % 2) : 16 * c + 8 * g;
+      const bool in = live && d < head_dim && scale != 0.f;
+      i32x4_t x = *reinterpret_cast<const i32x4_t *>(static_cast<const elt *>(row) + (in ? d : 0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[i] = in ? x[i] ^ (scale < 0.f ? (int)0x80008000 : 0) : 0;
+      qf.v[c] = __builtin_bit_cast(h8, x);
+    }
+  }
+
+  // K fragments of the tile at byte `at`.
+  struct KF {
+    i32x4_t v[BN / 32][NK];
+  };
+  __device__ __forceinline__ static void read_k(const Bases &bs, int at, KF &kf) {
+    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+        kf.v[b][c] = *(const lds_i32x4 *)(uintptr_t)(bs.k[c] + at + b * 32 * ROW);
+  }
+  __device__ __forceinline__ static void qk(const KF &kf, const QF &qf, f16v (&s)[BN / 32]) {
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b) {
+      s[b] = f16v{};
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        if constexpr (F8) {
+          s[b] = X::mfma(widen(kf.v[b][c][0], kf.v[b][c][1]), qf.v[2 * c], s[b]);
+          s[b] = X::mfma(widen(kf.v[b][c][2], kf.v[b][c][3]), qf.v[2 * c + 1], s[b]);
+        } else {
+          s[b] = X::mfma(__builtin_bit_cast(h8, kf.v[b][c]), qf.v[c], s[b]);
+        }
+      }
+    }
+  }
+  // V fragments of dim blocks b0 .. b0 + N - 1.
+  template <int N> struct VF {
+    i32x4_t v[N][BN / 16]; // e4m3: .xy
+  };
+  template <int N>
+  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<N> &vf) {
+#pragma unroll
+    for (int bd = 0; bd < N; ++bd)
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        const uint32_t a = bs.v[b0 + bd] + at + c * 16 * ROW;
+        if constexpr (F8) {
+          typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+          const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(uintptr_t)a);
+          vf.v[bd][c][0] = x[0], vf.v[bd][c][1] = x[1];
+        } else {
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)a);
+          const i16x4_t hi =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)(a + 8 * ROW));
+          vf.v[bd][c] =
+              __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      }
+  }
+  template <int N>
+  __device__ __forceinline__ static void pv(const VF<N> &vf, int b0, const h8 (&pf)[BN / 16],
+                                            f16v (&acc)[D / 32]) {
+#pragma unroll
+    for (int bd = 0; bd < N; ++bd)
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        h8 x;
+        if constexpr (F8)
+          x = widen(vf.v[bd][c][0], vf.v[bd][c][1]);
+        else
+          x = __builtin_bit_cast(h8, vf.v[bd][c]);
+        acc[b0 + bd] = X::mfma(x, pf[c], acc[b0 + bd]);
+      }
+  }
+
+  // One block's softmax: s are its scores (times qk_scale > 0 they are base-2 exponents); MASK:
+  // bit n of `seen` says that the lane's row attends to key n of the block.  Updates the row's
+  // reference m (both lanes of a row hold the same), the lane's part of the sum l, and acc; p as
+  // MFMA operands.  m follows the maximum only when that has grown by more than 8, so p is
+  // up to 2^8 (in range in both types, and rounded by the same relative half step), and
+  // acc is seldom rescaled.
+  template <bool MASK>
+  __device__ __forceinline__ static void softmax(f16v (&s)[BN / 32], uint64_t seen, float qk_scale,
+                                                 f16v (&acc)[D / 32], float &m, float &l,
+                                                 h8 (&pf)[BN / 16]) {
+    if constexpr (MASK) {
+      const uint64_t mine = seen >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b) {
+        const uint32_t w = (uint32_t)(mine >> (32 * b));
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[b][r] = (w >> (8 * (r / 4) + r % 4)) & 1 ? s[b][r] : -INFINITY;
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        mx = fmaxf(mx, s[b][r]);
+    mx = X::xmax(mx) * qk_scale;
+    if (__any(mx > m + 8.f)) {
+      const float to = mx > m + 8.f ? mx : m;
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+      l *= alpha;
+#pragma unroll
+      for (int bd = 0; bd < D / 32; ++bd)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[bd][r] *= alpha;
+      m = to;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], qk_scale, -base));
+        sum += s[b][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int c = 0; c < BN / 16; ++c)
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        pf[c][t] = (elt)s[c / 2][8 * (c % 2) + t];
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Pages into LDS
+// ---------------------------------------------------------------------------
+
+// One wave's view of a table row: lane i holds entry `first` + i (-1: no page).
+struct PageRow {
+  const int32_t *row;
+  int64_t width;
+  uint32_t pages;
+  int shift, first, ids;
+  uint64_t holes; // lanes without a page
+
+  // Holds the entries of keys [n, n + 64).
+  __device__ __forceinline__ void hold(int n, bool anew) {
+    const int e0 = n >> shift, e1 = (n + 63) >> shift;
+    if (!anew && e0 >= first && e1 < first + 64)
+      return;
+    first = e0;
+    const int64_t e = (int64_t)e0 + (threadIdx.x & 63);
+    ids = -1;
+    if (e < width)
+      ids = row[e];
+    if ((uint32_t)ids >= pages)
+      ids = -1;
+    holes = __ballot(ids < 0);
+  }
+  // Which of the BN keys from n on, before `end`, have a page.
+  template <int BN> __device__ __forceinline__ uint64_t there(int n, int end) const {
+    const uint64_t all = ~0ull >> (64 - BN);
+    const int e0 = (n >> shift) - first, e1 = ((n + BN - 1) >> shift) - first;
+    const uint64_t span = (~0ull >> (63 - (e1 - e0))) << e0;
+    if (!(holes & span) && n + BN <= end)
+      return all;
+    const int key = n + (threadIdx.x & 63);
+    const int id = __shfl(ids, ((key >> shift) - first) & 63);
+    return __ballot(key < end && id >= 0) & all;
+  }
+};
+
+// k or v of one kv head; run: rows that one resource covers, a power of two that divides
+// a page and what a wave loads of a block.
+struct PageSide {
+  const uint8_t *base;
+  int64_t sp, st;
+  int run;
+};
+
+// Loads `first` .. first + U - 1 of the block of keys from n on into the tile at `lds`; rows
+// from `end` on come as zeros.
+template <class A, int U>
+__device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd, int n, int end,
+                                           int first, const uint32_t (&off)[U], uint32_t lds,
+                                           int row_bytes) {
+  typedef AttnFwd<64, true, 32, 64> X;
+  auto resource = [&](int key) {
+    const int id = lane_value(pr.ids, ((key >> pr.shift) - pr.first) & 63);
+    const int slot = key & ((1 << pr.shift) - 1);
+    const uint8_t *at = sd.base + (uint64_t)(uint32_t)id * (uint64_t)sd.sp +
+                        (uint64_t)(uint32_t)slot * (uint64_t)sd.st;
+    const int live = end - key < sd.run ? end - key : sd.run;
+    const uint32_t bytes = (uint32_t)(live - 1) * (uint32_t)sd.st + (uint32_t)row_bytes;
+    return make_rsrc(at, id < 0 || live <= 0 ? 0 : bytes);
+  };
+  // N resources of U / N loads each
+  auto fast = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const i32x4_t rsrc = resource(n + A::R * (first + U / N * i));
+#pragma unroll
+      for (int u = U / N * i; u < U / N * (i + 1); ++u)
+        X::dma16(off[u], rsrc, 0, lds + (first + u) * 1024);
+    }
+  };
+  if (sd.run >= U * A::R)
+    fast(std::integral_constant<int, 1>());
+  else if (U % 2 == 0 && 2 * sd.run >= U * A::R)
+    fast(std::integral_constant<int, U % 2 ? 1 : 2>());
+  else if (U % 4 == 0 && 4 * sd.run >= U * A::R)
+    fast(std::integral_constant<int, U % 4 ? 1 : 4>());
+  else { // pages of fewer rows; maybe fewer than a load has: the lanes of one at a time
+    const int lr = (threadIdx.x & 63) / A::CPR;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma nounroll
+      for (int r0 = 0; r0 < A::R; r0 += sd.run) {
+        const i32x4_t rsrc = resource(n + A::R * (first + u) + r0);
+        if (sd.run >= A::R || (lr & ~(sd.run - 1)) == r0)
+          X::dma16(off[u], rsrc, 0, lds + (first + u) * 1024);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Which blocks are whose
+// ---------------------------------------------------------------------------
+
+// A unit of work: rows r0 .. r0 + rows - 1 of sequence b and kv head hk, whose tokens begin at
+// row t0 of q and at position pos0, and of its steps those from s0 to s1.  Cut in parts,
+// this one is `part`; part j is that of workgroup w0 + j, in its first place of the workspace, but
+// part 0 in place slot0 (a workgroup's run has a cut unit at its beginning or at its end).
+struct PagedUnit {
+  int64_t pos0;
+  int t0, r0, rows, hk, b, len, lo, hi; // keys [lo, hi)
+  uint32_t s0, s1, parts, part, w0, slot0;
+};
+
+// The keys [lo, hi) of rows [r0, r1) of a sequence of `len` keys whose first new token has
+// position `at`.
+__device__ __forceinline__ void paged_keys(const PagedAttnArgs &p, int64_t at, int len, int r0, int r1,
+                                           int &lo, int &hi) {
+  const int64_t last = at + (uint32_t)(r1 - 1) / (uint32_t)p.G + 1;
+  const int64_t first = at + (uint32_t)r0 / (uint32_t)p.G - p.window + 1;
+  hi = len;
+  if (p.causal && last < hi)
+    hi = last < 0 ? 0 : (int)last;
+  lo = p.window > 0 && first > 0 ? (int)(first < hi ? first : hi) : 0;
+}
+
+// Deals out the units.  Blocks of BN keys in steps of WPS blocks (those that the waves of a
+// workgroup take side by side); a unit has one step at least, so that its rows are written.  The first
+// wave goes through this, a lane per sequence (64 at a time, in LDS) or block of rows; sums
+// across lanes.
+struct PagedSchedState {
+  int64_t pos0[64];
+  int t0[64], n[64], len[64];
+  uint32_t cost[64];
+  int cb, b, rb, hk;
+  uint32_t S, share, pos, end, s0, w; // S: steps of a kv head
+  PagedUnit unit; // rows 0: the end
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)(uint32_t)uniform((int)v) | (int64_t)uniform((int)(v >> 32)) << 32;
+}
+
+template <int BM, int BN, int WPS> struct PagedSched {
+  const PagedAttnArgs &p;
+  PagedSchedState &st;
+  const int lane = threadIdx.x & 63;
+
+  __device__ __forceinline__ PagedSched(const PagedAttnArgs &a, PagedSchedState &s) : p(a), st(s) {}
+
+  __device__ __forceinline__ uint32_t upto(uint32_t v) const { // inclusive sum over lanes
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(v, d);
+      v += lane >= d ? o : 0;
+    }
+    return v;
+  }
+  __device__ __forceinline__ static uint32_t steps_of(int lo, int hi) {
+    if (hi <= lo)
+      return 1;
+    const int blocks = (int)(((uint32_t)hi + BN - 1) / BN) - lo / BN;
+    return (blocks + WPS - 1) / WPS;
+  }
+  __device__ __forceinline__ uint32_t unit_steps(int64_t at, int len, int nr, int k) const {
+    if (k * (int64_t)BM >= nr)
+      return 0;
+    int lo, hi;
+    paged_keys(p, at, len, k * BM, nr - k * BM < BM ? nr : k * BM + BM, lo, hi);
+    return steps_of(lo, hi);
+  }
+  // The 64 sequences from `first` on; returns this lane's steps.
+  __device__ __forceinline__ uint32_t load_chunk(int first) {
+    const int q = first + lane;
+    int n = 0, t0 = 0, len = 0;
+    int64_t pos0 = 0;
+    if (q < p.B) {
+      const int raw = p.kv_len[q];
+      if (p.cu_q) {
+        const int a = p.cu_q[q], z = p.cu_q[q + 1];
+        t0 = a > 0 ? a : 0;
+        const int t1 = z < p.T ? z : p.T;
+        n = t1 > t0 ? t1 - t0 : 0;
+        pos0 = (int64_t)raw - z + t0;
+      } else {
+        t0 = q, n = 1, pos0 = (int64_t)raw - 1;
+      }
+      len = raw < 0 ? 0 : raw < p.most ? raw : p.most;
+    }
+    const int nr = n * p.G;
+    uint32_t cost = 0;
+    for (int k = 0; k < 2; ++k)
+      if (nr <= 2 * BM)
+        cost += unit_steps(pos0, len, nr, k);
+    // sequences of many blocks of rows: a lane per block
+    for (uint64_t big = __ballot(nr > 2 * BM); big; big &= big - 1) {
+      const int from = __builtin_ctzll(big);
+      const int64_t at = (int64_t)(uint32_t)lane_value((int)pos0, from) |
+                         (int64_t)lane_value((int)(pos0 >> 32), from) << 32;
+      const int ln = lane_value(len, from), rows = lane_value(nr, from);
+      uint32_t c = 0;
+      for (int k = lane; k * (int64_t)BM < rows; k += 64)
+        c += unit_steps(at, ln, rows, k);
+      c = lane_value(upto(c), 63);
+      if (lane == from)
+        cost = c;
+    }
+    st.pos0[lane] = pos0, st.t0[lane] = t0, st.n[lane] = n, st.len[lane] = len;
+    st.cost[lane] = cost;
+    st.cb = first;
+    return cost;
+  }
+
+  // The run of workgroup w of `grid`.
+  __device__ __forceinline__ void init(uint32_t w, uint32_t grid) {
+    uint32_t mine = 0;
+    for (int c = 0; c < p.B; c += 64)
+      mine += load_chunk(c);
+    const uint32_t S = lane_value(upto(mine), 63), total = S * p.Hkv;
+    uint32_t share = (total + grid - 1) / grid;
+    share = share > p.min_share ? share : p.min_share;
+    const uint64_t at = (uint64_t)share * w;
+    st.w = w, st.S = S, st.share = share;
+    st.pos = st.end = 0;
+    if (at >= total)
+      return;
+    const uint32_t pos = (uint32_t)at;
+    st.pos = pos, st.end = total - pos < share ? total : pos + share;
+    const int hk = pos / S;
+    uint32_t rem = pos - hk * S;
+    st.hk = hk;
+    int i = 0;
+    // (The loops end at the last sequence and block also if lengths change meanwhile.)
+    for (int c = 0; c < p.B; c += 64) {
+      const uint32_t cost = p.B > 64 ? load_chunk(c) : st.cost[lane];
+      const uint32_t upto_me = upto(cost), all = lane_value(upto_me, 63);
+      if (rem < all) {
+        i = __builtin_ctzll(__ballot(rem < upto_me));
+        st.b = c + i;
+        rem -= lane_value(upto_me, i) - lane_value(cost, i);
+        break;
+      }
+      rem -= all;
+    }
+    // the block of rows
+    const int rows = uniform(st.n[i]) * p.G, ln = uniform(st.len[i]);
+    const int64_t p0 = uniform64(st.pos0[i]);
+    int rb = 0;
+    if (rows > BM)
+      for (; (int64_t)rb * BM < rows; rb += 64) {
+        const uint32_t c = unit_steps(p0, ln, rows, rb + lane);
+        const uint32_t upto_me = upto(c), all = lane_value(upto_me, 63);
+        if (rem < all) {
+          const int j = __builtin_ctzll(__ballot(rem < upto_me));
+          rem -= lane_value(upto_me, j) - lane_value(c, j);
+          rb += j;
+          break;
+        }
+        rem -= all;
+      }
+    st.rb = rb, st.s0 = rem;
+  }
+
+  // The next unit of the run, into st.unit.
+  __device__ __forceinline__ void get() {
+    const uint32_t pos = uniform(st.pos), end = uniform(st.end), s0 = uniform(st.s0);
+    PagedUnit u;
+    u.rows = 0;
+    if (pos < end) {
+      u.b = uniform(st.b), u.hk = uniform(st.hk);
+      const int i = u.b - uniform(st.cb), nr = uniform(st.n[i]) * p.G;
+      int rb = uniform(st.rb);
+      u.t0 = st.t0[i], u.len = uniform(st.len[i]), u.pos0 = uniform64(st.pos0[i]);
+      u.r0 = rb * BM;
+      u.rows = nr - u.r0 < BM ? nr - u.r0 : BM;
+      paged_keys(p, u.pos0, u.len, u.r0, u.r0 + u.rows, u.lo, u.hi);
+      const uint32_t steps = steps_of(u.lo, u.hi);
+      u.s0 = s0, u.s1 = steps - s0 < end - pos ? steps : s0 + (end - pos);
+      u.parts = 1, u.part = 0, u.w0 = 0, u.slot0 = 0;
+      if (u.s1 - u.s0 < steps) {
+        const uint32_t share = uniform(st.share), first = pos - s0;
+        u.w0 = first / share;
+        u.parts = (first + steps - 1) / share - u.w0 + 1;
+        u.part = uniform(st.w) - u.w0;
+        u.slot0 = first == u.w0 * share ? 0 : 1;
+      }
+      st.pos = pos + u.s1 - u.s0, st.s0 = 0;
+      if (pos + u.s1 - u.s0 < end) { // there is another
+        if ((rb + 1) * (int64_t)BM < nr) {
+          st.rb = rb + 1;
+        } else {
+          st.rb = 0;
+          uint64_t later = __ballot(st.cost[lane] > 0) & (i == 63 ? 0 : ~0ull << (i + 1));
+          int c = uniform(st.cb), hk = u.hk;
+          while (!later && hk < p.Hkv) {
+            c += 64;
+            if (c >= p.B)
+              c = 0, ++hk;
+            later = __ballot((p.B > 64 ? load_chunk(c) : st.cost[lane]) > 0);
+          }
+          if (!later || hk >= p.Hkv)
+            st.end = 0;
+          st.b = c + (later ? __builtin_ctzll(later) : 0), st.hk = hk;
+        }
+      }
+    }
+    st.unit = u;
+  }
+};
+
+// The unit as scalars.
+__device__ __forceinline__ PagedUnit paged_unit(const volatile PagedUnit &s) {
+  PagedUnit u;
+  u.pos0 = uniform64(s.pos0);
+  u.t0 = uniform(s.t0), u.r0 = uniform(s.r0), u.rows = uniform(s.rows), u.hk = uniform(s.hk);
+  u.b = uniform(s.b), u.len = uniform(s.len), u.lo = uniform(s.lo), u.hi = uniform(s.hi);
+  u.s0 = uniform(s.s0), u.s1 = uniform(s.s1), u.parts = uniform(s.parts), u.part = uniform(s.part);
+  u.w0 = uniform(s.w0), u.slot0 = uniform(s.slot0);
+  return u;
+}
+
+// The kernel's arguments, read again from here on (they are not kept in registers through
+// the loop before).
+__device__ __forceinline__ const PagedAttnArgs &paged_args() {
+  auto *a = (const __attribute__((address_space(4))) PagedAttnArgs *)
+      __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const PagedAttnArgs *)a;
+}
+
+// Rows that belong to no sequence: zero.
+template <class T> __device__ __forceinline__ void paged_zero_rows(const PagedAttnArgs &p) {
+  if (!p.cu_q)
+    return;
+  int a = p.cu_q[0], z = p.cu_q[p.B];
+  a = a < 0 ? 0 : a < p.T ? a : p.T;
+  z = z < a ? a : z < p.T ? z : p.T;
+  for (int64_t i = blockIdx.x; i < a + p.T - z; i += gridDim.x) {
+    const int64_t t = i < a ? i : z + i - a;
+    for (int h = 0; h < p.Hq; ++h) {
+      for (int d = threadIdx.x; d < p.head_dim; d += blockDim.x)
+        static_cast<T *>(p.o)[t * p.o_st + h * p.o_sh + d] = (T)0.f;
+      if (threadIdx.x == 0 && p.lse)
+        p.lse[t * p.Hq + h] = -INFINITY;
+    }
+  }
+}
+
+// A workgroup's place in the order of work: the 8 XCDs take contiguous runs.
+__device__ __forceinline__ uint32_t paged_place() {
+  const uint32_t n = gridDim.x, b = blockIdx.x;
+  return n % 8 == 0 ? (b % 8) * (n / 8) + b / 8 : b;
+}
+
+// One part's arrival: true in the last workgroup of the unit.  Data moves between
+// workgroups with the SC1 policy only (decode_i8.h): stores are acknowledged before the count,
+// loads follow it.
+__device__ __forceinline__ bool paged_arrive(uint32_t *counter, uint32_t parts, int *flag) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t old =
+        __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = old + 1 == parts;
+    if (last)
+      __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *reinterpret_cast<volatile int *>(flag) = last;
+  }
+  __syncthreads();
+  const bool last = __builtin_amdgcn_readfirstlane(*reinterpret_cast<volatile int *>(flag));
+  __syncthreads(); // the flag's next use
+  return last;
+}
+
+// Joins (m1, l1, x1) to (m, l, x): sums relative to 2^m.
+template <class V>
+__device__ __forceinline__ void paged_join(float &m, float &l, V &x, float m1, float l1,
+                                           const V &x1) {
+  if (m1 == -INFINITY)
+    return;
+  const float to = fmaxf(m, m1);
+  const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+  const float a1 = __builtin_amdgcn_exp2f(m1 - to);
+  l = l * a + l1 * a1;
+  x = x * a + x1 * a1;
+  m = to;
+}
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// Few rows: the waves of a workgroup share out the keys
+// ---------------------------------------------------------------------------
+
+// 32 rows a unit (decoding, some drafted tokens).  Every wave goes through its own run of
+// blocks, K and V each in one LDS tile of its own that is loaded again as soon as its
+// fragments are in registers, with no barrier; at the end the four join in LDS.  Bound by
+// memory: 8 waves a CU keep up to 16 KiB each in flight.
+template <class A>
+__global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
+  constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024;
+  typedef typename A::elt elt;
+  typedef PagedSched<32, BN, 4> Sched;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * A::TILE];
+  __shared__ float ms[4][32], ls[4][32];
+  __shared__ PagedSchedState st;
+  __shared__ int flag;
+  static_assert(D * 128 <= 2 * A::TILE, "a wave's sums fit its tiles");
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row_bytes = args.head_dim * A::ESZ;
+
+  paged_zero_rows<elt>(args);
+  if (wave == 0)
+    Sched(args, st).init(paged_place(), gridDim.x);
+
+  const uint32_t k_lds = lds_addr(smem[wave]), v_lds = k_lds + A::TILE;
+  typename A::Bases bs;
+  A::bases(k_lds, v_lds, bs);
+  uint32_t ko[U], vo[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    ko[u] = A::template offset<false>(u, (uint32_t)args.k_st, args.k_run, row_bytes);
+    vo[u] = A::template offset<true>(u, (uint32_t)args.v_st, args.v_run, row_bytes);
+  }
+  const bool whole_loads = args.k_run >= A::R && args.v_run >= A::R;
+
+  for (;;) {
+    const PagedAttnArgs &p = paged_args();
+    if (wave == 0)
+      Sched(p, st).get();
     __syncthreads();
-    const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float base = mn == -INFINITY ? 0.f : mn;
-    ps[tid] = exp2f(s - base);
-    pg[tid] = page < 0 ? -1 : page * p.v_sp + slot * p.v_st + hk * p.v_sh;
+    const PagedUnit un = paged_unit(st.unit);
+    if (un.rows <= 0)
+      return;
+    const float ks = p.k_scale ? p.k_scale[un.hk] : 1.f;
+    float scale = p.qk_scale * ks;
+    const int r = lane & 31, rr = un.r0 + (r < un.rows ? r : 0);
+    const int64_t tok = un.t0 + (uint32_t)rr / (uint32_t)p.G;
+    const int head = un.hk * p.G + (uint32_t)rr % (uint32_t)p.G;
+    typename A::QF qf;
+    A::load_q(static_cast<const elt *>(p.q) + tok * p.q_st + head * p.q_sh, r < un.rows,
+              p.head_dim, scale, qf);
+    scale = scale == 0.f ? 1.f : fabsf(scale);
+    int lo, hi; // of the lane's row
+    paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
+    // keys that every row attends to
+    int lo_all, hi_all, skip;
+    paged_keys(p, un.pos0, un.len, un.r0, un.r0 + 1, skip, hi_all);
+    paged_keys(p, un.pos0, un.len, un.r0 + un.rows - 1, un.r0 + un.rows, lo_all, skip);
+
+    // this wave's blocks
+    int k0 = 0, k1 = 0;
+    if (un.hi > un.lo) {
+      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
+      const int w0 = first + 4 * (int)un.s0;
+      const int w1 = last - first < 4 * (int64_t)un.s1 ? last : first + 4 * (int)un.s1;
+      const int q = (w1 - w0 + 3) / 4;
+      k0 = w0 + wave * q < w1 ? w0 + wave * q : w1;
+      k1 = k0 + q < w1 ? k0 + q : w1;
+    }
+    float m = -INFINITY, l = 0.f;
+    typename A::f16v acc[D / 32], s[BN / 32];
+#pragma unroll
+    for (int bd = 0; bd < D / 32; ++bd)
+      acc[bd] = typename A::f16v{};
+    PageRow pr{p.table + un.b * p.table_s, p.table_width, p.pages, p.page_shift, 0, -1, 0};
+    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
+    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
+    uint64_t here = 0, next_here = 0;
+    if (k0 < k1) {
+      paged_vmcnt<0>(); // the loads below are counted
+      pr.hold(k0 * BN, true);
+      here = pr.template there<BN>(k0 * BN, un.hi);
+      issue_rows<A, U>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
+      issue_rows<A, U>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
+    }
+    for (int k = k0; k < k1; ++k) {
+      const int n0 = k * BN;
+      if (whole_loads)
+        paged_vmcnt<U>();
+      else
+        paged_vmcnt<0>();
+      {
+        typename A::KF kf;
+        A::read_k(bs, 0, kf);
+        paged_lgkmcnt0();
+        if (k + 1 < k1) {
+          pr.hold(n0 + BN, false);
+          next_here = pr.template there<BN>(n0 + BN, un.hi);
+          issue_rows<A, U>(pr, sk, n0 + BN, un.hi, 0, ko, k_lds, row_bytes);
+        }
+        A::qk(kf, qf, s);
+      }
+      typename A::h8 pf[BN / 16];
+      const uint64_t all = ~0ull >> (64 - BN);
+      if (here == all && n0 >= lo_all && n0 + BN <= hi_all) {
+        A::template softmax<false>(s, 0, scale, acc, m, l, pf);
+      } else {
+        const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
+        uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
+        seen &= a < 64 ? ~0ull << a : 0;
+        A::template softmax<true>(s, seen & here, scale, acc, m, l, pf);
+      }
+      if (whole_loads && k + 1 < k1)
+        paged_vmcnt<U>();
+      else
+        paged_vmcnt<0>();
+      constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
+#pragma unroll
+      for (int b0 = 0; b0 < D / 32; b0 += VG) {
+        typename A::template VF<VG> vf;
+        A::template read_v<VG>(bs, 0, b0, vf);
+        if (b0 + VG == D / 32) {
+          paged_lgkmcnt0();
+          if (k + 1 < k1)
+            issue_rows<A, U>(pr, sv, n0 + BN, un.hi, 0, vo, v_lds, row_bytes);
+        }
+        A::template pv<VG>(vf, b0, pf, acc);
+      }
+      here = next_here;
+    }
+
+    // The waves' sums: quads of 4 dims in lane order in each one's own tiles (all its loads
+    // have landed).
+    l = A::X::xsum(l);
+    const PagedAttnArgs &pe = paged_args();
+    const PagedUnit ue = paged_unit(st.unit);
+    const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
+    if (k0 < k1) {
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q)
+        *reinterpret_cast<f32x4v *>(smem[wave] + (q * 64 + lane) * 16) =
+            f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
+                   acc[q / 4][4 * (q % 4) + 2], acc[q / 4][4 * (q % 4) + 3]};
+    }
+    if (g == 0)
+      ms[wave][lane & 31] = m, ls[wave][lane & 31] = l;
     __syncthreads();
-    const float alpha = exp2f(m - base);
-    l *= alpha;
-    acc *= alpha;
-    m = mn;
-    const int n = hi - j0 < 256 ? (int)(hi - j0) : 256;
-    for (int i = 0; i < n; ++i) {
-      if (pg[i] < 0)
+    const int dq = pe.head_dim / 4, items = ue.rows * dq;
+    const int64_t part_bytes = 32 * (D + 2) * 4;
+    uint8_t *const unit_parts = pe.parts;
+    auto part_at = [&](uint32_t j) {
+      const uint64_t slot = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
+      return __builtin_amdgcn_make_buffer_rsrc(unit_parts + slot * part_bytes, 0, (int)part_bytes,
+                                               0x00020000);
+    };
+    auto finish = [&](int row, int qd, float mm, float ll, f32x4v x) {
+      const int ro = ue.r0 + row;
+      const int64_t t = ue.t0 + ro / pe.G;
+      const int h = ue.hk * pe.G + ro % pe.G;
+      const float f = ll == 0.f ? 0.f : vs / ll;
+      typename A::h4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = (elt)(x[e] * f);
+      *reinterpret_cast<typename A::h4 *>(static_cast<elt *>(pe.o) + t * pe.o_st + h * pe.o_sh +
+                                          4 * qd) = y;
+      if (qd == 0 && pe.lse)
+        pe.lse[t * pe.Hq + h] = ll == 0.f ? -INFINITY : mm + __builtin_log2f(ll);
+    };
+    constexpr int kSC1 = 16;
+    for (int it = tid; it < items; it += 256) {
+      const int row = it / dq, qd = it % dq;
+      float mm = -INFINITY, ll = 0.f;
+      f32x4v x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int wv = 0; wv < 4; ++wv)
+        paged_join(mm, ll, x, ms[wv][row], ls[wv][row],
+                   *reinterpret_cast<const f32x4v *>(
+                       smem[wv] + ((qd >> 1) * 64 + row + 32 * (qd & 1)) * 16));
+      if (ue.parts == 1) {
+        finish(row, qd, mm, ll, x);
+      } else {
+        const auto mine = part_at(ue.part);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4_t, x), mine,
+                                               (row * D + 4 * qd) * 4, 0, kSC1);
+        if (qd == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), mine, (32 * D + row) * 4, 0,
+                                                kSC1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(ll), mine,
+                                                (32 * D + 32 + row) * 4, 0, kSC1);
+        }
+      }
+    }
+    __syncthreads(); // the tiles' and ms' next use
+    if (ue.parts == 1 || !paged_arrive(&pe.counters[ue.w0], ue.parts, &flag))
+      continue;
+    // Last: all parts, in order.  Threads past one set of items take other parts.
+    const int groups = items < 256 ? 256 / items : 1;
+    for (int base = 0; base < items; base += 256) {
+      const int gi = items < 256 ? tid / items : 0, it = items < 256 ? tid % items : base + tid;
+      const bool on = gi < groups && it < items;
+      const int row = on ? it / dq : 0, qd = on ? it % dq : 0;
+      float mm = -INFINITY, ll = 0.f;
+      f32x4v x = {0.f, 0.f, 0.f, 0.f};
+      constexpr int NJ = 8; // parts in flight
+      for (uint32_t j0 = gi; j0 < ue.parts; j0 += NJ * groups) {
+        float pm[NJ], pl[NJ];
+        i32x4_t px[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const uint32_t jj = j0 + j * groups;
+          pm[j] = -INFINITY;
+          if (on && jj < ue.parts) {
+            const uint64_t slot = 2ull * (ue.w0 + jj) + (jj == 0 ? ue.slot0 : 0);
+            const auto all = __builtin_amdgcn_make_buffer_rsrc(unit_parts, 0, 0x7fffffff, 0x00020000);
+            const int at = (int)(slot * part_bytes);
+            px[j] = __builtin_bit_cast(
+                i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, at + (row * D + 4 * qd) * 4, 0, kSC1));
+            pm[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, at + (32 * D + row) * 4, 0, kSC1));
+            pl[j] = __int_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(all, at + (32 * D + 32 + row) * 4, 0, kSC1));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          paged_join(mm, ll, x, pm[j], pl[j], __builtin_bit_cast(f32x4v, px[j]));
+      }
+      if (groups > 1) {
+        f32x4v *const xs = reinterpret_cast<f32x4v *>(smem[0]);
+        float *const mls = reinterpret_cast<float *>(smem[0] + 4096);
+        xs[tid] = x;
+        mls[tid] = mm, mls[256 + tid] = ll;
+        __syncthreads();
+        if (tid < items) {
+          for (int k = 1; k < groups; ++k)
+            paged_join(mm, ll, x, mls[k * items + tid], mls[256 + k * items + tid],
+                       xs[k * items + tid]);
+          finish(row, qd, mm, ll, x);
+        }
+        __syncthreads();
+      } else if (on) {
+        finish(row, qd, mm, ll, x);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the waves of a workgroup share the keys
+// ---------------------------------------------------------------------------
+
+// 128 rows a unit, 32 a wave (chunks of a prompt).  Iteration j holds S_j, computes S_{j+1}
+// beside the softmax of S_j, then adds P_j V_j; K and V have two LDS slots each, loaded one
+// block ahead, and one barrier a block.
+template <class A>
+__global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kernel(PagedAttnArgs args) {
+  constexpr int D = A::D, BN = A::BN, U = A::TILE / 4096; // loads of a wave
+  typedef typename A::elt elt;
+  typedef PagedSched<128, BN, 1> Sched;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * A::TILE];
+  __shared__ PagedSchedState st;
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row_bytes = args.head_dim * A::ESZ;
+
+  paged_zero_rows<elt>(args);
+  if (wave == 0)
+    Sched(args, st).init(paged_place(), gridDim.x);
+
+  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * A::TILE;
+  typename A::Bases bs;
+  A::bases(k_lds, v_lds, bs);
+  uint32_t ko[U], vo[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    ko[u] = A::template offset<false>(U * wave + u, (uint32_t)args.k_st, args.k_run, row_bytes);
+    vo[u] = A::template offset<true>(U * wave + u, (uint32_t)args.v_st, args.v_run, row_bytes);
+  }
+
+  for (;;) {
+    const PagedAttnArgs &p = paged_args();
+    if (wave == 0)
+      Sched(p, st).get();
+    __syncthreads();
+    const PagedUnit un = paged_unit(st.unit);
+    if (un.rows <= 0)
+      return;
+    const float ks = p.k_scale ? p.k_scale[un.hk] : 1.f;
+    float scale = p.qk_scale * ks;
+    const int w_rows = un.rows - 32 * wave; // of this wave
+    const bool busy = w_rows > 0;
+    const int r = 32 * wave + (lane & 31), rr = un.r0 + (r < un.rows ? r : 0);
+    const int64_t tok = un.t0 + (uint32_t)rr / (uint32_t)p.G;
+    const int head = un.hk * p.G + (uint32_t)rr % (uint32_t)p.G;
+    typename A::QF qf;
+    A::load_q(static_cast<const elt *>(p.q) + tok * p.q_st + head * p.q_sh, r < un.rows,
+              p.head_dim, scale, qf);
+    scale = scale == 0.f ? 1.f : fabsf(scale);
+    int lo, hi;
+    paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
+    // of the wave's rows: keys that all attend to, and keys that any does
+    int lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;
+    if (busy) {
+      const int a = un.r0 + 32 * wave, z = un.r0 + (un.rows < 32 * wave + 32 ? un.rows : 32 * wave + 32);
+      paged_keys(p, un.pos0, un.len, a, a + 1, lo_any, hi_all);
+      paged_keys(p, un.pos0, un.len, z - 1, z, lo_all, hi_any);
+    }
+
+    int k0 = 0, k1 = 0;
+    if (un.hi > un.lo) {
+      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
+      k0 = first + (int)un.s0;
+      k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
+    }
+    float m = -INFINITY, l = 0.f;
+    typename A::f16v acc[D / 32], s[BN / 32];
+#pragma unroll
+    for (int bd = 0; bd < D / 32; ++bd)
+      acc[bd] = typename A::f16v{};
+    PageRow pr{p.table + un.b * p.table_s, p.table_width, p.pages, p.page_shift, 0, -1, 0};
+    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
+    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
+    uint64_t here[3] = {0, 0, 0}; // of blocks j, j + 1, j + 2
+
+    auto issue_k = [&](int k, int slot) {
+      issue_rows<A, U>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
+    };
+    auto issue_v = [&](int k, int slot) {
+      issue_rows<A, U>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
+    };
+    auto live = [&](int k) { return busy && k * BN < hi_any && k * BN + BN > lo_any; };
+    if (k0 < k1) {
+      paged_vmcnt<0>(); // the loads below are counted
+      pr.hold(k0 * BN, true);
+      here[0] = pr.template there<BN>(k0 * BN, un.hi);
+      issue_k(k0, 0);
+      issue_v(k0, 0);
+      if (k0 + 1 < k1) {
+        pr.hold((k0 + 1) * BN, false);
+        here[1] = pr.template there<BN>((k0 + 1) * BN, un.hi);
+        issue_k(k0 + 1, 1);
+      }
+      paged_vmcnt<0>();
+    }
+    __syncthreads();
+    if (k0 < k1 && live(k0)) {
+      typename A::KF kf;
+      A::read_k(bs, 0, kf);
+      A::qk(kf, qf, s);
+    }
+    __syncthreads(); // K slot 0 is loaded again
+    auto iter = [&](int k, auto slot_c) {
+      constexpr int SL = decltype(slot_c)::value;
+      if (k + 1 < k1)
+        issue_v(k + 1, 1 - SL);
+      if (k + 2 < k1) {
+        pr.hold((k + 2) * BN, false);
+        here[2] = pr.template there<BN>((k + 2) * BN, un.hi);
+        issue_k(k + 2, SL);
+      }
+      typename A::f16v sn[BN / 32];
+      if (k + 1 < k1 && live(k + 1)) {
+        typename A::KF kf;
+        A::read_k(bs, (1 - SL) * A::TILE, kf);
+        A::qk(kf, qf, sn);
+      }
+      if (live(k)) {
+        const int n0 = k * BN;
+        typename A::h8 pf[BN / 16];
+        const uint64_t all = ~0ull >> (64 - BN);
+        if (here[0] == all && n0 >= lo_all && n0 + BN <= hi_all) {
+          A::template softmax<false>(s, 0, scale, acc, m, l, pf);
+        } else {
+          const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
+          uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
+          seen &= a < 64 ? ~0ull << a : 0;
+          A::template softmax<true>(s, seen & here[0], scale, acc, m, l, pf);
+        }
+        constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
+#pragma unroll
+        for (int b0 = 0; b0 < D / 32; b0 += VG) {
+          typename A::template VF<VG> vf;
+          A::template read_v<VG>(bs, SL * A::TILE, b0, vf);
+          A::template pv<VG>(vf, b0, pf, acc);
+        }
+      }
+#pragma unroll
+      for (int b2 = 0; b2 < BN / 32; ++b2)
+        s[b2] = sn[b2];
+      here[0] = here[1], here[1] = here[2];
+      paged_vmcnt<0>();
+      __syncthreads();
+    };
+    int k = k0;
+    for (; k + 1 < k1; k += 2) {
+      iter(k, std::integral_constant<int, 0>());
+      iter(k + 1, std::integral_constant<int, 1>());
+    }
+    if (k < k1)
+      iter(k, std::integral_constant<int, 0>());
+
+    l = A::X::xsum(l);
+    const PagedAttnArgs &pe = paged_args();
+    const PagedUnit ue = paged_unit(st.unit);
+    __syncthreads(); // (the first wave writes the next one there)
+    const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
+    const int r_e = 32 * wave + (lane & 31), rr_e = ue.r0 + (r_e < ue.rows ? r_e : 0);
+    const bool busy_e = ue.rows > 32 * wave;
+    const int64_t tok_e = ue.t0 + (uint32_t)rr_e / (uint32_t)pe.G;
+    const int head_e = ue.hk * pe.G + (uint32_t)rr_e % (uint32_t)pe.G;
+    const int64_t part_bytes = 128 * (D + 2) * 4;
+    constexpr int kSC1 = 16;
+    if (ue.parts > 1) {
+      // (lane order: quads of a wave side by side)
+      const uint64_t slot = 2ull * (ue.w0 + ue.part) + (ue.part == 0 ? ue.slot0 : 0);
+      const auto mine = __builtin_amdgcn_make_buffer_rsrc(pe.parts + slot * part_bytes, 0,
+                                                          (int)part_bytes, 0x00020000);
+      if (busy_e) {
+#pragma unroll
+        for (int q = 0; q < D / 8; ++q)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(i32x4_t, f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
+                                                 acc[q / 4][4 * (q % 4) + 2],
+                                                 acc[q / 4][4 * (q % 4) + 3]}),
+              mine, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1);
+        if (g == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(m), mine, (128 * D + r_e) * 4, 0, kSC1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(l), mine, (128 * D + 128 + r_e) * 4, 0,
+                                                kSC1);
+        }
+      }
+      if (!paged_arrive(&pe.counters[ue.w0], ue.parts, &flag))
         continue;
-      l += ps[i];
-      if (tid < p.head_dim)
-        acc += ps[i] * cache_f32<T, C>(p.vc + pg[i] * sizeof(C), tid);
+      if (busy_e) {
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int bd = 0; bd < D / 32; ++bd)
+          acc[bd] = typename A::f16v{};
+        for (uint32_t j = 0; j < ue.parts; ++j) {
+          const uint64_t from = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
+          const auto part = __builtin_amdgcn_make_buffer_rsrc(pe.parts + from * part_bytes, 0,
+                                                              (int)part_bytes, 0x00020000);
+          i32x4_t x[D / 8];
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+            x[q] = __builtin_bit_cast(
+                i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                             part, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1));
+          const float m1 = __int_as_float(
+              __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + r_e) * 4, 0, kSC1));
+          const float l1 = __int_as_float(
+              __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + 128 + r_e) * 4, 0, kSC1));
+          if (m1 == -INFINITY)
+            continue;
+          const float to = fmaxf(m, m1);
+          const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+          const float a1 = __builtin_amdgcn_exp2f(m1 - to);
+          l = l * a + l1 * a1;
+          m = to;
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[q / 4][4 * (q % 4) + e] =
+                  acc[q / 4][4 * (q % 4) + e] * a + __int_as_float(x[q][e]) * a1;
+        }
+      }
+    }
+    if (r_e < ue.rows) {
+      const float f = l == 0.f ? 0.f : vs / l;
+      elt *const orow = static_cast<elt *>(pe.o) + tok_e * pe.o_st + head_e * pe.o_sh;
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const int d = 32 * (q / 4) + 8 * (q % 4) + 4 * g;
+        typename A::h4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = (elt)(acc[q / 4][4 * (q % 4) + e] * f);
+        if (d < pe.head_dim)
+          *reinterpret_cast<typename A::h4 *>(orow + d) = y;
+      }
+      if (g == 0 && pe.lse)
+        pe.lse[tok_e * pe.Hq + head_e] = l == 0.f ? -INFINITY : m + __builtin_log2f(l);
     }
   }
-  if (tid < p.head_dim)
-    static_cast<T *>(p.o)[t * p.o_st + h * p.o_sh + tid] =
-        (T)(l > 0.f ? acc / l * (p.v_scale ? p.v_scale[hk] : 1.f) : 0.f);
-  if (tid == 0 && p.lse)
-    p.lse[t * p.Hq + h] = l > 0.f ? m + log2f(l) : -INFINITY;
 }
 
 } // namespace txk
