@@ -240,45 +240,35 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
       }
   }
 
-  // One block's softmax: s are its scores (times qk_scale > 0 they are base-2 exponents); MASK:
-  // bit n of `seen` says that the lane's row attends to key n of the block.  Updates the row's
-  // reference m (both lanes of a row hold the same), the lane's part of the sum l, and acc; p as
-  // MFMA operands.  m follows the maximum only when that has grown by more than 8, so p is
-  // up to 2^8 (in range in both types, and rounded by the same relative half step), and
-  // acc is seldom rescaled.
-  template <bool MASK>
-  __device__ __forceinline__ static void softmax(f16v (&s)[BN / 32], uint64_t seen, float qk_scale,
+  // Scores of keys that the lane's row does not attend to (bit n of `seen`: it does to key n of
+  // the block).
+  __device__ __forceinline__ static void mask(f16v (&s)[BN / 32], uint64_t seen) {
+    const uint64_t mine = seen >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+    for (int b = 0; b < BN / 32; ++b) {
+      const uint32_t w = (uint32_t)(mine >> (32 * b));
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[b][r] = (w >> (8 * (r / 4) + r % 4)) & 1 ? s[b][r] : -INFINITY;
+    }
+  }
+
+  // One block's softmax: s are its scores (times qk_scale > 0 they are base-2 exponents).
+  // Updates the row's maximum m (both lanes of a row hold the same), the lane's part of the sum
+  // l, and acc; p as MFMA operands.
+  __device__ __forceinline__ static void softmax(f16v (&s)[BN / 32], float qk_scale,
                                                  f16v (&acc)[D / 32], float &m, float &l,
                                                  h8 (&pf)[BN / 16]) {
-    if constexpr (MASK) {
-      const uint64_t mine = seen >> (4 * ((threadIdx.x & 63) >> 5));
-#pragma unroll
-      for (int b = 0; b < BN / 32; ++b) {
-        const uint32_t w = (uint32_t)(mine >> (32 * b));
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[b][r] = (w >> (8 * (r / 4) + r % 4)) & 1 ? s[b][r] : -INFINITY;
-      }
-    }
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < BN / 32; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         mx = fmaxf(mx, s[b][r]);
-    mx = X::xmax(mx) * qk_scale;
-    if (__any(mx > m + 8.f)) {
-      const float to = mx > m + 8.f ? mx : m;
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
-      l *= alpha;
-#pragma unroll
-      for (int bd = 0; bd < D / 32; ++bd)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          acc[bd][r] *= alpha;
-      m = to;
-    }
-    const float base = m == -INFINITY ? 0.f : m;
+    const float to = fmaxf(m, X::xmax(mx) * qk_scale);
+    const float base = to == -INFINITY ? 0.f : to;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);
+    m = to;
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < BN / 32; ++b)
@@ -287,12 +277,17 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
         s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], qk_scale, -base));
         sum += s[b][r];
       }
-    l += sum;
+    l = l * alpha + sum;
 #pragma unroll
     for (int c = 0; c < BN / 16; ++c)
 #pragma unroll
       for (int t = 0; t < 8; ++t)
         pf[c][t] = (elt)s[c / 2][8 * (c % 2) + t];
+#pragma unroll
+    for (int bd = 0; bd < D / 32; ++bd)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[bd][r] *= alpha;
   }
 };
 
@@ -303,8 +298,7 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
 // One wave's view of a table row: lane i holds entry `first` + i (-1: no page).
 struct PageRow {
   const int32_t *row;
-  int64_t width;
-  uint32_t pages;
+  uint32_t width, pages;
   int shift, first, ids;
   uint64_t holes; // lanes without a page
 
@@ -314,11 +308,9 @@ struct PageRow {
     if (!anew && e0 >= first && e1 < first + 64)
       return;
     first = e0;
-    const int64_t e = (int64_t)e0 + (threadIdx.x & 63);
-    ids = -1;
-    if (e < width)
-      ids = row[e];
-    if ((uint32_t)ids >= pages)
+    const uint32_t e = e0 + (threadIdx.x & 63);
+    ids = row[e < width ? e : 0];
+    if (e >= width || (uint32_t)ids >= pages)
       ids = -1;
     holes = __ballot(ids < 0);
   }
@@ -641,7 +633,7 @@ template <class T> __device__ __forceinline__ void paged_zero_rows(const PagedAt
 // A workgroup's place in the order of work: the 8 XCDs take contiguous runs.
 __device__ __forceinline__ uint32_t paged_place() {
   const uint32_t n = gridDim.x, b = blockIdx.x;
-  return n % 8 == 0 ? (b % 8) * (n / 8) + b / 8 : b;
+  return b;
 }
 
 // One part's arrival: true in the last workgroup of the unit.  Data moves between
@@ -756,7 +748,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
 #pragma unroll
     for (int bd = 0; bd < D / 32; ++bd)
       acc[bd] = typename A::f16v{};
-    PageRow pr{p.table + un.b * p.table_s, p.table_width, p.pages, p.page_shift, 0, -1, 0};
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift, 0, -1, 0};
     const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
     uint64_t here = 0, next_here = 0;
@@ -786,14 +778,13 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
       }
       typename A::h8 pf[BN / 16];
       const uint64_t all = ~0ull >> (64 - BN);
-      if (here == all && n0 >= lo_all && n0 + BN <= hi_all) {
-        A::template softmax<false>(s, 0, scale, acc, m, l, pf);
-      } else {
+      if (here != all || n0 < lo_all || n0 + BN > hi_all) {
         const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
         uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
         seen &= a < 64 ? ~0ull << a : 0;
-        A::template softmax<true>(s, seen & here, scale, acc, m, l, pf);
+        A::mask(s, seen & here);
       }
+      A::softmax(s, scale, acc, m, l, pf);
       if (whole_loads && k + 1 < k1)
         paged_vmcnt<U>();
       else
@@ -1002,7 +993,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
 #pragma unroll
     for (int bd = 0; bd < D / 32; ++bd)
       acc[bd] = typename A::f16v{};
-    PageRow pr{p.table + un.b * p.table_s, p.table_width, p.pages, p.page_shift, 0, -1, 0};
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift, 0, -1, 0};
     const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
     uint64_t here[3] = {0, 0, 0}; // of blocks j, j + 1, j + 2
@@ -1053,14 +1044,13 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
         const int n0 = k * BN;
         typename A::h8 pf[BN / 16];
         const uint64_t all = ~0ull >> (64 - BN);
-        if (here[0] == all && n0 >= lo_all && n0 + BN <= hi_all) {
-          A::template softmax<false>(s, 0, scale, acc, m, l, pf);
-        } else {
+        if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
           const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
           uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
           seen &= a < 64 ? ~0ull << a : 0;
-          A::template softmax<true>(s, seen & here[0], scale, acc, m, l, pf);
+          A::mask(s, seen & here[0]);
         }
+        A::softmax(s, scale, acc, m, l, pf);
         constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
 #pragma unroll
         for (int b0 = 0; b0 < D / 32; b0 += VG) {
