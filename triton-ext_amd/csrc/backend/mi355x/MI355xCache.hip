@@ -504,6 +504,11 @@ extern "C" TX_API int tx_paged_attn_launch(const tx_paged_attn_plan *plan, const
   a.k_sp = d.k_sp * ce, a.k_st = d.k_st * ce, a.k_sh = d.k_sh * ce;
   a.v_sp = d.v_sp * ce, a.v_st = d.v_st * ce, a.v_sh = d.v_sh * ce;
   a.pages = (uint32_t)d.pages, a.min_share = 1;
+  a.g_mul = a.g_shift = 0;
+  if (const int64_t G = d.Hq / d.Hkv; G > 1) { // ceil(2^(31 + s) / G), 2^s >= G
+    const int sh = log2of(G);
+    a.g_mul = (uint32_t)((((uint64_t)1 << (31 + sh)) + G - 1) / G), a.g_shift = sh - 1;
+  }
   a.T = (int32_t)d.T, a.B = (int32_t)d.B, a.G = d.Hq / d.Hkv, a.Hq = d.Hq, a.Hkv = d.Hkv;
   a.head_dim = d.head_dim, a.page_shift = log2of(d.page_size);
   a.causal = d.causal, a.window = d.window;

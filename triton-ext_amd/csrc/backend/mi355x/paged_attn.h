@@ -44,6 +44,7 @@ struct PagedAttnArgs {
   int64_t q_st, q_sh, o_st, o_sh;
   int64_t k_sp, k_st, k_sh, v_sp, v_st, v_sh; // bytes
   uint32_t pages, min_share;
+  uint32_t g_mul, g_shift; // n / G = mulhi(n, g_mul) >> g_shift for n < 2^31 (G 1: g_mul 0)
   int32_t most; // keys that a table row has place for
   int32_t T, B, G, Hq, Hkv, head_dim, page_shift, causal, window;
   int32_t k_run, v_run; // rows of one resource
@@ -158,14 +159,22 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   struct QF {
     h8 v[D / 16];
   };
-  __device__ __forceinline__ static void load_q(const void *row, bool live, int head_dim,
-                                                float scale, QF &qf) {
+  __device__ __forceinline__ static int q_dim(int c) {
     const int g = (threadIdx.x & 63) >> 5;
+    return F8 ? 32 * (c / 2) + 16 * g + 8 * (c % 2) : 16 * c + 8 * g;
+  }
+  __device__ __forceinline__ static void load_q(const void *row, int head_dim, QF &qf) {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      const int d = F8 ? 32 * (c / 2) + 16 * g + 8 * (c % 2) : 16 * c + 8 * g;
-      const bool in = live && d < head_dim && scale != 0.f;
-      i32x4_t x = *reinterpret_cast<const i32x4_t *>(static_cast<const elt *>(row) + (in ? d : 0));
+      const int d = q_dim(c);
+      qf.v[c] = *reinterpret_cast<const h8 *>(static_cast<const elt *>(row) + (d < head_dim ? d : 0));
+    }
+  }
+  __device__ __forceinline__ static void settle_q(bool live, int head_dim, float scale, QF &qf) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const bool in = live && q_dim(c) < head_dim && scale != 0.f;
+      i32x4_t x = __builtin_bit_cast(i32x4_t, qf.v[c]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         x[i] = in ? x[i] ^ (scale < 0.f ? (int)0x80008000 : 0) : 0;
@@ -299,20 +308,26 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
 struct PageRow {
   const int32_t *row;
   uint32_t width, pages;
-  int shift, first, ids;
-  uint64_t holes; // lanes without a page
+  int shift, first = 0, ids = -1;
+  uint64_t holes = 0; // lanes without a page
 
-  // Holds the entries of keys [n, n + 64).
-  __device__ __forceinline__ void hold(int n, bool anew) {
-    const int e0 = n >> shift, e1 = (n + 63) >> shift;
-    if (!anew && e0 >= first && e1 < first + 64)
-      return;
-    first = e0;
-    const uint32_t e = e0 + (threadIdx.x & 63);
+  // Holds the entries of keys [n, n + 64); first their load (any entry past the row's end),
+  // then their use.
+  __device__ __forceinline__ void load(int n) {
+    first = n >> shift;
+    const uint32_t e = first + (threadIdx.x & 63);
     ids = row[e < width ? e : 0];
-    if (e >= width || (uint32_t)ids >= pages)
+  }
+  __device__ __forceinline__ void settle() {
+    if (first + (threadIdx.x & 63) >= width || (uint32_t)ids >= pages)
       ids = -1;
     holes = __ballot(ids < 0);
+  }
+  __device__ __forceinline__ void hold(int n) {
+    if (((n + 63) >> shift) >= first + 64) {
+      load(n);
+      settle();
+    }
   }
   // Which of the BN keys from n on, before `end`, have a page.
   template <int BN> __device__ __forceinline__ uint64_t there(int n, int end) const {
@@ -395,12 +410,17 @@ struct PagedUnit {
   uint32_t s0, s1, parts, part, w0, slot0;
 };
 
+// The token of a row.
+__device__ __forceinline__ int paged_token(const PagedAttnArgs &p, int row) {
+  return p.g_mul ? __umulhi((uint32_t)row, p.g_mul) >> p.g_shift : row;
+}
+
 // The keys [lo, hi) of rows [r0, r1) of a sequence of `len` keys whose first new token has
 // position `at`.
 __device__ __forceinline__ void paged_keys(const PagedAttnArgs &p, int64_t at, int len, int r0, int r1,
                                            int &lo, int &hi) {
-  const int64_t last = at + (uint32_t)(r1 - 1) / (uint32_t)p.G + 1;
-  const int64_t first = at + (uint32_t)r0 / (uint32_t)p.G - p.window + 1;
+  const int64_t last = at + paged_token(p, r1 - 1) + 1;
+  const int64_t first = at + paged_token(p, r0) - p.window + 1;
   hi = len;
   if (p.causal && last < hi)
     hi = last < 0 ? 0 : (int)last;
@@ -408,8 +428,8 @@ __device__ __forceinline__ void paged_keys(const PagedAttnArgs &p, int64_t at, i
 }
 
 // Deals out the units.  Blocks of BN keys in steps of WPS blocks (those that the waves of a
-// workgroup take side by side); a unit has one step at least, so that its rows are written.  The first
-// wave goes through this, a lane per sequence (64 at a time, in LDS) or block of rows; sums
+// workgroup take side by side); a unit has one step at least, so that its rows are written, and
+// begins with OV more that stand for what its beginning and end cost.  The first wave goes through this, a lane per sequence (64 at a time, in LDS) or block of rows; sums
 // across lanes.
 struct PagedSchedState {
   int64_t pos0[64];
@@ -417,7 +437,7 @@ struct PagedSchedState {
   uint32_t cost[64];
   int cb, b, rb, hk;
   uint32_t S, share, pos, end, s0, w; // S: steps of a kv head
-  PagedUnit unit; // rows 0: the end
+  PagedUnit unit[2]; // the current one and the next; rows 0: the end
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -425,19 +445,21 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return (int64_t)(uint32_t)uniform((int)v) | (int64_t)uniform((int)(v >> 32)) << 32;
 }
 
-template <int BM, int BN, int WPS> struct PagedSched {
+template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
   const PagedAttnArgs &p;
   PagedSchedState &st;
   const int lane = threadIdx.x & 63;
 
   __device__ __forceinline__ PagedSched(const PagedAttnArgs &a, PagedSchedState &s) : p(a), st(s) {}
 
-  __device__ __forceinline__ uint32_t upto(uint32_t v) const { // inclusive sum over lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(v, d);
-      v += lane >= d ? o : 0;
-    }
+  // Inclusive sum over lanes, by DPP: rows of 16 lanes, then the rows.
+  __device__ __forceinline__ static uint32_t upto(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false); // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false); // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
     return v;
   }
   __device__ __forceinline__ static uint32_t steps_of(int lo, int hi) {
@@ -451,7 +473,7 @@ template <int BM, int BN, int WPS> struct PagedSched {
       return 0;
     int lo, hi;
     paged_keys(p, at, len, k * BM, nr - k * BM < BM ? nr : k * BM + BM, lo, hi);
-    return steps_of(lo, hi);
+    return OV + steps_of(lo, hi);
   }
   // The 64 sequences from `first` on; returns this lane's steps.
   __device__ __forceinline__ uint32_t load_chunk(int first) {
@@ -545,50 +567,53 @@ template <int BM, int BN, int WPS> struct PagedSched {
     st.rb = rb, st.s0 = rem;
   }
 
-  // The next unit of the run, into st.unit.
-  __device__ __forceinline__ void get() {
-    const uint32_t pos = uniform(st.pos), end = uniform(st.end), s0 = uniform(st.s0);
+  // The next unit of the run, into `to`.
+  __device__ __forceinline__ void get(PagedUnit &to) {
+    const uint32_t end = uniform(st.end), share = uniform(st.share);
+    uint32_t pos = uniform(st.pos), s0 = uniform(st.s0);
+    int cb = uniform(st.cb), b = uniform(st.b), hk = uniform(st.hk), rb = uniform(st.rb);
     PagedUnit u;
     u.rows = 0;
-    if (pos < end) {
-      u.b = uniform(st.b), u.hk = uniform(st.hk);
-      const int i = u.b - uniform(st.cb), nr = uniform(st.n[i]) * p.G;
-      int rb = uniform(st.rb);
+    while (pos < end && u.rows == 0) {
+      const int i = b - cb, nr = uniform(st.n[i]) * p.G;
+      u.b = b, u.hk = hk;
       u.t0 = st.t0[i], u.len = uniform(st.len[i]), u.pos0 = uniform64(st.pos0[i]);
       u.r0 = rb * BM;
-      u.rows = nr - u.r0 < BM ? nr - u.r0 : BM;
-      paged_keys(p, u.pos0, u.len, u.r0, u.r0 + u.rows, u.lo, u.hi);
-      const uint32_t steps = steps_of(u.lo, u.hi);
-      u.s0 = s0, u.s1 = steps - s0 < end - pos ? steps : s0 + (end - pos);
-      u.parts = 1, u.part = 0, u.w0 = 0, u.slot0 = 0;
-      if (u.s1 - u.s0 < steps) {
-        const uint32_t share = uniform(st.share), first = pos - s0;
-        u.w0 = first / share;
-        u.parts = (first + steps - 1) / share - u.w0 + 1;
-        u.part = uniform(st.w) - u.w0;
-        u.slot0 = first == u.w0 * share ? 0 : 1;
-      }
-      st.pos = pos + u.s1 - u.s0, st.s0 = 0;
-      if (pos + u.s1 - u.s0 < end) { // there is another
-        if ((rb + 1) * (int64_t)BM < nr) {
-          st.rb = rb + 1;
-        } else {
-          st.rb = 0;
-          uint64_t later = __ballot(st.cost[lane] > 0) & (i == 63 ? 0 : ~0ull << (i + 1));
-          int c = uniform(st.cb), hk = u.hk;
-          while (!later && hk < p.Hkv) {
-            c += 64;
-            if (c >= p.B)
-              c = 0, ++hk;
-            later = __ballot((p.B > 64 ? load_chunk(c) : st.cost[lane]) > 0);
-          }
-          if (!later || hk >= p.Hkv)
-            st.end = 0;
-          st.b = c + (later ? __builtin_ctzll(later) : 0), st.hk = hk;
+      const int rows = nr - u.r0 < BM ? nr - u.r0 : BM;
+      paged_keys(p, u.pos0, u.len, u.r0, u.r0 + rows, u.lo, u.hi);
+      const uint32_t cost = OV + steps_of(u.lo, u.hi);
+      const uint32_t s1 = cost - s0 < end - pos ? cost : s0 + (end - pos);
+      if (s1 > OV) {
+        u.rows = rows;
+        u.s0 = (s0 > OV ? s0 : OV) - OV, u.s1 = s1 - OV;
+        u.parts = 1, u.part = 0, u.w0 = 0, u.slot0 = 0;
+        if (u.s1 - u.s0 < cost - OV) {
+          const uint32_t first = pos - s0;
+          u.w0 = (first + OV) / share;
+          u.parts = (first + cost - 1) / share - u.w0 + 1;
+          u.part = uniform(st.w) - u.w0;
+          u.slot0 = first < u.w0 * share ? 0 : 1;
         }
       }
+      pos += s1 - s0, s0 = 0;
+      if (pos >= end)
+        break;
+      if ((++rb) * (int64_t)BM >= nr) {
+        rb = 0;
+        uint64_t later = __ballot(st.cost[lane] > 0) & (i == 63 ? 0 : ~0ull << (i + 1));
+        while (!later && hk < p.Hkv) {
+          cb += 64;
+          if (cb >= p.B)
+            cb = 0, ++hk;
+          later = __ballot((p.B > 64 ? load_chunk(cb) : st.cost[lane]) > 0);
+        }
+        if (!later || hk >= p.Hkv)
+          pos = end;
+        b = cb + (later ? __builtin_ctzll(later) : 0);
+      }
     }
-    st.unit = u;
+    st.pos = pos, st.s0 = 0, st.b = b, st.hk = hk, st.rb = rb;
+    to = u;
   }
 };
 
@@ -684,7 +709,7 @@ template <class A>
 __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
   constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024;
   typedef typename A::elt elt;
-  typedef PagedSched<32, BN, 4> Sched;
+  typedef PagedSched<32, BN, 4, 2> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * A::TILE];
   __shared__ float ms[4][32], ls[4][32];
   __shared__ PagedSchedState st;
@@ -694,9 +719,12 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row_bytes = args.head_dim * A::ESZ;
 
-  paged_zero_rows<elt>(args);
-  if (wave == 0)
-    Sched(args, st).init(paged_place(), gridDim.x);
+  if (wave == 0) {
+    Sched sched(args, st);
+    sched.init(paged_place(), gridDim.x);
+    sched.get(st.unit[0]);
+  }
+  __syncthreads();
 
   const uint32_t k_lds = lds_addr(smem[wave]), v_lds = k_lds + A::TILE;
   typename A::Bases bs;
@@ -709,30 +737,12 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
   }
   const bool whole_loads = args.k_run >= A::R && args.v_run >= A::R;
 
-  for (;;) {
+  for (int turn = 0;; turn ^= 1) {
     const PagedAttnArgs &p = paged_args();
-    if (wave == 0)
-      Sched(p, st).get();
-    __syncthreads();
-    const PagedUnit un = paged_unit(st.unit);
+    const PagedUnit un = paged_unit(st.unit[turn]);
     if (un.rows <= 0)
-      return;
-    const float ks = p.k_scale ? p.k_scale[un.hk] : 1.f;
-    float scale = p.qk_scale * ks;
-    const int r = lane & 31, rr = un.r0 + (r < un.rows ? r : 0);
-    const int64_t tok = un.t0 + (uint32_t)rr / (uint32_t)p.G;
-    const int head = un.hk * p.G + (uint32_t)rr % (uint32_t)p.G;
-    typename A::QF qf;
-    A::load_q(static_cast<const elt *>(p.q) + tok * p.q_st + head * p.q_sh, r < un.rows,
-              p.head_dim, scale, qf);
-    scale = scale == 0.f ? 1.f : fabsf(scale);
-    int lo, hi; // of the lane's row
-    paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
-    // keys that every row attends to
-    int lo_all, hi_all, skip;
-    paged_keys(p, un.pos0, un.len, un.r0, un.r0 + 1, skip, hi_all);
-    paged_keys(p, un.pos0, un.len, un.r0 + un.rows - 1, un.r0 + un.rows, lo_all, skip);
-
+      break;
+    paged_vmcnt<0>(); // the loads below are counted
     // this wave's blocks
     int k0 = 0, k1 = 0;
     if (un.hi > un.lo) {
@@ -743,22 +753,41 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
       k0 = w0 + wave * q < w1 ? w0 + wave * q : w1;
       k1 = k0 + q < w1 ? k0 + q : w1;
     }
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
+    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
+    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
+    // The table, Q and the first blocks are under way together, and meanwhile the first wave
+    // looks up the next unit.
+    if (k0 < k1)
+      pr.load(k0 * BN);
+    const int r = lane & 31, rr = un.r0 + (r < un.rows ? r : 0);
+    const int of = paged_token(p, rr), head = un.hk * p.G + rr - of * p.G;
+    typename A::QF qf;
+    A::load_q(static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh,
+              p.head_dim, qf);
+    uint64_t here = 0, next_here = 0;
+    if (k0 < k1) {
+      pr.settle();
+      here = pr.template there<BN>(k0 * BN, un.hi);
+      issue_rows<A, U>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
+      issue_rows<A, U>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
+    }
+    if (wave == 0)
+      Sched(p, st).get(st.unit[turn ^ 1]);
+    int lo, hi; // of the lane's row
+    paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
+    // keys that every row attends to
+    int lo_all, hi_all, skip;
+    paged_keys(p, un.pos0, un.len, un.r0, un.r0 + 1, skip, hi_all);
+    paged_keys(p, un.pos0, un.len, un.r0 + un.rows - 1, un.r0 + un.rows, lo_all, skip);
+    float scale = p.qk_scale * (p.k_scale ? p.k_scale[un.hk] : 1.f);
+    A::settle_q(r < un.rows, p.head_dim, scale, qf);
+    scale = scale == 0.f ? 1.f : fabsf(scale);
     float m = -INFINITY, l = 0.f;
     typename A::f16v acc[D / 32], s[BN / 32];
 #pragma unroll
     for (int bd = 0; bd < D / 32; ++bd)
       acc[bd] = typename A::f16v{};
-    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift, 0, -1, 0};
-    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
-    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
-    uint64_t here = 0, next_here = 0;
-    if (k0 < k1) {
-      paged_vmcnt<0>(); // the loads below are counted
-      pr.hold(k0 * BN, true);
-      here = pr.template there<BN>(k0 * BN, un.hi);
-      issue_rows<A, U>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
-      issue_rows<A, U>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
-    }
     for (int k = k0; k < k1; ++k) {
       const int n0 = k * BN;
       if (whole_loads)
@@ -770,7 +799,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
         A::read_k(bs, 0, kf);
         paged_lgkmcnt0();
         if (k + 1 < k1) {
-          pr.hold(n0 + BN, false);
+          pr.hold(n0 + BN);
           next_here = pr.template there<BN>(n0 + BN, un.hi);
           issue_rows<A, U>(pr, sk, n0 + BN, un.hi, 0, ko, k_lds, row_bytes);
         }
@@ -808,7 +837,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
     // have landed).
     l = A::X::xsum(l);
     const PagedAttnArgs &pe = paged_args();
-    const PagedUnit ue = paged_unit(st.unit);
+    const PagedUnit ue = paged_unit(st.unit[turn]);
     const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
     if (k0 < k1) {
 #pragma unroll
@@ -830,8 +859,8 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
     };
     auto finish = [&](int row, int qd, float mm, float ll, f32x4v x) {
       const int ro = ue.r0 + row;
-      const int64_t t = ue.t0 + ro / pe.G;
-      const int h = ue.hk * pe.G + ro % pe.G;
+      const int of = paged_token(pe, ro), h = ue.hk * pe.G + ro - of * pe.G;
+      const int64_t t = ue.t0 + of;
       const float f = ll == 0.f ? 0.f : vs / ll;
       typename A::h4 y;
 #pragma unroll
@@ -918,6 +947,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
       }
     }
   }
+  paged_zero_rows<elt>(args);
 }
 
 // ---------------------------------------------------------------------------
@@ -931,7 +961,7 @@ template <class A>
 __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kernel(PagedAttnArgs args) {
   constexpr int D = A::D, BN = A::BN, U = A::TILE / 4096; // loads of a wave
   typedef typename A::elt elt;
-  typedef PagedSched<128, BN, 1> Sched;
+  typedef PagedSched<128, BN, 1, 4> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * A::TILE];
   __shared__ PagedSchedState st;
   __shared__ int flag;
@@ -939,9 +969,12 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row_bytes = args.head_dim * A::ESZ;
 
-  paged_zero_rows<elt>(args);
-  if (wave == 0)
-    Sched(args, st).init(paged_place(), gridDim.x);
+  if (wave == 0) {
+    Sched sched(args, st);
+    sched.init(paged_place(), gridDim.x);
+    sched.get(st.unit[0]);
+  }
+  __syncthreads();
 
   const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * A::TILE;
   typename A::Bases bs;
@@ -953,26 +986,52 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     vo[u] = A::template offset<true>(U * wave + u, (uint32_t)args.v_st, args.v_run, row_bytes);
   }
 
-  for (;;) {
+  for (int turn = 0;; turn ^= 1) {
     const PagedAttnArgs &p = paged_args();
-    if (wave == 0)
-      Sched(p, st).get();
-    __syncthreads();
-    const PagedUnit un = paged_unit(st.unit);
+    const PagedUnit un = paged_unit(st.unit[turn]);
     if (un.rows <= 0)
-      return;
-    const float ks = p.k_scale ? p.k_scale[un.hk] : 1.f;
-    float scale = p.qk_scale * ks;
-    const int w_rows = un.rows - 32 * wave; // of this wave
-    const bool busy = w_rows > 0;
+      break;
+    paged_vmcnt<0>(); // the loads below are counted
+    int k0 = 0, k1 = 0;
+    if (un.hi > un.lo) {
+      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
+      k0 = first + (int)un.s0;
+      k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
+    }
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
+    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
+    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
+    uint64_t here[3] = {0, 0, 0}; // of blocks j, j + 1, j + 2
+    auto issue_k = [&](int k, int slot) {
+      issue_rows<A, U>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
+    };
+    auto issue_v = [&](int k, int slot) {
+      issue_rows<A, U>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
+    };
+    // The table, Q and the first blocks are under way together, and meanwhile the first wave
+    // looks up the next unit.
+    if (k0 < k1)
+      pr.load(k0 * BN);
+    const bool busy = un.rows > 32 * wave;
     const int r = 32 * wave + (lane & 31), rr = un.r0 + (r < un.rows ? r : 0);
-    const int64_t tok = un.t0 + (uint32_t)rr / (uint32_t)p.G;
-    const int head = un.hk * p.G + (uint32_t)rr % (uint32_t)p.G;
+    const int of = paged_token(p, rr), head = un.hk * p.G + rr - of * p.G;
     typename A::QF qf;
-    A::load_q(static_cast<const elt *>(p.q) + tok * p.q_st + head * p.q_sh, r < un.rows,
-              p.head_dim, scale, qf);
-    scale = scale == 0.f ? 1.f : fabsf(scale);
-    int lo, hi;
+    A::load_q(static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh,
+              p.head_dim, qf);
+    if (k0 < k1) {
+      pr.settle();
+      here[0] = pr.template there<BN>(k0 * BN, un.hi);
+      issue_k(k0, 0);
+      issue_v(k0, 0);
+      if (k0 + 1 < k1) {
+        pr.hold((k0 + 1) * BN);
+        here[1] = pr.template there<BN>((k0 + 1) * BN, un.hi);
+        issue_k(k0 + 1, 1);
+      }
+    }
+    if (wave == 0)
+      Sched(p, st).get(st.unit[turn ^ 1]);
+    int lo, hi; // of the lane's row
     paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
     // of the wave's rows: keys that all attend to, and keys that any does
     int lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;
@@ -981,43 +1040,16 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
       paged_keys(p, un.pos0, un.len, a, a + 1, lo_any, hi_all);
       paged_keys(p, un.pos0, un.len, z - 1, z, lo_all, hi_any);
     }
-
-    int k0 = 0, k1 = 0;
-    if (un.hi > un.lo) {
-      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
-      k0 = first + (int)un.s0;
-      k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
-    }
+    auto live = [&](int k) { return busy && k * BN < hi_any && k * BN + BN > lo_any; };
+    float scale = p.qk_scale * (p.k_scale ? p.k_scale[un.hk] : 1.f);
+    A::settle_q(r < un.rows, p.head_dim, scale, qf);
+    scale = scale == 0.f ? 1.f : fabsf(scale);
     float m = -INFINITY, l = 0.f;
     typename A::f16v acc[D / 32], s[BN / 32];
 #pragma unroll
     for (int bd = 0; bd < D / 32; ++bd)
       acc[bd] = typename A::f16v{};
-    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift, 0, -1, 0};
-    const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
-    const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
-    uint64_t here[3] = {0, 0, 0}; // of blocks j, j + 1, j + 2
-
-    auto issue_k = [&](int k, int slot) {
-      issue_rows<A, U>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
-    };
-    auto issue_v = [&](int k, int slot) {
-      issue_rows<A, U>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
-    };
-    auto live = [&](int k) { return busy && k * BN < hi_any && k * BN + BN > lo_any; };
-    if (k0 < k1) {
-      paged_vmcnt<0>(); // the loads below are counted
-      pr.hold(k0 * BN, true);
-      here[0] = pr.template there<BN>(k0 * BN, un.hi);
-      issue_k(k0, 0);
-      issue_v(k0, 0);
-      if (k0 + 1 < k1) {
-        pr.hold((k0 + 1) * BN, false);
-        here[1] = pr.template there<BN>((k0 + 1) * BN, un.hi);
-        issue_k(k0 + 1, 1);
-      }
-      paged_vmcnt<0>();
-    }
+    paged_vmcnt<0>();
     __syncthreads();
     if (k0 < k1 && live(k0)) {
       typename A::KF kf;
@@ -1030,7 +1062,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
       if (k + 1 < k1)
         issue_v(k + 1, 1 - SL);
       if (k + 2 < k1) {
-        pr.hold((k + 2) * BN, false);
+        pr.hold((k + 2) * BN);
         here[2] = pr.template there<BN>((k + 2) * BN, un.hi);
         issue_k(k + 2, SL);
       }
@@ -1076,13 +1108,13 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
 
     l = A::X::xsum(l);
     const PagedAttnArgs &pe = paged_args();
-    const PagedUnit ue = paged_unit(st.unit);
-    __syncthreads(); // (the first wave writes the next one there)
+    const PagedUnit ue = paged_unit(st.unit[turn]);
+    __syncthreads(); // (the first wave will write the unit after the next there)
     const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
     const int r_e = 32 * wave + (lane & 31), rr_e = ue.r0 + (r_e < ue.rows ? r_e : 0);
     const bool busy_e = ue.rows > 32 * wave;
-    const int64_t tok_e = ue.t0 + (uint32_t)rr_e / (uint32_t)pe.G;
-    const int head_e = ue.hk * pe.G + (uint32_t)rr_e % (uint32_t)pe.G;
+    const int of_e = paged_token(pe, rr_e), head_e = ue.hk * pe.G + rr_e - of_e * pe.G;
+    const int64_t tok_e = ue.t0 + of_e;
     const int64_t part_bytes = 128 * (D + 2) * 4;
     constexpr int kSC1 = 16;
     if (ue.parts > 1) {
@@ -1158,6 +1190,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
         pe.lse[tok_e * pe.Hq + head_e] = l == 0.f ? -INFINITY : m + __builtin_log2f(l);
     }
   }
+  paged_zero_rows<elt>(args);
 }
 
 } // namespace txk
