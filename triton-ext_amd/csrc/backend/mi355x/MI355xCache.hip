@@ -568,27 +568,41 @@ int checkPages(const tx_page_desc *d, void *const *caches) {
   return TX_OK;
 }
 
-bool anyNull(std::initializer_list<const void *> ps) {
-  for (const void *p : ps)
-    if (!p)
+// Whether an array is NULL that a call on books of these extents reads or writes.
+bool anyNull(const tx_page_desc &d, std::initializer_list<const void *> of_S,
+             std::initializer_list<const void *> of_table, std::initializer_list<const void *> of_P) {
+  for (const void *p : of_S)
+    if (!p && d.S)
+      return true;
+  for (const void *p : of_table)
+    if (!p && d.S && d.W)
+      return true;
+  for (const void *p : of_P)
+    if (!p && d.P)
       return true;
   return false;
 }
-
 BookArgs bookArgs(const tx_page_desc &d, const int32_t *table, const int32_t *len,
                   const int32_t *refs, int32_t *table_out, int32_t *len_out, int32_t *refs_out,
                   int32_t *count, void *workspace) {
   BookArgs a = {};
-  a.S = d.S, a.W = d.W, a.P = d.P, a.n = d.n, a.page_shift = log2of(d.page_size);
+  a.W = d.W, a.S = (int32_t)d.S, a.P = (int32_t)d.P, a.n = (int32_t)d.n;
+  a.page_shift = log2of(d.page_size);
   a.table = table, a.len = len, a.refs = refs;
   a.table_out = table_out, a.len_out = len_out, a.refs_out = refs_out, a.count = count;
-  a.free_list = static_cast<int32_t *>(workspace);
-  if (workspace) {
-    a.prefix = a.free_list + d.P;
-    a.src = a.free_list + d.P;
-    a.dst = a.src + std::max(d.P, d.n);
-  }
+  a.table_in_place = table_out == table, a.refs_in_place = refs_out == refs;
+  a.src = static_cast<int32_t *>(workspace);
+  if (workspace)
+    a.dst = a.src + 2 * std::max(d.P, d.n);
   return a;
+}
+
+// Workgroups over the table's rows: about 2048 entries (or counts) each; `alone`: one.
+int64_t bookGrid(const tx_page_desc &d, bool alone, BookArgs &a) {
+  int64_t grid = std::max(cdiv(d.S * d.W, 2048), cdiv(d.P, 4096));
+  grid = alone ? 1 : std::min<int64_t>(std::max<int64_t>(grid, 1), 256);
+  a.rows = (int32_t)std::min<int64_t>(std::max<int64_t>(cdiv(d.S, grid), 1), kBookRows);
+  return grid;
 }
 
 int launchCopy(const tx_page_desc &d, void *const *caches, const int32_t *src, const int32_t *dst,
@@ -599,7 +613,7 @@ int launchCopy(const tx_page_desc &d, void *const *caches, const int32_t *src, c
   for (int i = 0; i < d.caches; ++i) {
     a.base[i] = static_cast<uint8_t *>(caches[i]);
     a.stride[i] = d.stride[i], a.bytes[i] = d.bytes[i];
-    pieces = std::max(pieces, cdiv(d.bytes[i], 4096));
+    pieces = std::max(pieces, cdiv(d.bytes[i], 16384));
   }
   if (d.caches == 0 || most == 0 || pieces == 0)
     return TX_OK;
@@ -619,7 +633,9 @@ extern "C" TX_API int tx_page_workspace(const tx_page_desc *desc, int64_t *bytes
     return rc;
   if (!bytes)
     return fail(TX_ERR_INVALID, "bytes is NULL");
-  *bytes = 4 * (desc->P + std::max<int64_t>(desc->S + 1, 2 * std::max(desc->P, desc->n)));
+  // lists of pages to copy (a page and its place each, and the places found), and the bits of
+  // page_compact where they do not fit LDS
+  *bytes = 12 * std::max(desc->P, desc->n) + 8 + 12 * (cdiv(desc->P, 64) + 1);
   return TX_OK;
 }
 
@@ -647,8 +663,7 @@ extern "C" TX_API int tx_page_reserve(const tx_page_desc *desc, const int32_t *p
   const int rc = checkPageDesc(desc);
   if (rc != TX_OK)
     return rc;
-  if (anyNull({page_table, kv_len, refs, new_len, table_out, len_out, refs_out, missing}) &&
-      desc->S && desc->W && desc->P)
+  if (anyNull(*desc, {kv_len, new_len, len_out}, {page_table, table_out}, {refs, refs_out}))
     return fail(TX_ERR_INVALID, "NULL array");
   if (!missing || !workspace)
     return fail(TX_ERR_INVALID, "missing or workspace is NULL");
@@ -657,7 +672,9 @@ extern "C" TX_API int tx_page_reserve(const tx_page_desc *desc, const int32_t *p
   BookArgs a = bookArgs(*desc, page_table, kv_len, refs, table_out, len_out, refs_out, missing,
                         workspace);
   a.new_len = new_len;
-  hipLaunchKernelGGL(page_reserve_kernel, dim3(1), dim3(kBookThreads), 0,
+  const bool alone = refs_out == refs || len_out == kv_len || len_out == new_len;
+  const int64_t grid = bookGrid(*desc, alone, a);
+  hipLaunchKernelGGL(page_reserve_kernel, dim3((uint32_t)grid), dim3(kBookThreads), 0,
                      static_cast<hipStream_t>(stream), a);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;
@@ -673,20 +690,23 @@ extern "C" TX_API int tx_page_fork(const tx_page_desc *desc, void *const *caches
   const int rc = checkPages(desc, caches);
   if (rc != TX_OK)
     return rc;
-  if (anyNull({page_table, kv_len, refs, table_out, len_out, refs_out}) && desc->S && desc->W &&
-      desc->P)
+  if (anyNull(*desc, {kv_len, len_out}, {page_table, table_out}, {refs, refs_out}))
     return fail(TX_ERR_INVALID, "NULL array");
   if (desc->n && (!parent || !child))
     return fail(TX_ERR_INVALID, "parent or child is NULL");
   if (!missing || !workspace)
     return fail(TX_ERR_INVALID, "missing or workspace is NULL");
+  if (!aligned(workspace, 8))
+    return fail(TX_ERR_WORKSPACE, "workspace must be 8-byte aligned");
   if (!tx_device_available())
     return fail(TX_ERR_NO_DEVICE, "no gfx950 device visible");
   hipStream_t s = static_cast<hipStream_t>(stream);
   BookArgs a = bookArgs(*desc, page_table, kv_len, refs, table_out, len_out, refs_out, missing,
                         workspace);
   a.parent = parent, a.child = child;
-  hipLaunchKernelGGL(page_fork_kernel, dim3(1), dim3(kBookThreads), 0, s, a);
+  // one for the children, others for the rows to copy
+  const int64_t grid = a.table_in_place && len_out == kv_len ? 1 : 1 + bookGrid(*desc, false, a);
+  hipLaunchKernelGGL(page_fork_kernel, dim3((uint32_t)grid), dim3(kBookThreads), 0, s, a);
   TX_HIP_CHECK(hipGetLastError());
   return launchCopy(*desc, caches, a.src, a.dst, nullptr, desc->n, s);
 }
@@ -699,8 +719,7 @@ extern "C" TX_API int tx_page_free(const tx_page_desc *desc, const int32_t *page
   const int rc = checkPageDesc(desc);
   if (rc != TX_OK)
     return rc;
-  if (anyNull({page_table, kv_len, refs, drop, table_out, len_out, refs_out}) && desc->S &&
-      desc->W && desc->P)
+  if (anyNull(*desc, {kv_len, drop, len_out}, {page_table, table_out}, {refs, refs_out}))
     return fail(TX_ERR_INVALID, "NULL array");
   if (desc->S == 0)
     if (desc->P == 0 || refs_out == refs)
@@ -710,8 +729,20 @@ extern "C" TX_API int tx_page_free(const tx_page_desc *desc, const int32_t *page
   BookArgs a = bookArgs(*desc, page_table, kv_len, refs, table_out, len_out, refs_out, nullptr,
                         nullptr);
   a.drop = drop;
-  hipLaunchKernelGGL(page_free_kernel, dim3(1), dim3(kBookThreads), 0,
-                     static_cast<hipStream_t>(stream), a);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!a.refs_in_place && desc->P > 0) {
+    hipLaunchKernelGGL(book_copy_kernel, dim3((uint32_t)std::min<int64_t>(cdiv(desc->P, 256), 1024)),
+                       dim3(256), 0, s, refs_out, refs, desc->P);
+    TX_HIP_CHECK(hipGetLastError());
+  }
+  if (desc->S == 0)
+    return TX_OK;
+  // a row's threads: 64 .. 512 by its length
+  int64_t tw = 64;
+  while (tw < desc->W && tw < kBookThreads)
+    tw *= 2;
+  const int64_t grid = std::min<int64_t>(cdiv(desc->S, kBookThreads / tw), 1024);
+  hipLaunchKernelGGL(page_free_kernel, dim3((uint32_t)grid), dim3(kBookThreads), 0, s, a);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;
 }
@@ -724,16 +755,23 @@ extern "C" TX_API int tx_page_compact(const tx_page_desc *desc, void *const *cac
   const int rc = checkPages(desc, caches);
   if (rc != TX_OK)
     return rc;
-  if (anyNull({page_table, table_out}) && desc->S && desc->W)
+  if (anyNull(*desc, {}, {page_table, table_out}, {refs, refs_out}))
     return fail(TX_ERR_INVALID, "NULL array");
-  if ((anyNull({refs, refs_out}) && desc->P) || !moved || !workspace)
-    return fail(TX_ERR_INVALID, "refs, moved or workspace is NULL");
+  if (!moved || !workspace)
+    return fail(TX_ERR_INVALID, "moved or workspace is NULL");
+  if (!aligned(workspace, 8))
+    return fail(TX_ERR_WORKSPACE, "workspace must be 8-byte aligned");
   if (!tx_device_available())
     return fail(TX_ERR_NO_DEVICE, "no gfx950 device visible");
   hipStream_t s = static_cast<hipStream_t>(stream);
   BookArgs a = bookArgs(*desc, page_table, nullptr, refs, table_out, nullptr, refs_out, moved,
                         workspace);
-  hipLaunchKernelGGL(page_compact_kernel, dim3(1), dim3(kBookThreads), 0, s, a);
+  const bool in_lds = cdiv(desc->P, 64) <= kBookMasks;
+  if (!in_lds)
+    a.masks = reinterpret_cast<uint64_t *>(
+        static_cast<uint8_t *>(workspace) + (12 * std::max(desc->P, desc->n) + 7) / 8 * 8);
+  const int64_t grid = bookGrid(*desc, a.refs_in_place || !in_lds, a);
+  hipLaunchKernelGGL(page_compact_kernel, dim3((uint32_t)grid), dim3(kBookThreads), 0, s, a);
   TX_HIP_CHECK(hipGetLastError());
   return launchCopy(*desc, caches, a.src, a.dst, moved, desc->P, s);
 }

@@ -1,10 +1,14 @@
 // The books of a paged cache (page table, lengths, reference counts) and the moves
 // of its pages.
 //
-// The books are integers of a few hundred KiB at most: one workgroup of 1024
-// threads goes through them with prefix sums, so that free pages are taken in
-// ascending order whatever the timing.  Pages are copied by a kernel of their own
-// that takes its list (and, compacting, its length) from device memory.
+// The books are integers: what bounds these kernels is the chain of their phases, not the bytes.
+// So a launch has as many workgroups as the table's rows fill, and every one works out
+// by itself what it needs of the others' part (sums over the sequences, which pages
+// are free), rather than wait for it.  That needs the books that all read to stay as they are:
+// where counts or lengths are written in place, the launch has one workgroup.  Free pages are
+// taken in ascending order whatever the timing, so results do not depend on it.
+// Pages are copied by a kernel of their own that takes its list (and, compacting, its
+// length) from device memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -14,31 +18,33 @@
 
 namespace txk {
 
-constexpr int kBookThreads = 1024;
+constexpr int kBookThreads = 512, kBookWaves = kBookThreads / 64;
+constexpr int kBookRows = 512; // rows of the table that a workgroup takes at a time
 
 struct BookArgs {
-  int64_t S, W, P, n;
-  int32_t page_shift;
+  int64_t W;
+  int32_t S, P, n, page_shift;
+  int32_t rows;              // rows of a workgroup, at most kBookRows
+  int32_t table_in_place, refs_in_place;
   const int32_t *table, *len, *refs;
   const int32_t *new_len, *parent, *child;
   const uint8_t *drop;
   int32_t *table_out, *len_out, *refs_out, *count;
-  int32_t *free_list; // [P]: free pages in ascending order; compact: the map of pages
-  int32_t *src, *dst; // [P] (compact) or [n] (fork): pages to copy
-  int32_t *prefix;    // [S + 1] (reserve)
+  int32_t *src, *dst;        // pages to copy: [P / 2] (compact) or [n] (fork)
+  uint64_t *masks;           // compact: [P / 64], and the sums after them; NULL: in LDS
 };
 
 // Sum over the workgroup of v in all threads before this one; total in `all`.
 __device__ __forceinline__ int book_scan(int v, int &all) {
-  __shared__ int part[kBookThreads / 64];
+  __shared__ int part[kBookWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int o = __shfl_up(s, d);
-    if (lane >= d)
-      s += o;
-  }
+  s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xf, 0xf, false); // row_shr 1, 2, 4, 8
+  s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xf, 0xf, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xf, 0xf, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xf, 0xf, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xa, 0xf, false); // row_bcast 15, 31
+  s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xc, 0xf, false);
   __syncthreads(); // the last call's reads of `part`
   if (lane == 63)
     part[wave] = s;
@@ -46,7 +52,7 @@ __device__ __forceinline__ int book_scan(int v, int &all) {
   int before = 0;
   all = 0;
 #pragma unroll
-  for (int w = 0; w < kBookThreads / 64; ++w) {
+  for (int w = 0; w < kBookWaves; ++w) {
     if (w < wave)
       before += part[w];
     all += part[w];
@@ -54,94 +60,204 @@ __device__ __forceinline__ int book_scan(int v, int &all) {
   return before + s - v;
 }
 
-// The free pages in ascending order into free_list; returns how many there are.
-__device__ __forceinline__ int64_t book_free_list(const BookArgs &p) {
-  int64_t free_pages = 0;
-  for (int64_t base = 0; base < p.P; base += kBookThreads) {
-    const int64_t i = base + threadIdx.x;
-    const int is_free = i < p.P && p.refs[i] == 0;
-    int all;
-    const int at = book_scan(is_free, all);
-    if (is_free)
-      p.free_list[free_pages + at] = (int32_t)i;
-    free_pages += all;
-  }
-  return free_pages;
-}
-
-__device__ __forceinline__ void book_copy(int32_t *to, const int32_t *from, int64_t n) {
-  if (to != from)
-    for (int64_t i = threadIdx.x; i < n; i += kBookThreads)
-      to[i] = from[i];
-}
-
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int shift) {
   return (tokens + (1ll << shift) - 1) >> shift;
 }
 
-__global__ void __launch_bounds__(kBookThreads) page_reserve_kernel(BookArgs p) {
-  const int64_t nfree = book_free_list(p);
-  const int64_t most = p.W << p.page_shift;
-  auto after = [&](int64_t s) { // the length that sequence s gets
-    const int64_t want = p.new_len[s] < most ? p.new_len[s] : most;
-    return want > p.len[s] ? want : (int64_t)p.len[s];
-  };
-  auto held = [&](int64_t s) {
-    const int64_t h = pages_of(p.len[s] > 0 ? p.len[s] : 0, p.page_shift);
-    return h < p.W ? h : p.W;
-  };
-  int64_t wanted = 0;
-  for (int64_t base = 0; base < p.S; base += kBookThreads) {
-    const int64_t s = base + threadIdx.x;
-    int need = 0;
-    if (s < p.S) {
-      const int64_t to = pages_of(after(s), p.page_shift);
-      need = (int)((to < p.W ? to : p.W) - held(s));
-      need = need > 0 ? need : 0;
-    }
-    int all;
-    const int at = book_scan(need, all);
-    if (s < p.S)
-      p.prefix[s] = (int32_t)(wanted + at);
-    wanted += all;
-  }
+// The free pages in ascending order, until `wanted` of them are found: f(rank, page) for each of
+// those.  Returns how many there are (at most `wanted`); cut: the last of them (-1: none).
+template <class F>
+__device__ __forceinline__ int64_t book_free_pages(const int32_t *refs, int64_t P, int64_t wanted,
+                                                   int64_t &cut, F f) {
+  constexpr int N = 4, STEP = N * kBookThreads;
+  __shared__ int last;
   if (threadIdx.x == 0)
-    p.prefix[p.S] = (int32_t)wanted;
-  book_copy(p.refs_out, p.refs, p.P);
+    last = -1;
+  int64_t found = 0;
+  auto load = [&](int64_t base, int (&r)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t i = base + N * (int64_t)threadIdx.x + k;
+      r[k] = refs[i < P ? i : 0];
+      if (i >= P)
+        r[k] = 1;
+    }
+  };
+  int r[N], ahead[N];
+  if (wanted > 0 && P > 0)
+    load(0, r);
+  for (int64_t base = 0; base < P && found < wanted; base += STEP) {
+    if (base + STEP < P)
+      load(base + STEP, ahead);
+    int mine = 0, all;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      mine += r[k] == 0;
+    int64_t rank = found + book_scan(mine, all);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (r[k] == 0) {
+        const int page = (int)(base + N * (int64_t)threadIdx.x + k);
+        if (rank < wanted)
+          f(rank, page);
+        if (rank == wanted - 1)
+          last = page;
+        ++rank;
+      }
+    found += all;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      r[k] = ahead[k];
+  }
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < p.S * p.W; i += kBookThreads) {
-    const int64_t s = i / p.W, w = i % p.W, first = held(s);
-    const int64_t rank = p.prefix[s] + w - first;
-    if (w < first || rank >= p.prefix[s + 1]) {
-      p.table_out[i] = p.table[i];
-      continue;
-    }
-    const int32_t page = rank < nfree ? p.free_list[rank] : -1;
-    p.table_out[i] = page;
-    if (page >= 0)
-      p.refs_out[page] = 1;
-  }
-  if (threadIdx.x == 0)
-    *p.count = (int32_t)(wanted > nfree ? wanted - nfree : 0);
-  __syncthreads(); // len_out may be len
-  for (int64_t base = 0; base < p.S; base += kBookThreads) {
-    const int64_t s = base + threadIdx.x;
-    if (s < p.S)
-      p.len_out[s] = (int32_t)after(s);
-  }
+  cut = found < wanted ? P - 1 : last;
+  __syncthreads(); // `last` again
+  return found < wanted ? found : wanted;
 }
 
+// New pages for the sequences.  Every workgroup sums the needs of all sequences, goes through the
+// counts as far as there are pages wanted (a page that it finds goes straight to its place in
+// the workgroup's rows), and then writes its rows and its share of the counts: a free page up
+// to the last one taken has been taken.
+__global__ void __launch_bounds__(kBookThreads) page_reserve_kernel(BookArgs p) {
+  __shared__ int pre[kBookRows + 1];   // pages that the sequences up to this row of ours want
+  __shared__ int held_of[kBookRows];
+  const int tid = threadIdx.x;
+  const int64_t most = p.W << p.page_shift;
+  auto after = [&](int64_t len, int64_t to) { // the length that a sequence gets
+    const int64_t want = to < most ? to : most;
+    return want > len ? want : len;
+  };
+  auto held = [&](int64_t len) {
+    const int64_t h = pages_of(len > 0 ? len : 0, p.page_shift);
+    return (int)(h < p.W ? h : p.W);
+  };
+  auto need = [&](int64_t len, int64_t to) {
+    const int64_t h = pages_of(after(len, to), p.page_shift);
+    const int x = (int)(h < p.W ? h : p.W) - held(len);
+    return x > 0 ? x : 0;
+  };
+  int64_t nfree = 0, cut = -1, wanted = 0;
+  for (int64_t s0 = (int64_t)blockIdx.x * p.rows; s0 < p.S; s0 += (int64_t)gridDim.x * p.rows) {
+    const int rows = (int)(p.S - s0 < p.rows ? p.S - s0 : p.rows);
+    int before = 0, all = 0, x;
+    for (int64_t s = tid; s < p.S; s += kBookThreads) {
+      const int v = need(p.len[s], p.new_len[s]);
+      all += v;
+      before += s < s0 ? v : 0;
+    }
+    book_scan(all, x);
+    wanted = x;
+    book_scan(before, x);
+    const int64_t first_rank = x;
+    int mine = 0;
+    if (tid < rows) {
+      const int64_t len = p.len[s0 + tid];
+      mine = need(len, p.new_len[s0 + tid]);
+      held_of[tid] = held(len);
+    }
+    const int at = book_scan(mine, x);
+    if (tid < rows)
+      pre[tid] = at;
+    if (tid == 0)
+      pre[rows] = x;
+    const int ours = x;
+    __syncthreads();
+    nfree = book_free_pages(p.refs, p.P, wanted, cut, [&](int64_t rank, int page) {
+      const int64_t r = rank - first_rank;
+      if (r < 0 || r >= ours)
+        return;
+      int lo = 0, hi = rows; // pre[lo] <= r < pre[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (pre[mid] <= r)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      p.table_out[(s0 + lo) * p.W + held_of[lo] + (r - pre[lo])] = page;
+    });
+    // the other entries
+    int tw = 64; // threads of a row
+    while (tw < p.W && tw < kBookThreads)
+      tw *= 2;
+    for (int r = tid / tw; r < rows; r += kBookThreads / tw) {
+      const int64_t row = (s0 + r) * p.W;
+      const int h = held_of[r], fresh = pre[r + 1] - pre[r];
+      const int64_t got = nfree - first_rank - pre[r]; // of `fresh`
+      if (p.table_in_place) {
+        for (int64_t w = (got > 0 ? got : 0) + (tid & (tw - 1)); w < fresh; w += tw)
+          p.table_out[row + h + w] = -1;
+        continue;
+      }
+      for (int64_t w = tid & (tw - 1); w < p.W; w += tw) {
+        const int64_t k = w - h;
+        if (k < 0 || k >= fresh)
+          p.table_out[row + w] = p.table[row + w];
+        else if (k >= got)
+          p.table_out[row + w] = -1;
+      }
+    }
+    __syncthreads(); // pre, held_of
+  }
+  if (p.refs_in_place) {
+    for (int64_t i = tid; i <= cut; i += kBookThreads)
+      if (p.refs[i] == 0)
+        p.refs_out[i] = 1;
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * kBookThreads + tid; i < p.P;
+         i += (int64_t)gridDim.x * kBookThreads) {
+      const int r = p.refs[i];
+      p.refs_out[i] = r == 0 && i <= cut ? 1 : r;
+    }
+  }
+  // (len_out may be len, with one workgroup: every need has been summed)
+  for (int64_t s = (int64_t)blockIdx.x * kBookThreads + tid; s < p.S;
+       s += (int64_t)gridDim.x * kBookThreads)
+    p.len_out[s] = (int32_t)after(p.len[s], p.new_len[s]);
+  if (blockIdx.x == 0 && tid == 0)
+    *p.count = (int32_t)(wanted - nfree);
+}
+
+// Workgroup 0 makes the children; the others copy the rows of who is not one.
 __global__ void __launch_bounds__(kBookThreads) page_fork_kernel(BookArgs p) {
-  const int64_t nfree = book_free_list(p);
-  book_copy(p.refs_out, p.refs, p.P);
-  book_copy(p.table_out, p.table, p.S * p.W);
-  book_copy(p.len_out, p.len, p.S);
-  __syncthreads();
-  int64_t wanted = 0;
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    __shared__ int is_child[kBookRows];
+    for (int64_t s0 = (int64_t)(blockIdx.x - 1) * p.rows; s0 < p.S;
+         s0 += (int64_t)(gridDim.x - 1) * p.rows) {
+      const int rows = (int)(p.S - s0 < p.rows ? p.S - s0 : p.rows);
+      __syncthreads();
+      for (int r = tid; r < rows; r += kBookThreads)
+        is_child[r] = 0;
+      __syncthreads();
+      for (int i = tid; i < p.n; i += kBookThreads) {
+        const int64_t a = p.parent[i], c = p.child[i];
+        if (a >= 0 && a < p.S && c >= s0 && c < s0 + rows)
+          is_child[c - s0] = 1;
+      }
+      __syncthreads();
+      int tw = 64;
+      while (tw < p.W && tw < kBookThreads)
+        tw *= 2;
+      for (int r = tid / tw; r < rows; r += kBookThreads / tw)
+        if (!is_child[r])
+          for (int64_t w = tid & (tw - 1); w < p.W; w += tw)
+            p.table_out[(s0 + r) * p.W + w] = p.table[(s0 + r) * p.W + w];
+      for (int r = tid; r < rows; r += kBookThreads)
+        if (!is_child[r])
+          p.len_out[s0 + r] = p.len[s0 + r];
+    }
+    return;
+  }
+  if (!p.refs_in_place)
+    for (int64_t i = tid; i < p.P; i += kBookThreads)
+      p.refs_out[i] = p.refs[i];
   // src[i], dst[i]: the last page of child i's parent and its copy (-1: none)
-  for (int64_t base = 0; base < p.n; base += kBookThreads) {
-    const int64_t i = base + threadIdx.x;
-    int open = 0, last = -1;
+  int64_t wanted = 0;
+  for (int base = 0; base < p.n; base += kBookThreads) {
+    const int i = base + tid;
+    int open = 0, last = -1, all;
     if (i < p.n) {
       const int64_t a = p.parent[i], c = p.child[i];
       if (a >= 0 && a < p.S && c >= 0 && c < p.S) {
@@ -151,100 +267,185 @@ __global__ void __launch_bounds__(kBookThreads) page_fork_kernel(BookArgs p) {
           last = p.table[a * p.W + used - 1];
       }
     }
-    int all;
     const int at = book_scan(open, all);
     if (i < p.n) {
-      const int32_t page = open && wanted + at < nfree ? p.free_list[wanted + at] : -1;
       p.src[i] = last;
-      p.dst[i] = page;
-      if (page >= 0)
-        p.refs_out[page] = 1;
+      p.dst[i] = open ? (int)(wanted + at) : -1; // its rank, until the pages are known
     }
     wanted += all;
   }
+  int64_t cut;
+  const int64_t nfree =
+      book_free_pages(p.refs, p.P, wanted, cut, [&](int64_t rank, int page) {
+        p.src[p.n + rank] = page; // (src and dst have place for 2 n)
+      });
   __syncthreads();
-  for (int64_t j = threadIdx.x; j < p.n * p.W; j += kBookThreads) {
-    const int64_t i = j / p.W, w = j % p.W;
+  for (int i = tid; i < p.n; i += kBookThreads) {
+    const int rank = p.dst[i];
+    const int page = rank >= 0 && rank < nfree ? p.src[p.n + rank] : -1;
+    p.dst[i] = page;
+    if (page >= 0)
+      p.refs_out[page] = 1;
+  }
+  __syncthreads();
+  int tw = 64;
+  while (tw < p.W && tw < kBookThreads)
+    tw *= 2;
+  for (int i = tid / tw; i < p.n; i += kBookThreads / tw) {
     const int64_t a = p.parent[i], c = p.child[i];
     if (a < 0 || a >= p.S || c < 0 || c >= p.S)
       continue;
     const int64_t len = p.len[a] > 0 ? p.len[a] : 0, used = pages_of(len, p.page_shift);
     const bool open = (len & ((1 << p.page_shift) - 1)) != 0;
-    int32_t page = -1;
-    if (w < used) {
-      page = p.table[a * p.W + w];
-      if (open && w == used - 1)
-        page = p.dst[i];
-      else if (page >= 0 && page < p.P)
-        atomicAdd(&p.refs_out[page], 1);
+    for (int64_t w = tid & (tw - 1); w < p.W; w += tw) {
+      int32_t page = -1;
+      if (w < used) {
+        page = p.table[a * p.W + w];
+        if (open && w == used - 1)
+          page = p.dst[i];
+        else if (page >= 0 && page < p.P)
+          atomicAdd(&p.refs_out[page], 1);
+      }
+      p.table_out[c * p.W + w] = page;
+      if (w == 0)
+        p.len_out[c] = (int32_t)len;
     }
-    p.table_out[c * p.W + w] = page;
-    if (w == 0)
-      p.len_out[c] = (int32_t)len;
   }
-  if (threadIdx.x == 0)
-    *p.count = (int32_t)(wanted > nfree ? wanted - nfree : 0);
+  if (tid == 0)
+    *p.count = (int32_t)(wanted - nfree);
 }
 
-__global__ void __launch_bounds__(kBookThreads) page_free_kernel(BookArgs p) {
-  book_copy(p.refs_out, p.refs, p.P);
-  __syncthreads();
-  for (int64_t i = threadIdx.x; i < p.S * p.W; i += kBookThreads) {
-    const int64_t s = i / p.W, w = i % p.W;
-    const int32_t page = p.table[i];
-    if (p.drop[s]) {
-      if (w < pages_of(p.len[s] > 0 ? p.len[s] : 0, p.page_shift) && page >= 0 && page < p.P)
-        atomicSub(&p.refs_out[page], 1);
-      p.table_out[i] = -1;
-    } else {
-      p.table_out[i] = page;
-    }
-  }
-  __syncthreads(); // len_out may be len
-  for (int64_t s = threadIdx.x; s < p.S; s += kBookThreads)
-    p.len_out[s] = p.drop[s] ? 0 : p.len[s];
+__global__ void __launch_bounds__(256) book_copy_kernel(int32_t *to, const int32_t *from, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    to[i] = from[i];
 }
+
+// refs_out holds the counts already.  A row's entries, then its length (which may be in place).
+__global__ void __launch_bounds__(kBookThreads) page_free_kernel(BookArgs p) {
+  const int tid = threadIdx.x;
+  int tw = 64;
+  while (tw < p.W && tw < kBookThreads)
+    tw *= 2;
+  const int per = kBookThreads / tw;
+  for (int64_t s0 = (int64_t)blockIdx.x * per; s0 < p.S; s0 += (int64_t)gridDim.x * per) {
+    const int64_t s = s0 + tid / tw;
+    const bool on = s < p.S;
+    const int len = on ? p.len[s] : 0;
+    const bool drop = on && p.drop[s];
+    const int64_t used = pages_of(len > 0 ? len : 0, p.page_shift);
+    for (int64_t w = tid & (tw - 1); on && w < p.W; w += tw) {
+      if (drop) {
+        const int32_t page = p.table[s * p.W + w];
+        if (w < used && page >= 0 && page < p.P)
+          atomicSub(&p.refs_out[page], 1);
+        p.table_out[s * p.W + w] = -1;
+      } else if (!p.table_in_place) {
+        p.table_out[s * p.W + w] = p.table[s * p.W + w];
+      }
+    }
+    __syncthreads(); // len_out may be len
+    if (on && (tid & (tw - 1)) == 0)
+      p.len_out[s] = drop ? 0 : len;
+  }
+}
+
+// With U pages in use: which pages are, as bits, and how many of them lie before each 64, from which
+// every workgroup finds by itself where a page goes and where it came from.
+constexpr int kBookMasks = 4096; // 64 pages each, in LDS
 
 __global__ void __launch_bounds__(kBookThreads) page_compact_kernel(BookArgs p) {
-  int used = 0, n;
-  for (int64_t base = 0; base < p.P; base += kBookThreads) {
-    const int64_t i = base + threadIdx.x;
-    book_scan(i < p.P && p.refs[i] > 0, n);
-    used += n;
+  __shared__ uint64_t lds_masks[kBookMasks];
+  __shared__ int lds_sums[kBookMasks + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = (int)(((int64_t)p.P + 63) / 64);
+  uint64_t *const masks = p.masks ? p.masks : lds_masks;
+  int *const sums = p.masks ? reinterpret_cast<int *>(p.masks + groups) : lds_sums;
+  constexpr int N = 8; // groups a wave has under way
+  for (int g0 = wave * N; g0 < groups; g0 += kBookWaves * N) {
+    int r[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t i = 64 * (int64_t)(g0 + k) + lane;
+      r[k] = p.refs[i < p.P ? i : 0];
+      if (i >= p.P)
+        r[k] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint64_t live = __ballot(r[k] > 0);
+      if (lane == 0 && g0 + k < groups)
+        masks[g0 + k] = live;
+    }
   }
-  // holes below `used` and used pages from there on, as many of the one as of the other
-  int64_t holes = 0, movers = 0;
-  for (int64_t base = 0; base < p.P; base += kBookThreads) {
-    const int64_t i = base + threadIdx.x;
-    const bool live = i < p.P && p.refs[i] > 0;
-    const int hole = i < used && !live, mover = i >= used && live;
+  __syncthreads();
+  int used = 0;
+  for (int base = 0; base < groups; base += kBookThreads) {
+    const int g = base + tid;
     int all;
-    const int at = book_scan(hole, all);
-    if (hole)
-      p.dst[holes + at] = (int32_t)i;
-    holes += all;
-    const int at2 = book_scan(mover, all);
-    if (mover)
-      p.src[movers + at2] = (int32_t)i;
-    movers += all;
-    if (i < p.P)
-      p.free_list[i] = (int32_t)i;
+    const int at = book_scan(g < groups ? __popcll(masks[g]) : 0, all);
+    if (g < groups)
+      sums[g] = used + at;
+    used += all;
   }
-  book_copy(p.refs_out, p.refs, p.P);
+  if (tid == 0)
+    sums[groups] = used;
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < movers; i += kBookThreads) {
-    const int32_t a = p.src[i], b = p.dst[i];
-    p.free_list[a] = b;
-    p.refs_out[b] = p.refs_out[a];
-    p.refs_out[a] = 0;
+  auto live_below = [&](int page) {
+    const int g = page >> 6, b = page & 63;
+    return g >= groups ? used : sums[g] + __popcll(masks[g] & ((1ull << b) - 1));
+  };
+  // the k-th page that is in use (or, `free`, that is not)
+  auto select = [&](int k, bool free) {
+    int lo = 0, hi = groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      const int at = free ? (int)(64 * (int64_t)mid - sums[mid]) : sums[mid];
+      if (at <= k)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    k -= free ? (int)(64 * (int64_t)lo - sums[lo]) : sums[lo];
+    const uint64_t m = free ? ~masks[lo] : masks[lo];
+    int at = 0; // the k-th bit of m
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+      const int c = __popcll((m >> at) & ((1ull << d) - 1));
+      if (c <= k)
+        k -= c, at += d;
+    }
+    return 64 * lo + at;
+  };
+  const int stay = live_below(used), movers = used - stay; // pages in use below U, and past it
+  const int64_t first = (int64_t)blockIdx.x * kBookThreads + tid,
+                step = (int64_t)gridDim.x * kBookThreads;
+  for (int64_t m = first; m < movers; m += step) {
+    const int a = select(stay + (int)m, false), b = select((int)m, true);
+    p.src[m] = a, p.dst[m] = b;
+    if (p.refs_in_place) {
+      p.refs_out[b] = p.refs[a];
+      p.refs_out[a] = 0;
+    }
   }
-  __syncthreads();
-  for (int64_t i = threadIdx.x; i < p.S * p.W; i += kBookThreads) {
-    const int32_t page = p.table[i];
-    p.table_out[i] = page >= 0 && page < p.P ? p.free_list[page] : page;
+  if (!p.refs_in_place)
+    for (int64_t i = first; i < p.P; i += step) {
+      const bool live = masks[i >> 6] >> (i & 63) & 1;
+      int from = (int)i;
+      if (i < used && !live)
+        from = select(stay + (int)i - live_below((int)i), false);
+      const int r = p.refs[from];
+      p.refs_out[i] = i >= used && live ? 0 : r;
+    }
+  const int64_t entries = p.S * p.W;
+  for (int64_t i = first; i < entries; i += step) {
+    int page = p.table[i];
+    // (an entry may name a page that is not in use: it stays)
+    if (page >= used && page < p.P && (masks[page >> 6] >> (page & 63) & 1))
+      page = select(live_below(page) - stay, true);
+    p.table_out[i] = page;
   }
-  if (threadIdx.x == 0)
-    *p.count = (int32_t)movers;
+  if (blockIdx.x == 0 && tid == 0)
+    *p.count = movers;
 }
 
 struct PageCopyArgs {
@@ -256,18 +457,35 @@ struct PageCopyArgs {
   int64_t stride[TX_PAGE_CACHES], bytes[TX_PAGE_CACHES];
 };
 
-// blockIdx.y: the cache.  Pieces of 4 KiB (256 threads x 16 bytes).
+// blockIdx.y: the cache.  Pieces of 16 KiB (256 threads x 4 x 16 bytes, all four loads before
+// the stores).  Bound by memory.
 __global__ void __launch_bounds__(256) page_copy_kernel(PageCopyArgs p) {
   const int c = blockIdx.y;
-  const int64_t n = p.count ? *p.count : p.n;
-  const int64_t pieces = (p.bytes[c] + 4095) / 4096;
-  for (int64_t w = blockIdx.x; w < n * pieces; w += gridDim.x) {
-    const int64_t i = w / pieces, at = (w % pieces) * 4096 + threadIdx.x * 16;
+  const int64_t bytes = p.bytes[c], stride = p.stride[c];
+  uint8_t *const base = p.base[c];
+  const uint32_t n = (uint32_t)(p.count ? *p.count : p.n);
+  const uint32_t pieces = (uint32_t)((bytes + 16383) / 16384);
+  if (pieces == 0)
+    return;
+  uint32_t i = blockIdx.x / pieces, at_piece = blockIdx.x - i * pieces;
+  const uint32_t step_i = gridDim.x / pieces, step_p = gridDim.x - step_i * pieces;
+  while (i < n) {
     const int64_t a = p.src[i], b = p.dst[i];
-    if (a < 0 || a >= p.P || b < 0 || b >= p.P || a == b || at >= p.bytes[c])
-      continue;
-    *reinterpret_cast<u32x4 *>(p.base[c] + b * p.stride[c] + at) =
-        *reinterpret_cast<const u32x4 *>(p.base[c] + a * p.stride[c] + at);
+    if (a >= 0 && a < p.P && b >= 0 && b < p.P && a != b) {
+      const int64_t at = (int64_t)at_piece * 16384 + threadIdx.x * 16;
+      u32x4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + 4096 * k < bytes)
+          x[k] = *reinterpret_cast<const u32x4 *>(base + a * stride + at + 4096 * k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + 4096 * k < bytes)
+          *reinterpret_cast<u32x4 *>(base + b * stride + at + 4096 * k) = x[k];
+    }
+    i += step_i, at_piece += step_p;
+    if (at_piece >= pieces)
+      at_piece -= pieces, ++i;
   }
 }
 
