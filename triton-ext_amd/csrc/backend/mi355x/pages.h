@@ -253,63 +253,95 @@ __global__ void __launch_bounds__(kBookThreads) page_fork_kernel(BookArgs p) {
   if (!p.refs_in_place)
     for (int64_t i = tid; i < p.P; i += kBookThreads)
       p.refs_out[i] = p.refs[i];
-  // src[i], dst[i]: the last page of child i's parent and its copy (-1: none)
-  int64_t wanted = 0;
-  for (int base = 0; base < p.n; base += kBookThreads) {
+  // src[i], dst[i]: the last page of child i's parent and its copy (-1: none).  A batch of children
+  // is looked up once, into LDS.
+  struct Child {
+    int a, c, len, rank; // parent (-1: the pair is skipped), child, rank of the page it wants or -1
+  };
+  __shared__ Child kids[kBookThreads];
+  auto look_up = [&](int base, int &last, int64_t before) {
     const int i = base + tid;
-    int open = 0, last = -1, all;
+    Child k{-1, 0, 0, -1};
+    int open = 0, all;
+    last = -1;
     if (i < p.n) {
-      const int64_t a = p.parent[i], c = p.child[i];
+      const int a = p.parent[i], c = p.child[i];
       if (a >= 0 && a < p.S && c >= 0 && c < p.S) {
-        const int64_t len = p.len[a] > 0 ? p.len[a] : 0, used = pages_of(len, p.page_shift);
-        open = (len & ((1 << p.page_shift) - 1)) != 0 && used <= p.W;
+        const int len = p.len[a];
+        k.a = a, k.c = c, k.len = len > 0 ? len : 0;
+        const int64_t used = pages_of(k.len, p.page_shift);
+        open = (k.len & ((1 << p.page_shift) - 1)) != 0 && used <= p.W;
         if (open)
           last = p.table[a * p.W + used - 1];
       }
     }
     const int at = book_scan(open, all);
-    if (i < p.n) {
-      p.src[i] = last;
-      p.dst[i] = open ? (int)(wanted + at) : -1; // its rank, until the pages are known
-    }
-    wanted += all;
+    k.rank = open ? (int)before + at : -1;
+    kids[tid] = k;
+    return all;
+  };
+  int64_t wanted = 0;
+  for (int base = 0; base < p.n; base += kBookThreads) {
+    int last;
+    wanted += look_up(base, last, wanted);
+    if (base + tid < p.n)
+      p.src[base + tid] = last;
   }
   int64_t cut;
-  const int64_t nfree =
-      book_free_pages(p.refs, p.P, wanted, cut, [&](int64_t rank, int page) {
-        p.src[p.n + rank] = page; // (src and dst have place for 2 n)
-      });
-  __syncthreads();
-  for (int i = tid; i < p.n; i += kBookThreads) {
-    const int rank = p.dst[i];
-    const int page = rank >= 0 && rank < nfree ? p.src[p.n + rank] : -1;
-    p.dst[i] = page;
-    if (page >= 0)
-      p.refs_out[page] = 1;
-  }
-  __syncthreads();
+  const int64_t nfree = book_free_pages(p.refs, p.P, wanted, cut, [&](int64_t rank, int page) {
+    p.src[p.n + rank] = page; // (src has place for 2 n)
+    p.refs_out[page] = 1;
+  });
   int tw = 64;
   while (tw < p.W && tw < kBookThreads)
     tw *= 2;
-  for (int i = tid / tw; i < p.n; i += kBookThreads / tw) {
-    const int64_t a = p.parent[i], c = p.child[i];
-    if (a < 0 || a >= p.S || c < 0 || c >= p.S)
-      continue;
-    const int64_t len = p.len[a] > 0 ? p.len[a] : 0, used = pages_of(len, p.page_shift);
-    const bool open = (len & ((1 << p.page_shift) - 1)) != 0;
-    for (int64_t w = tid & (tw - 1); w < p.W; w += tw) {
-      int32_t page = -1;
-      if (w < used) {
-        page = p.table[a * p.W + w];
-        if (open && w == used - 1)
-          page = p.dst[i];
-        else if (page >= 0 && page < p.P)
-          atomicAdd(&p.refs_out[page], 1);
-      }
-      p.table_out[c * p.W + w] = page;
-      if (w == 0)
-        p.len_out[c] = (int32_t)len;
+  const int per = kBookThreads / tw;
+  int64_t before = 0;
+  for (int base = 0; base < p.n; base += kBookThreads) {
+    if (p.n > kBookThreads) { // (else kids holds them)
+      int last;
+      __syncthreads();
+      before += look_up(base, last, before);
     }
+    __syncthreads();
+    if (base + tid < p.n) {
+      const int rank = kids[tid].rank;
+      kids[tid].rank = rank < 0 ? -2 : rank < nfree ? p.src[p.n + rank] : -1; // the page; -2: none
+      p.dst[base + tid] = kids[tid].rank < 0 ? -1 : kids[tid].rank;
+    }
+    __syncthreads();
+    const int m = p.n - base < kBookThreads ? p.n - base : kBookThreads;
+    constexpr int N = 4; // rows under way
+    for (int i0 = tid / tw; i0 < m; i0 += N * per)
+      for (int64_t w = tid & (tw - 1); w < p.W; w += tw) {
+        int page[N];
+        bool shared[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int i = i0 + k * per;
+          const Child kid = kids[i < m ? i : 0];
+          const int64_t used = pages_of(kid.len, p.page_shift);
+          shared[k] = i < m && kid.a >= 0 && w < used;
+          page[k] = -1;
+          if (shared[k]) {
+            if (kid.rank != -2 && w == used - 1)
+              page[k] = kid.rank, shared[k] = false;
+            else
+              page[k] = p.table[kid.a * p.W + w];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int i = i0 + k * per;
+          if (i >= m || kids[i].a < 0)
+            continue;
+          if (shared[k] && page[k] >= 0 && page[k] < p.P)
+            atomicAdd(&p.refs_out[page[k]], 1);
+          p.table_out[kids[i].c * p.W + w] = page[k];
+        }
+      }
+    if (base + tid < p.n && kids[tid].a >= 0)
+      p.len_out[kids[tid].c] = kids[tid].len;
   }
   if (tid == 0)
     *p.count = (int32_t)(wanted - nfree);

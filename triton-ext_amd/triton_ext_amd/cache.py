@@ -21,29 +21,45 @@ import math
 from . import capi
 from .dot import _current_stream, _tx_of, workspace_for
 
-_plans = {}
+# What a call's checks found for arguments of one form (shapes, strides, types, devices and
+# scalars: _form), so that a call of the same form goes to the launch at once.  Nothing here depends
+# on a tensor's address or contents.
+_forms = {}
+
+
+def _form(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _keep(form, found):
+    if len(_forms) >= 4096:  # a program of ever new sizes
+        _forms.clear()
+    _forms[form] = found
+    return found
 
 
 def _plan(kind, desc_type, plan_type, key):
-    """The plan of a descriptor with these fields in order, kept by its fields."""
-    full = (kind,) + key
-    p = _plans.get(full)
-    if p is None:
-        p = plan_type()
-        capi.check(getattr(capi.load(), f"tx_{kind}_plan_create")(
-            ctypes.byref(desc_type(*key)), ctypes.byref(p)))
-        if len(_plans) >= 4096:  # a program of ever new sizes
-            _plans.clear()
-        _plans[full] = p
+    """The plan of a descriptor with these fields in order."""
+    p = plan_type()
+    capi.check(getattr(capi.load(), f"tx_{kind}_plan_create")(
+        ctypes.byref(desc_type(*key)), ctypes.byref(p)))
     return p
 
 
-def _int32(t, name, dims):
+def _is_int32(t, name, dims):
     import torch
     if t.dtype != torch.int32 or t.dim() != dims:
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension(s), got "
                          f"{t.dtype} {tuple(t.shape)}")
+
+
+def _dense(t):
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _int32(t, name, dims):
+    _is_int32(t, name, dims)
+    return _dense(t)
 
 
 def _same_device(device, **tensors):
@@ -59,6 +75,16 @@ def _dense_last(t):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _new(t):
+    """A new tensor like t, dense, with its last dimension contiguous (empty_like is the
+    cheapest call that makes one)."""
+    import torch
+    out = torch.empty_like(t)
+    if out.stride(-1) != 1 and out.shape[-1] > 1:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return out
 
 
 def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, context=4096,
@@ -106,6 +132,30 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     <= D: the dims past it are copied.  The pairs are dims (i, i + rot_dim / 2), or
     (2 i, 2 i + 1) when interleaved.  inverse: the transposed map, which takes the
     gradient of the result to that of x.  out may be x itself."""
+    form = ("rotary", _form(x), _form(positions), _form(inv_freq), bool(interleaved),
+            float(scale), bool(inverse), _form(out))
+    found = _forms.get(form)
+    if found is None:
+        _rotary_checks(x, positions, inv_freq, out)
+        # what the kernel does not take as it lies is copied, and the copy's form looked up
+        xc = _dense_last(x)
+        pc, fc = positions.contiguous(), inv_freq.contiguous()
+        if xc is not x or pc is not positions or fc is not inv_freq:
+            return rotary(xc, pc, fc, interleaved=interleaved, scale=scale, inverse=inverse,
+                          out=out, stream=stream)
+        found = _keep(form, _rotary_plan(x, positions, inv_freq, interleaved, scale, inverse,
+                                         _new(x) if out is None else out))
+    if out is None:
+        out = _new(x)
+    rc = capi.load().tx_rotary_launch(found, x.data_ptr(), positions.data_ptr(),
+                                      inv_freq.data_ptr(), out.data_ptr(),
+                                      _current_stream(x.device) if stream is None else stream)
+    if rc:
+        capi.check(rc)
+    return out
+
+
+def _rotary_checks(x, positions, inv_freq, out):
     import torch
     if x.dim() not in (3, 4):
         raise ValueError(f"x must be [T, H, D] or [Z, H, N, D], got {tuple(x.shape)}")
@@ -116,40 +166,32 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise NotImplementedError(f"x: fp32, fp16 and bf16 are implemented, got {x.dtype}")
     _same_device(x.device, positions=positions, inv_freq=inv_freq, out=out)
-    x = _dense_last(x)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype
+                            or (out.stride(-1) != 1 and out.shape[-1] > 1)):
         raise ValueError("out must be as x, with its last dimension contiguous")
+    N = x.shape[0] if x.dim() == 3 else x.shape[2]
+    if positions.shape != (N,) and (x.dim() == 3 or positions.shape != (x.shape[0], N)):
+        raise ValueError(f"positions must be [{N}]" + (f" or [{x.shape[0]}, {N}]" if x.dim() == 4
+                                                       else "") + f", got {tuple(positions.shape)}")
+
+
+def _rotary_plan(x, positions, inv_freq, interleaved, scale, inverse, out):
     xs, os_ = x.stride(), out.stride()
     if x.dim() == 3:
         (N, H, D), Z = x.shape, 1
-        if positions.shape != (N,):
-            raise ValueError(f"positions must be [{N}], got {tuple(positions.shape)}")
         st = (0, xs[0], xs[1], 0, os_[0], os_[1])
-        pos_sz = 0
     else:
         Z, H, N, D = x.shape
-        if positions.shape == (Z, N):
-            pos_sz = N
-        elif positions.shape == (N,):
-            pos_sz = 0
-        else:
-            raise ValueError(f"positions must be [{N}] or [{Z}, {N}], got {tuple(positions.shape)}")
         st = (xs[0], xs[2], xs[1], os_[0], os_[2], os_[1])
-    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    p = _plan("rotary", capi.RotaryDesc, capi.RotaryPlan,
-              (Z, N, H, D, 2 * inv_freq.shape[0], _tx_of(x.dtype), int(bool(interleaved)),
-               int(bool(inverse)), 8 * positions.element_size(), float(scale), 0, pos_sz) + st)
-    if stream is None:
-        stream = _current_stream(x.device)
-    capi.check(capi.load().tx_rotary_launch(ctypes.byref(p), x.data_ptr(), positions.data_ptr(),
-                                            inv_freq.data_ptr(), out.data_ptr(), stream))
-    return out
+    return ctypes.byref(_plan(
+        "rotary", capi.RotaryDesc, capi.RotaryPlan,
+        (Z, N, H, D, 2 * inv_freq.shape[0], _tx_of(x.dtype), int(bool(interleaved)),
+         int(bool(inverse)), 8 * positions.element_size(), float(scale), 0,
+         N if positions.dim() == 2 else 0) + st))
 
 
 def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, dtype):
-    """What paged_append and paged_attention ask alike; the index arrays, contiguous."""
+    """What paged_append and paged_attention ask alike."""
     import torch
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
         raise ValueError("k_cache and v_cache must share one [pages, page_size, Hkv, D] shape and "
@@ -172,7 +214,7 @@ def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, 
             page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table must be an int32 [sequences, entries] tensor with contiguous "
                          "rows")
-    kv_len = _int32(kv_len, "kv_len", 1)
+    _is_int32(kv_len, "kv_len", 1)
     B = kv_len.shape[0]
     if page_table.shape[0] != B:
         raise ValueError(f"page_table has {page_table.shape[0]} rows, kv_len {B}")
@@ -180,19 +222,17 @@ def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, 
         if T != B:
             raise ValueError(f"{T} new tokens of {B} sequences: give cu_q")
     else:
-        cu_q = _int32(cu_q, "cu_q", 1)
+        _is_int32(cu_q, "cu_q", 1)
         if cu_q.shape[0] != B + 1:
             raise ValueError(f"cu_q must be [{B + 1}], got {tuple(cu_q.shape)}")
-    return page_table, kv_len, cu_q
 
 
 def _tokens(t, name, heads, D, dtype, T):
-    """t [T, heads, D] with D contiguous."""
+    """Refuses t unless it is [T, heads, D]."""
     if t.dim() != 3 or tuple(t.shape) != (T, heads, D):
         raise ValueError(f"{name} must be [{T}, {heads}, {D}], got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    return _dense_last(t)
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=None, inv_freq=None,
@@ -207,6 +247,47 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     The pages must be there (page_reserve); a token without one is not written.  fp16 or
     bf16; a float8_e4m3fn cache holds k / k_scale[head] and v / v_scale[head] (fp32 [Hkv];
     None: 1), saturated.  Rows of q from cu_q[B] on come back as they are."""
+    form = ("append", _form(k), _form(v), _form(k_cache), _form(v_cache), _form(page_table),
+            _form(kv_len), _form(cu_q), _form(q), _form(inv_freq), bool(interleaved),
+            float(scale), _form(k_scale), _form(v_scale), _form(q_out))
+    found = _forms.get(form)
+    if found is None:
+        _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, k_scale,
+                       v_scale, q_out)
+        given = (k, v, kv_len, cu_q, q, inv_freq)
+        dense = tuple(None if t is None else f(t) for f, t in zip(
+            (_dense_last, _dense_last, _dense, _dense, _dense_last, _dense), given))
+        if any(a is not b for a, b in zip(dense, given)):  # copied, and the copies' form looked up
+            k, v, kv_len, cu_q, q, inv_freq = dense
+            return paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q=q,
+                                inv_freq=inv_freq, interleaved=interleaved, scale=scale,
+                                k_scale=k_scale, v_scale=v_scale, q_out=q_out, stream=stream)
+        T, Hkv, D = k.shape
+        Hq, q_st = 0, (0, 0, 0, 0)
+        if q is not None:
+            if q_out is None:
+                q_out = _new(q)
+            Hq, q_st = q.shape[1], q.stride()[:2] + q_out.stride()[:2]
+        found = _keep(form, ctypes.byref(_plan(
+            "paged_append", capi.PagedAppendDesc, capi.PagedAppendPlan,
+            (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D,
+             0 if inv_freq is None else 2 * inv_freq.shape[0], k_cache.shape[1], _tx_of(k.dtype),
+             _tx_of(k_cache.dtype), int(bool(interleaved)), int(cu_q is not None), float(scale))
+            + q_st + k.stride()[:2] + v.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
+            + (page_table.stride(0),))))
+    if q is not None and q_out is None:
+        q_out = _new(q)
+    rc = capi.load().tx_paged_append_launch(
+        found, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
+        v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(inv_freq),
+        _ptr(k_scale), _ptr(v_scale), _current_stream(k.device) if stream is None else stream)
+    if rc:
+        capi.check(rc)
+    return q_out
+
+
+def _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, k_scale, v_scale,
+                   q_out):
     import torch
     if k.dim() != 3:
         raise ValueError(f"k must be [T, Hkv, D], got {tuple(k.shape)}")
@@ -214,41 +295,21 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     dtype = k.dtype
     if dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"k: fp16 and bf16 are implemented, got {dtype}")
-    k, v = _dense_last(k), _tokens(v, "v", Hkv, D, dtype, T)
-    page_table, kv_len, cu_q = _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale,
-                                             v_scale, T, Hkv, D, dtype)
+    _tokens(v, "v", Hkv, D, dtype, T)
+    _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, dtype)
     _same_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
                  kv_len=kv_len, cu_q=cu_q, q=q, inv_freq=inv_freq, k_scale=k_scale,
                  v_scale=v_scale, q_out=q_out)
-    rot = 0
-    if inv_freq is not None:
-        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
-            raise ValueError("inv_freq must be an fp32 vector")
-        inv_freq = inv_freq.contiguous()
-        rot = 2 * inv_freq.shape[0]
-    Hq, q_st = 0, (0, 0, 0, 0)
-    if q is not None:
-        Hq = q.shape[1] if q.dim() == 3 else 0
-        q = _tokens(q, "q", Hq, D, dtype, T)
-        if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
-        elif q_out.shape != q.shape or q_out.dtype != dtype or (D > 1 and q_out.stride(2) != 1):
-            raise ValueError("q_out must be as q, with its last dimension contiguous")
-        q_st = q.stride()[:2] + q_out.stride()[:2]
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    p = _plan("paged_append", capi.PagedAppendDesc, capi.PagedAppendPlan,
-              (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D, rot,
-               k_cache.shape[1], _tx_of(dtype), _tx_of(k_cache.dtype), int(bool(interleaved)),
-               int(cu_q is not None), float(scale)) + q_st + k.stride()[:2] + v.stride()[:2]
-              + k_cache.stride()[:3] + v_cache.stride()[:3] + (page_table.stride(0),))
-    if stream is None:
-        stream = _current_stream(k.device)
-    capi.check(capi.load().tx_paged_append_launch(
-        ctypes.byref(p), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
-        v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(inv_freq),
-        _ptr(k_scale), _ptr(v_scale), stream))
-    return q_out
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1):
+        raise ValueError("inv_freq must be an fp32 vector")
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+        return
+    _tokens(q, "q", q.shape[1] if q.dim() == 3 else 0, D, dtype, T)
+    if q_out is not None and (q_out.shape != q.shape or q_out.dtype != dtype
+                              or (D > 1 and q_out.stride(2) != 1)):
+        raise ValueError("q_out must be as q, with its last dimension contiguous")
 
 
 def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_scale, causal=True,
@@ -264,40 +325,62 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     o [T, Hq, D], with return_lse also log2 of the sum of e^(score), fp32 [T, Hq] (-inf
     where nothing is attended to).  cu_q as for paged_append."""
     import torch
+    form = ("attention", _form(q), _form(k_cache), _form(v_cache), _form(page_table),
+            _form(kv_len), _form(cu_q), float(sm_scale), bool(causal), int(window), _form(k_scale), _form(v_scale),
+            _form(out))
+    found = _forms.get(form)
+    if found is None or q.data_ptr() % 16:
+        _attention_checks(q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, out)
+        s0, s1, s2 = q.stride()
+        qc = q
+        if q.shape[2] % 8 == 0 and (s2 != 1 or s0 % 8 or s1 % 8 or q.data_ptr() % 16):
+            qc = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
+        given = (kv_len, cu_q)
+        dense = (_dense(kv_len), None if cu_q is None else _dense(cu_q))
+        if qc is not q or dense[0] is not given[0] or dense[1] is not given[1]:
+            return paged_attention(qc, k_cache, v_cache, page_table, *dense, sm_scale=sm_scale,
+                                   causal=causal, window=window, k_scale=k_scale, v_scale=v_scale,
+                                   out=out, return_lse=return_lse, workspace=workspace,
+                                   stream=stream)
+        if out is None:
+            out = _new(q)
+        T, Hq, D = q.shape
+        p = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
+                  (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq,
+                   k_cache.shape[2], D, k_cache.shape[1], _tx_of(q.dtype), _tx_of(k_cache.dtype),
+                   int(bool(causal)), int(window), int(cu_q is not None), float(sm_scale))
+                  + q.stride()[:2] + out.stride()[:2] + k_cache.stride()[:3]
+                  + v_cache.stride()[:3] + (page_table.stride(0),))
+        found = _keep(form, (ctypes.byref(p), p))
+    if out is None:
+        out = _new(q)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    if stream is None:
+        stream = _current_stream(q.device)
+    ws = workspace if workspace is not None else workspace_for(found[1], q.device, stream)
+    rc = capi.load().tx_paged_attn_launch(
+        found[0], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+        kv_len.data_ptr(), _ptr(cu_q), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), _ptr(lse),
+        _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), stream)
+    if rc:
+        capi.check(rc)
+    return (out, lse) if return_lse else out
+
+
+def _attention_checks(q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, out):
+    import torch
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, D], got {tuple(q.shape)}")
     T, Hq, D = q.shape
     dtype = q.dtype
     if dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"q: fp16 and bf16 are implemented, got {dtype}")
-    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
-    page_table, kv_len, cu_q = _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale,
-                                             v_scale, T, Hkv, D, dtype)
+    _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T,
+                  k_cache.shape[2] if k_cache.dim() == 4 else 0, D, dtype)
     _same_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, kv_len=kv_len,
                  cu_q=cu_q, k_scale=k_scale, v_scale=v_scale, out=out)
-    s0, s1, s2 = q.stride()
-    if s2 != 1 or s0 % 8 or s1 % 8 or q.data_ptr() % 16:
-        q = torch.empty((T, Hq, D), dtype=dtype, device=q.device).copy_(q)
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1):
         raise ValueError("out must be as q, with its last dimension contiguous")
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    p = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
-              (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D,
-               k_cache.shape[1], _tx_of(dtype), _tx_of(k_cache.dtype), int(bool(causal)),
-               int(window), int(cu_q is not None), float(sm_scale)) + q.stride()[:2]
-              + out.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
-              + (page_table.stride(0),))
-    if stream is None:
-        stream = _current_stream(q.device)
-    ws = workspace if workspace is not None else workspace_for(p, q.device, stream)
-    capi.check(capi.load().tx_paged_attn_launch(
-        ctypes.byref(p), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(k_scale), _ptr(v_scale),
-        out.data_ptr(), _ptr(lse), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
-        stream))
-    return (out, lse) if return_lse else out
 
 
 # ---------------------------------------------------------------------------
@@ -317,61 +400,55 @@ def _page_bytes(t, name, P):
     return t.stride(0) * e, n * e
 
 
-def _caches(d, caches, P, device):
-    if len(caches) > capi.PAGE_CACHES:
-        raise ValueError(f"{len(caches)} caches: at most {capi.PAGE_CACHES} a call")
-    ptrs = (ctypes.c_void_p * max(len(caches), 1))()
-    d.caches = len(caches)
-    for i, t in enumerate(caches):
-        if t.device != device:
-            raise ValueError(f"cache {i} is on {t.device}, not on {device}")
-        d.stride[i], d.bytes[i] = _page_bytes(t, f"cache {i}", P)
-        ptrs[i] = t.data_ptr()
-    return ptrs
+def _pointers(caches):
+    return (ctypes.c_void_p * max(len(caches), 1))(*[t.data_ptr() for t in caches])
 
 
-def _books(page_table, kv_len, refs):
-    page_table, refs = _int32(page_table, "page_table", 2), _int32(refs, "refs", 1)
+_COUNTERS = 65536
+
+
+class _Pages:
+    """The descriptor of calls on pages, and what workspace_for asks of a plan: their scratch
+    memory.  The first 64 KiB of a workspace are the arrival counters of other launches."""
+
+    def __init__(self, caches, P, device, S=0, W=0, n=0, page_size=1):
+        if len(caches) > capi.PAGE_CACHES:
+            raise ValueError(f"{len(caches)} caches: at most {capi.PAGE_CACHES} a call")
+        d = self.desc = capi.PageDesc()
+        d.S, d.W, d.P, d.n, d.page_size, d.caches = S, W, P, n, page_size, len(caches)
+        for i, t in enumerate(caches):
+            if t.device != device:
+                raise ValueError(f"cache {i} is on {t.device}, not on {device}")
+            d.stride[i], d.bytes[i] = _page_bytes(t, f"cache {i}", P)
+        self.ref, need = ctypes.byref(d), ctypes.c_int64(0)
+        capi.check(capi.load().tx_page_workspace(self.ref, ctypes.byref(need)))
+        self.workspace_bytes = _COUNTERS + need.value
+
+    def scratch(self, device, stream):
+        return workspace_for(self, device, stream).data_ptr() + _COUNTERS
+
+
+def _book_checks(page_table, kv_len, refs, out, **more):
+    """Refuses books that do not go together; `more`: int32 vectors, `out` the books to write."""
+    _is_int32(page_table, "page_table", 2)
+    _is_int32(refs, "refs", 1)
     if kv_len is not None:
-        kv_len = _int32(kv_len, "kv_len", 1)
+        _is_int32(kv_len, "kv_len", 1)
         if kv_len.shape[0] != page_table.shape[0]:
             raise ValueError(f"page_table has {page_table.shape[0]} rows, kv_len "
                              f"{kv_len.shape[0]}")
-    _same_device(page_table.device, kv_len=kv_len, refs=refs)
-    d = capi.PageDesc()
-    (d.S, d.W), d.P = page_table.shape, refs.shape[0]
-    d.page_size = 1
-    return d, page_table, kv_len, refs
-
-
-def _new_books(out, *like):
-    """The books to write: `out`, checked, or new ones."""
-    import torch
+    for name, t in more.items():
+        _is_int32(t, name, 1)
+    _same_device(page_table.device, kv_len=kv_len, refs=refs, **more)
     if out is None:
-        return tuple(torch.empty_like(t) for t in like)
+        return
+    like = tuple(t for t in (page_table, kv_len, refs) if t is not None)
     if len(out) != len(like):
         raise ValueError(f"out must be {len(like)} tensors")
     for t, u in zip(out, like):
         if t.shape != u.shape or t.dtype != u.dtype or t.device != u.device or not t.is_contiguous():
             raise ValueError(f"out must be contiguous and as the books read: {tuple(t.shape)} "
                              f"{t.dtype} for {tuple(u.shape)} {u.dtype}")
-    return tuple(out)
-
-
-_COUNTERS = 65536
-
-
-class _Need:
-    """What workspace_for asks of a plan: the scratch memory of a call on pages.  The first
-    64 KiB of a workspace are the arrival counters of other launches."""
-
-    def __init__(self, d):
-        n = ctypes.c_int64(0)
-        capi.check(capi.load().tx_page_workspace(ctypes.byref(d), ctypes.byref(n)))
-        self.workspace_bytes = _COUNTERS + n.value
-
-    def scratch(self, device, stream):
-        return workspace_for(self, device, stream).data_ptr() + _COUNTERS
 
 
 def page_copy(caches, src, dst, *, stream=None):
@@ -383,15 +460,14 @@ def page_copy(caches, src, dst, *, stream=None):
         raise ValueError("src and dst must be of one length")
     if not caches:
         return
-    d = capi.PageDesc()
-    d.P, d.n, d.page_size = caches[0].shape[0], src.shape[0], 1
-    _same_device(src.device, dst=dst)
-    ptrs = _caches(d, caches, d.P, src.device)
-    _Need(d)
-    if stream is None:
-        stream = _current_stream(src.device)
-    capi.check(capi.load().tx_page_copy(ctypes.byref(d), ptrs, src.data_ptr(), dst.data_ptr(),
-                                        stream))
+    form = ("copy", _form(src), dst.device, *map(_form, caches))
+    found = _forms.get(form)
+    if found is None:
+        _same_device(src.device, dst=dst)
+        found = _keep(form, _Pages(caches, caches[0].shape[0], src.device, n=src.shape[0]))
+    capi.check(capi.load().tx_page_copy(
+        found.ref, _pointers(caches), src.data_ptr(), dst.data_ptr(),
+        _current_stream(src.device) if stream is None else stream))
 
 
 def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stream=None):
@@ -401,21 +477,30 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
     int32 scalar on the device; those entries are -1).  out: the three tensors to write,
     which may be those read."""
     import torch
-    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
-    new_len = _int32(new_len, "new_len", 1)
-    if new_len.shape != kv_len.shape:
-        raise ValueError("new_len must be as kv_len")
-    _same_device(refs.device, new_len=new_len)
-    d.page_size = page_size
-    t, n, r = _new_books(out, page_table, kv_len, refs)
-    missing = torch.empty((), dtype=torch.int32, device=refs.device)
-    need = _Need(d)
+    form = ("reserve", _form(page_table), _form(kv_len), _form(refs), _form(new_len), page_size,
+            None if out is None else tuple(map(_form, out)))
+    found = _forms.get(form)
+    if found is None:
+        _book_checks(page_table, kv_len, refs, out, new_len=new_len)
+        if new_len.shape != kv_len.shape:
+            raise ValueError("new_len must be as kv_len")
+        given = (page_table, kv_len, refs, new_len)
+        dense = tuple(map(_dense, given))
+        if any(a is not b for a, b in zip(dense, given)):
+            return page_reserve(*dense, page_size, out=out, stream=stream)
+        found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
+                                   page_size=page_size))
+    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    device = refs.device
+    missing = refs.new_empty(())
     if stream is None:
-        stream = _current_stream(refs.device)
-    capi.check(capi.load().tx_page_reserve(
-        ctypes.byref(d), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        stream = _current_stream(device)
+    rc = capi.load().tx_page_reserve(
+        found.ref, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
         new_len.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(), missing.data_ptr(),
-        need.scratch(refs.device, stream), stream))
+        found.scratch(device, stream), stream)
+    if rc:
+        capi.check(rc)
     return t, n, r, missing
 
 
@@ -425,27 +510,37 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
     to a free one.  Returns page_table, kv_len, refs and the missing pages, as page_reserve."""
     import torch
     caches = list(caches)
-    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
-    parent, child = _int32(parent, "parent", 1), _int32(child, "child", 1)
-    if parent.shape != child.shape:
-        raise ValueError("parent and child must be of one length")
-    if not caches:
-        raise ValueError("page_fork needs the caches: the size of a page is theirs")
-    _same_device(refs.device, parent=parent, child=child)
-    d.n, d.page_size = parent.shape[0], caches[0].shape[1]
-    ptrs = _caches(d, caches, d.P, refs.device)
-    for i, c in enumerate(caches):
-        if c.shape[1] != d.page_size:
-            raise ValueError(f"cache {i} has pages of {c.shape[1]} tokens, cache 0 of {d.page_size}")
-    t, n, r = _new_books(out, page_table, kv_len, refs)
-    missing = torch.empty((), dtype=torch.int32, device=refs.device)
-    need = _Need(d)
+    form = ("fork", _form(page_table), _form(kv_len), _form(refs), _form(parent), _form(child),
+            None if out is None else tuple(map(_form, out)), *map(_form, caches))
+    found = _forms.get(form)
+    if found is None:
+        _book_checks(page_table, kv_len, refs, out, parent=parent, child=child)
+        if parent.shape != child.shape:
+            raise ValueError("parent and child must be of one length")
+        if not caches:
+            raise ValueError("page_fork needs the caches: the size of a page is theirs")
+        given = (page_table, kv_len, refs, parent, child)
+        dense = tuple(map(_dense, given))
+        if any(a is not b for a, b in zip(dense, given)):
+            return page_fork(caches, *dense, out=out, stream=stream)
+        pages = _Pages(caches, refs.shape[0], refs.device, *page_table.shape, parent.shape[0],
+                       caches[0].shape[1])
+        for i, c in enumerate(caches):
+            if c.shape[1] != caches[0].shape[1]:
+                raise ValueError(f"cache {i} has pages of {c.shape[1]} tokens, cache 0 of "
+                                 f"{caches[0].shape[1]}")
+        found = _keep(form, pages)
+    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    device = refs.device
+    missing = refs.new_empty(())
     if stream is None:
-        stream = _current_stream(refs.device)
-    capi.check(capi.load().tx_page_fork(
-        ctypes.byref(d), ptrs, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        stream = _current_stream(device)
+    rc = capi.load().tx_page_fork(
+        found.ref, _pointers(caches), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
         parent.data_ptr(), child.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
-        missing.data_ptr(), need.scratch(refs.device, stream), stream))
+        missing.data_ptr(), found.scratch(device, stream), stream)
+    if rc:
+        capi.check(rc)
     return t, n, r, missing
 
 
@@ -453,19 +548,27 @@ def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=Non
     """Sequences with drop[s] (bool [S]) give their pages back and become empty.  Returns
     page_table, kv_len, refs; out as for page_reserve."""
     import torch
-    d, page_table, kv_len, refs = _books(page_table, kv_len, refs)
-    if drop.dtype not in (torch.bool, torch.uint8) or drop.shape != kv_len.shape:
-        raise ValueError("drop must be a bool tensor as long as kv_len")
-    drop = drop.contiguous()
-    _same_device(refs.device, drop=drop)
-    d.page_size = page_size
-    t, n, r = _new_books(out, page_table, kv_len, refs)
-    _Need(d)
-    if stream is None:
-        stream = _current_stream(refs.device)
-    capi.check(capi.load().tx_page_free(
-        ctypes.byref(d), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
-        drop.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(), stream))
+    form = ("free", _form(page_table), _form(kv_len), _form(refs), _form(drop), page_size,
+            None if out is None else tuple(map(_form, out)))
+    found = _forms.get(form)
+    if found is None:
+        _book_checks(page_table, kv_len, refs, out)
+        if drop.dtype not in (torch.bool, torch.uint8) or drop.shape != kv_len.shape:
+            raise ValueError("drop must be a bool tensor as long as kv_len")
+        _same_device(refs.device, drop=drop)
+        given = (page_table, kv_len, refs, drop)
+        dense = tuple(map(_dense, given))
+        if any(a is not b for a, b in zip(dense, given)):
+            return page_free(*dense, page_size, out=out, stream=stream)
+        found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
+                                   page_size=page_size))
+    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    rc = capi.load().tx_page_free(
+        found.ref, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
+        drop.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
+        _current_stream(refs.device) if stream is None else stream)
+    if rc:
+        capi.check(rc)
     return t, n, r
 
 
@@ -475,14 +578,23 @@ def page_compact(caches, page_table, refs, *, out=None, stream=None):
     page_table, refs and how many were moved (an int32 scalar on the device)."""
     import torch
     caches = list(caches)
-    d, page_table, _, refs = _books(page_table, None, refs)
-    ptrs = _caches(d, caches, d.P, refs.device)
-    t, r = _new_books(out, page_table, refs)
-    moved = torch.empty((), dtype=torch.int32, device=refs.device)
-    need = _Need(d)
+    form = ("compact", _form(page_table), _form(refs),
+            None if out is None else tuple(map(_form, out)), *map(_form, caches))
+    found = _forms.get(form)
+    if found is None:
+        _book_checks(page_table, None, refs, out)
+        dense = _dense(page_table), _dense(refs)
+        if dense[0] is not page_table or dense[1] is not refs:
+            return page_compact(caches, *dense, out=out, stream=stream)
+        found = _keep(form, _Pages(caches, refs.shape[0], refs.device, *page_table.shape))
+    t, r = (_new(page_table), _new(refs)) if out is None else out
+    device = refs.device
+    moved = refs.new_empty(())
     if stream is None:
-        stream = _current_stream(refs.device)
-    capi.check(capi.load().tx_page_compact(
-        ctypes.byref(d), ptrs, page_table.data_ptr(), refs.data_ptr(), t.data_ptr(), r.data_ptr(),
-        moved.data_ptr(), need.scratch(refs.device, stream), stream))
+        stream = _current_stream(device)
+    rc = capi.load().tx_page_compact(
+        found.ref, _pointers(caches), page_table.data_ptr(), refs.data_ptr(), t.data_ptr(),
+        r.data_ptr(), moved.data_ptr(), found.scratch(device, stream), stream)
+    if rc:
+        capi.check(rc)
     return t, r, moved
