@@ -443,7 +443,7 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   const int step = plan->variant ? 64 : 4 * splitBlock(D, f8);
   const double units = (double)d.B + (double)d.T * G / plan->rows;
   const double keys = (double)d.table_width * d.page_size;
-  const double steps = units * (keys / step + 1) * d.Hkv;
+  const double steps = units * (keys / step + 1 + (plan->variant ? kRowsOverhead : kSplitOverhead)) * d.Hkv;
   plan->units = (int32_t)std::min<double>(256 * per_cu, std::ceil(steps));
   plan->grid_x = plan->units;
   plan->slots = 2 * plan->units;

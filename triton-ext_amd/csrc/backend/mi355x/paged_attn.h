@@ -61,6 +61,9 @@ __device__ __forceinline__ void paged_lgkmcnt0() {
 __device__ __forceinline__ int lane_value(int v, int lane) {
   return __builtin_amdgcn_readlane(v, lane);
 }
+__device__ __forceinline__ int64_t lane_value64(int64_t v, int lane) {
+  return (int64_t)(uint32_t)lane_value((int)v, lane) | (int64_t)lane_value((int)(v >> 32), lane) << 32;
+}
 
 // ---------------------------------------------------------------------------
 // Fragments
@@ -263,8 +266,10 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   }
 
   // One block's softmax: s are its scores (times qk_scale > 0 they are base-2 exponents).
-  // Updates the row's maximum m (both lanes of a row hold the same), the lane's part of the sum
-  // l, and acc; p as MFMA operands.
+  // Updates the row's reference m (both lanes of a row hold the same), the lane's part of the sum
+  // l, and acc; p as MFMA operands.  m follows the row's maximum only when that has grown past
+  // it by 8, so acc is seldom rescaled; p is up to 2^8 then, in range in both types, and rounded by
+  // the same relative half step.
   __device__ __forceinline__ static void softmax(f16v (&s)[BN / 32], float qk_scale,
                                                  f16v (&acc)[D / 32], float &m, float &l,
                                                  h8 (&pf)[BN / 16]) {
@@ -274,10 +279,19 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         mx = fmaxf(mx, s[b][r]);
-    const float to = fmaxf(m, X::xmax(mx) * qk_scale);
-    const float base = to == -INFINITY ? 0.f : to;
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    m = to;
+    mx = X::xmax(mx) * qk_scale;
+    if (__builtin_expect(__any(mx > m + 8.f), 0)) {
+      const float to = mx > m + 8.f ? mx : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+      l *= alpha;
+#pragma unroll
+      for (int bd = 0; bd < D / 32; ++bd)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[bd][r] *= alpha;
+      m = to;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < BN / 32; ++b)
@@ -286,17 +300,12 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
         s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], qk_scale, -base));
         sum += s[b][r];
       }
-    l = l * alpha + sum;
+    l += sum;
 #pragma unroll
     for (int c = 0; c < BN / 16; ++c)
 #pragma unroll
       for (int t = 0; t < 8; ++t)
         pf[c][t] = (elt)s[c / 2][8 * (c % 2) + t];
-#pragma unroll
-    for (int bd = 0; bd < D / 32; ++bd)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        acc[bd][r] *= alpha;
   }
 };
 
@@ -350,13 +359,23 @@ struct PageSide {
   int run;
 };
 
+// 16 bytes a lane into LDS; NT: data that is read once.
+template <bool NT>
+__device__ __forceinline__ void paged_dma(uint32_t voff, const i32x4_t &rsrc, uint32_t lds) {
+  if constexpr (NT)
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds)
+                 : "memory");
+  else
+    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds)
+                 : "memory");
+}
+
 // Loads `first` .. first + U - 1 of the block of keys from n on into the tile at `lds`; rows
 // from `end` on come as zeros.
-template <class A, int U>
+template <class A, int U, bool NT>
 __device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd, int n, int end,
                                            int first, const uint32_t (&off)[U], uint32_t lds,
                                            int row_bytes) {
-  typedef AttnFwd<64, true, 32, 64> X;
   auto resource = [&](int key) {
     const int id = lane_value(pr.ids, ((key >> pr.shift) - pr.first) & 63);
     const int slot = key & ((1 << pr.shift) - 1);
@@ -374,7 +393,7 @@ __device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd
       const i32x4_t rsrc = resource(n + A::R * (first + U / N * i));
 #pragma unroll
       for (int u = U / N * i; u < U / N * (i + 1); ++u)
-        X::dma16(off[u], rsrc, 0, lds + (first + u) * 1024);
+        paged_dma<NT>(off[u], rsrc, lds + (first + u) * 1024);
     }
   };
   if (sd.run >= U * A::R)
@@ -391,7 +410,7 @@ __device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd
       for (int r0 = 0; r0 < A::R; r0 += sd.run) {
         const i32x4_t rsrc = resource(n + A::R * (first + u) + r0);
         if (sd.run >= A::R || (lr & ~(sd.run - 1)) == r0)
-          X::dma16(off[u], rsrc, 0, lds + (first + u) * 1024);
+          paged_dma<NT>(off[u], rsrc, lds + (first + u) * 1024);
       }
   }
 }
@@ -404,11 +423,15 @@ __device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd
 // row t0 of q and at position pos0, and of its steps those from s0 to s1.  Cut in parts,
 // this one is `part`; part j is that of workgroup w0 + j, in its first place of the workspace, but
 // part 0 in place slot0 (a workgroup's run has a cut unit at its beginning or at its end).
-struct PagedUnit {
+struct alignas(16) PagedUnit {
   int64_t pos0;
   int t0, r0, rows, hk, b, len, lo, hi; // keys [lo, hi)
   uint32_t s0, s1, parts, part, w0, slot0;
 };
+static_assert(sizeof(PagedUnit) == 64, "four 16-byte reads");
+
+// What a unit's beginning and end cost, in steps.
+constexpr uint32_t kSplitOverhead = 2, kRowsOverhead = 4;
 
 // The token of a row.
 __device__ __forceinline__ int paged_token(const PagedAttnArgs &p, int row) {
@@ -501,8 +524,7 @@ template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
     // sequences of many blocks of rows: a lane per block
     for (uint64_t big = __ballot(nr > 2 * BM); big; big &= big - 1) {
       const int from = __builtin_ctzll(big);
-      const int64_t at = (int64_t)(uint32_t)lane_value((int)pos0, from) |
-                         (int64_t)lane_value((int)(pos0 >> 32), from) << 32;
+      const int64_t at = lane_value64(pos0, from);
       const int ln = lane_value(len, from), rows = lane_value(nr, from);
       uint32_t c = 0;
       for (int k = lane; k * (int64_t)BM < rows; k += 64)
@@ -572,12 +594,14 @@ template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
     const uint32_t end = uniform(st.end), share = uniform(st.share);
     uint32_t pos = uniform(st.pos), s0 = uniform(st.s0);
     int cb = uniform(st.cb), b = uniform(st.b), hk = uniform(st.hk), rb = uniform(st.rb);
+    int my_n = st.n[lane], my_t0 = st.t0[lane], my_len = st.len[lane];
+    int64_t my_pos0 = st.pos0[lane];
     PagedUnit u;
     u.rows = 0;
     while (pos < end && u.rows == 0) {
-      const int i = b - cb, nr = uniform(st.n[i]) * p.G;
+      const int i = b - cb, nr = lane_value(my_n, i) * p.G;
       u.b = b, u.hk = hk;
-      u.t0 = st.t0[i], u.len = uniform(st.len[i]), u.pos0 = uniform64(st.pos0[i]);
+      u.t0 = lane_value(my_t0, i), u.len = lane_value(my_len, i), u.pos0 = lane_value64(my_pos0, i);
       u.r0 = rb * BM;
       const int rows = nr - u.r0 < BM ? nr - u.r0 : BM;
       paged_keys(p, u.pos0, u.len, u.r0, u.r0 + rows, u.lo, u.hi);
@@ -606,6 +630,7 @@ template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
           if (cb >= p.B)
             cb = 0, ++hk;
           later = __ballot((p.B > 64 ? load_chunk(cb) : st.cost[lane]) > 0);
+          my_n = st.n[lane], my_t0 = st.t0[lane], my_len = st.len[lane], my_pos0 = st.pos0[lane];
         }
         if (!later || hk >= p.Hkv)
           pos = end;
@@ -618,13 +643,20 @@ template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
 };
 
 // The unit as scalars.
-__device__ __forceinline__ PagedUnit paged_unit(const volatile PagedUnit &s) {
+__device__ __forceinline__ PagedUnit paged_unit(const PagedUnit &s) {
+  asm volatile("" ::: "memory"); // (read from LDS again)
+  i32x4_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = reinterpret_cast<const i32x4_t *>(&s)[i];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    v[i / 4][i % 4] = uniform(v[i / 4][i % 4]);
   PagedUnit u;
-  u.pos0 = uniform64(s.pos0);
-  u.t0 = uniform(s.t0), u.r0 = uniform(s.r0), u.rows = uniform(s.rows), u.hk = uniform(s.hk);
-  u.b = uniform(s.b), u.len = uniform(s.len), u.lo = uniform(s.lo), u.hi = uniform(s.hi);
-  u.s0 = uniform(s.s0), u.s1 = uniform(s.s1), u.parts = uniform(s.parts), u.part = uniform(s.part);
-  u.w0 = uniform(s.w0), u.slot0 = uniform(s.slot0);
+  u.pos0 = (int64_t)(uint32_t)v[0][0] | (int64_t)v[0][1] << 32;
+  u.t0 = v[0][2], u.r0 = v[0][3], u.rows = v[1][0], u.hk = v[1][1], u.b = v[1][2], u.len = v[1][3];
+  u.lo = v[2][0], u.hi = v[2][1], u.s0 = v[2][2], u.s1 = v[2][3];
+  u.parts = v[3][0], u.part = v[3][1], u.w0 = v[3][2], u.slot0 = v[3][3];
   return u;
 }
 
@@ -709,7 +741,7 @@ template <class A>
 __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
   constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024;
   typedef typename A::elt elt;
-  typedef PagedSched<32, BN, 4, 2> Sched;
+  typedef PagedSched<32, BN, 4, kSplitOverhead> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * A::TILE];
   __shared__ float ms[4][32], ls[4][32];
   __shared__ PagedSchedState st;
@@ -769,8 +801,8 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
     if (k0 < k1) {
       pr.settle();
       here = pr.template there<BN>(k0 * BN, un.hi);
-      issue_rows<A, U>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
-      issue_rows<A, U>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
+      issue_rows<A, U, true>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
+      issue_rows<A, U, true>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
     }
     if (wave == 0)
       Sched(p, st).get(st.unit[turn ^ 1]);
@@ -801,7 +833,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
         if (k + 1 < k1) {
           pr.hold(n0 + BN);
           next_here = pr.template there<BN>(n0 + BN, un.hi);
-          issue_rows<A, U>(pr, sk, n0 + BN, un.hi, 0, ko, k_lds, row_bytes);
+          issue_rows<A, U, true>(pr, sk, n0 + BN, un.hi, 0, ko, k_lds, row_bytes);
         }
         A::qk(kf, qf, s);
       }
@@ -826,7 +858,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
         if (b0 + VG == D / 32) {
           paged_lgkmcnt0();
           if (k + 1 < k1)
-            issue_rows<A, U>(pr, sv, n0 + BN, un.hi, 0, vo, v_lds, row_bytes);
+            issue_rows<A, U, true>(pr, sv, n0 + BN, un.hi, 0, vo, v_lds, row_bytes);
         }
         A::template pv<VG>(vf, b0, pf, acc);
       }
@@ -955,14 +987,17 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
 // ---------------------------------------------------------------------------
 
 // 128 rows a unit, 32 a wave (chunks of a prompt).  Iteration j holds S_j, computes S_{j+1}
-// beside the softmax of S_j, then adds P_j V_j; K and V have two LDS slots each, loaded one
-// block ahead, and one barrier a block.
+// beside the softmax of S_j, then adds P_j V_j.  K and V have NS LDS slots each, loaded NS blocks
+// ahead of S and NS - 1 ahead of P V, and one barrier a block.  Four slots where they fit (a block then
+// takes less time than a load from memory): mixed lengths with a window in heads of 64
+// 42 -> 33 us.
 template <class A>
 __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kernel(PagedAttnArgs args) {
   constexpr int D = A::D, BN = A::BN, U = A::TILE / 4096; // loads of a wave
+  constexpr int NS = A::TILE <= 8192 ? 4 : 2;
   typedef typename A::elt elt;
-  typedef PagedSched<128, BN, 1, 4> Sched;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * A::TILE];
+  typedef PagedSched<128, BN, 1, kRowsOverhead> Sched;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * NS * A::TILE];
   __shared__ PagedSchedState st;
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
@@ -976,7 +1011,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
   }
   __syncthreads();
 
-  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * A::TILE;
+  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + NS * A::TILE;
   typename A::Bases bs;
   A::bases(k_lds, v_lds, bs);
   uint32_t ko[U], vo[U];
@@ -985,6 +1020,8 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     ko[u] = A::template offset<false>(U * wave + u, (uint32_t)args.k_st, args.k_run, row_bytes);
     vo[u] = A::template offset<true>(U * wave + u, (uint32_t)args.v_st, args.v_run, row_bytes);
   }
+
+  const bool whole_loads = args.k_run >= A::R && args.v_run >= A::R;
 
   for (int turn = 0;; turn ^= 1) {
     const PagedAttnArgs &p = paged_args();
@@ -1001,12 +1038,12 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
     const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
-    uint64_t here[3] = {0, 0, 0}; // of blocks j, j + 1, j + 2
+    uint64_t here[NS + 1] = {}; // of blocks j .. j + NS
     auto issue_k = [&](int k, int slot) {
-      issue_rows<A, U>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
+      issue_rows<A, U, false>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
     };
     auto issue_v = [&](int k, int slot) {
-      issue_rows<A, U>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
+      issue_rows<A, U, false>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
     };
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
     // looks up the next unit.
@@ -1020,14 +1057,15 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
               p.head_dim, qf);
     if (k0 < k1) {
       pr.settle();
-      here[0] = pr.template there<BN>(k0 * BN, un.hi);
-      issue_k(k0, 0);
-      issue_v(k0, 0);
-      if (k0 + 1 < k1) {
-        pr.hold((k0 + 1) * BN);
-        here[1] = pr.template there<BN>((k0 + 1) * BN, un.hi);
-        issue_k(k0 + 1, 1);
-      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (k0 + i < k1) {
+          pr.hold((k0 + i) * BN);
+          here[i] = pr.template there<BN>((k0 + i) * BN, un.hi);
+          issue_k(k0 + i, i);
+          if (i < NS - 1)
+            issue_v(k0 + i, i);
+        }
     }
     if (wave == 0)
       Sched(p, st).get(st.unit[turn ^ 1]);
@@ -1059,17 +1097,18 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     __syncthreads(); // K slot 0 is loaded again
     auto iter = [&](int k, auto slot_c) {
       constexpr int SL = decltype(slot_c)::value;
-      if (k + 1 < k1)
-        issue_v(k + 1, 1 - SL);
-      if (k + 2 < k1) {
-        pr.hold((k + 2) * BN);
-        here[2] = pr.template there<BN>((k + 2) * BN, un.hi);
-        issue_k(k + 2, SL);
+      const bool ahead = k + NS < k1;
+      if (k + NS - 1 < k1)
+        issue_v(k + NS - 1, (SL + NS - 1) % NS);
+      if (ahead) {
+        pr.hold((k + NS) * BN);
+        here[NS] = pr.template there<BN>((k + NS) * BN, un.hi);
+        issue_k(k + NS, SL);
       }
       typename A::f16v sn[BN / 32];
       if (k + 1 < k1 && live(k + 1)) {
         typename A::KF kf;
-        A::read_k(bs, (1 - SL) * A::TILE, kf);
+        A::read_k(bs, (SL + 1) % NS * A::TILE, kf);
         A::qk(kf, qf, sn);
       }
       if (live(k)) {
@@ -1094,17 +1133,27 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
 #pragma unroll
       for (int b2 = 0; b2 < BN / 32; ++b2)
         s[b2] = sn[b2];
-      here[0] = here[1], here[1] = here[2];
-      paged_vmcnt<0>();
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        here[i] = here[i + 1];
+      // K_{k+2} and V_{k+1} have landed: NS - 2 iterations' loads came after them
+      if (whole_loads && ahead)
+        paged_vmcnt<2 * U * (NS - 2)>();
+      else
+        paged_vmcnt<0>();
       __syncthreads();
     };
-    int k = k0;
-    for (; k + 1 < k1; k += 2) {
-      iter(k, std::integral_constant<int, 0>());
-      iter(k + 1, std::integral_constant<int, 1>());
+    for (int k = k0; k < k1;) {
+      iter(k++, std::integral_constant<int, 0>());
+      if (k < k1)
+        iter(k++, std::integral_constant<int, 1>());
+      if constexpr (NS == 4) {
+        if (k < k1)
+          iter(k++, std::integral_constant<int, 2>());
+        if (k < k1)
+          iter(k++, std::integral_constant<int, 3>());
+      }
     }
-    if (k < k1)
-      iter(k, std::integral_constant<int, 0>());
 
     l = A::X::xsum(l);
     const PagedAttnArgs &pe = paged_args();
