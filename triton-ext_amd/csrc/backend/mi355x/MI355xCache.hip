@@ -379,7 +379,7 @@ int attnDims(int head_dim) {
   return head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
 }
 // Keys of a block in the split form: tiles of 8 KiB (4: e4m3 heads of 64; 16: heads of 256).
-int splitBlock(int D, bool f8) { return f8 || D == 64 ? 64 : 32; }
+int splitBlock(int D, bool f8) { return f8 && (D > 128 || D == 64) ? 64 : 32; }
 
 // Rows of a page that one buffer resource covers: as many as divide a page and the rows
 // that a wave loads, with 31-bit offsets.

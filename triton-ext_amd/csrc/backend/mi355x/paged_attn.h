@@ -733,20 +733,23 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // Few rows: the waves of a workgroup share out the keys
 // ---------------------------------------------------------------------------
 
+// LDS tiles that a wave has for K and for V.
+template <class A> constexpr int paged_split_slots() { return A::TILE <= 4096 ? 2 : 1; }
+
 // 32 rows a unit (decoding, some drafted tokens).  Every wave goes through its own run of
 // blocks, K and V each in one LDS tile of its own that is loaded again as soon as its
 // fragments are in registers, with no barrier; at the end the four join in LDS.  Bound by
 // memory: 8 waves a CU keep up to 16 KiB each in flight.
 template <class A>
-__global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
-  constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024;
+__global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
+  constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024, NS = paged_split_slots<A>();
   typedef typename A::elt elt;
   typedef PagedSched<32, BN, 4, kSplitOverhead> Sched;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * A::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * NS * A::TILE];
   __shared__ float ms[4][32], ls[4][32];
   __shared__ PagedSchedState st;
   __shared__ int flag;
-  static_assert(D * 128 <= 2 * A::TILE, "a wave's sums fit its tiles");
+  static_assert(D * 128 <= 2 * NS * A::TILE, "a wave's sums fit its tiles");
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row_bytes = args.head_dim * A::ESZ;
@@ -758,7 +761,7 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
   }
   __syncthreads();
 
-  const uint32_t k_lds = lds_addr(smem[wave]), v_lds = k_lds + A::TILE;
+  const uint32_t k_lds = lds_addr(smem[wave]), v_lds = k_lds + NS * A::TILE;
   typename A::Bases bs;
   A::bases(k_lds, v_lds, bs);
   uint32_t ko[U], vo[U];
@@ -797,12 +800,18 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
     typename A::QF qf;
     A::load_q(static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh,
               p.head_dim, qf);
-    uint64_t here = 0, next_here = 0;
+    uint64_t here[NS + 1] = {}; // of blocks k .. k + NS
     if (k0 < k1) {
       pr.settle();
-      here = pr.template there<BN>(k0 * BN, un.hi);
-      issue_rows<A, U, true>(pr, sk, k0 * BN, un.hi, 0, ko, k_lds, row_bytes);
-      issue_rows<A, U, true>(pr, sv, k0 * BN, un.hi, 0, vo, v_lds, row_bytes);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (k0 + i < k1) {
+          const int n = (k0 + i) * BN;
+          pr.hold(n);
+          here[i] = pr.template there<BN>(n, un.hi);
+          issue_rows<A, U, true>(pr, sk, n, un.hi, 0, ko, k_lds + i * A::TILE, row_bytes);
+          issue_rows<A, U, true>(pr, sv, n, un.hi, 0, vo, v_lds + i * A::TILE, row_bytes);
+        }
     }
     if (wave == 0)
       Sched(p, st).get(st.unit[turn ^ 1]);
@@ -820,49 +829,59 @@ __global__ void __launch_bounds__(256, A::TILE > 8192 ? 1 : 2) paged_attn_split_
 #pragma unroll
     for (int bd = 0; bd < D / 32; ++bd)
       acc[bd] = typename A::f16v{};
-    for (int k = k0; k < k1; ++k) {
-      const int n0 = k * BN;
-      if (whole_loads)
-        paged_vmcnt<U>();
+    auto iter = [&](int k, auto slot_c) {
+      constexpr int SL = decltype(slot_c)::value;
+      const int n0 = k * BN, na = n0 + NS * BN;
+      const bool ahead = k + NS < k1;
+      if (whole_loads && k + NS <= k1)
+        paged_vmcnt<(2 * NS - 1) * U>(); // all after K_k
       else
         paged_vmcnt<0>();
       {
         typename A::KF kf;
-        A::read_k(bs, 0, kf);
+        A::read_k(bs, SL * A::TILE, kf);
         paged_lgkmcnt0();
-        if (k + 1 < k1) {
-          pr.hold(n0 + BN);
-          next_here = pr.template there<BN>(n0 + BN, un.hi);
-          issue_rows<A, U, true>(pr, sk, n0 + BN, un.hi, 0, ko, k_lds, row_bytes);
+        if (ahead) {
+          pr.hold(na);
+          here[NS] = pr.template there<BN>(na, un.hi);
+          issue_rows<A, U, true>(pr, sk, na, un.hi, 0, ko, k_lds + SL * A::TILE, row_bytes);
         }
         A::qk(kf, qf, s);
       }
       typename A::h8 pf[BN / 16];
       const uint64_t all = ~0ull >> (64 - BN);
-      if (here != all || n0 < lo_all || n0 + BN > hi_all) {
+      if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
         const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
         uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
         seen &= a < 64 ? ~0ull << a : 0;
-        A::mask(s, seen & here);
+        A::mask(s, seen & here[0]);
       }
       A::softmax(s, scale, acc, m, l, pf);
-      if (whole_loads && k + 1 < k1)
-        paged_vmcnt<U>();
+      if (whole_loads && ahead)
+        paged_vmcnt<(2 * NS - 1) * U>(); // all after V_k
       else
         paged_vmcnt<0>();
       constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
 #pragma unroll
       for (int b0 = 0; b0 < D / 32; b0 += VG) {
         typename A::template VF<VG> vf;
-        A::template read_v<VG>(bs, 0, b0, vf);
+        A::template read_v<VG>(bs, SL * A::TILE, b0, vf);
         if (b0 + VG == D / 32) {
           paged_lgkmcnt0();
-          if (k + 1 < k1)
-            issue_rows<A, U, true>(pr, sv, n0 + BN, un.hi, 0, vo, v_lds, row_bytes);
+          if (ahead)
+            issue_rows<A, U, true>(pr, sv, na, un.hi, 0, vo, v_lds + SL * A::TILE, row_bytes);
         }
         A::template pv<VG>(vf, b0, pf, acc);
       }
-      here = next_here;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        here[i] = here[i + 1];
+    };
+    for (int k = k0; k < k1;) {
+      iter(k++, std::integral_constant<int, 0>());
+      if constexpr (NS == 2)
+        if (k < k1)
+          iter(k++, std::integral_constant<int, 1>());
     }
 
     // The waves' sums: quads of 4 dims in lane order in each one's own tiles (all its loads
