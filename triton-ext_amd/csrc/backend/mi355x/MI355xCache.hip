@@ -16,7 +16,7 @@ using namespace txk;
 namespace txk {
 typedef void (*PagedAttnFn)(PagedAttnArgs);
 // [64, 96, 128, 256 dims][bf16][e4m3 cache] (kernels_paged_*.hip)
-extern const PagedAttnFn kPagedAttnSplit[4][2][2], kPagedAttnRows[4][2][2];
+extern const PagedAttnFn kPagedAttnSplit16[4][2][2], kPagedAttnSplit[4][2][2], kPagedAttnRows[4][2][2];
 } // namespace txk
 
 namespace {
@@ -378,8 +378,10 @@ constexpr int64_t kAttnCounters = 65536; // the arrival counters that every work
 int attnDims(int head_dim) {
   return head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128 : 256;
 }
-// Keys of a block in the split form: tiles of 8 KiB (4: e4m3 heads of 64; 16: heads of 256).
-int splitBlock(int D, bool f8) { return f8 && (D > 128 || D == 64) ? 64 : 32; }
+// Forms of the kernel, by the rows of a unit: 16, 32 (the waves of a workgroup share out the keys,
+// in blocks of 32), 128 (they share the keys, in blocks of 64).
+enum { kAttn16 = 0, kAttn32 = 1, kAttn128 = 2 };
+constexpr int kSplitBlock = 32;
 
 // Rows of a page that one buffer resource covers: as many as divide a page and the rows
 // that a wave loads, with 31-bit offsets.
@@ -431,19 +433,22 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   plan->block_threads = 256;
   if (d.T == 0)
     return TX_OK;
-  // Up to 32 rows a sequence of one kv head: units of 32, their keys shared out among waves
-  // (memory bounds both forms there); more: units of 128.
-  const int64_t G = d.Hq / d.Hkv;
-  plan->variant = d.T * G > 32 * d.B;
-  plan->rows = plan->variant ? 128 : 32;
+  // The fewer rows a sequence has on average, the less of a unit's matrix and softmax work is
+  // for nothing; memory bounds the calls of few rows, whichever form.
+  const int64_t G = d.Hq / d.Hkv, rows = d.T * G;
+  plan->variant = rows <= 16 * d.B ? kAttn16 : rows <= 32 * d.B ? kAttn32 : kAttn128;
+  plan->rows = plan->variant == kAttn16 ? 16 : plan->variant == kAttn32 ? 32 : 128;
   const int D = attnDims(d.head_dim);
   const bool f8 = d.cache_type == TX_F8E4M3;
-  const int per_cu = D > 128 ? 1 : 2;
+  // workgroups that a CU has place for (64 KiB of LDS, 256 registers a lane)
+  const bool one = D > 128 && !(plan->variant == kAttn16 && f8);
+  const int per_cu = one ? 1 : 2;
   // the most steps of work there can be (a step: the keys a workgroup takes at a time)
-  const int step = plan->variant ? 64 : 4 * splitBlock(D, f8);
+  const bool split = plan->variant != kAttn128;
+  const int step = split ? 4 * kSplitBlock : 64;
   const double units = (double)d.B + (double)d.T * G / plan->rows;
   const double keys = (double)d.table_width * d.page_size;
-  const double steps = units * (keys / step + 1 + (plan->variant ? kRowsOverhead : kSplitOverhead)) * d.Hkv;
+  const double steps = units * (keys / step + 1 + (split ? kSplitOverhead : kRowsOverhead)) * d.Hkv;
   plan->units = (int32_t)std::min<double>(256 * per_cu, std::ceil(steps));
   plan->grid_x = plan->units;
   plan->slots = 2 * plan->units;
@@ -512,13 +517,14 @@ extern "C" TX_API int tx_paged_attn_launch(const tx_paged_attn_plan *plan, const
   a.T = (int32_t)d.T, a.B = (int32_t)d.B, a.G = d.Hq / d.Hkv, a.Hq = d.Hq, a.Hkv = d.Hkv;
   a.head_dim = d.head_dim, a.page_shift = log2of(d.page_size);
   a.causal = d.causal, a.window = d.window;
-  const int wave_rows = plan->variant ? 16 : splitBlock(D, f8);
+  const int wave_rows = plan->variant == kAttn128 ? 16 : kSplitBlock;
   a.k_run = runOf(wave_rows, d.page_size, a.k_st, d.head_dim * ce);
   a.v_run = runOf(wave_rows, d.page_size, a.v_st, d.head_dim * ce);
   a.qk_scale = d.sm_scale * 1.44269504f;
   const PagedAttnFn fn =
-      (plan->variant ? kPagedAttnRows
-                     : kPagedAttnSplit)[D == 64 ? 0 : D == 96 ? 1 : D == 128 ? 2 : 3]
+      (plan->variant == kAttn16 ? kPagedAttnSplit16
+       : plan->variant == kAttn32 ? kPagedAttnSplit
+                                  : kPagedAttnRows)[D == 64 ? 0 : D == 96 ? 1 : D == 128 ? 2 : 3]
                                        [d.dtype == TX_BF16][f8];
   hipLaunchKernelGGL(fn, dim3(plan->grid_x), dim3(plan->block_threads), 0,
                      static_cast<hipStream_t>(stream), a);

@@ -1,4 +1,4 @@
-// Table of the paged attention's kernels, few rows a sequence (paged_attn.h).
+// Table of the paged attention's kernels, up to 32 rows a sequence (paged_attn.h).
 
 #include "paged_attn.h"
 
@@ -8,13 +8,21 @@ typedef void (*PagedAttnFn)(PagedAttnArgs);
 extern const PagedAttnFn kPagedAttnSplit[4][2][2];
 // [64, 96, 128, 256 dims][bf16][e4m3 cache]
 const PagedAttnFn kPagedAttnSplit[4][2][2] = {
-    {{paged_attn_split_kernel<PagedFrag<64, false, false, 32>>, paged_attn_split_kernel<PagedFrag<64, false, true, 64>>},
-     {paged_attn_split_kernel<PagedFrag<64, true, false, 32>>, paged_attn_split_kernel<PagedFrag<64, true, true, 64>>}},
-    {{paged_attn_split_kernel<PagedFrag<96, false, false, 32>>, paged_attn_split_kernel<PagedFrag<96, false, true, 32>>},
-     {paged_attn_split_kernel<PagedFrag<96, true, false, 32>>, paged_attn_split_kernel<PagedFrag<96, true, true, 32>>}},
-    {{paged_attn_split_kernel<PagedFrag<128, false, false, 32>>, paged_attn_split_kernel<PagedFrag<128, false, true, 32>>},
-     {paged_attn_split_kernel<PagedFrag<128, true, false, 32>>, paged_attn_split_kernel<PagedFrag<128, true, true, 32>>}},
-    {{paged_attn_split_kernel<PagedFrag<256, false, false, 32>>, paged_attn_split_kernel<PagedFrag<256, false, true, 64>>},
-     {paged_attn_split_kernel<PagedFrag<256, true, false, 32>>, paged_attn_split_kernel<PagedFrag<256, true, true, 64>>}}};
+    {{paged_attn_split_kernel<PagedFrag<64, false, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<64, false, true, 32>>},
+     {paged_attn_split_kernel<PagedFrag<64, true, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<64, true, true, 32>>}},
+    {{paged_attn_split_kernel<PagedFrag<96, false, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<96, false, true, 32>>},
+     {paged_attn_split_kernel<PagedFrag<96, true, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<96, true, true, 32>>}},
+    {{paged_attn_split_kernel<PagedFrag<128, false, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<128, false, true, 32>>},
+     {paged_attn_split_kernel<PagedFrag<128, true, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<128, true, true, 32>>}},
+    {{paged_attn_split_kernel<PagedFrag<256, false, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<256, false, true, 32>>},
+     {paged_attn_split_kernel<PagedFrag<256, true, false, 32>>,
+      paged_attn_split_kernel<PagedFrag<256, true, true, 32>>}}};
 
 } // namespace txk

@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t lane_value64(int64_t v, int lane) {
 // lies at c ^ swizzle(r), so that the rows of one ds_read_b128 or transposed read fall on
 // different banks.
 template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
-  static constexpr int D = D_, BN = BN_;
+  static constexpr int D = D_, BN = BN_, ROWS = 32;
   static constexpr bool F8 = F8_;
   static constexpr int ESZ = F8 ? 1 : 2;
   static constexpr int ROW = (D == 96 ? 128 : D) * ESZ, TILE = BN * ROW, CPR = ROW / 16;
@@ -173,18 +173,22 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
       qf.v[c] = *reinterpret_cast<const h8 *>(static_cast<const elt *>(row) + (d < head_dim ? d : 0));
     }
   }
+  __device__ __forceinline__ static h8 settled(const h8 &q, bool live, float scale) {
+    i32x4_t x = __builtin_bit_cast(i32x4_t, q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = live && scale != 0.f ? x[i] ^ (scale < 0.f ? (int)0x80008000 : 0) : 0;
+    return __builtin_bit_cast(h8, x);
+  }
   __device__ __forceinline__ static void settle_q(bool live, int head_dim, float scale, QF &qf) {
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const bool in = live && q_dim(c) < head_dim && scale != 0.f;
-      i32x4_t x = __builtin_bit_cast(i32x4_t, qf.v[c]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = in ? x[i] ^ (scale < 0.f ? (int)0x80008000 : 0) : 0;
-      qf.v[c] = __builtin_bit_cast(h8, x);
-    }
+    for (int c = 0; c < D / 16; ++c)
+      qf.v[c] = settled(qf.v[c], live && q_dim(c) < head_dim, scale);
   }
 
+  typedef f16v Scores[BN / 32];
+  typedef f16v Acc[D / 32];
+  typedef h8 PF[BN / 16];
   // K fragments of the tile at byte `at`.
   struct KF {
     i32x4_t v[BN / 32][NK];
@@ -216,10 +220,10 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   template <int N> struct VF {
     i32x4_t v[N][BN / 16]; // e4m3: .xy
   };
-  template <int N>
-  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<N> &vf) {
+  static constexpr int VN = NV < 4 ? NV : NV % 4 ? 3 : 4; // dim blocks read together
+  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<VN> &vf) {
 #pragma unroll
-    for (int bd = 0; bd < N; ++bd)
+    for (int bd = 0; bd < VN; ++bd)
 #pragma unroll
       for (int c = 0; c < BN / 16; ++c) {
         const uint32_t a = bs.v[b0 + bd] + at + c * 16 * ROW;
@@ -236,11 +240,9 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
         }
       }
   }
-  template <int N>
-  __device__ __forceinline__ static void pv(const VF<N> &vf, int b0, const h8 (&pf)[BN / 16],
-                                            f16v (&acc)[D / 32]) {
+  __device__ __forceinline__ static void pv(const VF<VN> &vf, int b0, const PF &pf, Acc &acc) {
 #pragma unroll
-    for (int bd = 0; bd < N; ++bd)
+    for (int bd = 0; bd < VN; ++bd)
 #pragma unroll
       for (int c = 0; c < BN / 16; ++c) {
         h8 x;
@@ -306,6 +308,229 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
 #pragma unroll
       for (int t = 0; t < 8; ++t)
         pf[c][t] = (elt)s[c / 2][8 * (c % 2) + t];
+  }
+  __device__ __forceinline__ static float row_sum(float v) { return X::xsum(v); }
+  // acc as quads of 4 dims; where quad qd (dims 4 qd ..) of a row lies among them.
+  typedef float f4v __attribute__((ext_vector_type(4)));
+  static constexpr int QUADS = D / 8;
+  __device__ __forceinline__ static f4v quad(const Acc &acc, int q) {
+    return f4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1], acc[q / 4][4 * (q % 4) + 2],
+               acc[q / 4][4 * (q % 4) + 3]};
+  }
+  __device__ __forceinline__ static int quad_at(int row, int qd) {
+    return (qd >> 1) * 64 + row + 32 * (qd & 1);
+  }
+};
+
+// The same on 16 rows a wave (decoding): 16x16x32 MFMAs, half the matrix and softmax work of 32 rows.
+// Lane l holds of S^T row l%16 and keys 4 (l/16) + r of each 16; P's operand of 32 keys is those of
+// two such blocks, and V's rows are read in that order.
+template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag16 {
+  typedef PagedFrag<D_, BF, F8_, BN_> P32;
+  static constexpr int D = D_, BN = BN_, ROWS = 16;
+  static constexpr bool F8 = F8_;
+  static constexpr int ESZ = P32::ESZ, ROW = P32::ROW, TILE = P32::TILE, CPR = P32::CPR, R = P32::R;
+  typedef typename P32::X X;
+  typedef typename X::elt elt;
+  typedef typename X::h8 h8;
+  typedef typename X::h4 h4;
+  typedef float f4v __attribute__((ext_vector_type(4)));
+
+  __device__ __forceinline__ static f4v mfma(const h8 &a, const h8 &b, const f4v &c) {
+    if constexpr (BF)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  // A transposed read takes 16 rows x 32 bytes a half wave (keys 0-7), e4m3 16 rows (keys 0-7 and
+  // 16-23) x 16 bytes.
+  __device__ __forceinline__ static int vswz(int r) {
+    if constexpr (F8)
+      return ROW == 64    ? ((r >> 2) & 1) | ((r >> 3) & 2)
+             : ROW == 128 ? ((r >> 1) & 3) | ((r >> 2) & 4)
+                          : (r & 7) | ((r >> 1) & 8);
+    else
+      return ROW == 128 ? 2 * ((r >> 1) & 3) : 2 * (r & 7);
+  }
+  template <bool V>
+  __device__ __forceinline__ static uint32_t offset(int u, uint32_t st, int run, int row_bytes) {
+    const int lane = threadIdx.x & 63, row = R * u + lane / CPR, pos = lane % CPR;
+    const int c = pos ^ (V ? vswz(row) : P32::kswz(row));
+    return 16 * c >= row_bytes ? P32::kOOB : (uint32_t)(row & (run - 1)) * st + 16 * c;
+  }
+
+  //   K: key l%16, 16-byte chunk 4 c + l/16: dims 32 c + 8 (l/16) .. of MFMA c, or (e4m3) dims
+  //     64 c + 16 (l/16) .., 8 each of MFMAs 2 c and 2 c + 1 (96 dims: as 128, with zeros);
+  //   V, dim block bd of 16: 16-bit keys 4 (l/16) + (l%16)/4 (and 16 further); e4m3 keys
+  //     4 (l/16) + 0..3 and + 16..19 by (l%16)/2.
+  static constexpr int NK = F8 ? (D + 63) / 64 : D / 32, NQF = F8 ? 2 * NK : NK, NV = D / 16;
+  struct Bases {
+    uint32_t k[NK], v[NV];
+  };
+  __device__ __forceinline__ static void bases(uint32_t k_lds, uint32_t v_lds, Bases &bs) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+      bs.k[c] = k_lds + r * ROW + (((4 * c + g) ^ P32::kswz(r)) << 4);
+#pragma unroll
+    for (int bd = 0; bd < NV; ++bd) {
+      if constexpr (F8) {
+        const int j = r >> 1, key = 4 * g + (j & 3) + 16 * (j >> 2);
+        bs.v[bd] = v_lds + key * ROW + ((bd ^ vswz(key)) << 4) + 8 * (r & 1);
+      } else {
+        const int d = 16 * bd + 4 * (r & 3), key = 4 * g + (r >> 2);
+        bs.v[bd] = v_lds + key * ROW + (((d >> 3) ^ vswz(key)) << 4) + (d & 7) * 2;
+      }
+    }
+  }
+
+  struct QF {
+    h8 v[NQF];
+  };
+  __device__ __forceinline__ static int q_dim(int c) {
+    const int g = (threadIdx.x & 63) >> 4;
+    return F8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
+  }
+  __device__ __forceinline__ static void load_q(const void *row, int head_dim, QF &qf) {
+#pragma unroll
+    for (int c = 0; c < NQF; ++c) {
+      const int d = q_dim(c);
+      qf.v[c] = *reinterpret_cast<const h8 *>(static_cast<const elt *>(row) + (d < head_dim ? d : 0));
+    }
+  }
+  __device__ __forceinline__ static void settle_q(bool live, int head_dim, float scale, QF &qf) {
+#pragma unroll
+    for (int c = 0; c < NQF; ++c)
+      qf.v[c] = P32::settled(qf.v[c], live && q_dim(c) < head_dim, scale);
+  }
+
+  typedef f4v Scores[BN / 16];
+  typedef f4v Acc[D / 16];
+  struct KF {
+    i32x4_t v[BN / 16][NK];
+  };
+  __device__ __forceinline__ static void read_k(const Bases &bs, int at, KF &kf) {
+    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
+#pragma unroll
+    for (int b = 0; b < BN / 16; ++b)
+#pragma unroll
+      for (int c = 0; c < NK; ++c)
+        kf.v[b][c] = *(const lds_i32x4 *)(uintptr_t)(bs.k[c] + at + b * 16 * ROW);
+  }
+  __device__ __forceinline__ static void qk(const KF &kf, const QF &qf, Scores &s) {
+#pragma unroll
+    for (int b = 0; b < BN / 16; ++b)
+      s[b] = f4v{};
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int b = 0; b < BN / 16; ++b) { // independent sums side by side
+        if constexpr (F8) {
+          s[b] = mfma(P32::widen(kf.v[b][c][0], kf.v[b][c][1]), qf.v[2 * c], s[b]);
+          s[b] = mfma(P32::widen(kf.v[b][c][2], kf.v[b][c][3]), qf.v[2 * c + 1], s[b]);
+        } else {
+          s[b] = mfma(__builtin_bit_cast(h8, kf.v[b][c]), qf.v[c], s[b]);
+        }
+      }
+  }
+  template <int N> struct VF {
+    i32x4_t v[N][BN / 32]; // e4m3: .xy
+  };
+  static constexpr int VN = NV < 8 ? NV : NV % 8 ? 6 : 8; // dim blocks read together
+  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<VN> &vf) {
+#pragma unroll
+    for (int bd = 0; bd < VN; ++bd)
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) {
+        const uint32_t a = bs.v[b0 + bd] + at + c * 32 * ROW;
+        if constexpr (F8) {
+          typedef __attribute__((address_space(3))) typename P32::i32x2 lds_i32x2;
+          const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(uintptr_t)a);
+          vf.v[bd][c][0] = x[0], vf.v[bd][c][1] = x[1];
+        } else {
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)a);
+          const i16x4_t hi =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)(a + 16 * ROW));
+          vf.v[bd][c] =
+              __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      }
+  }
+  typedef h8 PF[BN / 32];
+  __device__ __forceinline__ static void pv(const VF<VN> &vf, int b0, const PF &pf, Acc &acc) {
+#pragma unroll
+    for (int c = 0; c < BN / 32; ++c)
+#pragma unroll
+      for (int bd = 0; bd < VN; ++bd) {
+        h8 x;
+        if constexpr (F8)
+          x = P32::widen(vf.v[bd][c][0], vf.v[bd][c][1]);
+        else
+          x = __builtin_bit_cast(h8, vf.v[bd][c]);
+        acc[b0 + bd] = mfma(x, pf[c], acc[b0 + bd]);
+      }
+  }
+  __device__ __forceinline__ static void mask(Scores &s, uint64_t seen) {
+    const uint64_t mine = seen >> (4 * ((threadIdx.x & 63) >> 4));
+#pragma unroll
+    for (int b = 0; b < BN / 16; ++b) {
+      const uint32_t w = (uint32_t)(mine >> (16 * b));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        s[b][r] = (w >> r) & 1 ? s[b][r] : -INFINITY;
+    }
+  }
+  // Across the lanes of a row (l%16).
+  __device__ __forceinline__ static float row_max(float v) {
+    v = X::xmax(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  __device__ __forceinline__ static float row_sum(float v) {
+    v = X::xsum(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  // As PagedFrag's.
+  __device__ __forceinline__ static void softmax(Scores &s, float qk_scale, Acc &acc, float &m,
+                                                 float &l, PF &pf) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < BN / 16; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        mx = fmaxf(mx, s[b][r]);
+    mx = row_max(mx) * qk_scale;
+    if (__builtin_expect(__any(mx > m + 8.f), 0)) {
+      const float to = mx > m + 8.f ? mx : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+      l *= alpha;
+#pragma unroll
+      for (int bd = 0; bd < NV; ++bd)
+        acc[bd] *= alpha;
+      m = to;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < BN / 16; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], qk_scale, -base));
+        sum += s[b][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int c = 0; c < BN / 32; ++c)
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        pf[c][t] = (elt)s[2 * c + t / 4][t % 4];
+  }
+  // acc as quads of 4 dims; where quad qd (dims 4 qd ..) of a row lies among them.
+  static constexpr int QUADS = D / 16;
+  __device__ __forceinline__ static f4v quad(const Acc &acc, int q) { return acc[q]; }
+  __device__ __forceinline__ static int quad_at(int row, int qd) {
+    return (qd >> 2) * 64 + row + 16 * (qd & 3);
   }
 };
 
@@ -733,24 +958,31 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // Few rows: the waves of a workgroup share out the keys
 // ---------------------------------------------------------------------------
 
-// LDS tiles that a wave has for K and for V.
-template <class A> constexpr int paged_split_slots() { return A::TILE <= 4096 ? 2 : 1; }
+// LDS tiles that a wave has for K and for V: 16 KiB in all, or as much as its sums fill.
+template <class A> constexpr int paged_split_slots() {
+  constexpr int want = A::ROWS * A::D * 4 > 16384 ? A::ROWS * A::D * 4 : 16384;
+  return want / (2 * A::TILE) > 0 ? want / (2 * A::TILE) : 1;
+}
+// 64 KiB of tiles leave a CU place for two workgroups.
+template <class A> constexpr int paged_split_groups() {
+  return 8 * paged_split_slots<A>() * A::TILE <= 65536 ? 2 : 1;
+}
 
-// 32 rows a unit (decoding, some drafted tokens).  Every wave goes through its own run of
+// 16 or 32 rows a unit (decoding, some drafted tokens).  Every wave goes through its own run of
 // blocks, K and V each in one LDS tile of its own that is loaded again as soon as its
 // fragments are in registers, with no barrier; at the end the four join in LDS.  Bound by
 // memory: 8 waves a CU keep up to 16 KiB each in flight.
 template <class A>
-__global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kernel(PagedAttnArgs args) {
-  constexpr int D = A::D, BN = A::BN, U = A::TILE / 1024, NS = paged_split_slots<A>();
+__global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split_kernel(PagedAttnArgs args) {
+  constexpr int D = A::D, BN = A::BN, ROWS = A::ROWS, U = A::TILE / 1024, NS = paged_split_slots<A>();
   typedef typename A::elt elt;
-  typedef PagedSched<32, BN, 4, kSplitOverhead> Sched;
+  typedef PagedSched<ROWS, BN, 4, kSplitOverhead> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4][2 * NS * A::TILE];
-  __shared__ float ms[4][32], ls[4][32];
+  __shared__ float ms[4][ROWS], ls[4][ROWS];
   __shared__ PagedSchedState st;
   __shared__ int flag;
-  static_assert(D * 128 <= 2 * NS * A::TILE, "a wave's sums fit its tiles");
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  static_assert(ROWS * D * 4 <= 2 * NS * A::TILE, "a wave's sums fit its tiles");
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row_bytes = args.head_dim * A::ESZ;
 
@@ -795,7 +1027,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
     // looks up the next unit.
     if (k0 < k1)
       pr.load(k0 * BN);
-    const int r = lane & 31, rr = un.r0 + (r < un.rows ? r : 0);
+    const int r = lane % ROWS, rr = un.r0 + (r < un.rows ? r : 0);
     const int of = paged_token(p, rr), head = un.hk * p.G + rr - of * p.G;
     typename A::QF qf;
     A::load_q(static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh,
@@ -825,10 +1057,8 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
     A::settle_q(r < un.rows, p.head_dim, scale, qf);
     scale = scale == 0.f ? 1.f : fabsf(scale);
     float m = -INFINITY, l = 0.f;
-    typename A::f16v acc[D / 32], s[BN / 32];
-#pragma unroll
-    for (int bd = 0; bd < D / 32; ++bd)
-      acc[bd] = typename A::f16v{};
+    typename A::Acc acc = {};
+    typename A::Scores s;
     auto iter = [&](int k, auto slot_c) {
       constexpr int SL = decltype(slot_c)::value;
       const int n0 = k * BN, na = n0 + NS * BN;
@@ -848,7 +1078,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
         }
         A::qk(kf, qf, s);
       }
-      typename A::h8 pf[BN / 16];
+      typename A::PF pf;
       const uint64_t all = ~0ull >> (64 - BN);
       if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
         const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
@@ -861,17 +1091,16 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
         paged_vmcnt<(2 * NS - 1) * U>(); // all after V_k
       else
         paged_vmcnt<0>();
-      constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
 #pragma unroll
-      for (int b0 = 0; b0 < D / 32; b0 += VG) {
-        typename A::template VF<VG> vf;
-        A::template read_v<VG>(bs, SL * A::TILE, b0, vf);
-        if (b0 + VG == D / 32) {
+      for (int b0 = 0; b0 < A::NV; b0 += A::VN) {
+        typename A::template VF<A::VN> vf;
+        A::read_v(bs, SL * A::TILE, b0, vf);
+        if (b0 + A::VN == A::NV) {
           paged_lgkmcnt0();
           if (ahead)
             issue_rows<A, U, true>(pr, sv, na, un.hi, 0, vo, v_lds + SL * A::TILE, row_bytes);
         }
-        A::template pv<VG>(vf, b0, pf, acc);
+        A::pv(vf, b0, pf, acc);
       }
 #pragma unroll
       for (int i = 0; i < NS; ++i)
@@ -879,29 +1108,33 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
     };
     for (int k = k0; k < k1;) {
       iter(k++, std::integral_constant<int, 0>());
-      if constexpr (NS == 2)
+      if constexpr (NS >= 2)
         if (k < k1)
           iter(k++, std::integral_constant<int, 1>());
+      if constexpr (NS == 4) {
+        if (k < k1)
+          iter(k++, std::integral_constant<int, 2>());
+        if (k < k1)
+          iter(k++, std::integral_constant<int, 3>());
+      }
     }
 
     // The waves' sums: quads of 4 dims in lane order in each one's own tiles (all its loads
     // have landed).
-    l = A::X::xsum(l);
+    l = A::row_sum(l);
     const PagedAttnArgs &pe = paged_args();
     const PagedUnit ue = paged_unit(st.unit[turn]);
     const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
     if (k0 < k1) {
 #pragma unroll
-      for (int q = 0; q < D / 8; ++q)
-        *reinterpret_cast<f32x4v *>(smem[wave] + (q * 64 + lane) * 16) =
-            f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
-                   acc[q / 4][4 * (q % 4) + 2], acc[q / 4][4 * (q % 4) + 3]};
+      for (int q = 0; q < A::QUADS; ++q)
+        *reinterpret_cast<f32x4v *>(smem[wave] + (q * 64 + lane) * 16) = A::quad(acc, q);
     }
-    if (g == 0)
-      ms[wave][lane & 31] = m, ls[wave][lane & 31] = l;
+    if (lane < ROWS)
+      ms[wave][lane] = m, ls[wave][lane] = l;
     __syncthreads();
     const int dq = pe.head_dim / 4, items = ue.rows * dq;
-    const int64_t part_bytes = 32 * (D + 2) * 4;
+    const int64_t part_bytes = ROWS * (D + 2) * 4;
     uint8_t *const unit_parts = pe.parts;
     auto part_at = [&](uint32_t j) {
       const uint64_t slot = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
@@ -931,7 +1164,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
       for (int wv = 0; wv < 4; ++wv)
         paged_join(mm, ll, x, ms[wv][row], ls[wv][row],
                    *reinterpret_cast<const f32x4v *>(
-                       smem[wv] + ((qd >> 1) * 64 + row + 32 * (qd & 1)) * 16));
+                       smem[wv] + A::quad_at(row, qd) * 16));
       if (ue.parts == 1) {
         finish(row, qd, mm, ll, x);
       } else {
@@ -939,10 +1172,10 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4_t, x), mine,
                                                (row * D + 4 * qd) * 4, 0, kSC1);
         if (qd == 0) {
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), mine, (32 * D + row) * 4, 0,
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), mine, (ROWS * D + row) * 4, 0,
                                                 kSC1);
           __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(ll), mine,
-                                                (32 * D + 32 + row) * 4, 0, kSC1);
+                                                (ROWS * D + ROWS + row) * 4, 0, kSC1);
         }
       }
     }
@@ -971,9 +1204,9 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_split_kern
             const int at = (int)(slot * part_bytes);
             px[j] = __builtin_bit_cast(
                 i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, at + (row * D + 4 * qd) * 4, 0, kSC1));
-            pm[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, at + (32 * D + row) * 4, 0, kSC1));
+            pm[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + row) * 4, 0, kSC1));
             pl[j] = __int_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(all, at + (32 * D + 32 + row) * 4, 0, kSC1));
+                __builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + ROWS + row) * 4, 0, kSC1));
           }
         }
 #pragma unroll
@@ -1141,12 +1374,11 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
           A::mask(s, seen & here[0]);
         }
         A::softmax(s, scale, acc, m, l, pf);
-        constexpr int VG = D / 32 < 4 ? D / 32 : D / 32 % 4 ? 3 : 4;
 #pragma unroll
-        for (int b0 = 0; b0 < D / 32; b0 += VG) {
-          typename A::template VF<VG> vf;
-          A::template read_v<VG>(bs, SL * A::TILE, b0, vf);
-          A::template pv<VG>(vf, b0, pf, acc);
+        for (int b0 = 0; b0 < A::NV; b0 += A::VN) {
+          typename A::template VF<A::VN> vf;
+          A::read_v(bs, SL * A::TILE, b0, vf);
+          A::pv(vf, b0, pf, acc);
         }
       }
 #pragma unroll
