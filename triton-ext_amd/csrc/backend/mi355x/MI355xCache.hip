@@ -53,14 +53,18 @@ int commonVec(int most, std::initializer_list<int64_t> n) {
   return v;
 }
 
-// Threads that share a token's heads: enough to give every CU 8 waves (64 x 8 x 256
-// threads), fewer where the tokens alone do; each goes through 4 heads at least
-// where there are tokens enough, since a thread's sines cost about what two heads do.
+// Threads that share a token's heads: enough to give every CU 32 waves (256 x 32 x 64
+// threads), fewer where the tokens alone do, since a thread's sines cost about what two heads do.
 int headLanes(int64_t tokens, int64_t items, int64_t heads) {
-  const int64_t want = 64 * 8 * 256;
+  const int64_t want = 256 * 32 * 64;
   int64_t lanes = cdiv(want, std::max<int64_t>(tokens * items, 1));
-  lanes = std::max<int64_t>(lanes, 1);
+  // (a batch of heads each)
+  lanes = std::max<int64_t>(std::min(lanes, cdiv(heads, tokens * items * heads > want ? kHeadBatch : 1)), 1);
   return (int)std::min<int64_t>(lanes, std::max<int64_t>(heads, 1));
+}
+// Workgroups of 256 for tokens of so many threads (RotaryPlace).
+int64_t tokenGrid(int64_t tokens, int64_t token_threads) {
+  return token_threads <= 256 ? cdiv(tokens, 256 / token_threads) : tokens * cdiv(token_threads, 256);
 }
 
 // Items of a head (rotary.h): runs of `vec` elements or pairs of them.
@@ -128,13 +132,14 @@ extern "C" TX_API int tx_rotary_plan_create(const tx_rotary_desc *desc, tx_rotar
   plan->vec = commonVec(vecOf(most, d.head_dim, d.rot_dim, d.interleaved),
                         {d.x_sz, d.x_sn, d.x_sh, d.o_sz, d.o_sn, d.o_sh});
   const int64_t items = itemsOf(d.head_dim, d.rot_dim, plan->vec, d.interleaved);
-  plan->head_lanes = headLanes(d.Z * d.N, items, d.H);
+  plan->head_lanes = (int)std::min<int64_t>(headLanes(d.Z * d.N, items, d.H), 65535);
   plan->block_threads = 256;
-  const int64_t threads = d.H == 0 ? 0 : d.Z * d.N * items * plan->head_lanes;
-  // (a base that is less aligned than vec runs at vec 1: 16 times the threads at most)
-  if (cdiv(threads * 16, 256) > INT32_MAX)
+  const bool token_fast = d.x_sh > d.x_sn && d.N > 1;
+  const int64_t per = token_fast ? items : items * plan->head_lanes;
+  // (a base that is less aligned than vec runs at vec 1, with 16 times the threads at most)
+  if (tokenGrid(d.Z * d.N, per) * 32 > INT32_MAX || items * plan->head_lanes > INT32_MAX / 32)
     return fail(TX_ERR_UNSUPPORTED, "grid above 2^31");
-  plan->grid_x = (int32_t)cdiv(threads, 256);
+  plan->grid_x = d.H == 0 ? 0 : (int32_t)tokenGrid(d.Z * d.N, per);
   return TX_OK;
 }
 
@@ -162,11 +167,10 @@ extern "C" TX_API int tx_rotary_launch(const tx_rotary_plan *plan, const void *x
   if (!tx_device_available())
     return fail(TX_ERR_NO_DEVICE, "no gfx950 device visible");
   int vec = plan->vec, lanes = plan->head_lanes;
-  int64_t grid = plan->grid_x;
   if (!aligned(x, vec * e) || !aligned(out, vec * e)) {
     vec = 1;
-    lanes = headLanes(d.Z * d.N, itemsOf(d.head_dim, d.rot_dim, 1, d.interleaved), d.H);
-    grid = cdiv(d.Z * d.N * itemsOf(d.head_dim, d.rot_dim, 1, d.interleaved) * lanes, 256);
+    lanes = (int)std::min<int64_t>(
+        headLanes(d.Z * d.N, itemsOf(d.head_dim, d.rot_dim, 1, d.interleaved), d.H), 65535);
   }
   RotaryArgs a;
   a.x = x, a.pos = positions, a.inv_freq = inv_freq, a.out = out;
@@ -175,6 +179,8 @@ extern "C" TX_API int tx_rotary_launch(const tx_rotary_plan *plan, const void *x
   a.o_sz = d.o_sz, a.o_sn = d.o_sn, a.o_sh = d.o_sh;
   a.H = (int32_t)d.H, a.head_dim = d.head_dim, a.rot = d.rot_dim;
   a.items = itemsOf(d.head_dim, d.rot_dim, vec, d.interleaved);
+  a.token_fast = d.x_sh > d.x_sn && d.N > 1;
+  a.token_threads = a.token_fast ? a.items : a.items * lanes;
   a.head_lanes = lanes, a.pos64 = d.pos_bits == 64, a.inverse = d.inverse, a.scale = d.scale;
   void (*fn[2][4])(RotaryArgs) = {};
   if (d.dtype == TX_F32)
@@ -183,7 +189,9 @@ extern "C" TX_API int tx_rotary_launch(const tx_rotary_plan *plan, const void *x
     rotaryKernels<_Float16>(fn);
   else
     rotaryKernels<__bf16>(fn);
-  hipLaunchKernelGGL(fn[d.interleaved][log2of(vec)], dim3((uint32_t)grid), dim3(256), 0,
+  const int64_t grid = tokenGrid(d.Z * d.N, a.token_threads);
+  hipLaunchKernelGGL(fn[d.interleaved][log2of(vec)],
+                     dim3((uint32_t)grid, a.token_fast ? (uint32_t)lanes : 1), dim3(256), 0,
                      static_cast<hipStream_t>(stream), a);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;
@@ -277,10 +285,10 @@ extern "C" TX_API int tx_paged_append_plan_create(const tx_paged_append_desc *de
   const int64_t heads = (int64_t)d.Hq + 2 * (int64_t)d.Hkv;
   plan->head_lanes = headLanes(d.T, items, heads);
   plan->block_threads = 256;
-  const int64_t threads = heads == 0 ? 0 : d.T * items * plan->head_lanes;
-  if (cdiv(threads * 16, 256) > INT32_MAX || heads > INT32_MAX)
+  const int64_t per = items * plan->head_lanes;
+  if (tokenGrid(d.T, per) * 32 > INT32_MAX || per > INT32_MAX / 32 || heads > INT32_MAX)
     return fail(TX_ERR_UNSUPPORTED, "grid above 2^31");
-  plan->grid_x = (int32_t)cdiv(threads, 256);
+  plan->grid_x = heads == 0 ? 0 : (int32_t)tokenGrid(d.T, per);
   return TX_OK;
 }
 
@@ -318,7 +326,6 @@ extern "C" TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, c
       return fail(TX_ERR_INVALID, "index, frequency and scale arrays must be 4-byte aligned");
   const void *tok[4] = {q, k, v, q_out};
   int vec = plan->vec, lanes = plan->head_lanes;
-  int64_t grid = plan->grid_x;
   bool whole = aligned(k_cache, vec * ce) && aligned(v_cache, vec * ce);
   for (const void *p : tok) {
     if (!aligned(p, 2))
@@ -332,9 +339,7 @@ extern "C" TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, c
   const int64_t heads = (int64_t)d.Hq + 2 * (int64_t)d.Hkv;
   if (!whole) {
     vec = 1;
-    const int64_t items = itemsOf(d.head_dim, d.rot_dim, 1, d.interleaved);
-    lanes = headLanes(d.T, items, heads);
-    grid = cdiv(d.T * items * lanes, 256);
+    lanes = headLanes(d.T, itemsOf(d.head_dim, d.rot_dim, 1, d.interleaved), heads);
   }
   AppendArgs a;
   a.q = q, a.k = k, a.v = v, a.q_out = q_out;
@@ -349,6 +354,7 @@ extern "C" TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, c
   a.vc_sp = d.vc_sp, a.vc_st = d.vc_st, a.vc_sh = d.vc_sh;
   a.B = (int32_t)d.B, a.Hq = d.Hq, a.Hkv = d.Hkv, a.head_dim = d.head_dim, a.rot = d.rot_dim;
   a.items = itemsOf(d.head_dim, d.rot_dim, vec, d.interleaved);
+  a.token_threads = a.items * lanes;
   a.head_lanes = lanes, a.page_shift = log2of(d.page_size), a.scale = d.scale;
   void (*fn[2][4])(AppendArgs);
   const bool f8 = d.cache_type == TX_F8E4M3;
@@ -360,7 +366,8 @@ extern "C" TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, c
     appendKernels<__bf16, uint8_t>(fn);
   else
     appendKernels<__bf16, __bf16>(fn);
-  hipLaunchKernelGGL(fn[d.interleaved][log2of(vec)], dim3((uint32_t)grid), dim3(256), 0,
+  hipLaunchKernelGGL(fn[d.interleaved][log2of(vec)],
+                     dim3((uint32_t)tokenGrid(d.T, a.token_threads)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), a);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;

@@ -9,7 +9,8 @@
 // elements of each half of the rotated part (halves layout), VEC adjacent elements
 // (interleaved), or VEC elements past rot_dim, which are copied.  So it forms its
 // VEC (or VEC / 2) sines once and goes through the token's heads, every
-// head_lanes-th of them.  Bound by memory: 16-byte loads and stores.
+// head_lanes-th of them, kHeadBatch at a time: their 16-byte loads are all under way before
+// the first store.  Bound by memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -26,6 +27,7 @@ struct RotaryArgs {
   const float *inv_freq;
   void *out;
   int64_t N, tokens; // tokens: Z * N
+  int32_t token_threads, token_fast; // RotaryPlace
   int64_t pos_sz, x_sz, x_sn, x_sh, o_sz, o_sn, o_sh;
   int32_t H, head_dim, rot, items, head_lanes, pos64, inverse;
   float scale;
@@ -41,7 +43,34 @@ struct AppendArgs {
   int64_t q_st, q_sh, o_st, o_sh, k_st, k_sh, v_st, v_sh;
   int64_t kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh;
   int32_t B, Hq, Hkv, head_dim, rot, items, head_lanes, page_shift;
+  int32_t token_threads;
   float scale;
+};
+
+constexpr int kHeadBatch = 4; // heads that a thread has under way
+
+// What a thread does: `item` of heads lane, lane + head_lanes, .. of a token.  A token has
+// token_threads = items x head_lanes threads, items fastest; a workgroup of 256 has whole tokens, or
+// a token whole workgroups.  token_fast (heads further apart than tokens): token_threads =
+// items, and the lane is blockIdx.y.
+struct RotaryPlace {
+  int64_t tok;
+  int item, lane;
+  __device__ __forceinline__ RotaryPlace(uint32_t token_threads, uint32_t items, bool token_fast) {
+    uint32_t in;
+    if (token_threads <= 256) {
+      const uint32_t per = 256 / token_threads, t = threadIdx.x / token_threads;
+      tok = t < per ? (int64_t)blockIdx.x * per + t : INT64_MAX;
+      in = threadIdx.x - t * token_threads;
+    } else {
+      const uint32_t blocks = (token_threads + 255) / 256, t = blockIdx.x / blocks;
+      in = (blockIdx.x - t * blocks) * 256 + threadIdx.x;
+      tok = in < token_threads ? (int64_t)t : INT64_MAX;
+    }
+    const uint32_t l = in / items;
+    item = in - l * items;
+    lane = token_fast ? blockIdx.y : l;
+  }
 };
 
 __device__ __forceinline__ float elt_to_f32(float x) { return x; }
@@ -51,13 +80,6 @@ __device__ __forceinline__ float elt_to_f32(__bf16 x) { return (float)x; }
 template <class T, int VEC> struct alignas(sizeof(T) * VEC) EltVec {
   T v[VEC];
 };
-template <class T, int VEC>
-__device__ __forceinline__ void load_f32(const T *p, float (&f)[VEC]) {
-  const EltVec<T, VEC> r = *reinterpret_cast<const EltVec<T, VEC> *>(p);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    f[i] = elt_to_f32(r.v[i]);
-}
 template <class T, int VEC>
 __device__ __forceinline__ void store_f32(T *p, const float (&f)[VEC]) {
   EltVec<T, VEC> r;
@@ -106,13 +128,18 @@ template <int VEC, bool INTER> struct RotaryItem {
         c[i] = 1.f, s[i] = 0.f;
     }
   }
-  // Loads the item of one head and rotates it (or not): y1 goes to `at`, y2 to `second`.
+  // The item of one head, and rotated (or not): y1 goes to `at`, y2 to `second`.
   template <class T>
-  __device__ __forceinline__ void apply(const T *head, bool rot_it, float (&y1)[VEC],
-                                        float (&y2)[VEC]) const {
-    load_f32<T, VEC>(head + at, y1);
-    if (second >= 0)
-      load_f32<T, VEC>(head + second, y2);
+  __device__ __forceinline__ void load(const T *head, EltVec<T, VEC> &x1, EltVec<T, VEC> &x2) const {
+    x1 = *reinterpret_cast<const EltVec<T, VEC> *>(head + at);
+    x2 = *reinterpret_cast<const EltVec<T, VEC> *>(head + (second >= 0 ? second : at));
+  }
+  template <class T>
+  __device__ __forceinline__ void apply(const EltVec<T, VEC> &x1, const EltVec<T, VEC> &x2,
+                                        bool rot_it, float (&y1)[VEC], float (&y2)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      y1[i] = elt_to_f32(x1.v[i]), y2[i] = elt_to_f32(x2.v[i]);
     if (!rotate || !rot_it)
       return;
     if constexpr (INTER && VEC > 1) {
@@ -135,27 +162,36 @@ template <int VEC, bool INTER> struct RotaryItem {
 
 template <class T, int VEC, bool INTER>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs p) {
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int item = (int)(idx % p.items);
-  const int64_t rest = idx / p.items;
-  const int lane = (int)(rest % p.head_lanes);
-  const int64_t tok = rest / p.head_lanes;
+  const RotaryPlace at(p.token_threads, p.items, p.token_fast);
+  const int64_t tok = at.tok;
   if (tok >= p.tokens)
     return;
-  const int64_t z = tok / p.N, n = tok % p.N;
+  const int64_t z = p.tokens == p.N ? 0 : tok / p.N, n = tok - z * p.N;
   const int64_t pi = z * p.pos_sz + n;
   const double pos = p.pos64 ? (double)static_cast<const int64_t *>(p.pos)[pi]
                              : (double)static_cast<const int32_t *>(p.pos)[pi];
-  const RotaryItem<VEC, INTER> it(item, p.rot, pos, p.inv_freq, p.scale, p.inverse);
+  const RotaryItem<VEC, INTER> it(at.item, p.rot, pos, p.inv_freq, p.scale, p.inverse);
   const T *x = static_cast<const T *>(p.x) + z * p.x_sz + n * p.x_sn;
   T *o = static_cast<T *>(p.out) + z * p.o_sz + n * p.o_sn;
-  for (int h = lane; h < p.H; h += p.head_lanes) {
-    float y1[VEC], y2[VEC];
-    it.template apply<T>(x + h * p.x_sh, true, y1, y2);
-    T *oh = o + h * p.o_sh;
-    store_f32<T, VEC>(oh + it.at, y1);
-    if (it.second >= 0)
-      store_f32<T, VEC>(oh + it.second, y2);
+  for (int h0 = at.lane; h0 < p.H; h0 += kHeadBatch * p.head_lanes) {
+    EltVec<T, VEC> x1[kHeadBatch], x2[kHeadBatch];
+#pragma unroll
+    for (int k = 0; k < kHeadBatch; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      it.template load<T>(x + (h < p.H ? h : h0) * p.x_sh, x1[k], x2[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeadBatch; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      if (h >= p.H)
+        break;
+      float y1[VEC], y2[VEC];
+      it.template apply<T>(x1[k], x2[k], true, y1, y2);
+      T *oh = o + h * p.o_sh;
+      store_f32<T, VEC>(oh + it.at, y1);
+      if (it.second >= 0)
+        store_f32<T, VEC>(oh + it.second, y2);
+    }
   }
 }
 
@@ -195,11 +231,8 @@ __device__ __forceinline__ void store_cache(uint8_t *head, int at, const float (
 // C: T, or uint8_t for e4m3.  Heads in the order q, k, v.
 template <class T, class C, int VEC, bool INTER>
 __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs p) {
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int item = (int)(idx % p.items);
-  const int64_t rest = idx / p.items;
-  const int lane = (int)(rest % p.head_lanes);
-  const int64_t t = rest / p.head_lanes;
+  const RotaryPlace at(p.token_threads, p.items, false);
+  const int64_t t = at.tok;
   if (t >= p.T)
     return;
   // Token t's sequence b, position and place in the cache (page < 0: none).
@@ -221,32 +254,46 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs p) {
       page = -1;
   }
   const int64_t slot = pos & ((1 << p.page_shift) - 1);
-  const RotaryItem<VEC, INTER> it(item, p.rot, (double)pos, p.inv_freq, p.scale, false);
-  const int heads = p.Hq + 2 * p.Hkv;
-  for (int h = lane; h < heads; h += p.head_lanes) {
-    float y1[VEC], y2[VEC];
-    if (h < p.Hq) {
-      it.template apply<T>(static_cast<const T *>(p.q) + t * p.q_st + h * p.q_sh, mine, y1, y2);
-      T *o = static_cast<T *>(p.q_out) + t * p.o_st + h * p.o_sh;
-      store_f32<T, VEC>(o + it.at, y1);
-      if (it.second >= 0)
-        store_f32<T, VEC>(o + it.second, y2);
-      continue;
+  const RotaryItem<VEC, INTER> it(at.item, p.rot, (double)pos, p.inv_freq, p.scale, false);
+  // (a token without a page: its q alone)
+  const int heads = page < 0 ? p.Hq : p.Hq + 2 * p.Hkv;
+  for (int h0 = at.lane; h0 < heads; h0 += kHeadBatch * p.head_lanes) {
+    EltVec<T, VEC> x1[kHeadBatch], x2[kHeadBatch];
+#pragma unroll
+    for (int k = 0; k < kHeadBatch; ++k) {
+      const int hh = h0 + k * p.head_lanes, h = hh < heads ? hh : h0;
+      const bool is_q = h < p.Hq, is_k = h < p.Hq + p.Hkv;
+      const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
+      const T *src = is_q   ? static_cast<const T *>(p.q) + t * p.q_st + h * p.q_sh
+                     : is_k ? static_cast<const T *>(p.k) + t * p.k_st + hk * p.k_sh
+                            : static_cast<const T *>(p.v) + t * p.v_st + hk * p.v_sh;
+      it.template load<T>(src, x1[k], x2[k]);
     }
-    if (page < 0)
-      return; // (the heads after this one are k's and v's too)
-    const bool is_k = h < p.Hq + p.Hkv;
-    const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
-    const T *src = is_k ? static_cast<const T *>(p.k) + t * p.k_st + hk * p.k_sh
-                        : static_cast<const T *>(p.v) + t * p.v_st + hk * p.v_sh;
-    it.template apply<T>(src, is_k, y1, y2);
-    const float *sc = is_k ? p.k_scale : p.v_scale;
-    const float scale = sc ? sc[hk] : 1.f;
-    uint8_t *dst = is_k ? p.kc + (page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh) * sizeof(C)
-                        : p.vc + (page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh) * sizeof(C);
-    store_cache<T, C, VEC>(dst, it.at, y1, scale);
-    if (it.second >= 0)
-      store_cache<T, C, VEC>(dst, it.second, y2, scale);
+#pragma unroll
+    for (int k = 0; k < kHeadBatch; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      if (h >= heads)
+        break;
+      float y1[VEC], y2[VEC];
+      if (h < p.Hq) {
+        it.template apply<T>(x1[k], x2[k], mine, y1, y2);
+        T *o = static_cast<T *>(p.q_out) + t * p.o_st + h * p.o_sh;
+        store_f32<T, VEC>(o + it.at, y1);
+        if (it.second >= 0)
+          store_f32<T, VEC>(o + it.second, y2);
+        continue;
+      }
+      const bool is_k = h < p.Hq + p.Hkv;
+      const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
+      it.template apply<T>(x1[k], x2[k], is_k, y1, y2);
+      const float *sc = is_k ? p.k_scale : p.v_scale;
+      const float scale = sc ? sc[hk] : 1.f;
+      uint8_t *dst = is_k ? p.kc + (page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh) * sizeof(C)
+                          : p.vc + (page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh) * sizeof(C);
+      store_cache<T, C, VEC>(dst, it.at, y1, scale);
+      if (it.second >= 0)
+        store_cache<T, C, VEC>(dst, it.second, y2, scale);
+    }
   }
 }
 
