@@ -1258,7 +1258,8 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
 
   if (wave == 0) {
     Sched sched(args, st);
-    sched.init(paged_place(), gridDim.x);
+    const uint32_t n = gridDim.x, b = blockIdx.x;
+    sched.init(n % 8 == 0 ? (b % 8) * (n / 8) + b / 8 : b, n);
     sched.get(st.unit[0]);
   }
   __syncthreads();

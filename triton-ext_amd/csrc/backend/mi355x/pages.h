@@ -509,11 +509,11 @@ __global__ void __launch_bounds__(256) page_copy_kernel(PageCopyArgs p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (at + 4096 * k < bytes)
-          x[k] = *reinterpret_cast<const u32x4 *>(base + a * stride + at + 4096 * k);
+          x[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + a * stride + at + 4096 * k));
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (at + 4096 * k < bytes)
-          *reinterpret_cast<u32x4 *>(base + b * stride + at + 4096 * k) = x[k];
+          __builtin_nontemporal_store(x[k], reinterpret_cast<u32x4 *>(base + b * stride + at + 4096 * k));
     }
     i += step_i, at_piece += step_p;
     if (at_piece >= pieces)
