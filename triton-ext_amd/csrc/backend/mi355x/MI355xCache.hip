@@ -447,9 +447,9 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   plan->rows = plan->variant == kAttn16 ? 16 : plan->variant == kAttn32 ? 32 : 128;
   const int D = attnDims(d.head_dim);
   const bool f8 = d.cache_type == TX_F8E4M3;
-  // workgroups that a CU has place for (64 KiB of LDS, 256 registers a lane)
+  // workgroups that a CU has place for (by LDS and registers)
   const bool one = D > 128 && !(plan->variant == kAttn16 && f8);
-  const int per_cu = one ? 1 : 2;
+  const int per_cu = one ? 1 : plan->variant == kAttn128 && D == 64 ? 3 : 2;
   // the most steps of work there can be (a step: the keys a workgroup takes at a time)
   const bool split = plan->variant != kAttn128;
   const int step = split ? 4 * kSplitBlock : 64;

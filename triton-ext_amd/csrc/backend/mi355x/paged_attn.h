@@ -196,17 +196,19 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   __device__ __forceinline__ static void read_k(const Bases &bs, int at, KF &kf) {
     typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
 #pragma unroll
-    for (int b = 0; b < BN / 32; ++b)
+    for (int c = 0; c < NK; ++c)
 #pragma unroll
-      for (int c = 0; c < NK; ++c)
+      for (int b = 0; b < BN / 32; ++b)
         kf.v[b][c] = *(const lds_i32x4 *)(uintptr_t)(bs.k[c] + at + b * 32 * ROW);
   }
   __device__ __forceinline__ static void qk(const KF &kf, const QF &qf, f16v (&s)[BN / 32]) {
 #pragma unroll
-    for (int b = 0; b < BN / 32; ++b) {
+    for (int b = 0; b < BN / 32; ++b)
       s[b] = f16v{};
 #pragma unroll
-      for (int c = 0; c < NK; ++c) {
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b) { // independent sums side by side
         if constexpr (F8) {
           s[b] = X::mfma(widen(kf.v[b][c][0], kf.v[b][c][1]), qf.v[2 * c], s[b]);
           s[b] = X::mfma(widen(kf.v[b][c][2], kf.v[b][c][3]), qf.v[2 * c + 1], s[b]);
@@ -214,16 +216,16 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
           s[b] = X::mfma(__builtin_bit_cast(h8, kf.v[b][c]), qf.v[c], s[b]);
         }
       }
-    }
   }
   // V fragments of dim blocks b0 .. b0 + N - 1.
   template <int N> struct VF {
     i32x4_t v[N][BN / 16]; // e4m3: .xy
   };
   static constexpr int VN = NV < 4 ? NV : NV % 4 ? 3 : 4; // dim blocks read together
-  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<VN> &vf) {
+  template <int N>
+  __device__ __forceinline__ static void read_v(const Bases &bs, int at, int b0, VF<N> &vf) {
 #pragma unroll
-    for (int bd = 0; bd < VN; ++bd)
+    for (int bd = 0; bd < N; ++bd)
 #pragma unroll
       for (int c = 0; c < BN / 16; ++c) {
         const uint32_t a = bs.v[b0 + bd] + at + c * 16 * ROW;
@@ -240,11 +242,12 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
         }
       }
   }
-  __device__ __forceinline__ static void pv(const VF<VN> &vf, int b0, const PF &pf, Acc &acc) {
+  template <int N>
+  __device__ __forceinline__ static void pv(const VF<N> &vf, int b0, const PF &pf, Acc &acc) {
 #pragma unroll
-    for (int bd = 0; bd < VN; ++bd)
+    for (int c = 0; c < BN / 16; ++c)
 #pragma unroll
-      for (int c = 0; c < BN / 16; ++c) {
+      for (int bd = 0; bd < N; ++bd) { // independent sums side by side
         h8 x;
         if constexpr (F8)
           x = widen(vf.v[bd][c][0], vf.v[bd][c][1]);
@@ -1238,18 +1241,19 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
 // Many rows: the waves of a workgroup share the keys
 // ---------------------------------------------------------------------------
 
-// 128 rows a unit, 32 a wave (chunks of a prompt).  Iteration j holds S_j, computes S_{j+1}
-// beside the softmax of S_j, then adds P_j V_j.  K and V have NS LDS slots each, loaded NS blocks
-// ahead of S and NS - 1 ahead of P V, and one barrier a block.  Four slots where they fit (a block then
-// takes less time than a load from memory): mixed lengths with a window in heads of 64
-// 42 -> 33 us.
+// 128 rows a unit, 32 a wave (chunks of a prompt).  K and V have two LDS slots each.  A block has
+// two barriers: after the first K_k is whole (and V_{k-1}'s slot free, for V_{k+1}), after the second
+// V_k is (and K_k's slot free, for K_{k+2}), so that loads have about two blocks' time to land.  All
+// of K's fragments are under way before the first of their MFMAs, all of V's before the softmax.  The
+// matrix cores and the softmax overlap between the workgroups of a CU.
+template <class A> constexpr int paged_rows_groups() { return A::D > 128 ? 1 : A::D > 64 ? 2 : 3; }
+
 template <class A>
-__global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kernel(PagedAttnArgs args) {
+__global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_kernel(PagedAttnArgs args) {
   constexpr int D = A::D, BN = A::BN, U = A::TILE / 4096; // loads of a wave
-  constexpr int NS = A::TILE <= 8192 ? 4 : 2;
   typedef typename A::elt elt;
   typedef PagedSched<128, BN, 1, kRowsOverhead> Sched;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * NS * A::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * A::TILE];
   __shared__ PagedSchedState st;
   __shared__ int flag;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
@@ -1264,7 +1268,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
   }
   __syncthreads();
 
-  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + NS * A::TILE;
+  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * A::TILE;
   typename A::Bases bs;
   A::bases(k_lds, v_lds, bs);
   uint32_t ko[U], vo[U];
@@ -1291,7 +1295,7 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
     const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
-    uint64_t here[NS + 1] = {}; // of blocks j .. j + NS
+    uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
     auto issue_k = [&](int k, int slot) {
       issue_rows<A, U, false>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
     };
@@ -1310,15 +1314,14 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
               p.head_dim, qf);
     if (k0 < k1) {
       pr.settle();
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        if (k0 + i < k1) {
-          pr.hold((k0 + i) * BN);
-          here[i] = pr.template there<BN>((k0 + i) * BN, un.hi);
-          issue_k(k0 + i, i);
-          if (i < NS - 1)
-            issue_v(k0 + i, i);
-        }
+      here[0] = pr.template there<BN>(k0 * BN, un.hi);
+      issue_k(k0, 0);
+      issue_v(k0, 0);
+      if (k0 + 1 < k1) {
+        pr.hold((k0 + 1) * BN);
+        here[1] = pr.template there<BN>((k0 + 1) * BN, un.hi);
+        issue_k(k0 + 1, 1);
+      }
     }
     if (wave == 0)
       Sched(p, st).get(st.unit[turn ^ 1]);
@@ -1336,37 +1339,36 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
     A::settle_q(r < un.rows, p.head_dim, scale, qf);
     scale = scale == 0.f ? 1.f : fabsf(scale);
     float m = -INFINITY, l = 0.f;
-    typename A::f16v acc[D / 32], s[BN / 32];
-#pragma unroll
-    for (int bd = 0; bd < D / 32; ++bd)
-      acc[bd] = typename A::f16v{};
+    typename A::Acc acc = {};
+    typename A::Scores s;
     paged_vmcnt<0>();
     __syncthreads();
-    if (k0 < k1 && live(k0)) {
-      typename A::KF kf;
-      A::read_k(bs, 0, kf);
-      A::qk(kf, qf, s);
-    }
-    __syncthreads(); // K slot 0 is loaded again
     auto iter = [&](int k, auto slot_c) {
       constexpr int SL = decltype(slot_c)::value;
-      const bool ahead = k + NS < k1;
-      if (k + NS - 1 < k1)
-        issue_v(k + NS - 1, (SL + NS - 1) % NS);
-      if (ahead) {
-        pr.hold((k + NS) * BN);
-        here[NS] = pr.template there<BN>((k + NS) * BN, un.hi);
-        issue_k(k + NS, SL);
-      }
-      typename A::f16v sn[BN / 32];
-      if (k + 1 < k1 && live(k + 1)) {
+      const int n0 = k * BN;
+      const bool on = live(k);
+      if (k + 1 < k1)
+        issue_v(k + 1, 1 - SL);
+      if (on) {
         typename A::KF kf;
-        A::read_k(bs, (SL + 1) % NS * A::TILE, kf);
-        A::qk(kf, qf, sn);
+        A::read_k(bs, SL * A::TILE, kf);
+        __builtin_amdgcn_sched_barrier(0);
+        A::qk(kf, qf, s);
       }
-      if (live(k)) {
-        const int n0 = k * BN;
-        typename A::h8 pf[BN / 16];
+      if (whole_loads && k + 1 < k1)
+        paged_vmcnt<2 * U>(); // all after V_k
+      else
+        paged_vmcnt<0>();
+      __syncthreads();
+      if (k + 2 < k1) {
+        pr.hold((k + 2) * BN);
+        here[2] = pr.template there<BN>((k + 2) * BN, un.hi);
+        issue_k(k + 2, SL);
+      }
+      if (on) {
+        typename A::template VF<A::NV> vf;
+        A::read_v(bs, SL * A::TILE, 0, vf);
+        __builtin_amdgcn_sched_barrier(0);
         const uint64_t all = ~0ull >> (64 - BN);
         if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
           const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
@@ -1374,23 +1376,13 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
           seen &= a < 64 ? ~0ull << a : 0;
           A::mask(s, seen & here[0]);
         }
+        typename A::PF pf;
         A::softmax(s, scale, acc, m, l, pf);
-#pragma unroll
-        for (int b0 = 0; b0 < A::NV; b0 += A::VN) {
-          typename A::template VF<A::VN> vf;
-          A::read_v(bs, SL * A::TILE, b0, vf);
-          A::pv(vf, b0, pf, acc);
-        }
+        A::pv(vf, 0, pf, acc);
       }
-#pragma unroll
-      for (int b2 = 0; b2 < BN / 32; ++b2)
-        s[b2] = sn[b2];
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        here[i] = here[i + 1];
-      // K_{k+2} and V_{k+1} have landed: NS - 2 iterations' loads came after them
-      if (whole_loads && ahead)
-        paged_vmcnt<2 * U * (NS - 2)>();
+      here[0] = here[1], here[1] = here[2];
+      if (whole_loads && k + 2 < k1)
+        paged_vmcnt<2 * U>(); // all after K_{k+1}
       else
         paged_vmcnt<0>();
       __syncthreads();
@@ -1399,12 +1391,6 @@ __global__ void __launch_bounds__(256, A::D > 128 ? 1 : 2) paged_attn_rows_kerne
       iter(k++, std::integral_constant<int, 0>());
       if (k < k1)
         iter(k++, std::integral_constant<int, 1>());
-      if constexpr (NS == 4) {
-        if (k < k1)
-          iter(k++, std::integral_constant<int, 2>());
-        if (k < k1)
-          iter(k++, std::integral_constant<int, 3>());
-      }
     }
 
     l = A::X::xsum(l);
