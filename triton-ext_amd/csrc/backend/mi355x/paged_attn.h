@@ -945,7 +945,7 @@ __device__ __forceinline__ bool paged_arrive(uint32_t *counter, uint32_t parts, 
 template <class V>
 __device__ __forceinline__ void paged_join(float &m, float &l, V &x, float m1, float l1,
                                            const V &x1) {
-  if (m1 == -INFINITY)
+  if (l1 == 0.f) // nothing (a NaN among the scores makes l NaN)
     return;
   const float to = fmaxf(m, m1);
   const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
@@ -1200,7 +1200,7 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           const uint32_t jj = j0 + j * groups;
-          pm[j] = -INFINITY;
+          pm[j] = -INFINITY, pl[j] = 0.f;
           if (on && jj < ue.parts) {
             const uint64_t slot = 2ull * (ue.w0 + jj) + (jj == 0 ? ue.slot0 : 0);
             const auto all = __builtin_amdgcn_make_buffer_rsrc(unit_parts, 0, 0x7fffffff, 0x00020000);
@@ -1444,7 +1444,7 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
               __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + r_e) * 4, 0, kSC1));
           const float l1 = __int_as_float(
               __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + 128 + r_e) * 4, 0, kSC1));
-          if (m1 == -INFINITY)
+          if (l1 == 0.f)
             continue;
           const float to = fmaxf(m, m1);
           const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);

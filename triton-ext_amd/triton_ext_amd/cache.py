@@ -78,13 +78,17 @@ def _ptr(t):
 
 
 def _new(t):
-    """A new tensor like t, dense, with its last dimension contiguous (empty_like is the
-    cheapest call that makes one)."""
+    """A new packed tensor like t."""
+    import torch
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _maker(t):
+    """What makes new tensors like t, with their last dimension contiguous: empty_like, the
+    cheapest call, where it does."""
     import torch
     out = torch.empty_like(t)
-    if out.stride(-1) != 1 and out.shape[-1] > 1:
-        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    return out
+    return torch.empty_like if out.stride(-1) == 1 or out.shape[-1] <= 1 else _new
 
 
 def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, context=4096,
@@ -143,11 +147,12 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
         if xc is not x or pc is not positions or fc is not inv_freq:
             return rotary(xc, pc, fc, interleaved=interleaved, scale=scale, inverse=inverse,
                           out=out, stream=stream)
-        found = _keep(form, _rotary_plan(x, positions, inv_freq, interleaved, scale, inverse,
-                                         _new(x) if out is None else out))
+        make = _maker(x)
+        found = _keep(form, (_rotary_plan(x, positions, inv_freq, interleaved, scale, inverse,
+                                          make(x) if out is None else out), make))
     if out is None:
-        out = _new(x)
-    rc = capi.load().tx_rotary_launch(found, x.data_ptr(), positions.data_ptr(),
+        out = found[1](x)
+    rc = capi.load().tx_rotary_launch(found[0], x.data_ptr(), positions.data_ptr(),
                                       inv_freq.data_ptr(), out.data_ptr(),
                                       _current_stream(x.device) if stream is None else stream)
     if rc:
@@ -263,22 +268,23 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
                                 inv_freq=inv_freq, interleaved=interleaved, scale=scale,
                                 k_scale=k_scale, v_scale=v_scale, q_out=q_out, stream=stream)
         T, Hkv, D = k.shape
-        Hq, q_st = 0, (0, 0, 0, 0)
+        Hq, q_st, make = 0, (0, 0, 0, 0), None
         if q is not None:
+            make = _maker(q)
             if q_out is None:
-                q_out = _new(q)
+                q_out = make(q)
             Hq, q_st = q.shape[1], q.stride()[:2] + q_out.stride()[:2]
-        found = _keep(form, ctypes.byref(_plan(
+        found = _keep(form, (ctypes.byref(_plan(
             "paged_append", capi.PagedAppendDesc, capi.PagedAppendPlan,
             (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D,
              0 if inv_freq is None else 2 * inv_freq.shape[0], k_cache.shape[1], _tx_of(k.dtype),
              _tx_of(k_cache.dtype), int(bool(interleaved)), int(cu_q is not None), float(scale))
             + q_st + k.stride()[:2] + v.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
-            + (page_table.stride(0),))))
+            + (page_table.stride(0),))), make))
     if q is not None and q_out is None:
-        q_out = _new(q)
+        q_out = found[1](q)
     rc = capi.load().tx_paged_append_launch(
-        found, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
+        found[0], _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
         v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(inv_freq),
         _ptr(k_scale), _ptr(v_scale), _current_stream(k.device) if stream is None else stream)
     if rc:
@@ -342,8 +348,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
                                    causal=causal, window=window, k_scale=k_scale, v_scale=v_scale,
                                    out=out, return_lse=return_lse, workspace=workspace,
                                    stream=stream)
+        make = _maker(q)
         if out is None:
-            out = _new(q)
+            out = make(q)
         T, Hq, D = q.shape
         p = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
                   (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq,
@@ -351,9 +358,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
                    int(bool(causal)), int(window), int(cu_q is not None), float(sm_scale))
                   + q.stride()[:2] + out.stride()[:2] + k_cache.stride()[:3]
                   + v_cache.stride()[:3] + (page_table.stride(0),))
-        found = _keep(form, (ctypes.byref(p), p))
+        found = _keep(form, (ctypes.byref(p), p, make))
     if out is None:
-        out = _new(q)
+        out = found[2](q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     if stream is None:
         stream = _current_stream(q.device)
@@ -420,6 +427,8 @@ class _Pages:
             if t.device != device:
                 raise ValueError(f"cache {i} is on {t.device}, not on {device}")
             d.stride[i], d.bytes[i] = _page_bytes(t, f"cache {i}", P)
+        import torch
+        self.new = torch.empty_like  # (of packed books)
         self.ref, need = ctypes.byref(d), ctypes.c_int64(0)
         capi.check(capi.load().tx_page_workspace(self.ref, ctypes.byref(need)))
         self.workspace_bytes = _COUNTERS + need.value
@@ -476,7 +485,6 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
     the other.  Returns page_table, kv_len, refs, and how many pages were missing (an
     int32 scalar on the device; those entries are -1).  out: the three tensors to write,
     which may be those read."""
-    import torch
     form = ("reserve", _form(page_table), _form(kv_len), _form(refs), _form(new_len), page_size,
             None if out is None else tuple(map(_form, out)))
     found = _forms.get(form)
@@ -490,7 +498,7 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
             return page_reserve(*dense, page_size, out=out, stream=stream)
         found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
                                    page_size=page_size))
-    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
     device = refs.device
     missing = refs.new_empty(())
     if stream is None:
@@ -508,7 +516,6 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
     """Sequences child[i] (empty rows, each named once) become copies of parent[i] that share
     its pages; a last page that is not full is copied, in every cache [P, page_size, ...],
     to a free one.  Returns page_table, kv_len, refs and the missing pages, as page_reserve."""
-    import torch
     caches = list(caches)
     form = ("fork", _form(page_table), _form(kv_len), _form(refs), _form(parent), _form(child),
             None if out is None else tuple(map(_form, out)), *map(_form, caches))
@@ -530,7 +537,7 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
                 raise ValueError(f"cache {i} has pages of {c.shape[1]} tokens, cache 0 of "
                                  f"{caches[0].shape[1]}")
         found = _keep(form, pages)
-    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
     device = refs.device
     missing = refs.new_empty(())
     if stream is None:
@@ -562,7 +569,7 @@ def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=Non
             return page_free(*dense, page_size, out=out, stream=stream)
         found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
                                    page_size=page_size))
-    t, n, r = (_new(page_table), _new(kv_len), _new(refs)) if out is None else out
+    t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
     rc = capi.load().tx_page_free(
         found.ref, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
         drop.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
@@ -576,7 +583,6 @@ def page_compact(caches, page_table, refs, *, out=None, stream=None):
     """Moves the pages in use (refs > 0) together: with U of them, those from U on go, in
     order, to the free ones below U, in every cache [P, ...] and in the books.  Returns
     page_table, refs and how many were moved (an int32 scalar on the device)."""
-    import torch
     caches = list(caches)
     form = ("compact", _form(page_table), _form(refs),
             None if out is None else tuple(map(_form, out)), *map(_form, caches))
@@ -587,7 +593,7 @@ def page_compact(caches, page_table, refs, *, out=None, stream=None):
         if dense[0] is not page_table or dense[1] is not refs:
             return page_compact(caches, *dense, out=out, stream=stream)
         found = _keep(form, _Pages(caches, refs.shape[0], refs.device, *page_table.shape))
-    t, r = (_new(page_table), _new(refs)) if out is None else out
+    t, r = tuple(map(found.new, (page_table, refs))) if out is None else out
     device = refs.device
     moved = refs.new_empty(())
     if stream is None:
