@@ -22,13 +22,18 @@ from . import capi
 from .dot import _current_stream, _tx_of, workspace_for
 
 # What a call's checks found for arguments of one form (shapes, strides, types, devices and
-# scalars: _form), so that a call of the same form goes to the launch at once.  Nothing here depends
-# on a tensor's address or contents.
+# numbers, as bytes), so that a call of the same form goes to the launch at once.  Nothing here
+# depends on a tensor's address or contents.
 _forms = {}
+_native = None
 
 
-def _form(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+def _calls():
+    """The module that makes forms and calls, loaded with the first call."""
+    global _native
+    if _native is None:
+        _native = capi.calls()
+    return _native
 
 
 def _keep(form, found):
@@ -39,11 +44,12 @@ def _keep(form, found):
 
 
 def _plan(kind, desc_type, plan_type, key):
-    """The plan of a descriptor with these fields in order."""
+    """The plan of a descriptor with these fields in order, and its launch: (function, address of
+    the plan, plan)."""
     p = plan_type()
     capi.check(getattr(capi.load(), f"tx_{kind}_plan_create")(
         ctypes.byref(desc_type(*key)), ctypes.byref(p)))
-    return p
+    return capi.address(f"tx_{kind}_launch"), ctypes.addressof(p), p
 
 
 def _is_int32(t, name, dims):
@@ -71,10 +77,6 @@ def _same_device(device, **tensors):
 def _dense_last(t):
     """t, or a copy, with its last dimension contiguous."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _new(t):
@@ -136,8 +138,9 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     <= D: the dims past it are copied.  The pairs are dims (i, i + rot_dim / 2), or
     (2 i, 2 i + 1) when interleaved.  inverse: the transposed map, which takes the
     gradient of the result to that of x.  out may be x itself."""
-    form = ("rotary", _form(x), _form(positions), _form(inv_freq), bool(interleaved),
-            float(scale), bool(inverse), _form(out))
+    native = _native or _calls()
+    form = native.form("rotary", x, positions, inv_freq, bool(interleaved), float(scale),
+                       bool(inverse), out)
     found = _forms.get(form)
     if found is None:
         _rotary_checks(x, positions, inv_freq, out)
@@ -150,11 +153,11 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
         make = _maker(x)
         found = _keep(form, (_rotary_plan(x, positions, inv_freq, interleaved, scale, inverse,
                                           make(x) if out is None else out), make))
+    (launch, plan, _), make = found
     if out is None:
-        out = found[1](x)
-    rc = capi.load().tx_rotary_launch(found[0], x.data_ptr(), positions.data_ptr(),
-                                      inv_freq.data_ptr(), out.data_ptr(),
-                                      _current_stream(x.device) if stream is None else stream)
+        out = make(x)
+    rc = native.call(launch, plan, x, positions, inv_freq, out,
+                     _current_stream(x.device) if stream is None else stream)
     if rc:
         capi.check(rc)
     return out
@@ -188,11 +191,11 @@ def _rotary_plan(x, positions, inv_freq, interleaved, scale, inverse, out):
     else:
         Z, H, N, D = x.shape
         st = (xs[0], xs[2], xs[1], os_[0], os_[2], os_[1])
-    return ctypes.byref(_plan(
+    return _plan(
         "rotary", capi.RotaryDesc, capi.RotaryPlan,
         (Z, N, H, D, 2 * inv_freq.shape[0], _tx_of(x.dtype), int(bool(interleaved)),
          int(bool(inverse)), 8 * positions.element_size(), float(scale), 0,
-         N if positions.dim() == 2 else 0) + st))
+         N if positions.dim() == 2 else 0) + st)
 
 
 def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, dtype):
@@ -252,9 +255,9 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     The pages must be there (page_reserve); a token without one is not written.  fp16 or
     bf16; a float8_e4m3fn cache holds k / k_scale[head] and v / v_scale[head] (fp32 [Hkv];
     None: 1), saturated.  Rows of q from cu_q[B] on come back as they are."""
-    form = ("append", _form(k), _form(v), _form(k_cache), _form(v_cache), _form(page_table),
-            _form(kv_len), _form(cu_q), _form(q), _form(inv_freq), bool(interleaved),
-            float(scale), _form(k_scale), _form(v_scale), _form(q_out))
+    native = _native or _calls()
+    form = native.form("append", k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
+                       bool(interleaved), float(scale), k_scale, v_scale, q_out)
     found = _forms.get(form)
     if found is None:
         _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, k_scale,
@@ -274,19 +277,19 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
             if q_out is None:
                 q_out = make(q)
             Hq, q_st = q.shape[1], q.stride()[:2] + q_out.stride()[:2]
-        found = _keep(form, (ctypes.byref(_plan(
+        found = _keep(form, (_plan(
             "paged_append", capi.PagedAppendDesc, capi.PagedAppendPlan,
             (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq, Hkv, D,
              0 if inv_freq is None else 2 * inv_freq.shape[0], k_cache.shape[1], _tx_of(k.dtype),
              _tx_of(k_cache.dtype), int(bool(interleaved)), int(cu_q is not None), float(scale))
             + q_st + k.stride()[:2] + v.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
-            + (page_table.stride(0),))), make))
+            + (page_table.stride(0),)), make))
+    (launch, plan, _), make = found
     if q is not None and q_out is None:
-        q_out = found[1](q)
-    rc = capi.load().tx_paged_append_launch(
-        found[0], _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(),
-        v_cache.data_ptr(), page_table.data_ptr(), kv_len.data_ptr(), _ptr(cu_q), _ptr(inv_freq),
-        _ptr(k_scale), _ptr(v_scale), _current_stream(k.device) if stream is None else stream)
+        q_out = make(q)
+    rc = native.call(launch, plan, q, k, v, q_out, k_cache, v_cache, page_table, kv_len, cu_q,
+                     inv_freq, k_scale, v_scale,
+                     _current_stream(k.device) if stream is None else stream)
     if rc:
         capi.check(rc)
     return q_out
@@ -331,9 +334,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     o [T, Hq, D], with return_lse also log2 of the sum of e^(score), fp32 [T, Hq] (-inf
     where nothing is attended to).  cu_q as for paged_append."""
     import torch
-    form = ("attention", _form(q), _form(k_cache), _form(v_cache), _form(page_table),
-            _form(kv_len), _form(cu_q), float(sm_scale), bool(causal), int(window), _form(k_scale), _form(v_scale),
-            _form(out))
+    native = _native or _calls()
+    form = native.form("attention", q, k_cache, v_cache, page_table, kv_len, cu_q, float(sm_scale),
+                       bool(causal), int(window), k_scale, v_scale, out)
     found = _forms.get(form)
     if found is None or q.data_ptr() % 16:
         _attention_checks(q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, out)
@@ -352,23 +355,22 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
         if out is None:
             out = make(q)
         T, Hq, D = q.shape
-        p = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
-                  (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq,
-                   k_cache.shape[2], D, k_cache.shape[1], _tx_of(q.dtype), _tx_of(k_cache.dtype),
-                   int(bool(causal)), int(window), int(cu_q is not None), float(sm_scale))
-                  + q.stride()[:2] + out.stride()[:2] + k_cache.stride()[:3]
-                  + v_cache.stride()[:3] + (page_table.stride(0),))
-        found = _keep(form, (ctypes.byref(p), p, make))
+        plan = _plan("paged_attn", capi.PagedAttnDesc, capi.PagedAttnPlan,
+                     (T, kv_len.shape[0], k_cache.shape[0], page_table.shape[1], Hq,
+                      k_cache.shape[2], D, k_cache.shape[1], _tx_of(q.dtype), _tx_of(k_cache.dtype),
+                      int(bool(causal)), int(window), int(cu_q is not None), float(sm_scale))
+                     + q.stride()[:2] + out.stride()[:2] + k_cache.stride()[:3]
+                     + v_cache.stride()[:3] + (page_table.stride(0),))
+        found = _keep(form, (plan, make))
+    (launch, plan, needs), make = found
     if out is None:
-        out = found[2](q)
+        out = make(q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     if stream is None:
         stream = _current_stream(q.device)
-    ws = workspace if workspace is not None else workspace_for(found[1], q.device, stream)
-    rc = capi.load().tx_paged_attn_launch(
-        found[0], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-        kv_len.data_ptr(), _ptr(cu_q), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), _ptr(lse),
-        _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), stream)
+    ws = workspace if workspace is not None else workspace_for(needs, q.device, stream)
+    rc = native.call(launch, plan, q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale,
+                     out, lse, ws, 0 if ws is None else ws.numel() * ws.element_size(), stream)
     if rc:
         capi.check(rc)
     return (out, lse) if return_lse else out
@@ -407,10 +409,6 @@ def _page_bytes(t, name, P):
     return t.stride(0) * e, n * e
 
 
-def _pointers(caches):
-    return (ctypes.c_void_p * max(len(caches), 1))(*[t.data_ptr() for t in caches])
-
-
 _COUNTERS = 65536
 
 
@@ -418,7 +416,7 @@ class _Pages:
     """The descriptor of calls on pages, and what workspace_for asks of a plan: their scratch
     memory.  The first 64 KiB of a workspace are the arrival counters of other launches."""
 
-    def __init__(self, caches, P, device, S=0, W=0, n=0, page_size=1):
+    def __init__(self, name, caches, P, device, S=0, W=0, n=0, page_size=1):
         if len(caches) > capi.PAGE_CACHES:
             raise ValueError(f"{len(caches)} caches: at most {capi.PAGE_CACHES} a call")
         d = self.desc = capi.PageDesc()
@@ -429,8 +427,9 @@ class _Pages:
             d.stride[i], d.bytes[i] = _page_bytes(t, f"cache {i}", P)
         import torch
         self.new = torch.empty_like  # (of packed books)
-        self.ref, need = ctypes.byref(d), ctypes.c_int64(0)
-        capi.check(capi.load().tx_page_workspace(self.ref, ctypes.byref(need)))
+        self.count = torch.empty((), dtype=torch.int32, device=device)  # what new counts are like
+        self.launch, self.ref, need = capi.address(name), ctypes.addressof(d), ctypes.c_int64(0)
+        capi.check(capi.load().tx_page_workspace(ctypes.byref(d), ctypes.byref(need)))
         self.workspace_bytes = _COUNTERS + need.value
 
     def scratch(self, device, stream):
@@ -469,14 +468,14 @@ def page_copy(caches, src, dst, *, stream=None):
         raise ValueError("src and dst must be of one length")
     if not caches:
         return
-    form = ("copy", _form(src), dst.device, *map(_form, caches))
+    native = _native or _calls()
+    form = native.form("copy", src, dst, caches)
     found = _forms.get(form)
     if found is None:
         _same_device(src.device, dst=dst)
-        found = _keep(form, _Pages(caches, caches[0].shape[0], src.device, n=src.shape[0]))
-    capi.check(capi.load().tx_page_copy(
-        found.ref, _pointers(caches), src.data_ptr(), dst.data_ptr(),
-        _current_stream(src.device) if stream is None else stream))
+        found = _keep(form, _Pages("tx_page_copy", caches, caches[0].shape[0], src.device, n=src.shape[0]))
+    capi.check(native.call(found.launch, found.ref, native.addresses(caches), src, dst,
+                           _current_stream(src.device) if stream is None else stream))
 
 
 def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stream=None):
@@ -485,8 +484,8 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
     the other.  Returns page_table, kv_len, refs, and how many pages were missing (an
     int32 scalar on the device; those entries are -1).  out: the three tensors to write,
     which may be those read."""
-    form = ("reserve", _form(page_table), _form(kv_len), _form(refs), _form(new_len), page_size,
-            None if out is None else tuple(map(_form, out)))
+    native = _native or _calls()
+    form = native.form("reserve", page_table, kv_len, refs, new_len, page_size, out)
     found = _forms.get(form)
     if found is None:
         _book_checks(page_table, kv_len, refs, out, new_len=new_len)
@@ -496,17 +495,15 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
         dense = tuple(map(_dense, given))
         if any(a is not b for a, b in zip(dense, given)):
             return page_reserve(*dense, page_size, out=out, stream=stream)
-        found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
+        found = _keep(form, _Pages("tx_page_reserve", (), refs.shape[0], refs.device, *page_table.shape,
                                    page_size=page_size))
     t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
     device = refs.device
-    missing = refs.new_empty(())
+    missing = found.new(found.count)
     if stream is None:
         stream = _current_stream(device)
-    rc = capi.load().tx_page_reserve(
-        found.ref, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
-        new_len.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(), missing.data_ptr(),
-        found.scratch(device, stream), stream)
+    rc = native.call(found.launch, found.ref, page_table, kv_len, refs, new_len, t, n, r, missing,
+                     found.scratch(device, stream), stream)
     if rc:
         capi.check(rc)
     return t, n, r, missing
@@ -517,8 +514,8 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
     its pages; a last page that is not full is copied, in every cache [P, page_size, ...],
     to a free one.  Returns page_table, kv_len, refs and the missing pages, as page_reserve."""
     caches = list(caches)
-    form = ("fork", _form(page_table), _form(kv_len), _form(refs), _form(parent), _form(child),
-            None if out is None else tuple(map(_form, out)), *map(_form, caches))
+    native = _native or _calls()
+    form = native.form("fork", page_table, kv_len, refs, parent, child, out, caches)
     found = _forms.get(form)
     if found is None:
         _book_checks(page_table, kv_len, refs, out, parent=parent, child=child)
@@ -530,7 +527,7 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
         dense = tuple(map(_dense, given))
         if any(a is not b for a, b in zip(dense, given)):
             return page_fork(caches, *dense, out=out, stream=stream)
-        pages = _Pages(caches, refs.shape[0], refs.device, *page_table.shape, parent.shape[0],
+        pages = _Pages("tx_page_fork", caches, refs.shape[0], refs.device, *page_table.shape, parent.shape[0],
                        caches[0].shape[1])
         for i, c in enumerate(caches):
             if c.shape[1] != caches[0].shape[1]:
@@ -539,13 +536,11 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
         found = _keep(form, pages)
     t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
     device = refs.device
-    missing = refs.new_empty(())
+    missing = found.new(found.count)
     if stream is None:
         stream = _current_stream(device)
-    rc = capi.load().tx_page_fork(
-        found.ref, _pointers(caches), page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
-        parent.data_ptr(), child.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
-        missing.data_ptr(), found.scratch(device, stream), stream)
+    rc = native.call(found.launch, found.ref, native.addresses(caches), page_table, kv_len, refs,
+                     parent, child, t, n, r, missing, found.scratch(device, stream), stream)
     if rc:
         capi.check(rc)
     return t, n, r, missing
@@ -555,8 +550,8 @@ def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=Non
     """Sequences with drop[s] (bool [S]) give their pages back and become empty.  Returns
     page_table, kv_len, refs; out as for page_reserve."""
     import torch
-    form = ("free", _form(page_table), _form(kv_len), _form(refs), _form(drop), page_size,
-            None if out is None else tuple(map(_form, out)))
+    native = _native or _calls()
+    form = native.form("free", page_table, kv_len, refs, drop, page_size, out)
     found = _forms.get(form)
     if found is None:
         _book_checks(page_table, kv_len, refs, out)
@@ -567,13 +562,11 @@ def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=Non
         dense = tuple(map(_dense, given))
         if any(a is not b for a, b in zip(dense, given)):
             return page_free(*dense, page_size, out=out, stream=stream)
-        found = _keep(form, _Pages((), refs.shape[0], refs.device, *page_table.shape,
+        found = _keep(form, _Pages("tx_page_free", (), refs.shape[0], refs.device, *page_table.shape,
                                    page_size=page_size))
     t, n, r = tuple(map(found.new, (page_table, kv_len, refs))) if out is None else out
-    rc = capi.load().tx_page_free(
-        found.ref, page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(),
-        drop.data_ptr(), t.data_ptr(), n.data_ptr(), r.data_ptr(),
-        _current_stream(refs.device) if stream is None else stream)
+    rc = native.call(found.launch, found.ref, page_table, kv_len, refs, drop, t, n, r,
+                     _current_stream(refs.device) if stream is None else stream)
     if rc:
         capi.check(rc)
     return t, n, r
@@ -584,23 +577,22 @@ def page_compact(caches, page_table, refs, *, out=None, stream=None):
     order, to the free ones below U, in every cache [P, ...] and in the books.  Returns
     page_table, refs and how many were moved (an int32 scalar on the device)."""
     caches = list(caches)
-    form = ("compact", _form(page_table), _form(refs),
-            None if out is None else tuple(map(_form, out)), *map(_form, caches))
+    native = _native or _calls()
+    form = native.form("compact", page_table, refs, out, caches)
     found = _forms.get(form)
     if found is None:
         _book_checks(page_table, None, refs, out)
         dense = _dense(page_table), _dense(refs)
         if dense[0] is not page_table or dense[1] is not refs:
             return page_compact(caches, *dense, out=out, stream=stream)
-        found = _keep(form, _Pages(caches, refs.shape[0], refs.device, *page_table.shape))
+        found = _keep(form, _Pages("tx_page_compact", caches, refs.shape[0], refs.device, *page_table.shape))
     t, r = tuple(map(found.new, (page_table, refs))) if out is None else out
     device = refs.device
-    moved = refs.new_empty(())
+    moved = found.new(found.count)
     if stream is None:
         stream = _current_stream(device)
-    rc = capi.load().tx_page_compact(
-        found.ref, _pointers(caches), page_table.data_ptr(), refs.data_ptr(), t.data_ptr(),
-        r.data_ptr(), moved.data_ptr(), found.scratch(device, stream), stream)
+    rc = native.call(found.launch, found.ref, native.addresses(caches), page_table, refs, t, r,
+                     moved, found.scratch(device, stream), stream)
     if rc:
         capi.check(rc)
     return t, r, moved

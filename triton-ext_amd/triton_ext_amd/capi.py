@@ -242,6 +242,29 @@ class TxError(RuntimeError):
         self.code = code
 
 
+def calls():
+    """The module _tx_calls (csrc/python/tx_calls.cpp): tensors' forms, and calls by address."""
+    mod = _libs.get("_tx_calls")
+    if mod is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (the module uses its libraries)
+        path = os.path.join(os.path.dirname(PKG_DIR), "lib", "_tx_calls.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built: run __graft_entry__.build() "
+                               "or `make -C triton-ext_amd`")
+        loader = importlib.machinery.ExtensionFileLoader("_tx_calls", path)
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tx_calls", loader))
+        loader.exec_module(mod)
+        _libs["_tx_calls"] = mod
+    return mod
+
+
+def address(name):
+    """Where the C function `name` of libmi355x_dot.so is, for calls().call."""
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+
+
 def check(rc):
     if rc != OK:
         msg = load().tx_get_last_error().decode(errors="replace")
