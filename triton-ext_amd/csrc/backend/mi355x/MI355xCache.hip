@@ -456,6 +456,9 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   const double units = (double)d.B + (double)d.T * G / plan->rows;
   const double keys = (double)d.table_width * d.page_size;
   const double steps = units * (keys / step + 1 + (split ? kSplitOverhead : kRowsOverhead)) * d.Hkv;
+  if (steps > INT32_MAX)
+    return fail(TX_ERR_UNSUPPORTED, "more than 2^31 blocks of keys for %lld tokens: fewer a call",
+                (long long)d.T);
   plan->units = (int32_t)std::min<double>(256 * per_cu, std::ceil(steps));
   plan->grid_x = plan->units;
   plan->slots = 2 * plan->units;
@@ -515,7 +518,7 @@ extern "C" TX_API int tx_paged_attn_launch(const tx_paged_attn_plan *plan, const
   a.q_st = d.q_st, a.q_sh = d.q_sh, a.o_st = d.o_st, a.o_sh = d.o_sh;
   a.k_sp = d.k_sp * ce, a.k_st = d.k_st * ce, a.k_sh = d.k_sh * ce;
   a.v_sp = d.v_sp * ce, a.v_st = d.v_st * ce, a.v_sh = d.v_sh * ce;
-  a.pages = (uint32_t)d.pages, a.min_share = 1;
+  a.pages = (uint32_t)d.pages;
   a.g_mul = a.g_shift = 0;
   if (const int64_t G = d.Hq / d.Hkv; G > 1) { // ceil(2^(31 + s) / G), 2^s >= G
     const int sh = log2of(G);
