@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
     float m = -INFINITY, l = 0.f;
     typename A::Acc acc = {};
     typename A::Scores s;
-    auto iter = [&](int k, auto slot_c) {
+    auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
       constexpr int SL = decltype(slot_c)::value;
       const int n0 = k * BN, na = n0 + NS * BN;
       const bool ahead = k + NS < k1;
@@ -370,12 +370,18 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
     const PageSide sk{p.kc + un.hk * p.k_sh, p.k_sp, p.k_st, p.k_run};
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
-    auto issue_k = [&](int k, int slot) {
-      issue_rows<A, U, false>(pr, sk, k * BN, un.hi, U * wave, ko, k_lds + slot * A::TILE, row_bytes);
+    // Keys that no other unit reads go past the caches (64 rows of each of 16 sequences of 16384 keys:
+    // 230 -> 209 us); those that others do must not (chunks of 2048: 955 -> 1150).
+    const bool once = un.alone;
+    auto issue = [&](const PageSide &sd, int k, const uint32_t (&off)[U],
+                     uint32_t lds) __attribute__((always_inline)) {
+      if (once)
+        issue_rows<A, U, true>(pr, sd, k * BN, un.hi, U * wave, off, lds, row_bytes);
+      else
+        issue_rows<A, U, false>(pr, sd, k * BN, un.hi, U * wave, off, lds, row_bytes);
     };
-    auto issue_v = [&](int k, int slot) {
-      issue_rows<A, U, false>(pr, sv, k * BN, un.hi, U * wave, vo, v_lds + slot * A::TILE, row_bytes);
-    };
+    auto issue_k = [&](int k, int slot) __attribute__((always_inline)) { issue(sk, k, ko, k_lds + slot * A::TILE); };
+    auto issue_v = [&](int k, int slot) __attribute__((always_inline)) { issue(sv, k, vo, v_lds + slot * A::TILE); };
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
     // looks up the next unit.
     if (k0 < k1)
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
     typename A::Scores s;
     paged_vmcnt<0>();
     __syncthreads();
-    auto iter = [&](int k, auto slot_c) {
+    auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
       constexpr int SL = decltype(slot_c)::value;
       const int n0 = k * BN;
       const bool on = live(k);
@@ -426,7 +432,8 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
       if (on) {
         typename A::KF kf;
         A::read_k(bs, SL * A::TILE, kf);
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (D <= 128)
+          __builtin_amdgcn_sched_barrier(0);
         A::qk(kf, qf, s);
       }
       if (whole_loads && k + 1 < k1)
@@ -440,7 +447,8 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
         issue_k(k + 2, SL);
       }
       if (on) {
-        typename A::template VF<A::NV> vf;
+        constexpr int VR = D <= 128 ? A::NV : A::VN; // dim blocks read ahead (256 dims: for want of registers)
+        typename A::template VF<VR> vf;
         A::read_v(bs, SL * A::TILE, 0, vf);
         __builtin_amdgcn_sched_barrier(0);
         const uint64_t all = ~0ull >> (64 - BN);
@@ -453,6 +461,11 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
         typename A::PF pf;
         A::softmax(s, scale, acc, m, l, pf);
         A::pv(vf, 0, pf, acc);
+#pragma unroll
+        for (int b0 = VR; b0 < A::NV; b0 += VR) {
+          A::read_v(bs, SL * A::TILE, b0, vf);
+          A::pv(vf, b0, pf, acc);
+        }
       }
       here[0] = here[1], here[1] = here[2];
       if (whole_loads && k + 2 < k1)

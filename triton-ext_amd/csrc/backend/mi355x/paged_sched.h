@@ -42,7 +42,7 @@ __device__ __forceinline__ int64_t lane_value64(int64_t v, int lane) {
 struct alignas(16) PagedUnit {
   int64_t pos0;
   int t0, r0, rows, hk, b, len, lo, hi; // keys [lo, hi)
-  uint32_t s0, s1, parts, part, w0, slot0;
+  uint32_t s0, s1, parts, part, w0, slot0 : 1, alone : 1; // alone: the sequence's only unit of hk
 };
 static_assert(sizeof(PagedUnit) == 64, "four 16-byte reads");
 
@@ -225,7 +225,7 @@ template <int BM, int BN, int WPS, uint32_t OV> struct PagedSched {
       if (s1 > OV) {
         u.rows = rows;
         u.s0 = (s0 > OV ? s0 : OV) - OV, u.s1 = s1 - OV;
-        u.parts = 1, u.part = 0, u.w0 = 0, u.slot0 = 0;
+        u.parts = 1, u.part = 0, u.w0 = 0, u.slot0 = 0, u.alone = rows == nr;
         if (u.s1 - u.s0 < cost - OV) {
           const uint32_t first = pos - s0;
           u.w0 = (first + OV) / share;
@@ -271,7 +271,7 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedUnit &s) {
   u.pos0 = (int64_t)(uint32_t)v[0][0] | (int64_t)v[0][1] << 32;
   u.t0 = v[0][2], u.r0 = v[0][3], u.rows = v[1][0], u.hk = v[1][1], u.b = v[1][2], u.len = v[1][3];
   u.lo = v[2][0], u.hi = v[2][1], u.s0 = v[2][2], u.s1 = v[2][3];
-  u.parts = v[3][0], u.part = v[3][1], u.w0 = v[3][2], u.slot0 = v[3][3];
+  u.parts = v[3][0], u.part = v[3][1], u.w0 = v[3][2], u.slot0 = v[3][3] & 1, u.alone = v[3][3] >> 1 & 1;
   return u;
 }
 
