@@ -107,7 +107,9 @@ TX_API int tx_paged_append_launch(const tx_paged_append_plan *plan, const void *
  * caches: k and v times k_scale[kv head], v_scale[kv head] (fp32; NULL: 1).  What
  * the cache holds where nothing is attended to may be anything, NaN included, outside
  * [0, kv_len) and in pages the table does not name.  Products on the matrix cores
- * with fp32 sums, softmax in fp32; p is rounded to q's type before p . v. */
+ * with fp32 sums, softmax in fp32; p (relative to a maximum of the row's keys up to there, and up to
+ * 2^8) is rounded to q's type before p . v.  A sequence has at most 2^31 - 128 tokens.  The
+ * order of sums depends on the lengths alone: the same call gives the same bits. */
 typedef struct tx_paged_attn_desc {
   int64_t T, B;
   int64_t pages, table_width;
@@ -123,10 +125,10 @@ typedef struct tx_paged_attn_desc {
 
 typedef struct tx_paged_attn_plan {
   tx_paged_attn_desc desc;
-  int32_t variant; /* the kernel */
-  int32_t rows;    /* query rows (token x head of one kv head) of a workgroup */
-  int32_t slots;   /* workspace places for parts of a row's keys */
-  int32_t units;   /* workgroups per kv head */
+  int32_t variant; /* the kernel: 0, 1: waves share out the keys, 2: the rows */
+  int32_t rows;    /* query rows (token x head of one kv head) of a unit of work: 16, 32, 128 */
+  int32_t slots;   /* workspace places for parts of a unit's keys */
+  int32_t units;   /* workgroups, which share all units' keys in equal runs */
   int32_t grid_x, block_threads;
   int64_t workspace_bytes; /* as tx_dot_launch's workspace: zeroed before its first use, never
                             * shared by launches that may overlap */
@@ -155,7 +157,7 @@ typedef struct tx_page_desc {
 } tx_page_desc;
 
 /* Checks desc, and gives the bytes of scratch memory that each of the calls below needs for
- * it (any contents). */
+ * it (any contents, 8-byte aligned). */
 TX_API int tx_page_workspace(const tx_page_desc *desc, int64_t *bytes);
 
 /* Page src[i] of every cache is copied to page dst[i], i < n.  Entries outside

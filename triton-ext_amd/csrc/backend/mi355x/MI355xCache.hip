@@ -441,7 +441,9 @@ extern "C" TX_API int tx_paged_attn_plan_create(const tx_paged_attn_desc *desc,
   if (d.T == 0)
     return TX_OK;
   // The fewer rows a sequence has on average, the less of a unit's matrix and softmax work is
-  // for nothing; memory bounds the calls of few rows, whichever form.
+  // for nothing; past a form's rows its units read the same keys again.  16 sequences of 16384 keys,
+  // heads of 128: 32 rows each 204 us in the form of 32, 224 in that of 128; 64 rows 374 and 209.  4
+  // rows each (32 sequences of up to 16384): 86 in the form of 16, 90 in that of 32.
   const int64_t G = d.Hq / d.Hkv, rows = d.T * G;
   plan->variant = rows <= 16 * d.B ? kAttn16 : rows <= 32 * d.B ? kAttn32 : kAttn128;
   plan->rows = plan->variant == kAttn16 ? 16 : plan->variant == kAttn32 ? 32 : 128;

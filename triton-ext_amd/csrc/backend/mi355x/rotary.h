@@ -10,7 +10,10 @@
 // (interleaved), or VEC elements past rot_dim, which are copied.  So it forms its
 // VEC (or VEC / 2) sines once and goes through the token's heads, every
 // head_lanes-th of them, kHeadBatch at a time: their 16-byte loads are all under way before
-// the first store.  Bound by memory.
+// the first store.  Bound by memory: (4, 32, 4096, 64) in fp16 with 32 dims rotated 23.9 us, 5.6
+// TB/s (one head at a time 32.9); 9001 tokens of 32 + 2 x 8 heads of 128 into an e4m3 cache 40.9 us, 5.0
+// TB/s (58.6).  Loads are non-temporal: what a projection left is read once (25.8 and 46.7 without).
+// A step's few tokens take 3.5 .. 4.5 us, less than the call on the host.
 #pragma once
 
 #include <hip/hip_runtime.h>
