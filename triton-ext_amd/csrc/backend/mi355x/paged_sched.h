@@ -70,8 +70,8 @@ __device__ __forceinline__ void paged_keys(const PagedAttnArgs &p, int64_t at, i
 
 // Deals out the units.  Blocks of BN keys in steps of WPS blocks (those that the waves of a
 // workgroup take side by side); a unit has one step at least, so that its rows are written, and
-// begins with OV more that stand for what its beginning and end cost.  The first wave goes through this, a lane per sequence (64 at a time, in LDS) or block of rows; sums
-// across lanes.
+// begins with OV more that stand for what its beginning and end cost.  The first wave goes through
+// this, a lane per sequence (64 at a time, in LDS) or block of rows; sums across lanes.
 struct PagedSchedState {
   int64_t pos0[64];
   int t0[64], n[64], len[64];

@@ -136,11 +136,14 @@ template <int VEC, bool INTER> struct RotaryItem {
   __device__ __forceinline__ void load(const T *head, EltVec<T, VEC> &x1, EltVec<T, VEC> &x2) const {
     if constexpr (sizeof(T) * VEC == 16) {
       typedef uint32_t q4 __attribute__((ext_vector_type(4)));
-      x1 = __builtin_bit_cast(EltVec<T , VEC>, __builtin_nontemporal_load(reinterpret_cast<const q4 *>(head + at)));
-      x2 = __builtin_bit_cast(EltVec<T , VEC>, __builtin_nontemporal_load(reinterpret_cast<const q4 *>(head + (second >= 0 ? second : at))));
+      const T *const head2 = head + (second >= 0 ? second : at);
+      x1 = __builtin_bit_cast(EltVec<T, VEC>,
+                              __builtin_nontemporal_load(reinterpret_cast<const q4 *>(head + at)));
+      x2 = __builtin_bit_cast(EltVec<T, VEC>,
+                              __builtin_nontemporal_load(reinterpret_cast<const q4 *>(head2)));
     } else {
-    x1 = *reinterpret_cast<const EltVec<T, VEC> *>(head + at);
-    x2 = *reinterpret_cast<const EltVec<T, VEC> *>(head + (second >= 0 ? second : at));
+      x1 = *reinterpret_cast<const EltVec<T, VEC> *>(head + at);
+      x2 = *reinterpret_cast<const EltVec<T, VEC> *>(head + (second >= 0 ? second : at));
     }
   }
   template <class T>
