@@ -214,6 +214,45 @@ def test_compact_pools_of_any_size(gpu, P, in_place):
     assert torch.equal(dev.cpu(), data)
 
 
+@pytest.mark.parametrize("S,W,P", [(1, 1, 1), (3, 100, 513), (4096, 1, 700), (4097, 1, 700),
+                                   (64, 64, 5000), (17, 241, 5000), (7, 40, 131072), (7, 40, 131073)])
+def test_forms_of_free(gpu, S, W, P):
+    """Entries and pages at and past where every workgroup goes through the table; pages that
+    several rows hold, holes, lengths past the table and below nothing."""
+    say("free", S, W, P)
+    g = gen(S + W)
+    page = 4
+    table = torch.randint(-1, min(P + 2, 200000), (S, W), generator=g).to(torch.int32)
+    table[:, : W // 3] = table[0, : W // 3]
+    table[0, 0] = P - 1
+    length = torch.randint(-3, W * page + 9, (S,), generator=g).to(torch.int32)
+    length[0] = W * page
+    refs = torch.randint(0, 1 << 20, (P,), generator=g).to(torch.int32)
+    drop = torch.rand(S, generator=g) < 0.5
+    drop[0] = True
+    held = (torch.arange(W)[None] < ((length + page - 1) // page)[:, None]) & drop[:, None]
+    given = table[held & (table >= 0) & (table < P)].long()
+    want = (torch.where(drop[:, None], -1, table), torch.where(drop, 0, length),
+            refs - torch.bincount(given, minlength=P).to(torch.int32))
+    for kind in (False, True):
+        t, n, r, d = (x.to(gpu) for x in (table, length, refs, drop))
+        got = tx.page_free(t, n, r, d, page, out=(t, n, r) if kind else None)
+        for x, y in zip(got, want):
+            assert torch.equal(x.cpu(), y)
+    assert int(given.numel()) > 0
+
+
+@pytest.mark.parametrize("S", [1, 5000])
+def test_free_of_rows_without_entries(gpu, S):
+    table = torch.empty((S, 0), dtype=torch.int32, device=gpu)
+    length = torch.full((S,), 3, dtype=torch.int32, device=gpu)
+    refs = torch.arange(9, dtype=torch.int32, device=gpu)
+    drop = torch.arange(S, device=gpu) % 2 == 0
+    t, n, r = tx.page_free(table, length, refs, drop, 4)
+    assert t.shape == (S, 0) and torch.equal(r, refs)
+    assert torch.equal(n, torch.where(drop, 0, length))
+
+
 # ---- together -----------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", [BF, E4M3])

@@ -748,6 +748,16 @@ extern "C" TX_API int tx_page_free(const tx_page_desc *desc, const int32_t *page
                         nullptr);
   a.drop = drop;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // One launch while a thread has few entries of the table; past it, or in place, a copy of the
+  // counts and atomics on them.
+  const bool apart = !a.table_in_place && len_out != kv_len;
+  if (apart && desc->P > 0 && desc->P <= 256 * kFreePages && desc->S * desc->W > 0 &&
+      desc->S * desc->W <= kFreeEntries) {
+    hipLaunchKernelGGL(page_free_small_kernel, dim3((uint32_t)cdiv(desc->P, kFreePages)),
+                       dim3(kBookThreads), 0, s, a);
+    TX_HIP_CHECK(hipGetLastError());
+    return TX_OK;
+  }
   if (!a.refs_in_place && desc->P > 0) {
     hipLaunchKernelGGL(book_copy_kernel, dim3((uint32_t)std::min<int64_t>(cdiv(desc->P, 256), 1024)),
                        dim3(256), 0, s, refs_out, refs, desc->P);
