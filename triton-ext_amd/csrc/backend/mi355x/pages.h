@@ -120,8 +120,8 @@ __device__ __forceinline__ int64_t book_free_pages(const int32_t *refs, int64_t 
 
 // New pages for the sequences.  Every workgroup sums the needs of all sequences, goes through the
 // counts as far as there are pages wanted (a page that it finds goes straight to its place in
-// the workgroup's rows), and then writes its rows and its share of the counts: a free page up
-// to the last one taken has been taken.
+// the workgroup's rows, of which there may be none), and then writes its rows and its share of the
+// counts: a free page up to the last one taken has been taken.
 __global__ void __launch_bounds__(kBookThreads) page_reserve_kernel(BookArgs p) {
   __shared__ int pre[kBookRows + 1];   // pages that the sequences up to this row of ours want
   __shared__ int held_of[kBookRows];
@@ -141,8 +141,11 @@ __global__ void __launch_bounds__(kBookThreads) page_reserve_kernel(BookArgs p) 
     return x > 0 ? x : 0;
   };
   int64_t nfree = 0, cut = -1, wanted = 0;
-  for (int64_t s0 = (int64_t)blockIdx.x * p.rows; s0 < p.S; s0 += (int64_t)gridDim.x * p.rows) {
-    const int rows = (int)(p.S - s0 < p.rows ? p.S - s0 : p.rows);
+  // (once also where there are no rows for it: its share of the counts asks for the last page taken)
+  int64_t s0 = (int64_t)blockIdx.x * p.rows;
+  do {
+    const int64_t left = p.S - s0;
+    const int rows = (int)(left < 0 ? 0 : left < p.rows ? left : p.rows);
     int before = 0, all = 0, x;
     for (int64_t s = tid; s < p.S; s += kBookThreads) {
       const int v = need(p.len[s], p.new_len[s]);
@@ -202,7 +205,8 @@ __global__ void __launch_bounds__(kBookThreads) page_reserve_kernel(BookArgs p) 
       }
     }
     __syncthreads(); // pre, held_of
-  }
+    s0 += (int64_t)gridDim.x * p.rows;
+  } while (s0 < p.S);
   if (p.refs_in_place) {
     for (int64_t i = tid; i <= cut; i += kBookThreads)
       if (p.refs[i] == 0)
