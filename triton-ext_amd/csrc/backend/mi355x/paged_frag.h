@@ -3,6 +3,7 @@
 #pragma once
 
 #include "attn_fwd.h"
+#include "page_rows.h"
 #include "paged_sched.h"
 
 namespace txk {
@@ -75,7 +76,7 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   __device__ __forceinline__ static uint32_t offset(int u, uint32_t st, int run, int row_bytes) {
     const int lane = threadIdx.x & 63, row = R * u + lane / CPR, pos = lane % CPR;
     const int c = pos ^ (V ? vswz(row) : kswz(row));
-    return 16 * c >= row_bytes ? kOOB : (uint32_t)(row & (run - 1)) * st + 16 * c;
+    return 16 * c >= row_bytes ? kOOB : page_run_row(row, run) * st + 16 * c;
   }
 
   // Per-lane LDS addresses of the fragment reads in a tile; the other fragments lie at
@@ -308,7 +309,7 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag16 {
   __device__ __forceinline__ static uint32_t offset(int u, uint32_t st, int run, int row_bytes) {
     const int lane = threadIdx.x & 63, row = R * u + lane / CPR, pos = lane % CPR;
     const int c = pos ^ (V ? vswz(row) : P32::kswz(row));
-    return 16 * c >= row_bytes ? P32::kOOB : (uint32_t)(row & (run - 1)) * st + 16 * c;
+    return 16 * c >= row_bytes ? P32::kOOB : page_run_row(row, run) * st + 16 * c;
   }
 
   //   K: key l%16, 16-byte chunk 4 c + l/16: dims 32 c + 8 (l/16) .. of MFMA c, or (e4m3) dims
@@ -562,34 +563,13 @@ __device__ __forceinline__ void issue_rows(const PageRow &pr, const PageSide &sd
     const uint32_t bytes = (uint32_t)(live - 1) * (uint32_t)sd.st + (uint32_t)row_bytes;
     return make_rsrc(at, id < 0 || live <= 0 ? 0 : bytes);
   };
-  // N resources of U / N loads each
-  auto fast = [&](auto count) {
-    constexpr int N = decltype(count)::value;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const i32x4_t rsrc = resource(n + A::R * (first + U / N * i));
-#pragma unroll
-      for (int u = U / N * i; u < U / N * (i + 1); ++u)
-        paged_dma<NT>(off[u], rsrc, lds + (first + u) * 1024);
-    }
-  };
-  if (sd.run >= U * A::R)
-    fast(std::integral_constant<int, 1>());
-  else if (U % 2 == 0 && 2 * sd.run >= U * A::R)
-    fast(std::integral_constant<int, U % 2 ? 1 : 2>());
-  else if (U % 4 == 0 && 4 * sd.run >= U * A::R)
-    fast(std::integral_constant<int, U % 4 ? 1 : 4>());
-  else { // pages of fewer rows; maybe fewer than a load has: the lanes of one at a time
-    const int lr = (threadIdx.x & 63) / A::CPR;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma nounroll
-      for (int r0 = 0; r0 < A::R; r0 += sd.run) {
-        const i32x4_t rsrc = resource(n + A::R * (first + u) + r0);
-        if (sd.run >= A::R || (lr & ~(sd.run - 1)) == r0)
+  const int lr = (threadIdx.x & 63) / A::CPR;
+  page_loads<U, A::R>(
+      first, sd.run, [&](int row) __attribute__((always_inline)) { return resource(n + row); },
+      [&](int u, const i32x4_t &rsrc, int r0) __attribute__((always_inline)) {
+        if (r0 < 0 || (lr & ~(sd.run - 1)) == r0)
           paged_dma<NT>(off[u], rsrc, lds + (first + u) * 1024);
-      }
-  }
+      });
 }
 
 } // namespace txk
