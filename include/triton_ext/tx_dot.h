@@ -253,6 +253,11 @@ TX_API const char *tx_get_last_error(void);
 TX_API const char *tx_kernel_name(int32_t kernel);
 /* 1 if a gfx950 device is visible to this process, else 0.  Never throws. */
 TX_API int tx_device_available(void);
+/* No counterpart in the reference.  *capture: 0, or the number of the capture into a graph that
+ * `stream` is part of, which no other capture of the process has.  A graph runs long after the calls
+ * that were captured, and in any order with others, so a workspace that it holds must stay its
+ * own, with a fill of the counters among its nodes. */
+TX_API int tx_stream_capture(void *stream, uint64_t *capture);
 
 #ifdef __cplusplus
 }

@@ -668,6 +668,17 @@ extern "C" TX_API int tx_device_available(void) {
   return cached[dev];
 }
 
+extern "C" TX_API int tx_stream_capture(void *stream, uint64_t *capture) {
+  clearError();
+  if (!capture)
+    return fail(TX_ERR_INVALID, "capture is NULL");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  TX_HIP_CHECK(hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id));
+  *capture = status == hipStreamCaptureStatusNone ? 0 : (uint64_t)id + 1;
+  return TX_OK;
+}
+
 extern "C" TX_API int tx_dot_plan_create(const tx_dot_desc *desc,
                                          tx_dot_plan *plan) {
   g_last_error.clear();

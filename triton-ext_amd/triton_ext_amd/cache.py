@@ -19,7 +19,7 @@ import ctypes
 import math
 
 from . import capi
-from .dot import _current_stream, _tx_of, workspace_for
+from .dot import _COUNTERS, _current_stream, _current_workspace, _tx_of, workspace_for
 
 # What a call's checks found for arguments of one form (shapes, strides, types, devices and
 # numbers, as bytes), so that a call of the same form goes to the launch at once.  Nothing here
@@ -366,9 +366,10 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     if out is None:
         out = make(q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    asked = workspace_for
     if stream is None:
-        stream = _current_stream(q.device)
-    ws = workspace if workspace is not None else workspace_for(needs, q.device, stream)
+        stream, asked = _current_stream(q.device), _current_workspace
+    ws = workspace if workspace is not None else asked(needs, q.device, stream)
     rc = native.call(launch, plan, q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale,
                      out, lse, ws, 0 if ws is None else ws.numel() * ws.element_size(), stream)
     if rc:
@@ -407,9 +408,6 @@ def _page_bytes(t, name, P):
             raise ValueError(f"{name}: a page must be one block of memory (strides {t.stride()})")
         n *= size
     return t.stride(0) * e, n * e
-
-
-_COUNTERS = 65536
 
 
 class _Pages:

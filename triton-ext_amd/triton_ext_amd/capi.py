@@ -157,6 +157,7 @@ EXPORTS = {
                               "tx_ring_reaches"],
     "libmi355x_dot.so": ["tx_dot_plan_create", "tx_dot_launch", "tx_dot_launch_noalloc",
                          "tx_get_last_error", "tx_kernel_name", "tx_device_available",
+                         "tx_stream_capture",
                          "tx_rotary_plan_create", "tx_rotary_launch",
                          "tx_paged_append_plan_create", "tx_paged_append_launch",
                          "tx_paged_attn_plan_create", "tx_paged_attn_launch",
@@ -224,6 +225,7 @@ def load(name="libmi355x_dot.so"):
                             ("paged_append", PagedAppendDesc, PagedAppendPlan),
                             ("paged_attn", PagedAttnDesc, PagedAttnPlan)):
             getattr(L, f"tx_{f}_plan_create").argtypes = [ctypes.POINTER(desc), ctypes.POINTER(pl)]
+        L.tx_stream_capture.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64)]
         L.tx_rotary_launch.argtypes = [ctypes.POINTER(RotaryPlan)] + [vp] * 5
         L.tx_paged_append_launch.argtypes = [ctypes.POINTER(PagedAppendPlan)] + [vp] * 13
         L.tx_paged_attn_launch.argtypes = ([ctypes.POINTER(PagedAttnPlan)] + [vp] * 11

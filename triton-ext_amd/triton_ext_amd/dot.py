@@ -3,6 +3,7 @@
 torch provides the device memory and the current HIP stream; all arithmetic
 runs in libmi355x_dot.so's kernels.
 """
+import contextlib
 import ctypes
 import math
 
@@ -10,7 +11,9 @@ from . import capi
 
 _TORCH_TYPES = {}
 _C_TYPES = {}
+_COUNTERS = 65536  # the arrival counters that every workspace begins with
 _workspaces = {}
+_captured = {}  # of the captures that are under way: (number of the capture, buffer)
 
 
 def _tx_of(dtype):
@@ -49,6 +52,16 @@ def _current_stream(device):
     if device.type != "cuda" or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@contextlib.contextmanager
+def _on_stream(device, stream):
+    """Makes the HIP stream of this handle torch's current one."""
+    import torch
+    s = (torch.cuda.ExternalStream(stream, device=device) if stream
+         else torch.cuda.default_stream(device))
+    with torch.cuda.device(device), torch.cuda.stream(s):
+        yield
 
 
 def _row_pitch(cols, elt_bytes):
@@ -206,30 +219,78 @@ def plan_for(a, b, out_dtype_tx, scale_mode=capi.SCALE_NONE, block=(0, 0, 0), fl
     return capi.plan(desc)
 
 
+def _capturing():
+    """Whether torch's current stream is being captured into a graph: from the first call on the
+    binding underneath torch.cuda.is_current_stream_capturing itself."""
+    global _capturing
+    import torch
+    _capturing = torch._C._cuda_isCurrentStreamCapturing
+    return _capturing()
+
+
+def _capture_of(device, stream):
+    """The number of the capture into a graph that `stream` is part of, 0 outside of one."""
+    if not _capturing() and stream == _current_stream(device):
+        return 0
+    number = ctypes.c_uint64(0)
+    capi.check(capi.load().tx_stream_capture(stream, ctypes.byref(number)))
+    return number.value
+
+
 def workspace_for(p, device, stream):
-    """A zero-initialised workspace of at least p.workspace_bytes, cached per
+    """A workspace of at least p.workspace_bytes with zeroed counters, cached per
     (device, stream): launches on one stream run one after another, so they
     may share it; launches on different streams may overlap and get their own.
 
-    Every plan's workspace starts with the decode kernel's arrival counters,
-    which must start at zero and which every completed launch leaves at zero
+    Every plan's workspace starts with the decode kernel's arrival counters
+    (64 KiB), which must start at zero and which every completed launch leaves at zero
     (the MX upcast writes only after them), so one buffer serves every plan.
     The buffer is allocated and zero-filled on `stream` itself, so the fill
     runs before any launch enqueued there after it, and torch's caching
     allocator orders the release of a buffer that grew too small after that
     stream's queued work.
+
+    A call that is captured into a graph gets a buffer of that capture's, whatever the eager
+    calls have: it comes from the graph's own memory, which torch keeps for as long as
+    the graph, and the fill of its counters is a node of the graph.  So the graph can be
+    replayed at any time, in any order with other graphs and after larger calls.
     """
-    import torch
     if p.workspace_bytes == 0:
         return None
-    key = (device if isinstance(device, torch.device) else torch.device(device), int(stream or 0))
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < p.workspace_bytes:
-        s = (torch.cuda.ExternalStream(int(stream), device=device) if stream
-             else torch.cuda.default_stream(device))
-        with torch.cuda.device(device), torch.cuda.stream(s):
-            ws = torch.zeros(int(p.workspace_bytes), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
+    if isinstance(device, (str, int)):
+        import torch
+        device = torch.device(device)
+    stream = int(stream or 0)
+    return _workspace(int(p.workspace_bytes), device, stream, _capture_of(device, stream))
+
+
+def _current_workspace(p, device, stream):
+    """workspace_for() of torch's current stream on `device`, with one question less."""
+    need = p.workspace_bytes
+    if need == 0:
+        return None
+    return _workspace(need, device, stream, _capture_of(device, stream) if _capturing() else 0)
+
+
+def _workspace(need, device, stream, capture):
+    key = (device, stream)
+    if not capture:
+        if _captured:  # the captures are over, and their graphs keep what they hold
+            _captured.clear()
+        ws = _workspaces.get(key)
+        if ws is not None and ws.numel() >= need:
+            return ws
+    import torch
+    if capture:
+        number, ws = _captured.get(key, (0, None))
+        if number != capture or ws.numel() < need:
+            with _on_stream(device, stream):
+                ws = torch.empty(need, dtype=torch.uint8, device=device)
+                ws[:_COUNTERS].zero_()
+            _captured[key] = (capture, ws)
+    else:
+        with _on_stream(device, stream):
+            ws = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
     return ws
 
 
@@ -294,9 +355,10 @@ def dot(a, b, out=None, out_dtype=None, scale_a=None, scale_b=None, scale_mode=N
                          "set exactly when acc is given")
     if M > 1 and ldc != p.desc.ldc:
         raise ValueError(f"out's row stride {ldc} differs from the plan's ldc {p.desc.ldc}")
+    asked = workspace_for
     if stream is None:
-        stream = _current_stream(a.device)
-    ws = workspace if workspace is not None else workspace_for(p, a.device, stream)
+        stream, asked = _current_stream(a.device), _current_workspace
+    ws = workspace if workspace is not None else asked(p, a.device, stream)
     L = capi.load()
     capi.check(L.tx_dot_launch(ctypes.byref(p), a.data_ptr(), b.data_ptr(), out.data_ptr(),
                                None if scale_a is None else scale_a.data_ptr(),
@@ -415,9 +477,10 @@ def dot_scaled(lhs, lhs_scale, lhs_format, rhs, rhs_scale, rhs_format, acc=None,
                          "set exactly when acc is given")
     if M > 1 and ldc != plan.desc.ldc:
         raise ValueError(f"out's row stride {ldc} differs from the plan's ldc {plan.desc.ldc}")
+    asked = workspace_for
     if stream is None:
-        stream = _current_stream(lhs.device)
-    ws = workspace_for(plan, lhs.device, stream)
+        stream, asked = _current_stream(lhs.device), _current_workspace
+    ws = asked(plan, lhs.device, stream)
     L = capi.load()
     capi.check(L.tx_dot_launch(ctypes.byref(plan), lhs.data_ptr(), rhs.data_ptr(),
                                out.data_ptr(),
