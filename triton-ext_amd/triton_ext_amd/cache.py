@@ -14,12 +14,16 @@ j % page_size.  A decoding step is
 and a chunk of several new tokens a sequence the same with cu_q, their starts in q, k
 and v.  Nothing here reads device memory on the host: every call can be captured into
 a graph and replayed with other contents.
+
+stream: the handle of the HIP stream to run on, torch's current one if None.  All of a call is in order
+on it: the copies of arguments that the kernels do not take as they lie, and the results, whose memory
+is that stream's.  The arguments have to be ready there.
 """
 import ctypes
 import math
 
 from . import capi
-from .dot import _COUNTERS, _current_stream, _current_workspace, _tx_of, workspace_for
+from .dot import _COUNTERS, _current_stream, _current_workspace, _on_stream, _tx_of
 
 # What a call's checks found for arguments of one form (shapes, strides, types, devices and
 # numbers, as bytes), so that a call of the same form goes to the launch at once.  Nothing here
@@ -66,6 +70,12 @@ def _dense(t):
 def _int32(t, name, dims):
     _is_int32(t, name, dims)
     return _dense(t)
+
+
+def _there(device, stream, f, *args, **kw):
+    """f with torch on `stream`, so that what it copies and allocates is in order with its launch."""
+    with _on_stream(device, stream):
+        return f(*args, **kw)
 
 
 def _same_device(device, **tensors):
@@ -138,6 +148,9 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     <= D: the dims past it are copied.  The pairs are dims (i, i + rot_dim / 2), or
     (2 i, 2 i + 1) when interleaved.  inverse: the transposed map, which takes the
     gradient of the result to that of x.  out may be x itself."""
+    if stream is not None and stream != _current_stream(x.device):
+        return _there(x.device, stream, rotary, x, positions, inv_freq, interleaved=interleaved,
+                      scale=scale, inverse=inverse, out=out)
     native = _native or _calls()
     form = native.form("rotary", x, positions, inv_freq, bool(interleaved), float(scale),
                        bool(inverse), out)
@@ -255,6 +268,10 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     The pages must be there (page_reserve); a token without one is not written.  fp16 or
     bf16; a float8_e4m3fn cache holds k / k_scale[head] and v / v_scale[head] (fp32 [Hkv];
     None: 1), saturated.  Rows of q from cu_q[B] on come back as they are."""
+    if stream is not None and stream != _current_stream(k.device):
+        return _there(k.device, stream, paged_append, k, v, k_cache, v_cache, page_table, kv_len,
+                      cu_q, q=q, inv_freq=inv_freq, interleaved=interleaved, scale=scale,
+                      k_scale=k_scale, v_scale=v_scale, q_out=q_out)
     native = _native or _calls()
     form = native.form("append", k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
                        bool(interleaved), float(scale), k_scale, v_scale, q_out)
@@ -333,6 +350,10 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     (times k_scale, v_scale, fp32 [Hkv]), D a multiple of 8 (e4m3: 16) up to 256.  Returns
     o [T, Hq, D], with return_lse also log2 of the sum of e^(score), fp32 [T, Hq] (-inf
     where nothing is attended to).  cu_q as for paged_append."""
+    if stream is not None and stream != _current_stream(q.device):
+        return _there(q.device, stream, paged_attention, q, k_cache, v_cache, page_table, kv_len, cu_q,
+                      sm_scale=sm_scale, causal=causal, window=window, k_scale=k_scale,
+                      v_scale=v_scale, out=out, return_lse=return_lse, workspace=workspace)
     import torch
     native = _native or _calls()
     form = native.form("attention", q, k_cache, v_cache, page_table, kv_len, cu_q, float(sm_scale),
@@ -366,10 +387,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     if out is None:
         out = make(q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    asked = workspace_for
     if stream is None:
-        stream, asked = _current_stream(q.device), _current_workspace
-    ws = workspace if workspace is not None else asked(needs, q.device, stream)
+        stream = _current_stream(q.device)
+    ws = workspace if workspace is not None else _current_workspace(needs, q.device, stream)
     rc = native.call(launch, plan, q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale,
                      out, lse, ws, 0 if ws is None else ws.numel() * ws.element_size(), stream)
     if rc:
@@ -431,7 +451,7 @@ class _Pages:
         self.workspace_bytes = _COUNTERS + need.value
 
     def scratch(self, device, stream):
-        return workspace_for(self, device, stream).data_ptr() + _COUNTERS
+        return _current_workspace(self, device, stream).data_ptr() + _COUNTERS
 
 
 def _book_checks(page_table, kv_len, refs, out, **more):
@@ -460,6 +480,8 @@ def _book_checks(page_table, kv_len, refs, out, **more):
 def page_copy(caches, src, dst, *, stream=None):
     """Copies page src[i] of every cache [P, ...] to page dst[i] (int32 [n]).  Entries
     outside [0, P) are skipped; no dst may be another dst, or a src but its own."""
+    if stream is not None and stream != _current_stream(src.device):
+        return _there(src.device, stream, page_copy, caches, src, dst)
     caches = list(caches)
     src, dst = _int32(src, "src", 1), _int32(dst, "dst", 1)
     if src.shape != dst.shape:
@@ -482,6 +504,9 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
     the other.  Returns page_table, kv_len, refs, and how many pages were missing (an
     int32 scalar on the device; those entries are -1).  out: the three tensors to write,
     which may be those read."""
+    if stream is not None and stream != _current_stream(refs.device):
+        return _there(refs.device, stream, page_reserve, page_table, kv_len, refs, new_len, page_size,
+                      out=out)
     native = _native or _calls()
     form = native.form("reserve", page_table, kv_len, refs, new_len, page_size, out)
     found = _forms.get(form)
@@ -511,6 +536,9 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
     """Sequences child[i] (empty rows, each named once) become copies of parent[i] that share
     its pages; a last page that is not full is copied, in every cache [P, page_size, ...],
     to a free one.  Returns page_table, kv_len, refs and the missing pages, as page_reserve."""
+    if stream is not None and stream != _current_stream(refs.device):
+        return _there(refs.device, stream, page_fork, caches, page_table, kv_len, refs, parent, child,
+                      out=out)
     caches = list(caches)
     native = _native or _calls()
     form = native.form("fork", page_table, kv_len, refs, parent, child, out, caches)
@@ -547,6 +575,9 @@ def page_fork(caches, page_table, kv_len, refs, parent, child, *, out=None, stre
 def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=None):
     """Sequences with drop[s] (bool [S]) give their pages back and become empty.  Returns
     page_table, kv_len, refs; out as for page_reserve."""
+    if stream is not None and stream != _current_stream(refs.device):
+        return _there(refs.device, stream, page_free, page_table, kv_len, refs, drop, page_size,
+                      out=out)
     import torch
     native = _native or _calls()
     form = native.form("free", page_table, kv_len, refs, drop, page_size, out)
@@ -574,6 +605,8 @@ def page_compact(caches, page_table, refs, *, out=None, stream=None):
     """Moves the pages in use (refs > 0) together: with U of them, those from U on go, in
     order, to the free ones below U, in every cache [P, ...] and in the books.  Returns
     page_table, refs and how many were moved (an int32 scalar on the device)."""
+    if stream is not None and stream != _current_stream(refs.device):
+        return _there(refs.device, stream, page_compact, caches, page_table, refs, out=out)
     caches = list(caches)
     native = _native or _calls()
     form = native.form("compact", page_table, refs, out, caches)
