@@ -50,6 +50,14 @@ def world(monkeypatch):
     monkeypatch.setattr(C, "_native", types.SimpleNamespace(form=native.form, call=launch,
                                                             addresses=native.addresses))
     monkeypatch.setattr(C, "_forms", {})
+    lib = capi.load()
+
+    class Library:
+        tx_dot_launch = tx_attn_fwd_launch = staticmethod(lambda *args: launch(*args))
+
+        def __getattr__(self, name):
+            return getattr(lib, name)
+    monkeypatch.setattr(capi, "load", lambda *name: Library())
     for module in (C, D):
         monkeypatch.setattr(module, "_current_stream", lambda device: w.now)
     monkeypatch.setattr(D, "_workspaces", {})
@@ -90,6 +98,13 @@ CALLS = {  # entry point, arguments, keywords
     "reserve": lambda: ("page_reserve", (ints(2, 4), ints(2), ints(8), ints(2), 16), {}),
     "fork": lambda: ("page_fork", (pools(), ints(2, 4), ints(2), ints(8), ints(1), ints(1)), {}),
     "free": lambda: ("page_free", (ints(2, 4), ints(2), ints(8), apart(2, dtype=torch.bool), 16), {}),
+    "dot": lambda: ("dot", (torch.zeros(40, 50, dtype=BF), torch.zeros(50, 60, dtype=BF)),
+                    {"acc": torch.zeros(40, 60)}),  # (rows not 16 bytes apart)
+    "dot, decode": lambda: ("dot", (torch.zeros(16, 4104, dtype=BF), torch.zeros(4104, 4096, dtype=BF)), {}),
+    "dot_scaled": lambda: ("dot_scaled", (torch.zeros(32, 64, dtype=torch.uint8), None, "e4m3",
+                                          torch.zeros(64, 40, dtype=torch.uint8), None, "e4m3"), {}),
+    "dense attention": lambda: ("attention", (torch.zeros(1, 1, 128, 32, dtype=BF).expand(1, 2, 128, 32),
+                                              *[torch.zeros(1, 2, 128, 32, dtype=BF)] * 2, True, 0.5), {}),
     "compact": lambda: ("page_compact", (pools(), ints(2, 4), ints(8)), {}),
 }
 

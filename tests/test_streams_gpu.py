@@ -105,3 +105,17 @@ def test_host_tensors_are_refused(gpu, stream):
                  lambda s: tx.page_compact([kc], t, r, stream=s)):
         with pytest.raises(ValueError):
             call(stream)
+
+
+def test_dots_and_dense_attention(gpu, busy):
+    say("stream=, dots")
+    g = gen(7)
+    a, b = randn(g, 70, 301, dtype=BF).to(gpu), randn(g, 301, 90, dtype=BF).to(gpu)
+    acc = randn(g, 70, 90).to(gpu)
+    both(lambda s: (tx.dot(a, b, acc=acc, stream=s),), busy)
+    few, wide = randn(g, 16, 4100, dtype=BF).to(gpu), randn(g, 4100, 4096, dtype=BF).to(gpu)
+    both(lambda s: (tx.dot(few, wide, stream=s),), busy)
+    x, y = (torch.randint(0, 100, n, generator=g).to(torch.uint8).to(gpu) for n in ((40, 64), (64, 72)))
+    both(lambda s: (tx.dot_scaled(x, None, "e4m3", y, None, "e4m3", stream=s),), busy)
+    q, k = randn(g, 2, 1, 256, 64, dtype=BF).to(gpu).expand(2, 4, 256, 64), randn(g, 2, 4, 256, 64, dtype=BF).to(gpu)
+    both(lambda s: tx.attention(q, k, k, True, 0.2, return_lse=True, stream=s), busy)

@@ -23,7 +23,7 @@ import ctypes
 import math
 
 from . import capi
-from .dot import _COUNTERS, _current_stream, _current_workspace, _on_stream, _tx_of
+from .dot import _COUNTERS, _current_stream, _current_workspace, _there, _tx_of
 
 # What a call's checks found for arguments of one form (shapes, strides, types, devices and
 # numbers, as bytes), so that a call of the same form goes to the launch at once.  Nothing here
@@ -70,12 +70,6 @@ def _dense(t):
 def _int32(t, name, dims):
     _is_int32(t, name, dims)
     return _dense(t)
-
-
-def _there(device, stream, f, *args, **kw):
-    """f with torch on `stream`, so that what it copies and allocates is in order with its launch."""
-    with _on_stream(device, stream):
-        return f(*args, **kw)
 
 
 def _same_device(device, **tensors):

@@ -64,6 +64,12 @@ def _on_stream(device, stream):
         yield
 
 
+def _there(device, stream, f, *args, **kw):
+    """f with torch on `stream`, so that what it copies and allocates is in order with its launch."""
+    with _on_stream(device, stream):
+        return f(*args, **kw)
+
+
 def _row_pitch(cols, elt_bytes):
     """Elements per row rounded up to a 16-byte multiple."""
     q = 16 // math.gcd(16, elt_bytes)
@@ -296,7 +302,9 @@ def _workspace(need, device, stream, capture):
 
 def dot(a, b, out=None, out_dtype=None, scale_a=None, scale_b=None, scale_mode=None,
         block=(0, 0, 0), flags=0, plan=None, workspace=None, stream=None, acc=None):
-    """C = epilogue(A @ B) on the current device's stream.
+    """C = epilogue(A @ B) on torch's current stream, or on the one whose handle `stream` is,
+    which then is torch's current one for all of the call (copies of operands and the result's
+    memory among it).
 
     scale_mode defaults to ROWCOL when int8 operands come with scales, to
     BLOCK128 for fp8 operands with scales, else NONE.  acc (fp32 or int32
@@ -311,6 +319,9 @@ def dot(a, b, out=None, out_dtype=None, scale_a=None, scale_b=None, scale_mode=N
     16-byte row strides.
     """
     import torch
+    if stream is not None and stream != _current_stream(a.device):
+        return _there(a.device, stream, dot, a, b, out, out_dtype, scale_a, scale_b, scale_mode, block,
+                      flags, plan, workspace, None, acc)
     ta = tx_type(a)
     if scale_mode is None:
         if scale_a is None:
@@ -355,10 +366,9 @@ def dot(a, b, out=None, out_dtype=None, scale_a=None, scale_b=None, scale_mode=N
                          "set exactly when acc is given")
     if M > 1 and ldc != p.desc.ldc:
         raise ValueError(f"out's row stride {ldc} differs from the plan's ldc {p.desc.ldc}")
-    asked = workspace_for
     if stream is None:
-        stream, asked = _current_stream(a.device), _current_workspace
-    ws = workspace if workspace is not None else asked(p, a.device, stream)
+        stream = _current_stream(a.device)
+    ws = workspace if workspace is not None else _current_workspace(p, a.device, stream)
     L = capi.load()
     capi.check(L.tx_dot_launch(ctypes.byref(p), a.data_ptr(), b.data_ptr(), out.data_ptr(),
                                None if scale_a is None else scale_a.data_ptr(),
@@ -396,6 +406,9 @@ def dot_scaled(lhs, lhs_scale, lhs_format, rhs, rhs_scale, rhs_format, acc=None,
     padded storage first.
     """
     import torch
+    if stream is not None and stream != _current_stream(lhs.device):
+        return _there(lhs.device, stream, dot_scaled, lhs, lhs_scale, lhs_format, rhs, rhs_scale,
+                      rhs_format, acc, fast_math, lhs_k_pack, rhs_k_pack, out_dtype, out, block, plan)
     for name, fmt in (("lhs_format", lhs_format), ("rhs_format", rhs_format)):
         if fmt not in ("e2m1", "e4m3", "e5m2", "bf16", "fp16"):
             raise ValueError(f"NYI: {name} {fmt}")
@@ -477,10 +490,9 @@ def dot_scaled(lhs, lhs_scale, lhs_format, rhs, rhs_scale, rhs_format, acc=None,
                          "set exactly when acc is given")
     if M > 1 and ldc != plan.desc.ldc:
         raise ValueError(f"out's row stride {ldc} differs from the plan's ldc {plan.desc.ldc}")
-    asked = workspace_for
     if stream is None:
-        stream, asked = _current_stream(lhs.device), _current_workspace
-    ws = asked(plan, lhs.device, stream)
+        stream = _current_stream(lhs.device)
+    ws = _current_workspace(plan, lhs.device, stream)
     L = capi.load()
     capi.check(L.tx_dot_launch(ctypes.byref(plan), lhs.data_ptr(), rhs.data_ptr(),
                                out.data_ptr(),
@@ -511,6 +523,9 @@ def attention(q, k, v, causal, sm_scale, USE_TMA=True, *, return_lse=False, plan
     return_lse, plan, stream and block are keyword-only.
     """
     import torch
+    if stream is not None and stream != _current_stream(q.device):
+        return _there(q.device, stream, attention, q, k, v, causal, sm_scale, USE_TMA,
+                      return_lse=return_lse, plan=plan, block=block)
     if q.dim() != 4 or k.shape != q.shape or v.shape != q.shape:
         raise ValueError(f"q, k, v must share one [Z, H, N_CTX, HEAD_DIM] shape: "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
