@@ -18,8 +18,11 @@ a graph and replayed with other contents.
 stream: the handle of the HIP stream to run on, torch's current one if None.  All of a call is in order
 on it: the copies of arguments that the kernels do not take as they lie, and the results, whose memory
 is that stream's.  The arguments have to be ready there.
+
+rotary has a gradient in torch's backward pass; the calls on the cache are for generation and have none.
 """
 import ctypes
+import functools
 import math
 
 from . import capi
@@ -141,10 +144,16 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     positions int32 or int64; inv_freq fp32 [rot_dim / 2] (rotary_frequencies), rot_dim
     <= D: the dims past it are copied.  The pairs are dims (i, i + rot_dim / 2), or
     (2 i, 2 i + 1) when interleaved.  inverse: the transposed map, which takes the
-    gradient of the result to that of x.  out may be x itself."""
+    gradient of the result to that of x; torch's backward pass calls it by itself where x
+    requires a gradient (positions and inv_freq get none).  out may be x itself; a result in
+    it has no gradient, so an x that requires one is refused."""
     if stream is not None and stream != _current_stream(x.device):
         return _there(x.device, stream, rotary, x, positions, inv_freq, interleaved=interleaved,
                       scale=scale, inverse=inverse, out=out)
+    if x.requires_grad and _grad_enabled():
+        if out is not None:
+            raise ValueError("out takes no gradient: x requires one (x.detach(), or torch.no_grad())")
+        return _differentiable()(x, positions, inv_freq, interleaved, scale, inverse)
     native = _native or _calls()
     form = native.form("rotary", x, positions, inv_freq, bool(interleaved), float(scale),
                        bool(inverse), out)
@@ -168,6 +177,32 @@ def rotary(x, positions, inv_freq, *, interleaved=False, scale=1.0, inverse=Fals
     if rc:
         capi.check(rc)
     return out
+
+
+def _grad_enabled():
+    import torch
+    return torch.is_grad_enabled()
+
+
+@functools.lru_cache(None)
+def _differentiable():
+    """rotary with its gradient."""
+    import torch
+
+    class Rotary(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, positions, inv_freq, interleaved, scale, inverse):
+            ctx.save_for_backward(positions, inv_freq)
+            ctx.how = interleaved, scale, inverse
+            return rotary(x, positions, inv_freq, interleaved=interleaved, scale=scale,
+                          inverse=inverse)
+
+        @staticmethod
+        def backward(ctx, dy):
+            interleaved, scale, inverse = ctx.how
+            return (rotary(dy, *ctx.saved_tensors, interleaved=interleaved, scale=scale,
+                           inverse=not inverse),) + (None,) * 5
+    return Rotary.apply
 
 
 def _rotary_checks(x, positions, inv_freq, out):
