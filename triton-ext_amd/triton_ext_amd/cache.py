@@ -24,6 +24,7 @@ rotary has a gradient in torch's backward pass; the calls on the cache are for g
 import ctypes
 import functools
 import math
+from operator import index
 
 from . import capi
 from .dot import _COUNTERS, _current_stream, _current_workspace, _there, _tx_of
@@ -537,6 +538,7 @@ def page_reserve(page_table, kv_len, refs, new_len, page_size, *, out=None, stre
         return _there(refs.device, stream, page_reserve, page_table, kv_len, refs, new_len, page_size,
                       out=out)
     native = _native or _calls()
+    page_size = index(page_size)
     form = native.form("reserve", page_table, kv_len, refs, new_len, page_size, out)
     found = _forms.get(form)
     if found is None:
@@ -609,6 +611,7 @@ def page_free(page_table, kv_len, refs, drop, page_size, *, out=None, stream=Non
                       out=out)
     import torch
     native = _native or _calls()
+    page_size = index(page_size)
     form = native.form("free", page_table, kv_len, refs, drop, page_size, out)
     found = _forms.get(form)
     if found is None:
