@@ -13,7 +13,8 @@
  *
  * All arrays are device memory; index arrays are int32.  No launch reads
  * lengths or tables on the host, so all can be captured into a graph and replayed with
- * other contents.  Contents out of range (a page outside [0, P), positions past
+ * other contents (a workspace then is the graph's alone, its counters cleared by a node of
+ * the graph).  Contents out of range (a page outside [0, P), positions past
  * the table, cu_q past T) are skipped by the kernels, never followed.  A plan
  * is a plain struct that the caller keeps; the launch plans its descriptor
  * again and refuses one that differs.  Errors: return codes and

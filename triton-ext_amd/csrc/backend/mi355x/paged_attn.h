@@ -324,9 +324,10 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
 // V_k is (and K_k's slot free, for K_{k+2}), so that loads have about two blocks' time to land.  All
 // of K's fragments are under way before the first of their MFMAs, all of V's before the softmax.
 // Bound by the matrix cores and the softmax's VALU work in turn: chunks of 2048 tokens of two
-// sequences of 11869 and 16384 keys, 32 heads of 128 over 8: 955 us, 920 TFLOP/s, the MFMAs busy 52%
-// of the time, the VALU 46%, at 1.7 GHz under the power limit (S_{k+1} computed beside the softmax of
-// S_k, which leaves registers for single fragments: 967; s_setprio around the MFMAs: 999).  24
+// sequences of 11869 and 16384 keys, 32 heads of 128 over 8: 970 us (960 .. 980 from card to card),
+// 907 TFLOP/s, the MFMAs busy 51% of the time, the VALU 46%, at 1.7 GHz under the power limit (S_{k+1}
+// computed beside the softmax of S_k, which leaves registers for single fragments: 1% more; s_setprio
+// around the MFMAs: 5% more).  24
 // sequences of 1 .. 300 tokens with a window, heads of 64: 36 us, bound by the beginning and end of
 // units (about 7 us each).
 template <class A> constexpr int paged_rows_groups() { return A::D > 128 ? 1 : A::D > 64 ? 2 : 3; }
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
 
   if (wave == 0) {
     Sched sched(args, st);
-    // the 8 XCDs take contiguous runs: a head's keys stay in one L2 (chunks of 2048: 987 -> 967 us)
+    // the 8 XCDs take contiguous runs: a head's keys stay in one L2 (chunks of 2048: 2% less)
     const uint32_t n = gridDim.x, b = blockIdx.x;
     sched.init(n % 8 == 0 ? (b % 8) * (n / 8) + b / 8 : b, n);
     sched.get(st.unit[0]);
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
     const PageSide sv{p.vc + un.hk * p.v_sh, p.v_sp, p.v_st, p.v_run};
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
     // Keys that no other unit reads go past the caches (64 rows of each of 16 sequences of 16384 keys:
-    // 230 -> 209 us); those that others do must not (chunks of 2048: 955 -> 1150).
+    // 230 -> 209 us); those that others do must not (chunks of 2048: 20% more).
     const bool once = un.alone;
     auto issue = [&](const PageSide &sd, int k, const uint32_t (&off)[U],
                      uint32_t lds) __attribute__((always_inline)) {

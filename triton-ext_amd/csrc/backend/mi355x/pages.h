@@ -7,7 +7,8 @@
 // are free), rather than wait for it.  That needs the books that all read to stay as they are:
 // where counts or lengths are written in place, the launch has one workgroup.  Free pages are
 // taken in ascending order whatever the timing, so results do not depend on it.
-// 256 rows of 512 entries and 65536 pages: page_reserve 6.9 us (one workgroup: 129); 64 rows of 256
+// 256 rows of 512 entries and 65536 pages: page_reserve 6.5 us (one workgroup: 129) where
+// free pages lie at the front, 34 a call where they come after 65000 that are held; 64 rows of 256
 // and 4096 pages: page_compact's books 9.3 us (19.6), page_free 4.7 and the counts' copy 2.2 (19.6);
 // 56 children of 64 entries: page_fork's 8.6 us (11).
 // Pages are copied by a kernel of their own that takes its list (and, compacting, its
