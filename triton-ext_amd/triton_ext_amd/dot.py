@@ -44,14 +44,24 @@ def _torch_dtype(tx):
     return _C_TYPES[tx]
 
 
+def _raw_stream(index):
+    """The handle of torch's current HIP stream on a device: from the first call on the binding
+    underneath torch.cuda.current_stream itself."""
+    global _raw_stream
+    import torch
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    return _raw_stream(index)
+
+
 def _current_stream(device):
     """The handle of torch's current HIP stream on `device`.  Asked of the
     binding underneath torch.cuda.current_stream, whose Stream object costs
-    1.8 us against 0.06 us here, on every call."""
-    import torch
-    if device.type != "cuda" or device.index is None:
+    1.8 us against 0.25 us here, on every call."""
+    index = device.index
+    if index is None or device.type != "cuda":
+        import torch
         return torch.cuda.current_stream(device).cuda_stream
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return _raw_stream(index)
 
 
 @contextlib.contextmanager
