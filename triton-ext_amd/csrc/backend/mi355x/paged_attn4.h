@@ -1,0 +1,617 @@
+// Attention of new tokens over a paged cache held in 4 bits (tx_cache4.h).  Units of work, their
+// schedule, softmax, masks and joins are those of paged_attn.h; keys and values come otherwise.
+//
+// A row of codes is 16 .. 128 bytes, a quarter of what LDS tiles of 16-bit pages are made for, so
+// they are loaded into registers, straight from the pages: of 16 keys, lane (m, g) takes the
+// g-th quarter of key m's row (of 256 dims: one 16-byte piece of each half) and its scales, one byte
+// each.  A piece is 8 bytes (heads of up to 64) or 16 (32 dims: one or two blocks), so the
+// conversion to 16 bits needs one or two factors.
+//
+// K: S^T = K . Q^T does not ask in which order dims are summed.  With m = lane % 16 the lane's
+// dims are an operand of the 16x16x32 MFMAs as they stand, Q is loaded in the same order, and K
+// never goes through LDS.  V: the product needs several keys of one dim in a lane, so with m =
+// lane / 4 its values are written into an LDS tile of 16-bit rows and read transposed.
+//
+// Lanes of keys that are not there read page 0 (there is one, or nothing is read); whatever it
+// holds, their scores are -inf and their V finite: a scale that may make no number is taken as 0
+// in V, and the key's score is NaN instead for the rows that attend to it.
+#pragma once
+
+#include "cache4.h"
+#include "cache4_rows.h"
+#include "paged_attn.h"
+
+namespace txk {
+
+struct Paged4Args {
+  PagedAttnArgs a; // (first: paged_args() reads it)
+  BlockScales ks, vs;
+};
+__device__ __forceinline__ const Paged4Args &paged4_args() {
+  return reinterpret_cast<const Paged4Args &>(paged_args());
+}
+
+// What a lane holds of one key's K or V row, in the order of its quarter g.
+template <int D, bool NV> struct Piece4 {
+  static constexpr int KW = D == 64 ? 2 : D == 256 ? 8 : 4; // dwords of 8 dims
+  static constexpr int SB = D == 64 ? 1 : (D == 256 ? 2 : 1) * (NV ? 2 : 1);
+  uint32_t w[KW], s[SB];
+
+  // The dims of dword c, and the scale among s that is theirs.
+  __device__ __forceinline__ static constexpr int dim(int c, int g) {
+    return D == 64 ? 16 * g + 8 * c : 128 * (c / 4) + 32 * g + 8 * (c % 4);
+  }
+  __device__ __forceinline__ static constexpr int scale_of(int c) {
+    return D == 64 ? 0 : NV ? c / 2 : c / 4;
+  }
+  __device__ __forceinline__ static constexpr int block_of(int j, int g) {
+    if (D == 64)
+      return NV ? g : g / 2;
+    return NV ? 8 * (j / 2) + 2 * g + j % 2 : 4 * j + g;
+  }
+};
+
+// Where lane (m, g) finds its pieces of K or V: the codes and scales of a head, and the lane's own
+// offsets from the first of 8 keys.  Pieces past head_dim are those of its beginning (Q is 0 there;
+// V's are not stored).
+template <int D, bool NV> struct Side4 {
+  typedef Piece4<D, NV> P;
+  const uint8_t *codes, *scales;
+  int64_t sp, st, ssp, sst;
+  int64_t row, srow;  // (m & 7) rows
+  uint32_t at[D == 256 ? 2 : 1];
+  int64_t sat[P::SB];
+  bool upper; // m & 8
+
+  __device__ __forceinline__ Side4(const uint8_t *c, int64_t sp_, int64_t st_, int64_t sh,
+                                   const BlockScales &bs, int hk, int head_dim, int m, int g)
+      : codes(c + hk * sh), scales(bs.s + hk * bs.sh), sp(sp_), st(st_), ssp(bs.sp), sst(bs.st),
+        row((m & 7) * st_), srow((m & 7) * bs.st), upper(m & 8) {
+    const int bytes = head_dim / 2;
+#pragma unroll
+    for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
+      const int o = D == 64 ? 8 * g : 64 * i + 16 * g;
+      at[i] = o < bytes ? o : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < P::SB; ++j) {
+      const int b = P::block_of(j, g);
+      sat[j] = (b < head_dim / (NV ? 16 : 32) ? b : 0) * bs.sb;
+    }
+  }
+  // The pieces of keys n + m; m is the lane's row again.
+  __device__ __forceinline__ void load(const PageRow &pr, int n, int m, P &x) const {
+    const uint8_t *c, *s;
+    if (pr.shift >= 3) { // 8 keys of one page
+      const int ea = (n >> pr.shift) - pr.first, eb = ((n + 8) >> pr.shift) - pr.first;
+      int a = lane_value(pr.ids, ea & 63), b = lane_value(pr.ids, eb & 63);
+      a = a < 0 ? 0 : a, b = b < 0 ? 0 : b;
+      const int mask = (1 << pr.shift) - 1, sa = n & mask, sb = (n + 8) & mask;
+      const uint8_t *const ca = codes + (int64_t)a * sp + (int64_t)sa * st;
+      const uint8_t *const cb = codes + (int64_t)b * sp + (int64_t)sb * st;
+      const uint8_t *const ka = scales + (int64_t)a * ssp + (int64_t)sa * sst;
+      const uint8_t *const kb = scales + (int64_t)b * ssp + (int64_t)sb * sst;
+      c = (upper ? cb : ca) + row;
+      s = (upper ? kb : ka) + srow;
+    } else {
+      const int key = n + m;
+      int a = __shfl(pr.ids, ((key >> pr.shift) - pr.first) & 63);
+      a = a < 0 ? 0 : a;
+      const int slot = key & ((1 << pr.shift) - 1);
+      c = codes + (int64_t)a * sp + (int64_t)slot * st;
+      s = scales + (int64_t)a * ssp + (int64_t)slot * sst;
+    }
+    typedef uint32_t w2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+    if constexpr (D == 64) {
+      const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2 *>(c + at[0]));
+      x.w[0] = v[0], x.w[1] = v[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < P::KW / 4; ++i) {
+        const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4 *>(c + at[i]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x.w[4 * i + e] = v[e];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < P::SB; ++j)
+      x.s[j] = __builtin_nontemporal_load(s + sat[j]);
+  }
+};
+
+// Q in the type that codes are computed in.  bf16 rows under e4m3 scales become fp16, times the
+// power of two that takes the row's largest magnitude to [2^7, 2^8): exact but for what is below
+// 2^-31 of that.  Returns what the row's scores are to be multiplied by.
+// x: the lane's dims of a row; the lanes of a row: those that `row_max` goes over.
+template <bool BF, int N, class F>
+__device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
+  if constexpr (!BF) {
+    return 1.f;
+  } else {
+    float mx = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mx = fmaxf(mx, fabsf(__uint_as_float((uint32_t)x[c][i] << 16)));
+        mx = fmaxf(mx, fabsf(__uint_as_float((uint32_t)x[c][i] & 0xffff0000u)));
+      }
+    mx = row_max(mx);
+    const int e = (__float_as_uint(mx) >> 23) & 255;
+    // (0, infinity: as it is)
+    const int up = e == 0 || e == 255 ? 0 : 134 - e < 127 ? 134 - e : 127;
+    const float f = __builtin_amdgcn_ldexpf(1.f, up);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const half2_t h = {(_Float16)(__uint_as_float((uint32_t)x[c][i] << 16) * f),
+                           (_Float16)(__uint_as_float((uint32_t)x[c][i] & 0xffff0000u) * f)};
+        x[c][i] = __builtin_bit_cast(uint32_t, h);
+      }
+    return __builtin_amdgcn_ldexpf(1.f, -up);
+  }
+}
+
+// Which of 16 keys (four adjacent lanes each) a lane's flag is set of.
+__device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
+  uint64_t x = lanes | lanes >> 1;
+  x |= x >> 2;
+  uint32_t r = 0;
+  for (int i = 0; i < 16; ++i)
+    r |= (uint32_t)(x >> (4 * i) & 1) << i;
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the waves of a workgroup share out the keys
+// ---------------------------------------------------------------------------
+
+// RT: blocks of 16 rows, which share the fragments of K and V.
+template <int D_, bool BF, bool NV_, int RT_> struct Paged4Split {
+  static constexpr int D = D_, BN = 32, RT = RT_, ROWS = 16 * RT;
+  static constexpr bool NV = NV_, CBF = BF && !NV;
+  typedef Code4<CBF, NV> Code;
+  typedef PagedFrag16<D, CBF, false, BN> P16; // of the values in 16 bits
+  typedef Piece4<D, NV> Piece;
+  typedef typename AttnFwd<64, BF, 32, 64>::elt elt; // of q and o
+  typedef typename AttnFwd<64, BF, 32, 64>::h4 h4;
+  typedef typename P16::h8 h8;
+  static constexpr int QUADS = RT * P16::QUADS;
+  static constexpr int TILE = P16::TILE, BYTES = TILE > ROWS * D * 4 ? TILE : ROWS * D * 4;
+  __device__ __forceinline__ static int quad_at(int row, int qd) {
+    return (row >> 4) * P16::QUADS * 64 + P16::quad_at(row & 15, qd);
+  }
+};
+
+// Workgroups of a CU: by LDS, and by registers where heads are long.
+template <class A> constexpr int paged4_split_groups() { return A::BYTES * 4 <= 81920 ? 2 : 1; }
+
+template <class A>
+__global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_split_kernel(Paged4Args args4) {
+  constexpr int D = A::D, BN = A::BN, RT = A::RT, ROWS = A::ROWS, NS = 2;
+  typedef typename A::P16 P16;
+  typedef typename A::Piece Piece;
+  typedef typename A::Code Code;
+  typedef typename A::elt elt;
+  typedef PagedSched<ROWS, BN, 4, kSplitOverhead> Sched;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4][A::BYTES];
+  __shared__ float ms[4][ROWS], ls[4][ROWS];
+  __shared__ PagedSchedState st;
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  if (wave == 0) {
+    Sched sched(args4.a, st);
+    sched.init(blockIdx.x, gridDim.x);
+    sched.get(st.unit[0]);
+  }
+  __syncthreads();
+
+  const uint32_t v_lds = lds_addr(smem[wave]);
+  typename P16::Bases bs;
+  P16::bases(v_lds, v_lds, bs);
+  const int km = lane & 15, kg = lane >> 4, vm = lane >> 2, vg = lane & 3;
+  uint32_t vw[Piece::KW]; // where the lane's values of V go in the tile (16 rows on: 16 * ROW)
+#pragma unroll
+  for (int c = 0; c < Piece::KW; ++c)
+    vw[c] = v_lds + vm * P16::ROW + (((Piece::dim(c, vg) / 8) ^ P16::vswz(vm)) << 4);
+
+  for (int turn = 0;; turn ^= 1) {
+    const Paged4Args &p4 = paged4_args();
+    const PagedAttnArgs &p = p4.a;
+    const PagedUnit un = paged_unit(st.unit[turn]);
+    if (un.rows <= 0)
+      break;
+    // this wave's blocks
+    int k0 = 0, k1 = 0;
+    if (un.hi > un.lo) {
+      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
+      const int w0 = first + 4 * (int)un.s0;
+      const int w1 = last - first < 4 * (int64_t)un.s1 ? last : first + 4 * (int)un.s1;
+      const int q = (w1 - w0 + 3) / 4;
+      k0 = w0 + wave * q < w1 ? w0 + wave * q : w1;
+      k1 = k0 + q < w1 ? k0 + q : w1;
+    }
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
+    const Side4<D, A::NV> sk(p.kc, p.k_sp, p.k_st, p.k_sh, p4.ks, un.hk, p.head_dim, km, kg);
+    const Side4<D, A::NV> sv(p.vc, p.v_sp, p.v_st, p.v_sh, p4.vs, un.hk, p.head_dim, vm, vg);
+    // The table, Q and the first blocks are under way together, and meanwhile the first wave
+    // looks up the next unit.
+    if (k0 < k1)
+      pr.load(k0 * BN);
+    u32x4 qf[RT][Piece::KW];
+    int rr[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = 16 * i + km;
+      rr[i] = un.r0 + (r < un.rows ? r : 0);
+      const int of = paged_token(p, rr[i]), head = un.hk * p.G + rr[i] - of * p.G;
+      const elt *row = static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh;
+#pragma unroll
+      for (int c = 0; c < Piece::KW; ++c) {
+        const int d = Piece::dim(c, kg);
+        qf[i][c] = *reinterpret_cast<const u32x4 *>(row + (d < p.head_dim ? d : 0));
+      }
+    }
+    Piece kp[NS][2], vp[NS][2];
+    uint64_t here[NS + 1] = {}; // of blocks k .. k + NS
+    if (k0 < k1) {
+      pr.settle();
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (k0 + i < k1) {
+          const int n = (k0 + i) * BN;
+          pr.hold(n);
+          here[i] = pr.template there<BN>(n, un.hi);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            sk.load(pr, n + 16 * b, km, kp[i][b]), sv.load(pr, n + 16 * b, vm, vp[i][b]);
+        }
+    }
+    if (wave == 0)
+      Sched(p, st).get(st.unit[turn ^ 1]);
+    int lo[RT], hi[RT]; // of the lane's rows
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+      paged_keys(p, un.pos0, un.len, rr[i], rr[i] + 1, lo[i], hi[i]);
+    // keys that every row attends to
+    int lo_all, hi_all, skip;
+    paged_keys(p, un.pos0, un.len, un.r0, un.r0 + 1, skip, hi_all);
+    paged_keys(p, un.pos0, un.len, un.r0 + un.rows - 1, un.r0 + un.rows, lo_all, skip);
+    const float scale0 = p.qk_scale * (p.k_scale ? p.k_scale[un.hk] : 1.f);
+    float scale[RT]; // of the lane's rows
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const bool live = 16 * i + km < un.rows;
+#pragma unroll
+      for (int c = 0; c < Piece::KW; ++c)
+        qf[i][c] = __builtin_bit_cast(
+            u32x4, P16::P32::settled(__builtin_bit_cast(typename P16::h8, qf[i][c]),
+                                     live && Piece::dim(c, kg) < p.head_dim, scale0));
+      scale[i] = scale0 == 0.f ? 1.f : fabsf(scale0);
+      if constexpr (A::NV)
+        scale[i] *= q4_to_f16<!std::is_same<elt, _Float16>::value>(
+            qf[i], [](float v) { return P16::row_max(v); });
+    }
+    float m[RT], l[RT];
+    typename P16::Acc acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+      for (int b = 0; b < P16::NV; ++b)
+        acc[i][b] = typename P16::f4v{};
+    }
+    auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
+      constexpr int SL = decltype(slot_c)::value;
+      const int n0 = k * BN, na = n0 + NS * BN;
+      typename P16::Scores s[RT];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Piece &x = kp[SL][b];
+        uint32_t f[Piece::SB];
+#pragma unroll
+        for (int j = 0; j < Piece::SB; ++j)
+          f[j] = Code::factor(x.s[j], false);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          s[i][b] = typename P16::f4v{};
+#pragma unroll
+        for (int c = 0; c < Piece::KW; ++c) {
+          const auto kf = __builtin_bit_cast(typename P16::h8, Code::eight(x.w[c], f[Piece::scale_of(c)]));
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            s[i][b] = P16::mfma(kf, __builtin_bit_cast(typename P16::h8, qf[i][c]), s[i][b]);
+        }
+      }
+      uint64_t none[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Piece &x = vp[SL][b];
+        uint32_t f[Piece::SB];
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < Piece::SB; ++j)
+          bad = bad || Code::bad(x.s[j]), f[j] = Code::factor(x.s[j], true);
+        none[b] = __ballot(bad);
+#pragma unroll
+        for (int c = 0; c < Piece::KW; ++c) {
+          typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+          *(lds_u32x4 *)(uintptr_t)(vw[c] + b * 16 * P16::ROW) = Code::eight(x.w[c], f[Piece::scale_of(c)]);
+        }
+      }
+      if (k + NS < k1) {
+        pr.hold(na);
+        here[NS] = pr.template there<BN>(na, un.hi);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          sk.load(pr, na + 16 * b, km, kp[SL][b]), sv.load(pr, na + 16 * b, vm, vp[SL][b]);
+      }
+      if (__builtin_expect((none[0] | none[1]) != 0, 0)) {
+        const uint32_t nan = (keys_of(none[0]) | keys_of(none[1]) << 16) >> (4 * kg);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[i][b][r] = nan >> (16 * b + r) & 1 ? __builtin_nanf("") : s[i][b][r];
+      }
+      const uint64_t all = ~0ull >> (64 - BN);
+      typename P16::PF pf[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
+          const int a = lo[i] - n0 < 0 ? 0 : lo[i] - n0, z = hi[i] - n0 < 0 ? 0 : hi[i] - n0;
+          uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
+          seen &= a < 64 ? ~0ull << a : 0;
+          P16::mask(s[i], seen & here[0]);
+        }
+        P16::softmax(s[i], scale[i], acc[i], m[i], l[i], pf[i]);
+      }
+#pragma unroll
+      for (int b0 = 0; b0 < P16::NV; b0 += P16::VN) {
+        typename P16::template VF<P16::VN> vf;
+        P16::read_v(bs, 0, b0, vf);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          P16::pv(vf, b0, pf[i], acc[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        here[i] = here[i + 1];
+    };
+    for (int k = k0; k < k1;) {
+      iter(k++, std::integral_constant<int, 0>());
+      if (k < k1)
+        iter(k++, std::integral_constant<int, 1>());
+    }
+
+    // The waves' sums: quads of 4 dims in lane order in each one's own tile.
+    const PagedAttnArgs &pe = paged_args();
+    const PagedUnit ue = paged_unit(st.unit[turn]);
+    const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      l[i] = P16::row_sum(l[i]);
+      if (k0 < k1) {
+#pragma unroll
+        for (int q = 0; q < P16::QUADS; ++q)
+          *reinterpret_cast<f32x4v *>(smem[wave] + ((i * P16::QUADS + q) * 64 + lane) * 16) =
+              P16::quad(acc[i], q);
+      }
+      if (lane < 16)
+        ms[wave][16 * i + lane] = m[i], ls[wave][16 * i + lane] = l[i];
+    }
+    paged_split_end<A>(pe, ue, vs, smem, ms, ls, &flag);
+  }
+  paged_zero_rows<elt>(args4.a);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the waves of a workgroup share the keys
+// ---------------------------------------------------------------------------
+
+// 128 rows a unit, 32 a wave.  Of a block of 64 keys each wave holds the codes of 16, converts them
+// into the tiles of 16-bit rows that all four read, and loads those of the next block: K and V have
+// two tiles each, one barrier a block.
+template <int D_, bool BF, bool NV_> struct Paged4Rows {
+  static constexpr int D = D_, BN = 64;
+  static constexpr bool NV = NV_, CBF = BF && !NV;
+  typedef Code4<CBF, NV> Code;
+  typedef PagedFrag<D, CBF, false, BN> P;
+  typedef Piece4<D, NV> Piece;
+  typedef typename AttnFwd<64, BF, 32, 64>::elt elt; // of q and o
+};
+template <class A> constexpr int paged4_rows_groups() { return A::D > 128 ? 1 : 2; }
+
+template <class A>
+__global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows_kernel(Paged4Args args4) {
+  constexpr int D = A::D, BN = A::BN;
+  typedef typename A::P P;
+  typedef typename A::Piece Piece;
+  typedef typename A::Code Code;
+  typedef typename A::elt elt;
+  typedef PagedSched<128, BN, 1, kRowsOverhead> Sched;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * P::TILE];
+  __shared__ PagedSchedState st;
+  __shared__ uint32_t nans[2][4]; // of each wave's 16 keys of a tile, those without numbers in V
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  if (wave == 0) {
+    Sched sched(args4.a, st);
+    const uint32_t n = gridDim.x, b = blockIdx.x; // (XCDs: as in paged_attn_rows_kernel)
+    sched.init(n % 8 == 0 ? (b % 8) * (n / 8) + b / 8 : b, n);
+    sched.get(st.unit[0]);
+  }
+  __syncthreads();
+
+  const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * P::TILE;
+  typename P::Bases bs;
+  P::bases(k_lds, v_lds, bs);
+  const int em = lane >> 2, eg = lane & 3, er = 16 * wave + em; // the key of a block that the lane converts
+  uint32_t kw[Piece::KW], vw[Piece::KW];
+#pragma unroll
+  for (int c = 0; c < Piece::KW; ++c) {
+    const int chunk = Piece::dim(c, eg) / 8;
+    kw[c] = k_lds + er * P::ROW + ((chunk ^ P::kswz(er)) << 4);
+    vw[c] = v_lds + er * P::ROW + ((chunk ^ P::vswz(er)) << 4);
+  }
+
+  for (int turn = 0;; turn ^= 1) {
+    const Paged4Args &p4 = paged4_args();
+    const PagedAttnArgs &p = p4.a;
+    const PagedUnit un = paged_unit(st.unit[turn]);
+    if (un.rows <= 0)
+      break;
+    int k0 = 0, k1 = 0;
+    if (un.hi > un.lo) {
+      const int first = un.lo / BN, last = (int)(((int64_t)un.hi + BN - 1) / BN);
+      k0 = first + (int)un.s0;
+      k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
+    }
+    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
+    const Side4<D, A::NV> sk(p.kc, p.k_sp, p.k_st, p.k_sh, p4.ks, un.hk, p.head_dim, em, eg);
+    const Side4<D, A::NV> sv(p.vc, p.v_sp, p.v_st, p.v_sh, p4.vs, un.hk, p.head_dim, em, eg);
+    uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
+    Piece kp, vp;
+    auto fetch = [&](int k) __attribute__((always_inline)) {
+      pr.hold(k * BN);
+      here[2] = pr.template there<BN>(k * BN, un.hi);
+      sk.load(pr, k * BN + 16 * wave, em, kp);
+      sv.load(pr, k * BN + 16 * wave, em, vp);
+    };
+    auto convert = [&](int slot) __attribute__((always_inline)) {
+      typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+      uint32_t fk[Piece::SB], fv[Piece::SB];
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < Piece::SB; ++j) {
+        fk[j] = Code::factor(kp.s[j], false), fv[j] = Code::factor(vp.s[j], true);
+        bad = bad || Code::bad(vp.s[j]);
+      }
+      const uint64_t none = __ballot(bad);
+      if (lane == 0)
+        nans[slot][wave] = none ? keys_of(none) : 0;
+#pragma unroll
+      for (int c = 0; c < Piece::KW; ++c) {
+        *(lds_u32x4 *)(uintptr_t)(kw[c] + slot * P::TILE) = Code::eight(kp.w[c], fk[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)(vw[c] + slot * P::TILE) = Code::eight(vp.w[c], fv[Piece::scale_of(c)]);
+      }
+    };
+    // The table, Q and the first blocks are under way together, and meanwhile the first wave
+    // looks up the next unit.
+    if (k0 < k1)
+      pr.load(k0 * BN);
+    const bool busy = un.rows > 32 * wave;
+    const int r = 32 * wave + (lane & 31), rr = un.r0 + (r < un.rows ? r : 0);
+    const int of = paged_token(p, rr), head = un.hk * p.G + rr - of * p.G;
+    const elt *qrow = static_cast<const elt *>(p.q) + (int64_t)(un.t0 + of) * p.q_st + head * p.q_sh;
+    u32x4 qx[D / 16];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const int d = P::q_dim(c);
+      qx[c] = *reinterpret_cast<const u32x4 *>(qrow + (d < p.head_dim ? d : 0));
+    }
+    if (k0 < k1) {
+      pr.settle();
+      fetch(k0);
+      here[0] = here[2];
+    }
+    if (wave == 0)
+      Sched(p, st).get(st.unit[turn ^ 1]);
+    int lo, hi; // of the lane's row
+    paged_keys(p, un.pos0, un.len, rr, rr + 1, lo, hi);
+    // of the wave's rows: keys that all attend to, and keys that any does
+    int lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;
+    if (busy) {
+      const int a = un.r0 + 32 * wave, z = un.r0 + (un.rows < 32 * wave + 32 ? un.rows : 32 * wave + 32);
+      paged_keys(p, un.pos0, un.len, a, a + 1, lo_any, hi_all);
+      paged_keys(p, un.pos0, un.len, z - 1, z, lo_all, hi_any);
+    }
+    auto live = [&](int k) { return busy && k * BN < hi_any && k * BN + BN > lo_any; };
+    const float scale0 = p.qk_scale * (p.k_scale ? p.k_scale[un.hk] : 1.f);
+    typename P::QF qf;
+    float scale = scale0 == 0.f ? 1.f : fabsf(scale0);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      qx[c] = __builtin_bit_cast(u32x4, P::settled(__builtin_bit_cast(typename P::h8, qx[c]),
+                                                   r < un.rows && P::q_dim(c) < p.head_dim, scale0));
+    if constexpr (A::NV)
+      scale *= q4_to_f16<!std::is_same<elt, _Float16>::value>(qx, [](float v) { return P::X::xmax(v); });
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      qf.v[c] = __builtin_bit_cast(typename P::h8, qx[c]);
+    float m = -INFINITY, l = 0.f;
+    typename P::Acc acc = {};
+    typename P::Scores s;
+    if (k0 < k1) {
+      convert(0);
+      if (k0 + 1 < k1) {
+        fetch(k0 + 1);
+        here[1] = here[2];
+      }
+    }
+    __syncthreads();
+    auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
+      constexpr int SL = decltype(slot_c)::value;
+      const int n0 = k * BN;
+      if (k + 1 < k1) {
+        convert(1 - SL);
+        if (k + 2 < k1)
+          fetch(k + 2);
+      }
+      if (live(k)) {
+        typename P::KF kf;
+        P::read_k(bs, SL * P::TILE, kf);
+        P::qk(kf, qf, s);
+        constexpr int VR = D <= 128 ? P::NV : P::VN;
+        typename P::template VF<VR> vf;
+        P::read_v(bs, SL * P::TILE, 0, vf);
+        uint64_t nan = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          nan |= (uint64_t)(uint32_t)uniform((int)nans[SL][w]) << (16 * w);
+        if (__builtin_expect(nan != 0, 0)) {
+          nan >>= 4 * g;
+#pragma unroll
+          for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              s[b][e] = nan >> (32 * b + 8 * (e / 4) + e % 4) & 1 ? __builtin_nanf("") : s[b][e];
+        }
+        if (here[0] != ~0ull || n0 < lo_all || n0 + BN > hi_all) {
+          const int a = lo - n0 < 0 ? 0 : lo - n0, z = hi - n0 < 0 ? 0 : hi - n0;
+          uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
+          seen &= a < 64 ? ~0ull << a : 0;
+          P::mask(s, seen & here[0]);
+        }
+        typename P::PF pf;
+        P::softmax(s, scale, acc, m, l, pf);
+        P::pv(vf, 0, pf, acc);
+#pragma unroll
+        for (int b0 = VR; b0 < P::NV; b0 += VR) {
+          P::read_v(bs, SL * P::TILE, b0, vf);
+          P::pv(vf, b0, pf, acc);
+        }
+      }
+      here[0] = here[1], here[1] = here[2];
+      __syncthreads();
+    };
+    for (int k = k0; k < k1;) {
+      iter(k++, std::integral_constant<int, 0>());
+      if (k < k1)
+        iter(k++, std::integral_constant<int, 1>());
+    }
+    paged_rows_end<P, elt>(st.unit[turn], acc, m, l, &flag);
+  }
+  paged_zero_rows<elt>(args4.a);
+}
+
+} // namespace txk

@@ -10,7 +10,7 @@ The product is the C-ABI in ../lib (headers in include/triton_ext/):
 
 This module binds them with ctypes (the binding a Python caller such as
 Triton's runtime would add) and offers `dot()` and its kin, and the paged cache
-(`rotary()`, `paged_append()`, `paged_attention()`, `page_*()`), over torch device
+(`rotary()`, `paged_append()`, `paged_attention()`, `paged_read()`, `page_*()`), over torch device
 tensors.
 torch is used only for device memory and streams.  There is no CPU fallback:
 if libmi355x_dot.so is missing, `load()` raises.
@@ -20,3 +20,4 @@ from .dot import (aligned_rows, attention, dot, dot_scaled, new_output, plan_for
                   workspace_for)
 from .cache import (page_compact, page_copy, page_fork, page_free, page_reserve,  # noqa: F401
                     paged_append, paged_attention, rotary, rotary_frequencies)
+from .cache4 import paged_read  # noqa: F401

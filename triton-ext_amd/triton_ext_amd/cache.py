@@ -12,7 +12,9 @@ j % page_size.  A decoding step is
     o = paged_attention(q, k_cache, v_cache, page_table, kv_len, sm_scale=D ** -0.5)
 
 and a chunk of several new tokens a sequence the same with cu_q, their starts in q, k
-and v.  Nothing here reads device memory on the host: every call can be captured into
+and v.  A cache may be held in 4 bits (k_block_scale and v_block_scale of both calls; the scales are
+caches of their own to page_fork and its kin), and paged_read gives back what a cache holds.  Nothing
+here reads device memory on the host: every call can be captured into
 a graph and replayed with other contents.
 
 stream: the handle of the HIP stream to run on, torch's current one if None.  All of a call is in order
@@ -42,6 +44,12 @@ def _calls():
     if _native is None:
         _native = capi.calls()
     return _native
+
+
+def _in_4_bits():
+    """The forms over caches of codes, loaded with the first call."""
+    from . import cache4
+    return cache4
 
 
 def _keep(form, found):
@@ -250,8 +258,8 @@ def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, 
     if tuple(k_cache.shape[2:]) != (Hkv, D):
         raise ValueError(f"the cache holds heads of {tuple(k_cache.shape[2:])}, not ({Hkv}, {D})")
     if k_cache.dtype != dtype and k_cache.dtype != torch.float8_e4m3fn:
-        raise NotImplementedError(f"a cache of {k_cache.dtype} under {dtype}: the same type, or "
-                                  "float8_e4m3fn")
+        raise NotImplementedError(f"a cache of {k_cache.dtype} under {dtype}: the same type, "
+                                  "float8_e4m3fn, or uint8 codes with block scales")
     if D > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
         raise ValueError("the caches' last dimension must be contiguous")
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
@@ -261,6 +269,11 @@ def _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, 
             raise ValueError(f"{name} is for float8_e4m3fn caches")
         if t.dtype != torch.float32 or t.shape != (Hkv,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous fp32 [{Hkv}] tensor")
+    _cache_books(page_table, kv_len, cu_q, T)
+
+
+def _cache_books(page_table, kv_len, cu_q, T):
+    import torch
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or (
             page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table must be an int32 [sequences, entries] tensor with contiguous "
@@ -287,8 +300,8 @@ def _tokens(t, name, heads, D, dtype, T):
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=None, inv_freq=None,
-                 interleaved=False, scale=1.0, k_scale=None, v_scale=None, q_out=None,
-                 stream=None):
+                 interleaved=False, scale=1.0, k_scale=None, v_scale=None, k_block_scale=None,
+                 v_block_scale=None, q_out=None, stream=None):
     """New tokens into a paged cache: k, v [T, Hkv, D] go to the pages of their sequences,
     k (and q [T, Hq, D], which is returned, in q_out if given) rotated at the token's
     position first when inv_freq is given (see rotary for interleaved and scale).
@@ -297,11 +310,26 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     one token each): row cu_q[b] + i of sequence b's n is its token kv_len[b] - n + i.
     The pages must be there (page_reserve); a token without one is not written.  fp16 or
     bf16; a float8_e4m3fn cache holds k / k_scale[head] and v / v_scale[head] (fp32 [Hkv];
-    None: 1), saturated.  Rows of q from cu_q[B] on come back as they are."""
+    None: 1), saturated.  Rows of q from cu_q[B] on come back as they are.
+
+    With k_block_scale and v_block_scale the cache is held in 4 bits: uint8 caches [pages, page_size,
+    Hkv, D / 2] of e2m1 codes (D a multiple of 32, the even dim in the low four bits), quantised as they
+    are written.  The block scales, in any strides, are uint8 [pages, page_size, Hkv, D / 32] (e8m0: the
+    least power of two 2^e with max |x| <= 7 * 2^e over 32 dims, e within [-125, 125] for bf16 and
+    [-23, 13] for fp16) or float8_e4m3fn [.., D / 16] (max |x| / 6, within [2^-9, 448]); codes go to
+    nearest, ties to even, saturated at 6; a block with a NaN or an infinity becomes NaN.  The fast
+    order in memory has a head's tokens together, torch.empty(pages, Hkv, page_size, D // 2).permute(0,
+    2, 1, 3), and of the scales those of one block of dims, torch.empty(pages, Hkv, D // 32,
+    page_size).permute(0, 3, 1, 2); pages of these are what page_copy and its kin move."""
     if stream is not None and stream != _current_stream(k.device):
         return _there(k.device, stream, paged_append, k, v, k_cache, v_cache, page_table, kv_len,
                       cu_q, q=q, inv_freq=inv_freq, interleaved=interleaved, scale=scale,
-                      k_scale=k_scale, v_scale=v_scale, q_out=q_out)
+                      k_scale=k_scale, v_scale=v_scale, k_block_scale=k_block_scale,
+                      v_block_scale=v_block_scale, q_out=q_out)
+    if k_block_scale is not None or v_block_scale is not None:
+        return _in_4_bits().append(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
+                                   interleaved, scale, k_scale, v_scale, k_block_scale,
+                                   v_block_scale, q_out, stream)
     native = _native or _calls()
     form = native.form("append", k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
                        bool(interleaved), float(scale), k_scale, v_scale, q_out)
@@ -342,8 +370,8 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     return q_out
 
 
-def _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, k_scale, v_scale,
-                   q_out):
+def _append_tokens(k, v, q, inv_freq, q_out):
+    """Refuses new tokens that do not go together."""
     import torch
     if k.dim() != 3:
         raise ValueError(f"k must be [T, Hkv, D], got {tuple(k.shape)}")
@@ -352,10 +380,6 @@ def _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq
     if dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"k: fp16 and bf16 are implemented, got {dtype}")
     _tokens(v, "v", Hkv, D, dtype, T)
-    _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, dtype)
-    _same_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
-                 kv_len=kv_len, cu_q=cu_q, q=q, inv_freq=inv_freq, k_scale=k_scale,
-                 v_scale=v_scale, q_out=q_out)
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1):
         raise ValueError("inv_freq must be an fp32 vector")
     if q is None:
@@ -368,9 +392,19 @@ def _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq
         raise ValueError("q_out must be as q, with its last dimension contiguous")
 
 
+def _append_checks(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, k_scale, v_scale,
+                   q_out):
+    _append_tokens(k, v, q, inv_freq, q_out)
+    T, Hkv, D = k.shape
+    _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T, Hkv, D, k.dtype)
+    _same_device(k.device, v=v, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                 kv_len=kv_len, cu_q=cu_q, q=q, inv_freq=inv_freq, k_scale=k_scale,
+                 v_scale=v_scale, q_out=q_out)
+
+
 def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_scale, causal=True,
-                    window=0, k_scale=None, v_scale=None, out=None, return_lse=False,
-                    workspace=None, stream=None):
+                    window=0, k_scale=None, v_scale=None, k_block_scale=None, v_block_scale=None,
+                    out=None, return_lse=False, workspace=None, stream=None):
     """Attention of the new tokens q [T, Hq, D] over a paged cache that holds them already
     (paged_append), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)).
 
@@ -379,11 +413,20 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     and rows from cu_q[B] on, get 0.  fp16 or bf16, the cache in q's type or float8_e4m3fn
     (times k_scale, v_scale, fp32 [Hkv]), D a multiple of 8 (e4m3: 16) up to 256.  Returns
     o [T, Hq, D], with return_lse also log2 of the sum of e^(score), fp32 [T, Hq] (-inf
-    where nothing is attended to).  cu_q as for paged_append."""
+    where nothing is attended to).  cu_q as for paged_append.
+
+    With k_block_scale and v_block_scale: over a cache held in 4 bits (see paged_append; D a multiple
+    of 32 up to 256), whose values are taken in q's type.  A row that attends to a token with a block
+    scale of NaN (or e8m0 above 2^125, fp16 q: 2^13) is NaN."""
     if stream is not None and stream != _current_stream(q.device):
         return _there(q.device, stream, paged_attention, q, k_cache, v_cache, page_table, kv_len, cu_q,
                       sm_scale=sm_scale, causal=causal, window=window, k_scale=k_scale,
-                      v_scale=v_scale, out=out, return_lse=return_lse, workspace=workspace)
+                      v_scale=v_scale, k_block_scale=k_block_scale, v_block_scale=v_block_scale,
+                      out=out, return_lse=return_lse, workspace=workspace)
+    if k_block_scale is not None or v_block_scale is not None:
+        return _in_4_bits().attention(q, k_cache, v_cache, page_table, kv_len, cu_q, sm_scale, causal,
+                                      window, k_scale, v_scale, k_block_scale, v_block_scale, out,
+                                      return_lse, workspace, stream)
     import torch
     native = _native or _calls()
     form = native.form("attention", q, k_cache, v_cache, page_table, kv_len, cu_q, float(sm_scale),
@@ -427,20 +470,23 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     return (out, lse) if return_lse else out
 
 
-def _attention_checks(q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, out):
+def _attention_q(q, out):
     import torch
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, D], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"q: fp16 and bf16 are implemented, got {q.dtype}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+        raise ValueError("out must be as q, with its last dimension contiguous")
+
+
+def _attention_checks(q, k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, out):
+    _attention_q(q, out)
     T, Hq, D = q.shape
-    dtype = q.dtype
-    if dtype not in (torch.float16, torch.bfloat16):
-        raise NotImplementedError(f"q: fp16 and bf16 are implemented, got {dtype}")
     _cache_checks(k_cache, v_cache, page_table, kv_len, cu_q, k_scale, v_scale, T,
-                  k_cache.shape[2] if k_cache.dim() == 4 else 0, D, dtype)
+                  k_cache.shape[2] if k_cache.dim() == 4 else 0, D, q.dtype)
     _same_device(q.device, k_cache=k_cache, v_cache=v_cache, page_table=page_table, kv_len=kv_len,
                  cu_q=cu_q, k_scale=k_scale, v_scale=v_scale, out=out)
-    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1):
-        raise ValueError("out must be as q, with its last dimension contiguous")
 
 
 # ---------------------------------------------------------------------------

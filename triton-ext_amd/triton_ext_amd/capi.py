@@ -1,4 +1,4 @@
-"""ctypes mirror of include/triton_ext/{TritonExtPassInfra,tx_dot,tx_passes,tx_attn,tx_cache}.h."""
+"""ctypes mirror of include/triton_ext/{TritonExtPassInfra,tx_dot,tx_passes,tx_attn,tx_cache,tx_cache4}.h."""
 import ctypes
 import os
 
@@ -119,6 +119,40 @@ class PagedAttnPlan(ctypes.Structure):
                 + _i64("workspace_bytes"))
 
 
+class BlockScales(ctypes.Structure):
+    _fields_ = _i32("mode reserved") + _i64("k_sp k_st k_sh k_sb v_sp v_st v_sh v_sb")
+
+
+class PagedAppend4Desc(ctypes.Structure):
+    _fields_ = [("c", PagedAppendDesc), ("s", BlockScales)]
+
+
+class PagedAppend4Plan(ctypes.Structure):
+    _fields_ = ([("desc", PagedAppend4Desc), ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
+                + _i32("whole head_lanes grid_x block_threads"))
+
+
+class PagedReadDesc(ctypes.Structure):
+    _fields_ = (_i64("T B pages table_width")
+                + _i32("Hkv head_dim page_size cache_type out_type ragged")
+                + _i64("kc_sp kc_st kc_sh vc_sp vc_st vc_sh k_st k_sh v_st v_sh table_s")
+                + [("s", BlockScales)])
+
+
+class PagedReadPlan(ctypes.Structure):
+    _fields_ = ([("desc", PagedReadDesc), ("bytes", ctypes.c_double)]
+                + _i32("vec head_lanes grid_x block_threads"))
+
+
+class PagedAttn4Desc(ctypes.Structure):
+    _fields_ = [("c", PagedAttnDesc), ("s", BlockScales)]
+
+
+class PagedAttn4Plan(ctypes.Structure):
+    _fields_ = ([("desc", PagedAttn4Desc)] + _i32("variant rows slots units grid_x block_threads")
+                + _i64("workspace_bytes"))
+
+
 PAGE_CACHES = 128  # TX_PAGE_CACHES
 
 
@@ -161,6 +195,9 @@ EXPORTS = {
                          "tx_rotary_plan_create", "tx_rotary_launch",
                          "tx_paged_append_plan_create", "tx_paged_append_launch",
                          "tx_paged_attn_plan_create", "tx_paged_attn_launch",
+                         "tx_paged_append4_plan_create", "tx_paged_append4_launch",
+                         "tx_paged_read_plan_create", "tx_paged_read_launch",
+                         "tx_paged_attn4_plan_create", "tx_paged_attn4_launch",
                          "tx_page_workspace", "tx_page_copy", "tx_page_reserve", "tx_page_fork",
                          "tx_page_free", "tx_page_compact"],
 }
@@ -223,13 +260,20 @@ def load(name="libmi355x_dot.so"):
         L.tx_attn_fwd_launch.argtypes = [ctypes.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp]
         for f, desc, pl in (("rotary", RotaryDesc, RotaryPlan),
                             ("paged_append", PagedAppendDesc, PagedAppendPlan),
-                            ("paged_attn", PagedAttnDesc, PagedAttnPlan)):
+                            ("paged_attn", PagedAttnDesc, PagedAttnPlan),
+                            ("paged_append4", PagedAppend4Desc, PagedAppend4Plan),
+                            ("paged_read", PagedReadDesc, PagedReadPlan),
+                            ("paged_attn4", PagedAttn4Desc, PagedAttn4Plan)):
             getattr(L, f"tx_{f}_plan_create").argtypes = [ctypes.POINTER(desc), ctypes.POINTER(pl)]
         L.tx_stream_capture.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64)]
         L.tx_rotary_launch.argtypes = [ctypes.POINTER(RotaryPlan)] + [vp] * 5
         L.tx_paged_append_launch.argtypes = [ctypes.POINTER(PagedAppendPlan)] + [vp] * 13
         L.tx_paged_attn_launch.argtypes = ([ctypes.POINTER(PagedAttnPlan)] + [vp] * 11
                                            + [ctypes.c_size_t, vp])
+        L.tx_paged_append4_launch.argtypes = [ctypes.POINTER(PagedAppend4Plan)] + [vp] * 15
+        L.tx_paged_read_launch.argtypes = [ctypes.POINTER(PagedReadPlan)] + [vp] * 12
+        L.tx_paged_attn4_launch.argtypes = ([ctypes.POINTER(PagedAttn4Plan)] + [vp] * 13
+                                            + [ctypes.c_size_t, vp])
         pd = ctypes.POINTER(PageDesc)
         L.tx_page_workspace.argtypes = [pd, ctypes.POINTER(i64)]
         for f, n in (("copy", 4), ("reserve", 10), ("fork", 12), ("free", 8), ("compact", 8)):
