@@ -374,6 +374,13 @@ extern "C" TX_API int tx_paged_attn4_plan_create(const tx_paged_attn4_desc *desc
     return rc;
   if (d.q_st % 8 || d.q_sh % 8 || d.o_st % 8 || d.o_sh % 8)
     return fail(TX_ERR_INVALID, "q and o strides must be multiples of 16 bytes");
+  // (the kernels' offsets from one of 16 tokens have 32 bits)
+  const tx_block_scales &s = desc->s;
+  const int64_t blocks = d.head_dim / (s.mode == TX_SCALE_MX32 ? 32 : 16), far = (int64_t)1 << 27;
+  if (d.page_size > 1 && (d.k_st >= far || d.v_st >= far || s.k_st >= far || s.v_st >= far))
+    return fail(TX_ERR_UNSUPPORTED, "tokens of a page 2^27 bytes apart");
+  if ((blocks - 1) * s.k_sb >= ((int64_t)1 << 31) || (blocks - 1) * s.v_sb >= ((int64_t)1 << 31))
+    return fail(TX_ERR_UNSUPPORTED, "scales of a head 2^31 bytes apart");
   if (d.T * (int64_t)(d.Hkv ? d.Hq / d.Hkv : 0) > INT32_MAX)
     return fail(TX_ERR_UNSUPPORTED, "more than 2^31 rows of a kv head");
   std::memset(plan, 0, sizeof(*plan));

@@ -51,65 +51,63 @@ template <int D, bool NV> struct Piece4 {
   }
 };
 
-// Where lane (m, g) finds its pieces of K or V: the codes and scales of a head, and the lane's own
-// offsets from the first of 8 keys.  Pieces past head_dim are those of its beginning (Q is 0 there;
-// V's are not stored).
-template <int D, bool NV> struct Side4 {
+// One wave's view of a table row: beside its entries, where their pages begin in the codes and scales of
+// K and of V (page 0 where there is none).
+struct PageRow4 : PageRow {
+  uint64_t at[4];
+
+  __device__ __forceinline__ void settle() {
+    PageRow::settle();
+    const Paged4Args &p = paged4_args();
+    const uint64_t id = ids < 0 ? 0 : ids;
+    at[0] = id * (uint64_t)p.a.k_sp, at[1] = id * (uint64_t)p.ks.sp;
+    at[2] = id * (uint64_t)p.a.v_sp, at[3] = id * (uint64_t)p.vs.sp;
+  }
+  __device__ __forceinline__ void hold(int n) {
+    if (((n + 63) >> shift) >= first + 64) {
+      load(n);
+      settle();
+    }
+  }
+};
+
+// Where lane (m, g) finds its pieces of K (V: of V) of 16 keys: the codes and scales of a head, which
+// are uniform, and the lane's offsets from the first key, of 32 bits.  Pieces past head_dim are those
+// of its beginning (Q is 0 there; V's are not stored).
+template <int D, bool NV, bool V> struct Side4 {
   typedef Piece4<D, NV> P;
   const uint8_t *codes, *scales;
-  int64_t sp, st, ssp, sst;
-  int64_t row, srow;  // (m & 7) rows
-  uint32_t at[D == 256 ? 2 : 1];
-  int64_t sat[P::SB];
-  bool upper; // m & 8
+  uint32_t st, sst;
+  uint32_t off[D == 256 ? 2 : 1], soff[P::SB];
 
-  __device__ __forceinline__ Side4(const uint8_t *c, int64_t sp_, int64_t st_, int64_t sh,
-                                   const BlockScales &bs, int hk, int head_dim, int m, int g)
-      : codes(c + hk * sh), scales(bs.s + hk * bs.sh), sp(sp_), st(st_), ssp(bs.sp), sst(bs.st),
-        row((m & 7) * st_), srow((m & 7) * bs.st), upper(m & 8) {
-    const int bytes = head_dim / 2;
+  __device__ __forceinline__ Side4(const Paged4Args &p, int hk, int m, int g) {
+    const BlockScales &bs = V ? p.vs : p.ks;
+    codes = (V ? p.a.vc : p.a.kc) + hk * (V ? p.a.v_sh : p.a.k_sh);
+    scales = bs.s + hk * bs.sh;
+    st = (uint32_t)(V ? p.a.v_st : p.a.k_st), sst = (uint32_t)bs.st;
+    const uint32_t row = p.a.page_shift >= 4 ? m : m & ((1 << p.a.page_shift) - 1);
+    const int bytes = p.a.head_dim / 2;
 #pragma unroll
     for (int i = 0; i < (D == 256 ? 2 : 1); ++i) {
       const int o = D == 64 ? 8 * g : 64 * i + 16 * g;
-      at[i] = o < bytes ? o : 0;
+      off[i] = row * st + (o < bytes ? o : 0);
     }
 #pragma unroll
     for (int j = 0; j < P::SB; ++j) {
       const int b = P::block_of(j, g);
-      sat[j] = (b < head_dim / (NV ? 16 : 32) ? b : 0) * bs.sb;
+      soff[j] = row * sst + (b < p.a.head_dim / (NV ? 16 : 32) ? b : 0) * (uint32_t)bs.sb;
     }
   }
-  // The pieces of keys n + m; m is the lane's row again.
-  __device__ __forceinline__ void load(const PageRow &pr, int n, int m, P &x) const {
-    const uint8_t *c, *s;
-    if (pr.shift >= 3) { // 8 keys of one page
-      const int ea = (n >> pr.shift) - pr.first, eb = ((n + 8) >> pr.shift) - pr.first;
-      int a = lane_value(pr.ids, ea & 63), b = lane_value(pr.ids, eb & 63);
-      a = a < 0 ? 0 : a, b = b < 0 ? 0 : b;
-      const int mask = (1 << pr.shift) - 1, sa = n & mask, sb = (n + 8) & mask;
-      const uint8_t *const ca = codes + (int64_t)a * sp + (int64_t)sa * st;
-      const uint8_t *const cb = codes + (int64_t)b * sp + (int64_t)sb * st;
-      const uint8_t *const ka = scales + (int64_t)a * ssp + (int64_t)sa * sst;
-      const uint8_t *const kb = scales + (int64_t)b * ssp + (int64_t)sb * sst;
-      c = (upper ? cb : ca) + row;
-      s = (upper ? kb : ka) + srow;
-    } else {
-      const int key = n + m;
-      int a = __shfl(pr.ids, ((key >> pr.shift) - pr.first) & 63);
-      a = a < 0 ? 0 : a;
-      const int slot = key & ((1 << pr.shift) - 1);
-      c = codes + (int64_t)a * sp + (int64_t)slot * st;
-      s = scales + (int64_t)a * ssp + (int64_t)slot * sst;
-    }
+  __device__ __forceinline__ void read(const uint8_t *c, const uint8_t *s, P &x) const {
     typedef uint32_t w2 __attribute__((ext_vector_type(2)));
     typedef uint32_t w4 __attribute__((ext_vector_type(4)));
     if constexpr (D == 64) {
-      const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2 *>(c + at[0]));
+      const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2 *>(c + off[0]));
       x.w[0] = v[0], x.w[1] = v[1];
     } else {
 #pragma unroll
       for (int i = 0; i < P::KW / 4; ++i) {
-        const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4 *>(c + at[i]));
+        const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4 *>(c + off[i]));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           x.w[4 * i + e] = v[e];
@@ -117,7 +115,34 @@ template <int D, bool NV> struct Side4 {
     }
 #pragma unroll
     for (int j = 0; j < P::SB; ++j)
-      x.s[j] = __builtin_nontemporal_load(s + sat[j]);
+      x.s[j] = __builtin_nontemporal_load(s + soff[j]);
+  }
+  // The pieces of N runs of 16 keys from n on, a multiple of 16 N; m is the lane's row again.
+  template <int N> __device__ __forceinline__ void load(const PageRow4 &pr, int n, int m, P (&x)[N]) const {
+    if (pr.shift >= 4) { // a run lies in one page
+      const uint8_t *c, *s;
+#pragma unroll
+      for (int b = 0; b < N; ++b) {
+        if (b == 0 || pr.shift < 5) {
+          const int key = n + 16 * b, e = ((key >> pr.shift) - pr.first) & 63;
+          const uint64_t slot = key & ((1 << pr.shift) - 1);
+          c = codes + (uint64_t)lane_value64(pr.at[V ? 2 : 0], e) + slot * st;
+          s = scales + (uint64_t)lane_value64(pr.at[V ? 3 : 1], e) + slot * sst;
+        } else {
+          c += 16ull * st, s += 16ull * sst;
+        }
+        read(c, s, x[b]);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < N; ++b) {
+        const int e = (((n + 16 * b + m) >> pr.shift) - pr.first) & 63;
+        auto of = [&](uint64_t v) {
+          return (uint64_t)(uint32_t)__shfl((int)v, e) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), e) << 32;
+        };
+        read(codes + of(pr.at[V ? 2 : 0]), scales + of(pr.at[V ? 3 : 1]), x[b]);
+      }
+    }
   }
 };
 
@@ -236,9 +261,9 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       k0 = w0 + wave * q < w1 ? w0 + wave * q : w1;
       k1 = k0 + q < w1 ? k0 + q : w1;
     }
-    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
-    const Side4<D, A::NV> sk(p.kc, p.k_sp, p.k_st, p.k_sh, p4.ks, un.hk, p.head_dim, km, kg);
-    const Side4<D, A::NV> sv(p.vc, p.v_sp, p.v_st, p.v_sh, p4.vs, un.hk, p.head_dim, vm, vg);
+    PageRow4 pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
+    const Side4<D, A::NV, false> sk(p4, un.hk, km, kg);
+    const Side4<D, A::NV, true> sv(p4, un.hk, vm, vg);
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
     // looks up the next unit.
     if (k0 < k1)
@@ -267,9 +292,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
           const int n = (k0 + i) * BN;
           pr.hold(n);
           here[i] = pr.template there<BN>(n, un.hi);
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            sk.load(pr, n + 16 * b, km, kp[i][b]), sv.load(pr, n + 16 * b, vm, vp[i][b]);
+          sk.load(pr, n, km, kp[i]), sv.load(pr, n, vm, vp[i]);
         }
     }
     if (wave == 0)
@@ -347,9 +370,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       if (k + NS < k1) {
         pr.hold(na);
         here[NS] = pr.template there<BN>(na, un.hi);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          sk.load(pr, na + 16 * b, km, kp[SL][b]), sv.load(pr, na + 16 * b, vm, vp[SL][b]);
+        sk.load(pr, na, km, kp[SL]), sv.load(pr, na, vm, vp[SL]);
       }
       if (__builtin_expect((none[0] | none[1]) != 0, 0)) {
         const uint32_t nan = (keys_of(none[0]) | keys_of(none[1]) << 16) >> (4 * kg);
@@ -476,11 +497,11 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       k0 = first + (int)un.s0;
       k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
     }
-    PageRow pr{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift};
-    const Side4<D, A::NV> sk(p.kc, p.k_sp, p.k_st, p.k_sh, p4.ks, un.hk, p.head_dim, em, eg);
-    const Side4<D, A::NV> sv(p.vc, p.v_sp, p.v_st, p.v_sh, p4.vs, un.hk, p.head_dim, em, eg);
+    PageRow4 pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
+    const Side4<D, A::NV, false> sk(p4, un.hk, em, eg);
+    const Side4<D, A::NV, true> sv(p4, un.hk, em, eg);
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
-    Piece kp, vp;
+    Piece kp[1], vp[1];
     auto fetch = [&](int k) __attribute__((always_inline)) {
       pr.hold(k * BN);
       here[2] = pr.template there<BN>(k * BN, un.hi);
@@ -493,16 +514,16 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       bool bad = false;
 #pragma unroll
       for (int j = 0; j < Piece::SB; ++j) {
-        fk[j] = Code::factor(kp.s[j], false), fv[j] = Code::factor(vp.s[j], true);
-        bad = bad || Code::bad(vp.s[j]);
+        fk[j] = Code::factor(kp[0].s[j], false), fv[j] = Code::factor(vp[0].s[j], true);
+        bad = bad || Code::bad(vp[0].s[j]);
       }
       const uint64_t none = __ballot(bad);
       if (lane == 0)
         nans[slot][wave] = none ? keys_of(none) : 0;
 #pragma unroll
       for (int c = 0; c < Piece::KW; ++c) {
-        *(lds_u32x4 *)(uintptr_t)(kw[c] + slot * P::TILE) = Code::eight(kp.w[c], fk[Piece::scale_of(c)]);
-        *(lds_u32x4 *)(uintptr_t)(vw[c] + slot * P::TILE) = Code::eight(vp.w[c], fv[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)(kw[c] + slot * P::TILE) = Code::eight(kp[0].w[c], fk[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)(vw[c] + slot * P::TILE) = Code::eight(vp[0].w[c], fv[Piece::scale_of(c)]);
       }
     };
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
