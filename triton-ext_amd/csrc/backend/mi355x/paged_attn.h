@@ -44,116 +44,6 @@ template <class A> constexpr int paged_split_groups() {
   return 8 * paged_split_slots<A>() * A::TILE <= 65536 ? 2 : 1;
 }
 
-// A unit's end: the four waves' sums (quads of 4 dims in smem[wave] by A::quad_at, and each row's
-// reference and sum in ms and ls) are joined, and written out, or left as one part of several, which
-// the last workgroup to arrive joins.  vs: the scale of v.
-template <class A, int BYTES>
-__device__ __forceinline__ void paged_split_end(const PagedAttnArgs &pe, const PagedUnit &ue, float vs,
-                                                uint8_t (&smem)[4][BYTES], float (&ms)[4][A::ROWS],
-                                                float (&ls)[4][A::ROWS], int *flag) {
-  constexpr int D = A::D, ROWS = A::ROWS;
-  typedef typename A::elt elt;
-  const int tid = threadIdx.x;
-  __syncthreads();
-  const int dq = pe.head_dim / 4, items = ue.rows * dq;
-  constexpr int64_t part_bytes = ROWS * (D + 2) * 4;
-  uint8_t *const unit_parts = pe.parts;
-  auto part_at = [&](uint32_t j) {
-    const uint64_t slot = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
-    return __builtin_amdgcn_make_buffer_rsrc(unit_parts + slot * part_bytes, 0, (int)part_bytes,
-                                             0x00020000);
-  };
-  auto finish = [&](int row, int qd, float mm, float ll, f32x4v x) {
-    const int ro = ue.r0 + row;
-    const int of = paged_token(pe, ro), h = ue.hk * pe.G + ro - of * pe.G;
-    const int64_t t = ue.t0 + of;
-    const float f = ll == 0.f ? 0.f : vs / ll;
-    typename A::h4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      y[e] = (elt)(x[e] * f);
-    *reinterpret_cast<typename A::h4 *>(static_cast<elt *>(pe.o) + t * pe.o_st + h * pe.o_sh +
-                                        4 * qd) = y;
-    if (qd == 0 && pe.lse)
-      pe.lse[t * pe.Hq + h] = ll == 0.f ? -INFINITY : mm + __builtin_log2f(ll);
-  };
-  constexpr int kSC1 = 16;
-  for (int it = tid; it < items; it += 256) {
-    const int row = it / dq, qd = it % dq;
-    float mm = -INFINITY, ll = 0.f;
-    f32x4v x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int wv = 0; wv < 4; ++wv)
-      paged_join(mm, ll, x, ms[wv][row], ls[wv][row],
-                 *reinterpret_cast<const f32x4v *>(
-                     smem[wv] + A::quad_at(row, qd) * 16));
-    if (ue.parts == 1) {
-      finish(row, qd, mm, ll, x);
-    } else {
-      const auto mine = part_at(ue.part);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4_t, x), mine,
-                                             (row * D + 4 * qd) * 4, 0, kSC1);
-      if (qd == 0) {
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), mine, (ROWS * D + row) * 4, 0,
-                                              kSC1);
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(ll), mine,
-                                              (ROWS * D + ROWS + row) * 4, 0, kSC1);
-      }
-    }
-  }
-  __syncthreads(); // the tiles' and ms' next use
-  if (ue.parts == 1 || !paged_arrive(&pe.counters[ue.w0], ue.parts, flag))
-    return;
-  // Last: all parts, in order.  Threads past one set of items take other parts.
-  const int groups = items < 256 ? 256 / items : 1;
-  for (int base = 0; base < items; base += 256) {
-    const int gi = items < 256 ? tid / items : 0, it = items < 256 ? tid % items : base + tid;
-    const bool on = gi < groups && it < items;
-    const int row = on ? it / dq : 0, qd = on ? it % dq : 0;
-    float mm = -INFINITY, ll = 0.f;
-    f32x4v x = {0.f, 0.f, 0.f, 0.f};
-    constexpr int NJ = 8; // parts in flight
-    for (uint32_t j0 = gi; j0 < ue.parts; j0 += NJ * groups) {
-      float pm[NJ], pl[NJ];
-      i32x4_t px[NJ];
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint32_t jj = j0 + j * groups;
-        pm[j] = -INFINITY, pl[j] = 0.f;
-        if (on && jj < ue.parts) {
-          const uint64_t slot = 2ull * (ue.w0 + jj) + (jj == 0 ? ue.slot0 : 0);
-          const auto all = __builtin_amdgcn_make_buffer_rsrc(unit_parts, 0, 0x7fffffff, 0x00020000);
-          const int at = (int)(slot * part_bytes);
-          px[j] = __builtin_bit_cast(
-              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, at + (row * D + 4 * qd) * 4, 0, kSC1));
-          pm[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + row) * 4, 0, kSC1));
-          pl[j] = __int_as_float(
-              __builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + ROWS + row) * 4, 0, kSC1));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        paged_join(mm, ll, x, pm[j], pl[j], __builtin_bit_cast(f32x4v, px[j]));
-    }
-    if (groups > 1) {
-      f32x4v *const xs = reinterpret_cast<f32x4v *>(smem[0]);
-      float *const mls = reinterpret_cast<float *>(smem[0] + 4096);
-      xs[tid] = x;
-      mls[tid] = mm, mls[256 + tid] = ll;
-      __syncthreads();
-      if (tid < items) {
-        for (int k = 1; k < groups; ++k)
-          paged_join(mm, ll, x, mls[k * items + tid], mls[256 + k * items + tid],
-                     xs[k * items + tid]);
-        finish(row, qd, mm, ll, x);
-      }
-      __syncthreads();
-    } else if (on) {
-      finish(row, qd, mm, ll, x);
-    }
-  }
-}
-
 // 16 or 32 rows a unit (decoding, some drafted tokens).  Every wave goes through its own run of
 // blocks, with LDS tiles of its own that are loaded again as soon as their fragments are in
 // registers, and no barrier; at the end the four join in LDS.  Bound by memory: 8 waves a CU
@@ -323,7 +213,104 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
     }
     if (lane < ROWS)
       ms[wave][lane] = m, ls[wave][lane] = l;
-    paged_split_end<A>(pe, ue, vs, smem, ms, ls, &flag);
+    __syncthreads();
+    const int dq = pe.head_dim / 4, items = ue.rows * dq;
+    const int64_t part_bytes = ROWS * (D + 2) * 4;
+    uint8_t *const unit_parts = pe.parts;
+    auto part_at = [&](uint32_t j) {
+      const uint64_t slot = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
+      return __builtin_amdgcn_make_buffer_rsrc(unit_parts + slot * part_bytes, 0, (int)part_bytes,
+                                               0x00020000);
+    };
+    auto finish = [&](int row, int qd, float mm, float ll, f32x4v x) {
+      const int ro = ue.r0 + row;
+      const int of = paged_token(pe, ro), h = ue.hk * pe.G + ro - of * pe.G;
+      const int64_t t = ue.t0 + of;
+      const float f = ll == 0.f ? 0.f : vs / ll;
+      typename A::h4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = (elt)(x[e] * f);
+      *reinterpret_cast<typename A::h4 *>(static_cast<elt *>(pe.o) + t * pe.o_st + h * pe.o_sh +
+                                          4 * qd) = y;
+      if (qd == 0 && pe.lse)
+        pe.lse[t * pe.Hq + h] = ll == 0.f ? -INFINITY : mm + __builtin_log2f(ll);
+    };
+    constexpr int kSC1 = 16;
+    for (int it = tid; it < items; it += 256) {
+      const int row = it / dq, qd = it % dq;
+      float mm = -INFINITY, ll = 0.f;
+      f32x4v x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int wv = 0; wv < 4; ++wv)
+        paged_join(mm, ll, x, ms[wv][row], ls[wv][row],
+                   *reinterpret_cast<const f32x4v *>(
+                       smem[wv] + A::quad_at(row, qd) * 16));
+      if (ue.parts == 1) {
+        finish(row, qd, mm, ll, x);
+      } else {
+        const auto mine = part_at(ue.part);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4_t, x), mine,
+                                               (row * D + 4 * qd) * 4, 0, kSC1);
+        if (qd == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), mine, (ROWS * D + row) * 4, 0,
+                                                kSC1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(ll), mine,
+                                                (ROWS * D + ROWS + row) * 4, 0, kSC1);
+        }
+      }
+    }
+    __syncthreads(); // the tiles' and ms' next use
+    if (ue.parts == 1 || !paged_arrive(&pe.counters[ue.w0], ue.parts, &flag))
+      continue;
+    // Last: all parts, in order.  Threads past one set of items take other parts.
+    const int groups = items < 256 ? 256 / items : 1;
+    for (int base = 0; base < items; base += 256) {
+      const int gi = items < 256 ? tid / items : 0, it = items < 256 ? tid % items : base + tid;
+      const bool on = gi < groups && it < items;
+      const int row = on ? it / dq : 0, qd = on ? it % dq : 0;
+      float mm = -INFINITY, ll = 0.f;
+      f32x4v x = {0.f, 0.f, 0.f, 0.f};
+      constexpr int NJ = 8; // parts in flight
+      for (uint32_t j0 = gi; j0 < ue.parts; j0 += NJ * groups) {
+        float pm[NJ], pl[NJ];
+        i32x4_t px[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const uint32_t jj = j0 + j * groups;
+          pm[j] = -INFINITY, pl[j] = 0.f;
+          if (on && jj < ue.parts) {
+            const uint64_t slot = 2ull * (ue.w0 + jj) + (jj == 0 ? ue.slot0 : 0);
+            const auto all = __builtin_amdgcn_make_buffer_rsrc(unit_parts, 0, 0x7fffffff, 0x00020000);
+            const int at = (int)(slot * part_bytes);
+            px[j] = __builtin_bit_cast(
+                i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, at + (row * D + 4 * qd) * 4, 0, kSC1));
+            pm[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + row) * 4, 0, kSC1));
+            pl[j] = __int_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(all, at + (ROWS * D + ROWS + row) * 4, 0, kSC1));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          paged_join(mm, ll, x, pm[j], pl[j], __builtin_bit_cast(f32x4v, px[j]));
+      }
+      if (groups > 1) {
+        f32x4v *const xs = reinterpret_cast<f32x4v *>(smem[0]);
+        float *const mls = reinterpret_cast<float *>(smem[0] + 4096);
+        xs[tid] = x;
+        mls[tid] = mm, mls[256 + tid] = ll;
+        __syncthreads();
+        if (tid < items) {
+          for (int k = 1; k < groups; ++k)
+            paged_join(mm, ll, x, mls[k * items + tid], mls[256 + k * items + tid],
+                       xs[k * items + tid]);
+          finish(row, qd, mm, ll, x);
+        }
+        __syncthreads();
+      } else if (on) {
+        finish(row, qd, mm, ll, x);
+      }
+    }
   }
   paged_zero_rows<elt>(args);
 }

@@ -180,6 +180,10 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
   }
 }
 
+// Counters of sets of parts begin here in the workspace's 16384 (those of units, and of other
+// launches, before them: a launch has at most 512 workgroups).
+constexpr uint32_t kSetCounters = 8192;
+
 // Which of 16 keys (four adjacent lanes each) a lane's flag is set of.
 __device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
   uint64_t x = lanes | lanes >> 1;
@@ -197,6 +201,7 @@ __device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
 // RT: blocks of 16 rows, which share the fragments of K and V.
 template <int D_, bool BF, bool NV_, int RT_> struct Paged4Split {
   static constexpr int D = D_, BN = 32, RT = RT_, ROWS = 16 * RT;
+  static constexpr int NS = D == 256 ? 1 : D == 64 ? (RT == 1 ? 6 : 4) : RT == 1 ? 3 : 2; // blocks that a wave has under way
   static constexpr bool NV = NV_, CBF = BF && !NV;
   typedef Code4<CBF, NV> Code;
   typedef PagedFrag16<D, CBF, false, BN> P16; // of the values in 16 bits
@@ -211,12 +216,166 @@ template <int D_, bool BF, bool NV_, int RT_> struct Paged4Split {
   }
 };
 
+// A unit's end: the four waves' sums (quads of 4 dims in smem[wave] by A::quad_at, and each row's
+// reference and sum in ms and ls) are joined, and written out, or left as one part of several.
+// The last workgroup to arrive joins the parts, in order; where that would be more than one round of
+// loads (R parts: 8 a thread, and threads past one set of items take others), the last of each R
+// joins those, and the last of all what these leave.  64 parts of 8 rows of 256 dims: a round takes 3
+// us, one after the other they took 25.  vs: the scale of v.
+template <class A, int BYTES>
+__device__ __forceinline__ void paged4_split_end(const PagedAttnArgs &pe, const PagedUnit &ue, float vs,
+                                                 uint8_t (&smem)[4][BYTES], float (&ms)[4][A::ROWS],
+                                                 float (&ls)[4][A::ROWS], int *flag) {
+  constexpr int D = A::D, ROWS = A::ROWS, NJ = 8, kSC1 = 16;
+  constexpr int part_bytes = ROWS * (D + 2) * 4;
+  typedef typename A::elt elt;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  const int dq = pe.head_dim / 4, items = ue.rows * dq;
+  uint8_t *const all = pe.parts;
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(all, 0, 0x7fffffff, 0x00020000);
+  // where part j is (a workgroup's two places: paged_sched.h)
+  auto part_at = [&](uint32_t j) { return (int)((2 * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0)) * (uint32_t)part_bytes); };
+  auto finish = [&](int row, int qd, float mm, float ll, f32x4v x) {
+    const int ro = ue.r0 + row;
+    const int of = paged_token(pe, ro), h = ue.hk * pe.G + ro - of * pe.G;
+    const int64_t t = ue.t0 + of;
+    const float f = ll == 0.f ? 0.f : vs / ll;
+    typename A::h4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      y[e] = (elt)(x[e] * f);
+    *reinterpret_cast<typename A::h4 *>(static_cast<elt *>(pe.o) + t * pe.o_st + h * pe.o_sh + 4 * qd) = y;
+    if (qd == 0 && pe.lse)
+      pe.lse[t * pe.Hq + h] = ll == 0.f ? -INFINITY : mm + __builtin_log2f(ll);
+  };
+  auto store = [&](int at, int row, int qd, float mm, float ll, f32x4v x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4_t, x), rsrc, at + (row * D + 4 * qd) * 4, 0, kSC1);
+    if (qd == 0) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(mm), rsrc, at + (ROWS * D + row) * 4, 0, kSC1);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(ll), rsrc, at + (ROWS * D + ROWS + row) * 4, 0, kSC1);
+    }
+  };
+  for (int it = tid; it < items; it += 256) {
+    const int row = it / dq, qd = it % dq;
+    float mm = -INFINITY, ll = 0.f;
+    f32x4v x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int wv = 0; wv < 4; ++wv)
+      paged_join(mm, ll, x, ms[wv][row], ls[wv][row],
+                 *reinterpret_cast<const f32x4v *>(smem[wv] + A::quad_at(row, qd) * 16));
+    if (ue.parts == 1)
+      finish(row, qd, mm, ll, x);
+    else
+      store(part_at(ue.part), row, qd, mm, ll, x);
+  }
+  __syncthreads(); // the tiles' and ms' next use
+  if (ue.parts == 1)
+    return;
+  const int groups = items < 256 ? 256 / items : 1;
+  // Joins `count` parts, the j-th at from(j).
+  auto join = [&](uint32_t count, auto from, auto emit) __attribute__((always_inline)) {
+    constexpr int IT = ROWS * D > 1024 ? 2 : 1; // items of a thread at a time
+    for (int base = 0; base < items; base += IT * 256) {
+      int row[IT], qd[IT];
+      bool on[IT];
+      float mm[IT], ll[IT];
+      f32x4v x[IT];
+      const int gi = groups > 1 ? tid / items : 0;
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int it = groups > 1 ? tid % items : base + i * 256 + tid;
+        on[i] = it < items && gi < groups && (i == 0 || groups == 1);
+        row[i] = on[i] ? it / dq : 0, qd[i] = on[i] ? it % dq : 0;
+        mm[i] = -INFINITY, ll[i] = 0.f, x[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+      }
+      for (uint32_t j0 = gi; j0 < count; j0 += NJ * groups) {
+        float pm[IT][NJ], pl[IT][NJ];
+        i32x4_t px[IT][NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const uint32_t jj = j0 + j * groups;
+          const int at = from(jj < count ? jj : 0);
+#pragma unroll
+          for (int i = 0; i < IT; ++i) {
+            pm[i][j] = -INFINITY, pl[i][j] = 0.f;
+            if (on[i] && jj < count) {
+              px[i][j] = __builtin_bit_cast(
+                  i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + (row[i] * D + 4 * qd[i]) * 4, 0, kSC1));
+              pm[i][j] = __int_as_float(
+                  __builtin_amdgcn_raw_buffer_load_b32(rsrc, at + (ROWS * D + row[i]) * 4, 0, kSC1));
+              pl[i][j] = __int_as_float(
+                  __builtin_amdgcn_raw_buffer_load_b32(rsrc, at + (ROWS * D + ROWS + row[i]) * 4, 0, kSC1));
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < IT; ++i)
+            paged_join(mm[i], ll[i], x[i], pm[i][j], pl[i][j], __builtin_bit_cast(f32x4v, px[i][j]));
+      }
+      if (groups > 1) {
+        f32x4v *const xs = reinterpret_cast<f32x4v *>(smem[0]);
+        float *const mls = reinterpret_cast<float *>(smem[0] + 4096);
+        xs[tid] = x[0];
+        mls[tid] = mm[0], mls[256 + tid] = ll[0];
+        __syncthreads();
+        if (tid < items) {
+          for (int k = 1; k < groups; ++k)
+            paged_join(mm[0], ll[0], x[0], mls[k * items + tid], mls[256 + k * items + tid], xs[k * items + tid]);
+          emit(row[0], qd[0], mm[0], ll[0], x[0]);
+        }
+        __syncthreads();
+      } else {
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+          if (on[i])
+            emit(row[i], qd[i], mm[i], ll[i], x[i]);
+      }
+    }
+  };
+  const uint32_t R = NJ * groups;
+  if (ue.parts > R) {
+    const uint32_t g = ue.part / R, n = ue.parts - g * R < R ? ue.parts - g * R : R, sets = (ue.parts + R - 1) / R;
+    // What the parts of set g leave: in the second place of a workgroup whose run lies within the unit,
+    // so that it has no other part (the first of the set, of set 0 the second); a last part alone
+    // is its set's.  Counters: apart from the units' own, that of the set's first workgroup.
+    auto set_at = [&](uint32_t k) {
+      return k * R + 1 == ue.parts ? part_at(k * R) : (int)((2 * (ue.w0 + (k ? k * R : 1)) + 1) * (uint32_t)part_bytes);
+    };
+    if (n > 1) {
+      if (!paged_arrive(&pe.counters[kSetCounters + ue.w0 + g * R], n, flag))
+        return;
+      const int to = set_at(g);
+      join(n, [&](uint32_t j) { return part_at(g * R + j); },
+           [&](int row, int qd, float mm, float ll, f32x4v x) { store(to, row, qd, mm, ll, x); });
+    }
+    if (!paged_arrive(&pe.counters[ue.w0], sets, flag))
+      return;
+    join(sets, set_at, finish);
+  } else {
+    if (!paged_arrive(&pe.counters[ue.w0], ue.parts, flag))
+      return;
+    join(ue.parts, part_at, finish);
+  }
+}
+
+// f(0), .. f(N - 1), of constants.
+template <int N, class F, int... I>
+__device__ __forceinline__ void each_slot(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F> __device__ __forceinline__ void each_slot(F f) {
+  each_slot<N>(f, std::make_integer_sequence<int, N>());
+}
+
 // Workgroups of a CU: by LDS, and by registers where heads are long.
 template <class A> constexpr int paged4_split_groups() { return A::BYTES * 4 <= 81920 ? 2 : 1; }
 
 template <class A>
 __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_split_kernel(Paged4Args args4) {
-  constexpr int D = A::D, BN = A::BN, RT = A::RT, ROWS = A::ROWS, NS = 2;
+  constexpr int D = A::D, BN = A::BN, RT = A::RT, ROWS = A::ROWS, NS = A::NS;
   typedef typename A::P16 P16;
   typedef typename A::Piece Piece;
   typedef typename A::Code Code;
@@ -283,7 +442,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       }
     }
     Piece kp[NS][2], vp[NS][2];
-    uint64_t here[NS + 1] = {}; // of blocks k .. k + NS
+    uint32_t here[NS + 1] = {}; // of blocks k .. k + NS
     if (k0 < k1) {
       pr.settle();
 #pragma unroll
@@ -291,7 +450,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
         if (k0 + i < k1) {
           const int n = (k0 + i) * BN;
           pr.hold(n);
-          here[i] = pr.template there<BN>(n, un.hi);
+          here[i] = (uint32_t)pr.template there<BN>(n, un.hi);
           sk.load(pr, n, km, kp[i]), sv.load(pr, n, vm, vp[i]);
         }
     }
@@ -369,7 +528,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       }
       if (k + NS < k1) {
         pr.hold(na);
-        here[NS] = pr.template there<BN>(na, un.hi);
+        here[NS] = (uint32_t)pr.template there<BN>(na, un.hi);
         sk.load(pr, na, km, kp[SL]), sv.load(pr, na, vm, vp[SL]);
       }
       if (__builtin_expect((none[0] | none[1]) != 0, 0)) {
@@ -382,11 +541,10 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
             for (int r = 0; r < 4; ++r)
               s[i][b][r] = nan >> (16 * b + r) & 1 ? __builtin_nanf("") : s[i][b][r];
       }
-      const uint64_t all = ~0ull >> (64 - BN);
       typename P16::PF pf[RT];
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        if (here[0] != all || n0 < lo_all || n0 + BN > hi_all) {
+        if (here[0] != ~0u || n0 < lo_all || n0 + BN > hi_all) {
           const int a = lo[i] - n0 < 0 ? 0 : lo[i] - n0, z = hi[i] - n0 < 0 ? 0 : hi[i] - n0;
           uint64_t seen = z < 64 ? (1ull << z) - 1 : ~0ull;
           seen &= a < 64 ? ~0ull << a : 0;
@@ -406,11 +564,11 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       for (int i = 0; i < NS; ++i)
         here[i] = here[i + 1];
     };
-    for (int k = k0; k < k1;) {
-      iter(k++, std::integral_constant<int, 0>());
-      if (k < k1)
-        iter(k++, std::integral_constant<int, 1>());
-    }
+    for (int k = k0; k < k1;)
+      each_slot<NS>([&](auto slot) __attribute__((always_inline)) {
+        if (k < k1)
+          iter(k++, slot);
+      });
 
     // The waves' sums: quads of 4 dims in lane order in each one's own tile.
     const PagedAttnArgs &pe = paged_args();
@@ -428,7 +586,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       if (lane < 16)
         ms[wave][16 * i + lane] = m[i], ls[wave][16 * i + lane] = l[i];
     }
-    paged_split_end<A>(pe, ue, vs, smem, ms, ls, &flag);
+    paged4_split_end<A>(pe, ue, vs, smem, ms, ls, &flag);
   }
   paged_zero_rows<elt>(args4.a);
 }
