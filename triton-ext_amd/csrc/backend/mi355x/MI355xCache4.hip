@@ -376,9 +376,9 @@ extern "C" TX_API int tx_paged_attn4_plan_create(const tx_paged_attn4_desc *desc
     return fail(TX_ERR_INVALID, "q and o strides must be multiples of 16 bytes");
   // (the kernels' offsets from one of 16 tokens have 32 bits)
   const tx_block_scales &s = desc->s;
-  const int64_t blocks = d.head_dim / (s.mode == TX_SCALE_MX32 ? 32 : 16), far = (int64_t)1 << 27;
+  const int64_t blocks = d.head_dim / (s.mode == TX_SCALE_MX32 ? 32 : 16), far = (int64_t)1 << 26;
   if (d.page_size > 1 && (d.k_st >= far || d.v_st >= far || s.k_st >= far || s.v_st >= far))
-    return fail(TX_ERR_UNSUPPORTED, "tokens of a page 2^27 bytes apart");
+    return fail(TX_ERR_UNSUPPORTED, "tokens of a page 2^26 bytes apart");
   if ((blocks - 1) * s.k_sb >= ((int64_t)1 << 31) || (blocks - 1) * s.v_sb >= ((int64_t)1 << 31))
     return fail(TX_ERR_UNSUPPORTED, "scales of a head 2^31 bytes apart");
   if (d.T * (int64_t)(d.Hkv ? d.Hq / d.Hkv : 0) > INT32_MAX)
@@ -478,6 +478,8 @@ extern "C" TX_API int tx_paged_attn4_launch(const tx_paged_attn4_plan *plan, con
   a.qk_scale = d.sm_scale * 1.44269504f;
   g.ks = scalesOf(k_block_scale, s.k_sp, s.k_st, s.k_sh, s.k_sb);
   g.vs = scalesOf(v_block_scale, s.v_sp, s.v_st, s.v_sh, s.v_sb);
+  g.packed = d.page_size >= 4 && aligned(k_block_scale, 4) && aligned(v_block_scale, 4) && s.k_st == 1 &&
+             s.v_st == 1 && commonVec(4, {s.k_sp, s.k_sh, s.k_sb, s.v_sp, s.v_sh, s.v_sb}) == 4;
   const int D = attnDims(d.head_dim), di = D == 64 ? 0 : D == 96 ? 1 : D == 128 ? 2 : 3;
   const bool bf = d.dtype == TX_BF16, nv = s.mode == TX_SCALE_NV16;
   const Paged4AttnFn fn = plan->variant == 2 ? kPaged4Rows[di][bf][nv] : kPaged4Split[plan->variant][di][bf][nv];

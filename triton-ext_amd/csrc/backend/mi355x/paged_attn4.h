@@ -26,18 +26,20 @@ namespace txk {
 struct Paged4Args {
   PagedAttnArgs a; // (first: paged_args() reads it)
   BlockScales ks, vs;
+  int32_t packed; // the scales of 4 keys from a multiple of 4 on are an aligned dword
 };
 __device__ __forceinline__ const Paged4Args &paged4_args() {
   return reinterpret_cast<const Paged4Args &>(paged_args());
 }
 
-// What a lane holds of one key's K or V row, in the order of its quarter g.
+// What a lane holds of one key's K or V row, in the order of its quarter g: KW dwords of 8 dims, under SB
+// block scales.
 template <int D, bool NV> struct Piece4 {
-  static constexpr int KW = D == 64 ? 2 : D == 256 ? 8 : 4; // dwords of 8 dims
+  static constexpr int KW = D == 64 ? 2 : D == 256 ? 8 : 4;
   static constexpr int SB = D == 64 ? 1 : (D == 256 ? 2 : 1) * (NV ? 2 : 1);
-  uint32_t w[KW], s[SB];
+  uint32_t w[KW];
 
-  // The dims of dword c, and the scale among s that is theirs.
+  // The dims of dword c, the scale that is theirs, and the block of scale j.
   __device__ __forceinline__ static constexpr int dim(int c, int g) {
     return D == 64 ? 16 * g + 8 * c : 128 * (c / 4) + 32 * g + 8 * (c % 4);
   }
@@ -71,20 +73,22 @@ struct PageRow4 : PageRow {
   }
 };
 
-// Where lane (m, g) finds its pieces of K (V: of V) of 16 keys: the codes and scales of a head, which
-// are uniform, and the lane's offsets from the first key, of 32 bits.  Pieces past head_dim are those
-// of its beginning (Q is 0 there; V's are not stored).
+__device__ __forceinline__ uint64_t lane_from(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__shfl((int)v, lane & 63) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane & 63) << 32;
+}
+
+// Where lane (m, g) finds its pieces of K (V: of V) of 16 keys: the codes of a head, which are
+// uniform, and the lane's offsets from the first key, of 32 bits.  Pieces past head_dim are those of
+// its beginning (Q is 0 there; V's are not stored).
 template <int D, bool NV, bool V> struct Side4 {
   typedef Piece4<D, NV> P;
-  const uint8_t *codes, *scales;
-  uint32_t st, sst;
-  uint32_t off[D == 256 ? 2 : 1], soff[P::SB];
+  const uint8_t *codes;
+  uint32_t st;
+  uint32_t off[D == 256 ? 2 : 1];
 
   __device__ __forceinline__ Side4(const Paged4Args &p, int hk, int m, int g) {
-    const BlockScales &bs = V ? p.vs : p.ks;
     codes = (V ? p.a.vc : p.a.kc) + hk * (V ? p.a.v_sh : p.a.k_sh);
-    scales = bs.s + hk * bs.sh;
-    st = (uint32_t)(V ? p.a.v_st : p.a.k_st), sst = (uint32_t)bs.st;
+    st = (uint32_t)(V ? p.a.v_st : p.a.k_st);
     const uint32_t row = p.a.page_shift >= 4 ? m : m & ((1 << p.a.page_shift) - 1);
     const int bytes = p.a.head_dim / 2;
 #pragma unroll
@@ -92,56 +96,135 @@ template <int D, bool NV, bool V> struct Side4 {
       const int o = D == 64 ? 8 * g : 64 * i + 16 * g;
       off[i] = row * st + (o < bytes ? o : 0);
     }
-#pragma unroll
-    for (int j = 0; j < P::SB; ++j) {
-      const int b = P::block_of(j, g);
-      soff[j] = row * sst + (b < p.a.head_dim / (NV ? 16 : 32) ? b : 0) * (uint32_t)bs.sb;
-    }
   }
-  __device__ __forceinline__ void read(const uint8_t *c, const uint8_t *s, P &x) const {
+  template <bool NT, class W> __device__ __forceinline__ static W take(const uint8_t *p) {
+    if constexpr (NT)
+      return __builtin_nontemporal_load(reinterpret_cast<const W *>(p));
+    else
+      return *reinterpret_cast<const W *>(p);
+  }
+  template <bool NT> __device__ __forceinline__ void read(const uint8_t *c, P &x) const {
     typedef uint32_t w2 __attribute__((ext_vector_type(2)));
     typedef uint32_t w4 __attribute__((ext_vector_type(4)));
     if constexpr (D == 64) {
-      const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2 *>(c + off[0]));
+      const w2 v = take<NT, w2>(c + off[0]);
       x.w[0] = v[0], x.w[1] = v[1];
     } else {
 #pragma unroll
       for (int i = 0; i < P::KW / 4; ++i) {
-        const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4 *>(c + off[i]));
+        const w4 v = take<NT, w4>(c + off[i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           x.w[4 * i + e] = v[e];
       }
     }
-#pragma unroll
-    for (int j = 0; j < P::SB; ++j)
-      x.s[j] = __builtin_nontemporal_load(s + soff[j]);
   }
-  // The pieces of N runs of 16 keys from n on, a multiple of 16 N; m is the lane's row again.
-  template <int N> __device__ __forceinline__ void load(const PageRow4 &pr, int n, int m, P (&x)[N]) const {
+  // The pieces of N runs of 16 keys from n on, a multiple of 16 N; m is the lane's row again.  NT: data
+  // that is read once.
+  template <bool NT, int N>
+  __device__ __forceinline__ void load(const PageRow4 &pr, int n, int m, P (&x)[N]) const {
     if (pr.shift >= 4) { // a run lies in one page
-      const uint8_t *c, *s;
+      const uint8_t *c;
 #pragma unroll
       for (int b = 0; b < N; ++b) {
         if (b == 0 || pr.shift < 5) {
           const int key = n + 16 * b, e = ((key >> pr.shift) - pr.first) & 63;
           const uint64_t slot = key & ((1 << pr.shift) - 1);
           c = codes + (uint64_t)lane_value64(pr.at[V ? 2 : 0], e) + slot * st;
-          s = scales + (uint64_t)lane_value64(pr.at[V ? 3 : 1], e) + slot * sst;
         } else {
-          c += 16ull * st, s += 16ull * sst;
+          c += 16ull * st;
         }
-        read(c, s, x[b]);
+        read<NT>(c, x[b]);
       }
     } else {
 #pragma unroll
-      for (int b = 0; b < N; ++b) {
-        const int e = (((n + 16 * b + m) >> pr.shift) - pr.first) & 63;
-        auto of = [&](uint64_t v) {
-          return (uint64_t)(uint32_t)__shfl((int)v, e) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), e) << 32;
-        };
-        read(codes + of(pr.at[V ? 2 : 0]), scales + of(pr.at[V ? 3 : 1]), x[b]);
+      for (int b = 0; b < N; ++b)
+        read<NT>(codes + lane_from(pr.at[V ? 2 : 0], ((n + 16 * b + m) >> pr.shift) - pr.first), x[b]);
+    }
+  }
+};
+
+// The block scales of KEYS keys' K and V: a lane holds dwords of 4 keys of a block each, in the order
+// [K, V][block][4 keys], which one or two loads of whole lines bring (a byte a lane and key took the
+// same memory 98 us where this takes 88: 4 sequences of up to 131072); the lanes that convert fetch their
+// byte from there.
+template <int D, bool NV, int KEYS> struct Scales4 {
+  typedef Piece4<D, NV> P;
+  static constexpr int NB = (D == 96 ? 128 : D) / (NV ? 16 : 32), QUADS = KEYS / 4, HALF = NB * QUADS;
+  static constexpr int W = (2 * HALF + 63) / 64;
+  struct Held {
+    uint32_t w[W];
+  };
+  const uint8_t *ks, *vs; // of the head
+  uint32_t kst, vst;
+  uint32_t off[W];        // of the lane's block and, where a page holds KEYS keys, its first key
+  int quad[W];            // that key
+  bool v[W];
+  bool packed;            // 4 keys of a block are a dword
+  uint32_t kfrom[P::SB], vfrom[P::SB], kshift, vshift;
+
+  // km, kg, vm, vg: as the lane has its pieces of K and V
+  __device__ __forceinline__ Scales4(const Paged4Args &p, int hk, int km, int kg, int vm, int vg) {
+    ks = p.ks.s + hk * p.ks.sh, vs = p.vs.s + hk * p.vs.sh;
+    kst = (uint32_t)p.ks.st, vst = (uint32_t)p.vs.st, packed = p.packed;
+    const int lane = threadIdx.x & 63, blocks = p.a.head_dim / (NV ? 16 : 32);
+#pragma unroll
+    for (int r = 0; r < W; ++r) {
+      const int i = (64 * r + lane) % (2 * HALF), b = i / QUADS % NB;
+      v[r] = i >= HALF, quad[r] = 4 * (i % QUADS);
+      const uint32_t st = v[r] ? vst : kst, sb = (uint32_t)(v[r] ? p.vs.sb : p.ks.sb);
+      off[r] = (b < blocks ? b : 0) * sb + (quad[r] & ((1 << p.a.page_shift) - 1)) * st;
+    }
+#pragma unroll
+    for (int j = 0; j < P::SB; ++j) {
+      kfrom[j] = 4 * ((P::block_of(j, kg) * QUADS + km / 4) & 63);
+      vfrom[j] = 4 * ((HALF + P::block_of(j, vg) * QUADS + vm / 4) & 63);
+    }
+    kshift = 8 * (km & 3), vshift = 8 * (vm & 3);
+  }
+  // Of the keys from n on, a multiple of KEYS.
+  __device__ __forceinline__ void load(const PageRow4 &pr, int n, Held &x) const {
+    const bool one = (1 << pr.shift) >= KEYS; // page
+    const uint8_t *bk = ks, *bv = vs;
+    if (one) {
+      const int e = ((n >> pr.shift) - pr.first) & 63;
+      const uint64_t slot = n & ((1 << pr.shift) - 1);
+      bk += (uint64_t)lane_value64(pr.at[1], e) + slot * kst;
+      bv += (uint64_t)lane_value64(pr.at[3], e) + slot * vst;
+    }
+#pragma unroll
+    for (int r = 0; r < W; ++r) {
+      const uint8_t *p = (v[r] ? bv : bk) + off[r];
+      if (packed) {
+        if (!one) {
+          const int e = ((n + quad[r]) >> pr.shift) - pr.first;
+          const uint64_t a = lane_from(pr.at[1], e), b = lane_from(pr.at[3], e);
+          p += v[r] ? b : a;
+        }
+        x.w[r] = *reinterpret_cast<const uint32_t *>(p);
+      } else {
+        uint32_t w = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int key = n + quad[r] + t, in = key & ((1 << pr.shift) - 1);
+          const int e = (key >> pr.shift) - pr.first;
+          const uint64_t a = lane_from(pr.at[1], e), b = lane_from(pr.at[3], e);
+          const int base = quad[r] & ((1 << pr.shift) - 1);
+          const uint32_t st = v[r] ? vst : kst;
+          const uint8_t *q = (v[r] ? vs + b : ks + a) + (off[r] - (uint64_t)base * st) + (uint64_t)in * st;
+          w |= (uint32_t)*q << (8 * t);
+        }
+        x.w[r] = w;
       }
+    }
+  }
+  // The scale bytes of the lane's pieces of run b.
+  template <bool V> __device__ __forceinline__ void of(const Held &x, int b, uint32_t (&s)[P::SB]) const {
+#pragma unroll
+    for (int j = 0; j < P::SB; ++j) {
+      const int r = ((V ? HALF : 0) + P::block_of(j, 0) * QUADS) / 64; // (the other g are in it too)
+      const uint32_t w = __builtin_amdgcn_ds_bpermute((V ? vfrom[j] : kfrom[j]) + 16 * b, x.w[r]);
+      s[j] = __builtin_amdgcn_ubfe(w, V ? vshift : kshift, 8);
     }
   }
 };
@@ -441,7 +524,9 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
         qf[i][c] = *reinterpret_cast<const u32x4 *>(row + (d < p.head_dim ? d : 0));
       }
     }
+    const Scales4<D, A::NV, BN> sc(p4, un.hk, km, kg, vm, vg);
     Piece kp[NS][2], vp[NS][2];
+    typename Scales4<D, A::NV, BN>::Held sp[NS];
     uint32_t here[NS + 1] = {}; // of blocks k .. k + NS
     if (k0 < k1) {
       pr.settle();
@@ -451,7 +536,8 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
           const int n = (k0 + i) * BN;
           pr.hold(n);
           here[i] = (uint32_t)pr.template there<BN>(n, un.hi);
-          sk.load(pr, n, km, kp[i]), sv.load(pr, n, vm, vp[i]);
+          sc.load(pr, n, sp[i]);
+          sk.template load<true>(pr, n, km, kp[i]), sv.template load<true>(pr, n, vm, vp[i]);
         }
     }
     if (wave == 0)
@@ -496,9 +582,10 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       for (int b = 0; b < 2; ++b) {
         const Piece &x = kp[SL][b];
         uint32_t f[Piece::SB];
+        sc.template of<false>(sp[SL], b, f);
 #pragma unroll
         for (int j = 0; j < Piece::SB; ++j)
-          f[j] = Code::factor(x.s[j], false);
+          f[j] = Code::factor(f[j], false);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
           s[i][b] = typename P16::f4v{};
@@ -515,10 +602,11 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       for (int b = 0; b < 2; ++b) {
         const Piece &x = vp[SL][b];
         uint32_t f[Piece::SB];
+        sc.template of<true>(sp[SL], b, f);
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < Piece::SB; ++j)
-          bad = bad || Code::bad(x.s[j]), f[j] = Code::factor(x.s[j], true);
+          bad = bad || Code::bad(f[j]), f[j] = Code::factor(f[j], true);
         none[b] = __ballot(bad);
 #pragma unroll
         for (int c = 0; c < Piece::KW; ++c) {
@@ -529,7 +617,8 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       if (k + NS < k1) {
         pr.hold(na);
         here[NS] = (uint32_t)pr.template there<BN>(na, un.hi);
-        sk.load(pr, na, km, kp[SL]), sv.load(pr, na, vm, vp[SL]);
+        sc.load(pr, na, sp[SL]);
+        sk.template load<true>(pr, na, km, kp[SL]), sv.template load<true>(pr, na, vm, vp[SL]);
       }
       if (__builtin_expect((none[0] | none[1]) != 0, 0)) {
         const uint32_t nan = (keys_of(none[0]) | keys_of(none[1]) << 16) >> (4 * kg);
@@ -659,21 +748,29 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
     const Side4<D, A::NV, false> sk(p4, un.hk, em, eg);
     const Side4<D, A::NV, true> sv(p4, un.hk, em, eg);
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
+    const Scales4<D, A::NV, 16> sc(p4, un.hk, em, eg, em, eg);
     Piece kp[1], vp[1];
+    typename Scales4<D, A::NV, 16>::Held sp;
+    const bool once = un.alone; // keys that no other unit reads go past the caches
     auto fetch = [&](int k) __attribute__((always_inline)) {
       pr.hold(k * BN);
       here[2] = pr.template there<BN>(k * BN, un.hi);
-      sk.load(pr, k * BN + 16 * wave, em, kp);
-      sv.load(pr, k * BN + 16 * wave, em, vp);
+      const int n = k * BN + 16 * wave;
+      sc.load(pr, n, sp);
+      if (once)
+        sk.template load<true>(pr, n, em, kp), sv.template load<true>(pr, n, em, vp);
+      else
+        sk.template load<false>(pr, n, em, kp), sv.template load<false>(pr, n, em, vp);
     };
     auto convert = [&](int slot) __attribute__((always_inline)) {
       typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
       uint32_t fk[Piece::SB], fv[Piece::SB];
+      sc.template of<false>(sp, 0, fk), sc.template of<true>(sp, 0, fv);
       bool bad = false;
 #pragma unroll
       for (int j = 0; j < Piece::SB; ++j) {
-        fk[j] = Code::factor(kp[0].s[j], false), fv[j] = Code::factor(vp[0].s[j], true);
-        bad = bad || Code::bad(vp[0].s[j]);
+        bad = bad || Code::bad(fv[j]);
+        fk[j] = Code::factor(fk[j], false), fv[j] = Code::factor(fv[j], true);
       }
       const uint64_t none = __ballot(bad);
       if (lane == 0)
