@@ -47,7 +47,8 @@ typedef struct tx_paged_append4_plan {
   tx_paged_append4_desc desc;
   double flops, bytes;
   int32_t whole; /* tokens are read 16 bytes at a time (the launch: where addresses allow it) */
-  int32_t head_lanes, grid_x, block_threads;
+  int32_t run;   /* how a thread has a head's dims: 0: 8 of them, 1: 8 of each half, 2: 8 in pairs */
+  int32_t head_lanes, grid_x, block_threads, reserved;
 } tx_paged_append4_plan;
 
 TX_API int tx_paged_append4_plan_create(const tx_paged_append4_desc *desc,

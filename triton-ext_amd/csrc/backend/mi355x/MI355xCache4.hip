@@ -60,9 +60,18 @@ BlockScales scalesOf(const void *p, int64_t sp, int64_t st, int64_t sh, int64_t 
   return BlockScales{static_cast<uint8_t *>(const_cast<void *>(p)), sp, st, sh, sb};
 }
 
-template <class T, bool NV> void append4Kernels(void (*(&k)[2][2])(Append4Args)) {
-  k[0][0] = paged_append4_kernel<T, NV, false, false>, k[0][1] = paged_append4_kernel<T, NV, false, true>;
-  k[1][0] = paged_append4_kernel<T, NV, true, false>, k[1][1] = paged_append4_kernel<T, NV, true, true>;
+template <class T, bool NV> void append4Kernels(void (*(&k)[3][2])(Append4Args)) {
+  k[0][0] = paged_append4_kernel<T, NV, kRunAlone, false>, k[0][1] = paged_append4_kernel<T, NV, kRunAlone, true>;
+  k[1][0] = paged_append4_kernel<T, NV, kRunHalves, false>, k[1][1] = paged_append4_kernel<T, NV, kRunHalves, true>;
+  k[2][0] = paged_append4_kernel<T, NV, kRunPairs, false>, k[2][1] = paged_append4_kernel<T, NV, kRunPairs, true>;
+}
+
+// How a thread has a head's dims (cache4_rows.h): halves where blocks end within them.
+int runOfAppend(const tx_paged_append_desc &d, int32_t mode) {
+  const int two = mode == TX_SCALE_MX32 ? 64 : 32;
+  if (d.interleaved && d.rot_dim)
+    return kRunPairs;
+  return d.rot_dim % two == 0 && (d.head_dim - d.rot_dim) % two == 0 ? kRunHalves : kRunAlone;
 }
 
 } // namespace
@@ -108,7 +117,8 @@ extern "C" TX_API int tx_paged_append4_plan_create(const tx_paged_append4_desc *
   plan->whole = commonVec(8, {d.Hq ? d.q_st : 0, d.Hq ? d.q_sh : 0, d.Hq ? d.o_st : 0, d.Hq ? d.o_sh : 0,
                               d.k_st, d.k_sh, d.v_st, d.v_sh}) == 8 &&
                 (d.interleaved || d.rot_dim % 16 == 0);
-  const int64_t items = d.head_dim / 8, heads = (int64_t)d.Hq + 2 * (int64_t)d.Hkv;
+  plan->run = runOfAppend(d, desc->s.mode);
+  const int64_t items = d.head_dim / (plan->run == kRunHalves ? 16 : 8), heads = (int64_t)d.Hq + 2 * (int64_t)d.Hkv;
   plan->head_lanes = headLanes(d.T, items, heads);
   plan->block_threads = 256;
   const int64_t per = items * plan->head_lanes;
@@ -172,14 +182,14 @@ extern "C" TX_API int tx_paged_append4_launch(const tx_paged_append4_plan *plan,
   a.kc_sp = d.kc_sp, a.kc_st = d.kc_st, a.kc_sh = d.kc_sh;
   a.vc_sp = d.vc_sp, a.vc_st = d.vc_st, a.vc_sh = d.vc_sh;
   a.B = (int32_t)d.B, a.Hq = d.Hq, a.Hkv = d.Hkv, a.head_dim = d.head_dim, a.rot = d.rot_dim;
-  a.items = d.head_dim / 8;
+  a.items = d.head_dim / (plan->run == kRunHalves ? 16 : 8);
   a.head_lanes = plan->head_lanes, a.token_threads = a.items * plan->head_lanes;
   a.page_shift = log2of(d.page_size), a.scale = d.scale;
   g.ks = scalesOf(k_block_scale, s.k_sp, s.k_st, s.k_sh, s.k_sb);
   g.vs = scalesOf(v_block_scale, s.v_sp, s.v_st, s.v_sh, s.v_sb);
   // values of the type at the ends: 6 * 2^hi is one, 0.5 * 2^lo is exact
   g.lo = d.dtype == TX_F16 ? -23 : -125, g.hi = d.dtype == TX_F16 ? 13 : 125;
-  void (*fn[2][2])(Append4Args);
+  void (*fn[3][2])(Append4Args);
   const bool nv = s.mode == TX_SCALE_NV16;
   if (d.dtype == TX_F16 && nv)
     append4Kernels<_Float16, true>(fn);
@@ -189,7 +199,7 @@ extern "C" TX_API int tx_paged_append4_launch(const tx_paged_append4_plan *plan,
     append4Kernels<__bf16, true>(fn);
   else
     append4Kernels<__bf16, false>(fn);
-  hipLaunchKernelGGL(fn[d.interleaved][whole], dim3((uint32_t)plan->grid_x), dim3(256), 0,
+  hipLaunchKernelGGL(fn[plan->run][whole], dim3((uint32_t)plan->grid_x), dim3(256), 0,
                      static_cast<hipStream_t>(stream), g);
   TX_HIP_CHECK(hipGetLastError());
   return TX_OK;
@@ -400,7 +410,7 @@ extern "C" TX_API int tx_paged_attn4_plan_create(const tx_paged_attn4_desc *desc
   const int step = split ? 128 : 64;
   const double units = (double)d.B + (double)d.T * G / plan->rows;
   const double keys = (double)d.table_width * d.page_size;
-  const double steps = units * (keys / step + 1 + (split ? kSplitOverhead : kRowsOverhead)) * d.Hkv;
+  const double steps = units * (keys / step + 1 + (split ? kSplit4Overhead : kRows4Overhead)) * d.Hkv;
   if (steps > INT32_MAX)
     return fail(TX_ERR_UNSUPPORTED, "more than 2^31 blocks of keys for %lld tokens: fewer a call",
                 (long long)d.T);

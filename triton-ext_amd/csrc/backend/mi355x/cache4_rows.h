@@ -1,10 +1,9 @@
 // New tokens into a 4-bit paged cache, and tokens out of any paged cache (tx_cache4.h).
 //
-// Append: a lane takes 8 adjacent dims of a head, so that a block's lanes (4, or 2 under e4m3
-// scales) are neighbours that find its largest magnitude by two DPP moves.  Rotated dims need
-// their partners, rot_dim / 2 further (halves) or in the same 8 (interleaved): the lane reads
-// them too.  A thread forms its 8 (or 4) sines once and goes through the token's heads, every
-// head_lanes-th of them.
+// Append: a lane takes 8 adjacent dims of a head, or 8 of each half of its rotated dims, so that a
+// block's lanes (4, or 2 under e4m3 scales) are neighbours that find its largest magnitude by two DPP
+// moves.  A token's sines are formed once, a pair a thread, and go through LDS; a thread then goes
+// through the token's heads, every head_lanes-th of them.
 //
 // Read: the same threads; a lane turns 8 dims into 16 or 32 bytes.  Both are bound by memory.
 #pragma once
@@ -88,130 +87,175 @@ __device__ __forceinline__ void store8(T *p, const float (&y)[8]) {
   }
 }
 
-// The turn of 8 adjacent dims: y = x c + partner s (with the sign of each dim's half).
-template <bool INTER> struct Turn8 {
-  bool any; // of the 8 dims is rotated
-  int dim, rot;
-  float c[INTER ? 4 : 8], s[INTER ? 4 : 8];
+// cos and sin of position * f, times scale: turn_of (rotary.h) with the turn's rounding to fp32 made good to
+// first order, since a key is quantised after it.
+__device__ __forceinline__ float2_t turn4_of(double pos, float f, float scale) {
+  double t = pos * (double)f * 0.15915494309189535; // turns
+  t -= rint(t);
+  const float turn = (float)t, rest = 6.2831853f * (float)(t - (double)turn);
+  float s, c;
+  sincospif(2.0f * turn, &s, &c);
+  return float2_t{(c - s * rest) * scale, (s + c * rest) * scale};
+}
 
-  __device__ __forceinline__ Turn8(int item, int rot_dim, double pos, const float *inv_freq, float scale)
-      : any(8 * item < rot_dim), dim(8 * item), rot(rot_dim) {
-    if (!any)
-      return;
+// How a thread has the dims of a head: 8 adjacent ones whose partners are elsewhere (any rot_dim), 8 of
+// each half of the rotated dims and of those past them (blocks lie within a half), or 8 of interleaved pairs.
+enum { kRunAlone = 0, kRunHalves = 1, kRunPairs = 2 };
+constexpr int kAppendSines = 2048; // pairs of a workgroup's tokens in LDS
+
+template <class T, bool NV, int MODE, bool WHOLE>
+__global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
+  constexpr int RUNS = MODE == kRunHalves ? 2 : 1, LANES = NV ? 2 : 4; // LANES of a block
+  constexpr int BATCH = RUNS == 2 ? 2 : 4;                             // heads that a thread has under way
+  __shared__ float2_t sines[kAppendSines];
+  const AppendArgs &p = args.a;
+  const RotaryPlace at(p.token_threads, p.items, false);
+  const int64_t t = at.tok;
+  const bool on = t < p.T;
+  TokenPlace pl = {};
+  if (on)
+    pl = token_place(t, p.cu_q, p.kv_len, p.B, p.table, p.table_s, p.table_width, p.pages, p.page_shift);
+  const int rot = p.rot, half = rot / 2;
+
+  // The token's sines, a pair a thread, in LDS; heads of more pairs than that: each thread its own.
+  const int per = p.token_threads <= 256 ? p.token_threads : 256, mine0 = (int)threadIdx.x / per * half;
+  const bool shared = (256 / per) * half <= kAppendSines;
+  if (shared && on)
+    for (int i = (int)threadIdx.x % per; i < half; i += per)
+      sines[mine0 + i] = turn4_of((double)pl.pos, p.inv_freq[i], p.scale);
+  __syncthreads();
+  if (!on)
+    return;
+
+  // dims d[r] .. d[r] + 7
+  int d[RUNS];
+  if constexpr (MODE == kRunHalves) {
+    const int pairs = rot / 16, i = at.item < pairs ? at.item : at.item - pairs;
+    const int from = at.item < pairs ? 0 : rot, n = at.item < pairs ? rot : p.head_dim - rot;
+    d[0] = from + 8 * i, d[RUNS - 1] = from + n / 2 + 8 * i;
+  } else {
+    d[0] = 8 * at.item;
+  }
+  const bool turned = d[0] < rot;
+  // of pair (dims j and j + half; or 2 j and 2 j + 1) that dim d[0] + i (or 2 i) is in: the sine has
+  // the sign that its partner comes with
+  constexpr int NP = MODE == kRunPairs ? 4 : 8;
+  float c[NP], s[NP];
 #pragma unroll
-    for (int i = 0; i < (INTER ? 4 : 8); ++i) {
-      const int d = INTER ? dim + 2 * i : dim + i;
-      c[i] = 1.f, s[i] = 0.f;
-      if (d < rot) {
-        const bool second = !INTER && d >= rot / 2;
-        turn_of(pos, inv_freq[INTER ? d / 2 : second ? d - rot / 2 : d], scale, !INTER && !second, c[i], s[i]);
-      }
+  for (int i = 0; i < NP; ++i) {
+    c[i] = 1.f, s[i] = 0.f;
+    const int dim = MODE == kRunPairs ? d[0] + 2 * i : d[0] + i;
+    if (dim < rot) {
+      const bool second = MODE == kRunAlone && dim >= half;
+      const int j = MODE == kRunPairs ? dim / 2 : second ? dim - half : dim;
+      const float2_t cs = shared ? sines[mine0 + j] : turn4_of((double)pl.pos, p.inv_freq[j], p.scale);
+      c[i] = cs[0], s[i] = MODE == kRunAlone && !second ? -cs[1] : cs[1];
     }
   }
-  // The partners of the 8 dims (halves; a dim past rot: itself).
-  template <class T, bool WHOLE>
-  __device__ __forceinline__ void load_partners(const T *head, EltVec<T, 8> &x) const {
-    if constexpr (!INTER) {
-      if constexpr (WHOLE) { // (rot / 2 is a multiple of 8)
-        load8<T, true>(head + (any ? dim < rot / 2 ? dim + rot / 2 : dim - rot / 2 : dim), x);
-      } else {
+
+  struct Loaded {
+    EltVec<T, 8> x[RUNS], partner;
+  };
+  auto load = [&](const T *head, Loaded &x, bool turn) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = dim + i;
-          x.v[i] = head[d >= rot ? d : d < rot / 2 ? d + rot / 2 : d - rot / 2];
+    for (int r = 0; r < RUNS; ++r)
+      load8<T, WHOLE>(head + d[r], x.x[r]);
+    if constexpr (MODE == kRunAlone)
+      if (turn && turned) {
+        if constexpr (WHOLE) { // (half is a multiple of 8)
+          load8<T, true>(head + (d[0] < half ? d[0] + half : d[0] - half), x.partner);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int dim = d[0] + i;
+            x.partner.v[i] = head[dim >= rot ? dim : dim < half ? dim + half : dim - half];
+          }
         }
       }
-    }
-  }
-  template <class T>
-  __device__ __forceinline__ void apply(const EltVec<T, 8> &x, const EltVec<T, 8> &partner, bool turn,
-                                        float (&y)[8]) const {
+  };
+  auto values = [&](const Loaded &x, bool turn, float (&y)[RUNS][8]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      y[i] = elt_to_f32(x.v[i]);
-    if (!any || !turn)
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[r][i] = elt_to_f32(x.x[r].v[i]);
+    if (!turn || !turned)
       return;
-    if constexpr (INTER) {
+    if constexpr (MODE == kRunHalves) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = y[2 * i], b = y[2 * i + 1];
-        if (dim + 2 * i < rot) {
-          y[2 * i] = a * c[i] - b * s[i];
-          y[2 * i + 1] = b * c[i] + a * s[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float a = y[0][i], b = y[RUNS - 1][i];
+        y[0][i] = a * c[i] - b * s[i], y[RUNS - 1][i] = b * c[i] + a * s[i];
+      }
+    } else if constexpr (MODE == kRunPairs) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const float a = y[0][2 * i], b = y[0][2 * i + 1];
+        if (d[0] + 2 * i < rot)
+          y[0][2 * i] = a * c[i] - b * s[i], y[0][2 * i + 1] = b * c[i] + a * s[i];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (dim + i < rot)
-          y[i] = y[i] * c[i] + elt_to_f32(partner.v[i]) * s[i];
+        if (d[0] + i < rot)
+          y[0][i] = y[0][i] * c[i] + elt_to_f32(x.partner.v[i]) * s[i];
     }
+  };
+  // f(head, its values) of heads lane, lane + head_lanes, ..
+  auto each = [&](const T *src, int64_t sh, int heads, bool turn, auto f) __attribute__((always_inline)) {
+    const T *head = src + at.lane * sh;
+    const int64_t step = p.head_lanes * sh;
+    for (int h0 = at.lane; h0 < heads; h0 += BATCH * p.head_lanes) {
+      Loaded x[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k, head += step)
+        if (h0 + k * p.head_lanes < heads)
+          load(head, x[k], turn);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int h = h0 + k * p.head_lanes;
+        if (h >= heads)
+          break;
+        float y[RUNS][8];
+        values(x[k], turn, y);
+        f(h, y);
+      }
+    }
+  };
+  if (p.Hq) {
+    T *const out = static_cast<T *>(p.q_out) + t * p.o_st;
+    each(static_cast<const T *>(p.q) + t * p.q_st, p.q_sh, p.Hq, pl.mine, [&](int h, float (&y)[RUNS][8]) {
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r)
+        store8<T, WHOLE>(out + h * p.o_sh + d[r], y[r]);
+    });
   }
-};
-
-// Heads in the order q, k, v.
-template <class T, bool NV, bool INTER, bool WHOLE>
-__global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
-  const AppendArgs &p = args.a;
-  const RotaryPlace at(p.token_threads, p.items, false);
-  const int64_t t = at.tok;
-  if (t >= p.T)
+  if (pl.page < 0) // a token without a page: its q alone
     return;
-  const TokenPlace pl = token_place(t, p.cu_q, p.kv_len, p.B, p.table, p.table_s, p.table_width, p.pages,
-                                    p.page_shift);
   const int64_t slot = pl.pos & ((1 << p.page_shift) - 1);
-  const Turn8<INTER> turn(at.item, p.rot, (double)pl.pos, p.inv_freq, p.scale);
-  constexpr int LANES = NV ? 2 : 4; // of a block
-  // (a token without a page: its q alone)
-  const int heads = pl.page < 0 ? p.Hq : p.Hq + 2 * p.Hkv;
-  for (int h0 = at.lane; h0 < heads; h0 += kHeadBatch * p.head_lanes) {
-    EltVec<T, 8> x[kHeadBatch], partner[kHeadBatch];
+  auto side = [&](const T *src, int64_t sh, bool turn, const float *head_scale, uint8_t *codes, int64_t ch,
+                  const BlockScales &bs) __attribute__((always_inline)) {
+    uint8_t *const scales = bs.s + pl.page * bs.sp + slot * bs.st;
+    each(src, sh, p.Hkv, turn, [&](int h, float (&y)[RUNS][8]) {
+      const float f = head_scale ? head_scale[h] : 1.f;
 #pragma unroll
-    for (int k = 0; k < kHeadBatch; ++k) {
-      const int hh = h0 + k * p.head_lanes, h = hh < heads ? hh : h0;
-      const bool is_q = h < p.Hq, is_k = h < p.Hq + p.Hkv;
-      const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
-      const T *src = is_q   ? static_cast<const T *>(p.q) + t * p.q_st + h * p.q_sh
-                     : is_k ? static_cast<const T *>(p.k) + t * p.k_st + hk * p.k_sh
-                            : static_cast<const T *>(p.v) + t * p.v_st + hk * p.v_sh;
-      load8<T, WHOLE>(src + turn.dim, x[k]);
-      if (is_k)
-        turn.template load_partners<T, WHOLE>(src, partner[k]);
-    }
+      for (int r = 0; r < RUNS; ++r) {
+        if (head_scale) {
 #pragma unroll
-    for (int k = 0; k < kHeadBatch; ++k) {
-      const int h = h0 + k * p.head_lanes;
-      if (h >= heads)
-        break;
-      float y[8];
-      if (h < p.Hq) {
-        turn.template apply<T>(x[k], partner[k], pl.mine, y);
-        store8<T, WHOLE>(static_cast<T *>(p.q_out) + t * p.o_st + h * p.o_sh + turn.dim, y);
-        continue;
+          for (int i = 0; i < 8; ++i)
+            y[r][i] = y[r][i] / f;
+        }
+        const uint32_t scale = block4_scale<NV>(block4_max<LANES>(y[r]), args.lo, args.hi);
+        *reinterpret_cast<uint32_t *>(codes + h * ch + d[r] / 2) = block4_codes<NV>(y[r], scale);
+        if (d[r] / 8 % LANES == 0)
+          scales[h * bs.sh + d[r] / (8 * LANES) * bs.sb] = scale;
       }
-      const bool is_k = h < p.Hq + p.Hkv;
-      const int hk = h - p.Hq - (is_k ? 0 : p.Hkv);
-      turn.template apply<T>(x[k], partner[k], is_k, y);
-      const float *sc = is_k ? p.k_scale : p.v_scale;
-      if (sc) {
-        const float f = sc[hk];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          y[i] = y[i] / f;
-      }
-      const uint32_t scale = block4_scale<NV>(block4_max<LANES>(y), args.lo, args.hi);
-      uint8_t *dst = is_k ? p.kc + pl.page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh
-                          : p.vc + pl.page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh;
-      *reinterpret_cast<uint32_t *>(dst + 4 * at.item) = block4_codes<NV>(y, scale);
-      if (at.item % LANES == 0) {
-        const int64_t blk = at.item / LANES;
-        if (is_k)
-          args.ks.s[pl.page * args.ks.sp + slot * args.ks.st + hk * args.ks.sh + blk * args.ks.sb] = scale;
-        else
-          args.vs.s[pl.page * args.vs.sp + slot * args.vs.st + hk * args.vs.sh + blk * args.vs.sb] = scale;
-      }
-    }
-  }
+    });
+  };
+  side(static_cast<const T *>(p.k) + t * p.k_st, p.k_sh, true, p.k_scale, p.kc + pl.page * p.kc_sp + slot * p.kc_st,
+       p.kc_sh, args.ks);
+  side(static_cast<const T *>(p.v) + t * p.v_st, p.v_sh, false, p.v_scale,
+       p.vc + pl.page * p.vc_sp + slot * p.vc_st, p.vc_sh, args.vs);
 }
 
 // ---------------------------------------------------------------------------
@@ -256,6 +300,8 @@ template <class C, int VEC> struct ReadItem {
         y[i] = elt_to_f32(e.v[i]);
     }
   }
+  // Writes the values without a head's factor, where that takes no arithmetic.
+  template <class O> __device__ __forceinline__ bool direct(O *) const { return false; }
 };
 template <bool NV> struct ReadItem<E2m1<NV>, 8> {
   uint32_t w, s;
@@ -264,9 +310,20 @@ template <bool NV> struct ReadItem<E2m1<NV>, 8> {
     s = scales[(d / (NV ? 16 : 32)) * bs.sb];
   }
   __device__ __forceinline__ void values(float (&y)[8]) const { codes4_f32<NV>(w, s, y); }
+  // (the conversions round code * scale once; NV: fp16 holds the products, as Code4 takes them)
+  template <class O> __device__ __forceinline__ bool direct(O *to) const {
+    constexpr bool BF = std::is_same<O, __bf16>::value, HF = std::is_same<O, _Float16>::value;
+    if constexpr ((BF && !NV) || HF) {
+      uint32_t f = s << 23;
+      if constexpr (NV)
+        f = Code4<false, true>::factor(s, false);
+      *reinterpret_cast<u32x4 *>(to) = Code4<BF, NV>::eight(w, f);
+      return true;
+    }
+    return false;
+  }
 };
 
-// Heads in the order k, v.
 template <class C, class O, int VEC, bool WHOLE>
 __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs p) {
   const RotaryPlace at(p.token_threads, p.items, false);
@@ -277,49 +334,47 @@ __global__ void __launch_bounds__(256) paged_read_kernel(ReadArgs p) {
                                     p.page_shift);
   const int64_t slot = pl.pos & ((1 << p.page_shift) - 1);
   const int d = at.item * VEC;
-  const int heads = 2 * p.Hkv;
-  for (int h0 = at.lane; h0 < heads; h0 += kHeadBatch * p.head_lanes) {
-    ReadItem<C, VEC> x[kHeadBatch];
-    if (pl.page >= 0) {
+  // heads lane, lane + head_lanes, ..
+  auto side = [&](const uint8_t *codes, int64_t sh, const BlockScales &bs, const float *head_scale, O *out,
+                  int64_t oh) __attribute__((always_inline)) {
+    const uint8_t *src = codes + at.lane * sh, *scales = bs.s + pl.page * bs.sp + slot * bs.st + at.lane * bs.sh;
+    O *to = out + at.lane * oh + d;
+    const int64_t step = p.head_lanes * sh, sstep = p.head_lanes * bs.sh, ostep = p.head_lanes * oh;
+    for (int h0 = at.lane; h0 < p.Hkv; h0 += kHeadBatch * p.head_lanes) {
+      ReadItem<C, VEC> x[kHeadBatch];
 #pragma unroll
-      for (int k = 0; k < kHeadBatch; ++k) {
-        const int hh = h0 + k * p.head_lanes, h = hh < heads ? hh : h0;
-        const bool is_k = h < p.Hkv;
-        const int hk = is_k ? h : h - p.Hkv;
-        const uint8_t *src = is_k ? p.kc + pl.page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh
-                                  : p.vc + pl.page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh;
-        const BlockScales &bs = is_k ? p.ks : p.vs;
-        x[k].load(src, d, bs, bs.s + pl.page * bs.sp + slot * bs.st + hk * bs.sh);
-      }
-    }
+      for (int k = 0; k < kHeadBatch; ++k, src += step, scales += sstep)
+        if (pl.page >= 0 && h0 + k * p.head_lanes < p.Hkv)
+          x[k].load(src, d, bs, scales);
 #pragma unroll
-    for (int k = 0; k < kHeadBatch; ++k) {
-      const int h = h0 + k * p.head_lanes;
-      if (h >= heads)
-        break;
-      const bool is_k = h < p.Hkv;
-      const int hk = is_k ? h : h - p.Hkv;
-      float y[VEC];
+      for (int k = 0; k < kHeadBatch; ++k, to += ostep) {
+        const int h = h0 + k * p.head_lanes;
+        if (h >= p.Hkv)
+          break;
+        if (VEC == 8 && WHOLE && pl.page >= 0 && !head_scale && x[k].template direct<O>(to))
+          continue;
+        float y[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        y[i] = 0.f;
-      if (pl.page >= 0) {
-        x[k].values(y);
-        if (const float *sc = is_k ? p.k_scale : p.v_scale) {
-          const float f = sc[hk];
+        for (int i = 0; i < VEC; ++i)
+          y[i] = 0.f;
+        if (pl.page >= 0) {
+          x[k].values(y);
+          if (head_scale) {
+            const float f = head_scale[h];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            y[i] *= f;
+            for (int i = 0; i < VEC; ++i)
+              y[i] *= f;
+          }
         }
+        if constexpr (VEC == 8)
+          store8<O, WHOLE>(to, y);
+        else
+          *to = (O)y[0];
       }
-      O *out = is_k ? static_cast<O *>(p.k) + t * p.k_st + hk * p.k_sh
-                    : static_cast<O *>(p.v) + t * p.v_st + hk * p.v_sh;
-      if constexpr (VEC == 8)
-        store8<O, WHOLE>(out + d, y);
-      else
-        out[d] = (O)y[0];
     }
-  }
+  };
+  side(p.kc + pl.page * p.kc_sp + slot * p.kc_st, p.kc_sh, p.ks, p.k_scale, static_cast<O *>(p.k) + t * p.k_st, p.k_sh);
+  side(p.vc + pl.page * p.vc_sp + slot * p.vc_st, p.vc_sh, p.vs, p.v_scale, static_cast<O *>(p.v) + t * p.v_st, p.v_sh);
 }
 
 } // namespace txk

@@ -263,6 +263,9 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
   }
 }
 
+// What a unit's beginning and end cost, in steps (paged_sched.h).
+constexpr uint32_t kSplit4Overhead = 3, kRows4Overhead = 6;
+
 // Counters of sets of parts begin here in the workspace's 16384 (those of units, and of other
 // launches, before them: a launch has at most 512 workgroups).
 constexpr uint32_t kSetCounters = 8192;
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
   typedef typename A::Piece Piece;
   typedef typename A::Code Code;
   typedef typename A::elt elt;
-  typedef PagedSched<ROWS, BN, 4, kSplitOverhead> Sched;
+  typedef PagedSched<ROWS, BN, 4, kSplit4Overhead> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4][A::BYTES];
   __shared__ float ms[4][ROWS], ls[4][ROWS];
   __shared__ PagedSchedState st;
@@ -704,7 +707,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
   typedef typename A::Piece Piece;
   typedef typename A::Code Code;
   typedef typename A::elt elt;
-  typedef PagedSched<128, BN, 1, kRowsOverhead> Sched;
+  typedef PagedSched<128, BN, 1, kRows4Overhead> Sched;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * P::TILE];
   __shared__ PagedSchedState st;
   __shared__ uint32_t nans[2][4]; // of each wave's 16 keys of a tile, those without numbers in V

@@ -129,7 +129,7 @@ class PagedAppend4Desc(ctypes.Structure):
 
 class PagedAppend4Plan(ctypes.Structure):
     _fields_ = ([("desc", PagedAppend4Desc), ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
-                + _i32("whole head_lanes grid_x block_threads"))
+                + _i32("whole run head_lanes grid_x block_threads reserved"))
 
 
 class PagedReadDesc(ctypes.Structure):
