@@ -57,10 +57,13 @@ __device__ __forceinline__ TokenPlace token_place(int64_t t, const int32_t *cu_q
   return r;
 }
 
-// 8 elements from p on; WHOLE: in one access.
-template <class T, bool WHOLE>
+// 8 elements from p on; WHOLE: in one access; NT: data that is read once.
+template <class T, bool WHOLE, bool NT>
 __device__ __forceinline__ void load8(const T *p, EltVec<T, 8> &x) {
-  if constexpr (WHOLE) {
+  if constexpr (WHOLE && NT) {
+    typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+    x = __builtin_bit_cast(EltVec<T, 8>, __builtin_nontemporal_load(reinterpret_cast<const w4 *>(p)));
+  } else if constexpr (WHOLE) {
     x = *reinterpret_cast<const EltVec<T, 8> *>(p);
   } else {
 #pragma unroll
@@ -159,11 +162,11 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
   auto load = [&](const T *head, Loaded &x, bool turn) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < RUNS; ++r)
-      load8<T, WHOLE>(head + d[r], x.x[r]);
+      load8<T, WHOLE, MODE != kRunAlone>(head + d[r], x.x[r]);
     if constexpr (MODE == kRunAlone)
       if (turn && turned) {
         if constexpr (WHOLE) { // (half is a multiple of 8)
-          load8<T, true>(head + (d[0] < half ? d[0] + half : d[0] - half), x.partner);
+          load8<T, true, false>(head + (d[0] < half ? d[0] + half : d[0] - half), x.partner);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {

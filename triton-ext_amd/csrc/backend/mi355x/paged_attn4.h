@@ -43,6 +43,9 @@ template <int D, bool NV> struct Piece4 {
   __device__ __forceinline__ static constexpr int dim(int c, int g) {
     return D == 64 ? 16 * g + 8 * c : 128 * (c / 4) + 32 * g + 8 * (c % 4);
   }
+  // Dword c's place in a 16-bit row of 16-byte chunks, from dword 0's: bits that dword 0's chunk (16 g,
+  // or 4 g chunks) has not set, so that a swizzle of the chunks commutes with it.
+  __device__ __forceinline__ static constexpr uint32_t at(int c) { return 2 * dim(c, 0); }
   __device__ __forceinline__ static constexpr int scale_of(int c) {
     return D == 64 ? 0 : NV ? c / 2 : c / 4;
   }
@@ -53,17 +56,22 @@ template <int D, bool NV> struct Piece4 {
   }
 };
 
-// One wave's view of a table row: beside its entries, where their pages begin in the codes and scales of
-// K and of V (page 0 where there is none).
-struct PageRow4 : PageRow {
-  uint64_t at[4];
+// One wave's view of a table row, and where an entry's page begins in the arrays: 0, 1: codes and scales of
+// K, 2, 3: of V (page 0 where there is none).  KEPT: found for all 64 entries at once (a wave that loads
+// all of a block by itself), else when asked for (8 registers less).
+template <bool KEPT> struct PageRow4 : PageRow {
+  uint64_t at[KEPT ? 4 : 1];
 
+  template <int I> __device__ __forceinline__ static uint64_t stride() {
+    const Paged4Args &p = paged4_args();
+    return (uint64_t)(I == 0 ? p.a.k_sp : I == 1 ? p.ks.sp : I == 2 ? p.a.v_sp : p.vs.sp);
+  }
   __device__ __forceinline__ void settle() {
     PageRow::settle();
-    const Paged4Args &p = paged4_args();
-    const uint64_t id = ids < 0 ? 0 : ids;
-    at[0] = id * (uint64_t)p.a.k_sp, at[1] = id * (uint64_t)p.ks.sp;
-    at[2] = id * (uint64_t)p.a.v_sp, at[3] = id * (uint64_t)p.vs.sp;
+    if constexpr (KEPT) {
+      const uint64_t id = ids < 0 ? 0 : ids;
+      at[0] = id * stride<0>(), at[1] = id * stride<1>(), at[2] = id * stride<2>(), at[3] = id * stride<3>();
+    }
   }
   __device__ __forceinline__ void hold(int n) {
     if (((n + 63) >> shift) >= first + 64) {
@@ -71,11 +79,20 @@ struct PageRow4 : PageRow {
       settle();
     }
   }
+  // Of entry `e` of those held, the same for all lanes; or each lane its own.
+  template <int I> __device__ __forceinline__ uint64_t place(int e) const {
+    if constexpr (KEPT)
+      return (uint64_t)lane_value64(at[I], e & 63);
+    const int id = lane_value(ids, e & 63);
+    return (uint64_t)(uint32_t)(id < 0 ? 0 : id) * stride<I>();
+  }
+  template <int I> __device__ __forceinline__ uint64_t places(int e) const {
+    if constexpr (KEPT)
+      return (uint64_t)(uint32_t)__shfl((int)at[I], e & 63) | (uint64_t)(uint32_t)__shfl((int)(at[I] >> 32), e & 63) << 32;
+    const int id = __shfl(ids, e & 63);
+    return (uint64_t)(uint32_t)(id < 0 ? 0 : id) * stride<I>();
+  }
 };
-
-__device__ __forceinline__ uint64_t lane_from(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__shfl((int)v, lane & 63) | (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane & 63) << 32;
-}
 
 // Where lane (m, g) finds its pieces of K (V: of V) of 16 keys: the codes of a head, which are
 // uniform, and the lane's offsets from the first key, of 32 bits.  Pieces past head_dim are those of
@@ -121,16 +138,16 @@ template <int D, bool NV, bool V> struct Side4 {
   }
   // The pieces of N runs of 16 keys from n on, a multiple of 16 N; m is the lane's row again.  NT: data
   // that is read once.
-  template <bool NT, int N>
-  __device__ __forceinline__ void load(const PageRow4 &pr, int n, int m, P (&x)[N]) const {
+  template <bool NT, int N, class Row>
+  __device__ __forceinline__ void load(const Row &pr, int n, int m, P (&x)[N]) const {
     if (pr.shift >= 4) { // a run lies in one page
       const uint8_t *c;
 #pragma unroll
       for (int b = 0; b < N; ++b) {
         if (b == 0 || pr.shift < 5) {
-          const int key = n + 16 * b, e = ((key >> pr.shift) - pr.first) & 63;
+          const int key = n + 16 * b;
           const uint64_t slot = key & ((1 << pr.shift) - 1);
-          c = codes + (uint64_t)lane_value64(pr.at[V ? 2 : 0], e) + slot * st;
+          c = codes + pr.template place<V ? 2 : 0>((key >> pr.shift) - pr.first) + slot * st;
         } else {
           c += 16ull * st;
         }
@@ -139,7 +156,7 @@ template <int D, bool NV, bool V> struct Side4 {
     } else {
 #pragma unroll
       for (int b = 0; b < N; ++b)
-        read<NT>(codes + lane_from(pr.at[V ? 2 : 0], ((n + 16 * b + m) >> pr.shift) - pr.first), x[b]);
+        read<NT>(codes + pr.template places<V ? 2 : 0>(((n + 16 * b + m) >> pr.shift) - pr.first), x[b]);
     }
   }
 };
@@ -148,7 +165,8 @@ template <int D, bool NV, bool V> struct Side4 {
 // [K, V][block][4 keys], which one or two loads of whole lines bring (a byte a lane and key took the
 // same memory 98 us where this takes 88: 4 sequences of up to 131072); the lanes that convert fetch their
 // byte from there.
-template <int D, bool NV, int KEYS> struct Scales4 {
+// ALIKE: the lane has the same piece of K and of V.
+template <int D, bool NV, int KEYS, bool ALIKE> struct Scales4 {
   typedef Piece4<D, NV> P;
   static constexpr int NB = (D == 96 ? 128 : D) / (NV ? 16 : 32), QUADS = KEYS / 4, HALF = NB * QUADS;
   static constexpr int W = (2 * HALF + 63) / 64;
@@ -161,7 +179,7 @@ template <int D, bool NV, int KEYS> struct Scales4 {
   int quad[W];            // that key
   bool v[W];
   bool packed;            // 4 keys of a block are a dword
-  uint32_t kfrom[P::SB], vfrom[P::SB], kshift, vshift;
+  uint32_t kfrom[P::SB], vfrom[ALIKE ? 1 : P::SB], kshift, vshift;
 
   // km, kg, vm, vg: as the lane has its pieces of K and V
   __device__ __forceinline__ Scales4(const Paged4Args &p, int hk, int km, int kg, int vm, int vg) {
@@ -178,19 +196,20 @@ template <int D, bool NV, int KEYS> struct Scales4 {
 #pragma unroll
     for (int j = 0; j < P::SB; ++j) {
       kfrom[j] = 4 * ((P::block_of(j, kg) * QUADS + km / 4) & 63);
-      vfrom[j] = 4 * ((HALF + P::block_of(j, vg) * QUADS + vm / 4) & 63);
+      if constexpr (!ALIKE)
+        vfrom[j] = 4 * ((HALF + P::block_of(j, vg) * QUADS + vm / 4) & 63);
     }
     kshift = 8 * (km & 3), vshift = 8 * (vm & 3);
   }
   // Of the keys from n on, a multiple of KEYS.
-  __device__ __forceinline__ void load(const PageRow4 &pr, int n, Held &x) const {
+  template <class Row> __device__ __forceinline__ void load(const Row &pr, int n, Held &x) const {
     const bool one = (1 << pr.shift) >= KEYS; // page
     const uint8_t *bk = ks, *bv = vs;
     if (one) {
-      const int e = ((n >> pr.shift) - pr.first) & 63;
+      const int e = (n >> pr.shift) - pr.first;
       const uint64_t slot = n & ((1 << pr.shift) - 1);
-      bk += (uint64_t)lane_value64(pr.at[1], e) + slot * kst;
-      bv += (uint64_t)lane_value64(pr.at[3], e) + slot * vst;
+      bk += pr.template place<1>(e) + slot * kst;
+      bv += pr.template place<3>(e) + slot * vst;
     }
 #pragma unroll
     for (int r = 0; r < W; ++r) {
@@ -198,7 +217,7 @@ template <int D, bool NV, int KEYS> struct Scales4 {
       if (packed) {
         if (!one) {
           const int e = ((n + quad[r]) >> pr.shift) - pr.first;
-          const uint64_t a = lane_from(pr.at[1], e), b = lane_from(pr.at[3], e);
+          const uint64_t a = pr.template places<1>(e), b = pr.template places<3>(e);
           p += v[r] ? b : a;
         }
         x.w[r] = *reinterpret_cast<const uint32_t *>(p);
@@ -208,7 +227,7 @@ template <int D, bool NV, int KEYS> struct Scales4 {
         for (int t = 0; t < 4; ++t) {
           const int key = n + quad[r] + t, in = key & ((1 << pr.shift) - 1);
           const int e = (key >> pr.shift) - pr.first;
-          const uint64_t a = lane_from(pr.at[1], e), b = lane_from(pr.at[3], e);
+          const uint64_t a = pr.template places<1>(e), b = pr.template places<3>(e);
           const int base = quad[r] & ((1 << pr.shift) - 1);
           const uint32_t st = v[r] ? vst : kst;
           const uint8_t *q = (v[r] ? vs + b : ks + a) + (off[r] - (uint64_t)base * st) + (uint64_t)in * st;
@@ -223,8 +242,9 @@ template <int D, bool NV, int KEYS> struct Scales4 {
 #pragma unroll
     for (int j = 0; j < P::SB; ++j) {
       const int r = ((V ? HALF : 0) + P::block_of(j, 0) * QUADS) / 64; // (the other g are in it too)
-      const uint32_t w = __builtin_amdgcn_ds_bpermute((V ? vfrom[j] : kfrom[j]) + 16 * b, x.w[r]);
-      s[j] = __builtin_amdgcn_ubfe(w, V ? vshift : kshift, 8);
+      const uint32_t at = !V ? kfrom[j] : ALIKE ? kfrom[j] + 4 * (HALF % 64) : vfrom[j % (ALIKE ? 1 : P::SB)];
+      const uint32_t w = __builtin_amdgcn_ds_bpermute(at + 16 * b, x.w[r]);
+      s[j] = __builtin_amdgcn_ubfe(w, V && !ALIKE ? vshift : kshift, 8);
     }
   }
 };
@@ -269,6 +289,12 @@ constexpr uint32_t kSplit4Overhead = 3, kRows4Overhead = 6;
 // Counters of sets of parts begin here in the workspace's 16384 (those of units, and of other
 // launches, before them: a launch has at most 512 workgroups).
 constexpr uint32_t kSetCounters = 8192;
+
+// x, as something that the compiler does not form other values from outside the loop.
+__device__ __forceinline__ uint32_t here_only(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // Which of 16 keys (four adjacent lanes each) a lane's flag is set of.
 __device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
@@ -485,10 +511,8 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
   typename P16::Bases bs;
   P16::bases(v_lds, v_lds, bs);
   const int km = lane & 15, kg = lane >> 4, vm = lane >> 2, vg = lane & 3;
-  uint32_t vw[Piece::KW]; // where the lane's values of V go in the tile (16 rows on: 16 * ROW)
-#pragma unroll
-  for (int c = 0; c < Piece::KW; ++c)
-    vw[c] = v_lds + vm * P16::ROW + (((Piece::dim(c, vg) / 8) ^ P16::vswz(vm)) << 4);
+  // where the lane's first 8 dims of V go in the tile (16 rows on: 16 * ROW; dword c: at ^ Piece::at(c))
+  const uint32_t vw = v_lds + vm * P16::ROW + (((Piece::dim(0, vg) / 8) ^ P16::vswz(vm)) << 4);
 
   for (int turn = 0;; turn ^= 1) {
     const Paged4Args &p4 = paged4_args();
@@ -506,7 +530,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
       k0 = w0 + wave * q < w1 ? w0 + wave * q : w1;
       k1 = k0 + q < w1 ? k0 + q : w1;
     }
-    PageRow4 pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
+    PageRow4<true> pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
     const Side4<D, A::NV, false> sk(p4, un.hk, km, kg);
     const Side4<D, A::NV, true> sv(p4, un.hk, vm, vg);
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
@@ -527,9 +551,9 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
         qf[i][c] = *reinterpret_cast<const u32x4 *>(row + (d < p.head_dim ? d : 0));
       }
     }
-    const Scales4<D, A::NV, BN> sc(p4, un.hk, km, kg, vm, vg);
+    const Scales4<D, A::NV, BN, false> sc(p4, un.hk, km, kg, vm, vg);
     Piece kp[NS][2], vp[NS][2];
-    typename Scales4<D, A::NV, BN>::Held sp[NS];
+    typename Scales4<D, A::NV, BN, false>::Held sp[NS];
     uint32_t here[NS + 1] = {}; // of blocks k .. k + NS
     if (k0 < k1) {
       pr.settle();
@@ -600,6 +624,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
             s[i][b] = P16::mfma(kf, __builtin_bit_cast(typename P16::h8, qf[i][c]), s[i][b]);
         }
       }
+      const uint32_t vto = here_only(vw);
       uint64_t none[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -614,7 +639,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
 #pragma unroll
         for (int c = 0; c < Piece::KW; ++c) {
           typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-          *(lds_u32x4 *)(uintptr_t)(vw[c] + b * 16 * P16::ROW) = Code::eight(x.w[c], f[Piece::scale_of(c)]);
+          *(lds_u32x4 *)(uintptr_t)((vto ^ Piece::at(c)) + b * 16 * P16::ROW) = Code::eight(x.w[c], f[Piece::scale_of(c)]);
         }
       }
       if (k + NS < k1) {
@@ -697,6 +722,32 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
   typedef PagedFrag<D, CBF, false, BN> P;
   typedef Piece4<D, NV> Piece;
   typedef typename AttnFwd<64, BF, 32, 64>::elt elt; // of q and o
+#ifndef VRX
+#define VRX 4
+#endif
+  // Fragments as P reads them, from one address each of K and V: those of the other chunks and dim blocks
+  // differ in bits that the first has not set.
+  __device__ __forceinline__ static void read_k(uint32_t k, int at, typename P::KF &kf) {
+    typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
+#pragma unroll
+    for (int c = 0; c < P::NK; ++c)
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b)
+        kf.v[b][c] = *(const lds_i32x4 *)(uintptr_t)((k ^ (32 * c)) + at + b * 32 * P::ROW);
+  }
+  template <int N>
+  __device__ __forceinline__ static void read_v(uint32_t v, int at, int b0, typename P::template VF<N> &vf) {
+#pragma unroll
+    for (int bd = 0; bd < N; ++bd)
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        const uint32_t a = (v ^ (64 * (b0 + bd))) + at + c * 16 * P::ROW;
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)a);
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)(a + 8 * P::ROW));
+        vf.v[bd][c] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+  }
+  static constexpr int VR = D == 128 ? VRX : D < 128 ? P::NV : P::VN; // dim blocks of V read ahead of the softmax
 };
 template <class A> constexpr int paged4_rows_groups() { return A::D > 128 ? 1 : 2; }
 
@@ -727,13 +778,8 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
   typename P::Bases bs;
   P::bases(k_lds, v_lds, bs);
   const int em = lane >> 2, eg = lane & 3, er = 16 * wave + em; // the key of a block that the lane converts
-  uint32_t kw[Piece::KW], vw[Piece::KW];
-#pragma unroll
-  for (int c = 0; c < Piece::KW; ++c) {
-    const int chunk = Piece::dim(c, eg) / 8;
-    kw[c] = k_lds + er * P::ROW + ((chunk ^ P::kswz(er)) << 4);
-    vw[c] = v_lds + er * P::ROW + ((chunk ^ P::vswz(er)) << 4);
-  }
+  const uint32_t kw = k_lds + er * P::ROW + (((Piece::dim(0, eg) / 8) ^ P::kswz(er)) << 4);
+  const uint32_t vw = v_lds + er * P::ROW + (((Piece::dim(0, eg) / 8) ^ P::vswz(er)) << 4);
 
   for (int turn = 0;; turn ^= 1) {
     const Paged4Args &p4 = paged4_args();
@@ -747,13 +793,13 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       k0 = first + (int)un.s0;
       k1 = first + (int)un.s1 < last ? first + (int)un.s1 : last;
     }
-    PageRow4 pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
+    PageRow4<false> pr{{p.table + un.b * p.table_s, (uint32_t)p.table_width, p.pages, p.page_shift}, {}};
     const Side4<D, A::NV, false> sk(p4, un.hk, em, eg);
     const Side4<D, A::NV, true> sv(p4, un.hk, em, eg);
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
-    const Scales4<D, A::NV, 16> sc(p4, un.hk, em, eg, em, eg);
+    const Scales4<D, A::NV, 16, true> sc(p4, un.hk, em, eg, em, eg);
     Piece kp[1], vp[1];
-    typename Scales4<D, A::NV, 16>::Held sp;
+    typename Scales4<D, A::NV, 16, true>::Held sp;
     const bool once = un.alone; // keys that no other unit reads go past the caches
     auto fetch = [&](int k) __attribute__((always_inline)) {
       pr.hold(k * BN);
@@ -775,13 +821,14 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
         bad = bad || Code::bad(fv[j]);
         fk[j] = Code::factor(fk[j], false), fv[j] = Code::factor(fv[j], true);
       }
+      const uint32_t kto = here_only(kw), vto = here_only(vw);
       const uint64_t none = __ballot(bad);
       if (lane == 0)
         nans[slot][wave] = none ? keys_of(none) : 0;
 #pragma unroll
       for (int c = 0; c < Piece::KW; ++c) {
-        *(lds_u32x4 *)(uintptr_t)(kw[c] + slot * P::TILE) = Code::eight(kp[0].w[c], fk[Piece::scale_of(c)]);
-        *(lds_u32x4 *)(uintptr_t)(vw[c] + slot * P::TILE) = Code::eight(vp[0].w[c], fv[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)((kto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(kp[0].w[c], fk[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)((vto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(vp[0].w[c], fv[Piece::scale_of(c)]);
       }
     };
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
@@ -841,18 +888,24 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
     auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
       constexpr int SL = decltype(slot_c)::value;
       const int n0 = k * BN;
-      if (k + 1 < k1) {
+      const bool on = live(k);
+      if (k + 1 < k1)
         convert(1 - SL);
-        if (k + 2 < k1)
-          fetch(k + 2);
-      }
-      if (live(k)) {
+      if (on) {
         typename P::KF kf;
-        P::read_k(bs, SL * P::TILE, kf);
+        A::read_k(here_only(bs.k[0]), SL * P::TILE, kf);
+        if constexpr (D <= 128)
+          __builtin_amdgcn_sched_barrier(0);
         P::qk(kf, qf, s);
-        constexpr int VR = D <= 128 ? P::NV : P::VN;
+      }
+      __builtin_amdgcn_sched_barrier(0); // (the codes' registers are K's fragments' before)
+      if (k + 2 < k1)
+        fetch(k + 2);
+      if (on) {
+        constexpr int VR = A::VR;
         typename P::template VF<VR> vf;
-        P::read_v(bs, SL * P::TILE, 0, vf);
+        A::read_v(here_only(bs.v[0]), SL * P::TILE, 0, vf);
+        __builtin_amdgcn_sched_barrier(0);
         uint64_t nan = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
@@ -876,7 +929,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
         P::pv(vf, 0, pf, acc);
 #pragma unroll
         for (int b0 = VR; b0 < P::NV; b0 += VR) {
-          P::read_v(bs, SL * P::TILE, b0, vf);
+          A::read_v(here_only(bs.v[0]), SL * P::TILE, b0, vf);
           P::pv(vf, b0, pf, acc);
         }
       }

@@ -46,10 +46,16 @@ def _calls():
     return _native
 
 
+_cache4 = None
+
+
 def _in_4_bits():
-    """The forms over caches of codes, loaded with the first call."""
-    from . import cache4
-    return cache4
+    """The forms over caches of codes (this module is theirs too, so they are looked up here)."""
+    global _cache4
+    if _cache4 is None:
+        from . import cache4
+        _cache4 = cache4
+    return _cache4
 
 
 def _keep(form, found):
@@ -327,9 +333,9 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
                       k_scale=k_scale, v_scale=v_scale, k_block_scale=k_block_scale,
                       v_block_scale=v_block_scale, q_out=q_out)
     if k_block_scale is not None or v_block_scale is not None:
-        return _in_4_bits().append(k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
-                                   interleaved, scale, k_scale, v_scale, k_block_scale,
-                                   v_block_scale, q_out, stream)
+        return (_cache4 or _in_4_bits()).append(
+            k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq, interleaved, scale,
+            k_scale, v_scale, k_block_scale, v_block_scale, q_out, stream)
     native = _native or _calls()
     form = native.form("append", k, v, k_cache, v_cache, page_table, kv_len, cu_q, q, inv_freq,
                        bool(interleaved), float(scale), k_scale, v_scale, q_out)
@@ -424,9 +430,9 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
                       v_scale=v_scale, k_block_scale=k_block_scale, v_block_scale=v_block_scale,
                       out=out, return_lse=return_lse, workspace=workspace)
     if k_block_scale is not None or v_block_scale is not None:
-        return _in_4_bits().attention(q, k_cache, v_cache, page_table, kv_len, cu_q, sm_scale, causal,
-                                      window, k_scale, v_scale, k_block_scale, v_block_scale, out,
-                                      return_lse, workspace, stream)
+        return (_cache4 or _in_4_bits()).attention(
+            q, k_cache, v_cache, page_table, kv_len, cu_q, sm_scale, causal, window, k_scale, v_scale,
+            k_block_scale, v_block_scale, out, return_lse, workspace, stream)
     import torch
     native = _native or _calls()
     form = native.form("attention", q, k_cache, v_cache, page_table, kv_len, cu_q, float(sm_scale),

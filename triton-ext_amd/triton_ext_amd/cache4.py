@@ -195,12 +195,14 @@ def paged_read(k_cache, v_cache, page_table, kv_len, cu_q=None, *, tokens=None, 
              int(cu_q is not None)) + k_cache.stride()[:3] + v_cache.stride()[:3]
             + (rows if k_out is None else k_out.stride()[:2])
             + (rows if v_out is None else v_out.stride()[:2]) + (page_table.stride(0),)
-            + (_scales_of(k_block_scale, v_block_scale),)), (T, Hkv, D), dtype))
-    (launch, plan, _), shape, dtype = found
+            + (_scales_of(k_block_scale, v_block_scale),)),
+            # what new rows are like: a view of one element, which empty_like makes packed
+            torch.empty((), dtype=dtype, device=device).expand(T, Hkv, D), torch.empty_like))
+    (launch, plan, _), like, make = found
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=device)
+        k_out = make(like)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=device)
+        v_out = make(like)
     rc = native.call(launch, plan, k_cache, v_cache, k_block_scale, v_block_scale, page_table, kv_len,
                      cu_q, k_scale, v_scale, k_out, v_out,
                      _current_stream(device) if stream is None else stream)
