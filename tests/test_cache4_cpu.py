@@ -151,14 +151,17 @@ def _attn4(**kw):
     return tx.load().tx_paged_attn4_plan_create(ctypes.byref(d), ctypes.byref(p)), p
 
 
-@pytest.mark.parametrize("T,B,G,rows", [(4, 4, 4, 16), (4, 4, 16, 16), (4, 4, 17, 32), (8, 1, 4, 32),
-                                        (9, 1, 4, 128), (0, 0, 4, 0), (300, 4, 1, 128)])
-def test_form_by_rows(T, B, G, rows):
-    rc, p = _attn4(T=T, B=B, Hq=2 * G, Hkv=2, ragged=1, q_st=2 * G * 256, o_st=2 * G * 256)
+@pytest.mark.parametrize("T,B,G,D,rows", [(4, 4, 4, 128, 16), (4, 4, 16, 64, 16), (4, 4, 17, 64, 32),
+                                          (8, 1, 4, 64, 32), (9, 1, 4, 64, 128), (9, 1, 4, 96, 32),
+                                          (16, 1, 4, 128, 32), (17, 1, 4, 128, 128), (0, 0, 4, 128, 0),
+                                          (300, 4, 1, 128, 128)])
+def test_form_by_rows(T, B, G, D, rows):
+    rc, p = _attn4(T=T, B=B, Hq=2 * G, Hkv=2, ragged=1, q_st=2 * G * 256, o_st=2 * G * 256, head_dim=D)
+    D = 128 if D == 128 else 96 if D == 96 else 64  # (the dims that a head is computed in)
     assert rc == tx.OK and p.rows == rows
     assert p.grid_x == p.units and p.slots == 2 * p.units and p.units * 4 <= 65536
     # the arrival counters, and a place for each part: sums, maximum and sum of p of every row
-    assert p.workspace_bytes == (65536 + p.slots * rows * 130 * 4 if T else 0)
+    assert p.workspace_bytes == (65536 + p.slots * rows * (D + 2) * 4 if T else 0)
 
 
 @pytest.mark.parametrize("kw,code", [

@@ -398,13 +398,17 @@ extern "C" TX_API int tx_paged_attn4_plan_create(const tx_paged_attn4_desc *desc
   plan->block_threads = 256;
   if (d.T == 0)
     return TX_OK;
-  // (as tx_paged_attn_plan_create)
-  const int64_t G = d.Hq / d.Hkv, rows = d.T * G;
-  plan->variant = rows <= 16 * d.B ? 0 : rows <= 32 * d.B ? 1 : 2;
-  plan->rows = plan->variant == 0 ? 16 : plan->variant == 1 ? 32 : 128;
+  // The fewer rows a sequence has on average, the less of a unit's matrix and softmax work is for
+  // nothing; past a form's rows its units convert the same keys again, which the form of 128 does once
+  // for all of its waves.  16 sequences of 16384 keys, heads of 128: 16 rows each 68 us in the form of 16,
+  // 82 in that of 32; 32 rows 89, and 146 in that of 128; 64 rows 160 and 175.  Heads of 64: 32 rows 67
+  // and 90, 64 rows 118 and 106.  8 sequences, heads of 256: 64 rows 131 and 170.
   const int D = attnDims(d.head_dim);
+  const int64_t G = d.Hq / d.Hkv, rows = d.T * G;
+  plan->variant = rows <= 16 * d.B ? 0 : rows <= (D > 64 ? 64 : 32) * d.B ? 1 : 2;
+  plan->rows = plan->variant == 0 ? 16 : plan->variant == 1 ? 32 : 128;
   // workgroups that a CU has place for (by LDS and registers)
-  const int per_cu = D > 128 && plan->variant > 0 ? 1 : 2;
+  const int per_cu = plan->variant == 0 ? 2 : D > 128 ? 1 : plan->variant == 2 && D == 64 ? 3 : 2;
   // the most steps of work there can be (a step: the keys a workgroup takes at a time)
   const bool split = plan->variant != 2;
   const int step = split ? 128 : 64;

@@ -32,6 +32,12 @@ __device__ __forceinline__ const Paged4Args &paged4_args() {
   return reinterpret_cast<const Paged4Args &>(paged_args());
 }
 
+// x, as something that the compiler does not form other values from outside the loop.
+__device__ __forceinline__ uint32_t here_only(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // What a lane holds of one key's K or V row, in the order of its quarter g: KW dwords of 8 dims, under SB
 // block scales.
 template <int D, bool NV> struct Piece4 {
@@ -213,25 +219,30 @@ template <int D, bool NV, int KEYS, bool ALIKE> struct Scales4 {
     }
 #pragma unroll
     for (int r = 0; r < W; ++r) {
-      const uint8_t *p = (v[r] ? bv : bk) + off[r];
-      if (packed) {
+      auto step = [&]() { return here_only(v[r] ? vst : kst); };
+      if (__builtin_expect(pr.shift >= 2, 1)) { // 4 keys of one page
+        const uint8_t *p = (v[r] ? bv : bk) + off[r];
         if (!one) {
           const int e = ((n + quad[r]) >> pr.shift) - pr.first;
           const uint64_t a = pr.template places<1>(e), b = pr.template places<3>(e);
           p += v[r] ? b : a;
         }
-        x.w[r] = *reinterpret_cast<const uint32_t *>(p);
+        if (__builtin_expect(packed, 1)) {
+          x.w[r] = *reinterpret_cast<const uint32_t *>(p);
+        } else {
+          const uint32_t st = step();
+          x.w[r] = (uint32_t)p[0] | (uint32_t)p[st] << 8 | (uint32_t)p[2ull * st] << 16 | (uint32_t)p[3ull * st] << 24;
+        }
       } else {
+        const int mask = (1 << pr.shift) - 1;
+        const uint32_t st = step();
         uint32_t w = 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int key = n + quad[r] + t, in = key & ((1 << pr.shift) - 1);
-          const int e = (key >> pr.shift) - pr.first;
+          const int key = n + quad[r] + t, e = (key >> pr.shift) - pr.first;
           const uint64_t a = pr.template places<1>(e), b = pr.template places<3>(e);
-          const int base = quad[r] & ((1 << pr.shift) - 1);
-          const uint32_t st = v[r] ? vst : kst;
-          const uint8_t *q = (v[r] ? vs + b : ks + a) + (off[r] - (uint64_t)base * st) + (uint64_t)in * st;
-          w |= (uint32_t)*q << (8 * t);
+          // (off's part of the quad's first key, whose slot is 0 in pages of 1 and 2)
+          w |= (uint32_t)((v[r] ? vs + b : ks + a) + off[r])[(uint64_t)(key & mask) * st] << (8 * t);
         }
         x.w[r] = w;
       }
@@ -290,12 +301,6 @@ constexpr uint32_t kSplit4Overhead = 3, kRows4Overhead = 6;
 // launches, before them: a launch has at most 512 workgroups).
 constexpr uint32_t kSetCounters = 8192;
 
-// x, as something that the compiler does not form other values from outside the loop.
-__device__ __forceinline__ uint32_t here_only(uint32_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // Which of 16 keys (four adjacent lanes each) a lane's flag is set of.
 __device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
   uint64_t x = lanes | lanes >> 1;
@@ -325,6 +330,20 @@ template <int D_, bool BF, bool NV_, int RT_> struct Paged4Split {
   static constexpr int TILE = P16::TILE, BYTES = TILE > ROWS * D * 4 ? TILE : ROWS * D * 4;
   __device__ __forceinline__ static int quad_at(int row, int qd) {
     return (row >> 4) * P16::QUADS * 64 + P16::quad_at(row & 15, qd);
+  }
+  // V fragments of dim blocks b0 .. b0 + VN - 1 as P16 reads them, from the first one's address: the others
+  // differ in bits that it has not set.
+  static constexpr int VN = D == 256 ? 4 : P16::VN;
+  __device__ __forceinline__ static void read_v(const typename P16::Bases &bs, int b0, i32x4_t (&vf)[VN]) {
+    const uint32_t v = here_only(bs.v[0]);
+#pragma unroll
+    for (int bd = 0; bd < VN; ++bd) {
+      // (heads of 256: 15 registers less; of 128 it costs 4%)
+      const uint32_t a = D == 256 ? v ^ (32 * (b0 + bd)) : bs.v[b0 + bd];
+      const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)a);
+      const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)(a + 16 * P16::ROW));
+      vf[bd] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
   }
 };
 
@@ -670,12 +689,14 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
         P16::softmax(s[i], scale[i], acc[i], m[i], l[i], pf[i]);
       }
 #pragma unroll
-      for (int b0 = 0; b0 < P16::NV; b0 += P16::VN) {
-        typename P16::template VF<P16::VN> vf;
-        P16::read_v(bs, 0, b0, vf);
+      for (int b0 = 0; b0 < P16::NV; b0 += A::VN) {
+        i32x4_t vf[A::VN];
+        A::read_v(bs, b0, vf);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
-          P16::pv(vf, b0, pf[i], acc[i]);
+#pragma unroll
+          for (int bd = 0; bd < A::VN; ++bd)
+            acc[i][b0 + bd] = P16::mfma(__builtin_bit_cast(typename P16::h8, vf[bd]), pf[i][0], acc[i][b0 + bd]);
       }
 #pragma unroll
       for (int i = 0; i < NS; ++i)
@@ -749,7 +770,7 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
   }
   static constexpr int VR = D == 128 ? VRX : D < 128 ? P::NV : P::VN; // dim blocks of V read ahead of the softmax
 };
-template <class A> constexpr int paged4_rows_groups() { return A::D > 128 ? 1 : 2; }
+template <class A> constexpr int paged4_rows_groups() { return A::D > 128 ? 1 : A::D > 64 ? 2 : 3; }
 
 template <class A>
 __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows_kernel(Paged4Args args4) {
@@ -798,23 +819,25 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
     const Side4<D, A::NV, true> sv(p4, un.hk, em, eg);
     uint64_t here[3] = {}; // of blocks k, k + 1, k + 2
     const Scales4<D, A::NV, 16, true> sc(p4, un.hk, em, eg, em, eg);
-    Piece kp[1], vp[1];
-    typename Scales4<D, A::NV, 16, true>::Held sp;
+    struct Codes { // of 16 keys
+      Piece k[1], v[1];
+      typename Scales4<D, A::NV, 16, true>::Held s;
+    } next;
     const bool once = un.alone; // keys that no other unit reads go past the caches
-    auto fetch = [&](int k) __attribute__((always_inline)) {
+    auto fetch = [&](int k, Codes &x) __attribute__((always_inline)) {
       pr.hold(k * BN);
       here[2] = pr.template there<BN>(k * BN, un.hi);
       const int n = k * BN + 16 * wave;
-      sc.load(pr, n, sp);
+      sc.load(pr, n, x.s);
       if (once)
-        sk.template load<true>(pr, n, em, kp), sv.template load<true>(pr, n, em, vp);
+        sk.template load<true>(pr, n, em, x.k), sv.template load<true>(pr, n, em, x.v);
       else
-        sk.template load<false>(pr, n, em, kp), sv.template load<false>(pr, n, em, vp);
+        sk.template load<false>(pr, n, em, x.k), sv.template load<false>(pr, n, em, x.v);
     };
-    auto convert = [&](int slot) __attribute__((always_inline)) {
+    auto convert = [&](int slot, const Codes &x) __attribute__((always_inline)) {
       typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
       uint32_t fk[Piece::SB], fv[Piece::SB];
-      sc.template of<false>(sp, 0, fk), sc.template of<true>(sp, 0, fv);
+      sc.template of<false>(x.s, 0, fk), sc.template of<true>(x.s, 0, fv);
       bool bad = false;
 #pragma unroll
       for (int j = 0; j < Piece::SB; ++j) {
@@ -827,8 +850,8 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
         nans[slot][wave] = none ? keys_of(none) : 0;
 #pragma unroll
       for (int c = 0; c < Piece::KW; ++c) {
-        *(lds_u32x4 *)(uintptr_t)((kto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(kp[0].w[c], fk[Piece::scale_of(c)]);
-        *(lds_u32x4 *)(uintptr_t)((vto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(vp[0].w[c], fv[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)((kto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(x.k[0].w[c], fk[Piece::scale_of(c)]);
+        *(lds_u32x4 *)(uintptr_t)((vto ^ Piece::at(c)) + slot * P::TILE) = Code::eight(x.v[0].w[c], fv[Piece::scale_of(c)]);
       }
     };
     // The table, Q and the first blocks are under way together, and meanwhile the first wave
@@ -845,10 +868,22 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       const int d = P::q_dim(c);
       qx[c] = *reinterpret_cast<const u32x4 *>(qrow + (d < p.head_dim ? d : 0));
     }
+    // (two blocks' codes at once where there are registers for them)
+    constexpr bool BOTH = D <= 64;
+    Codes other;
+    Codes &begin = BOTH ? other : next;
+    auto second = [&]() __attribute__((always_inline)) {
+      if (k0 + 1 < k1) {
+        fetch(k0 + 1, next);
+        here[1] = here[2];
+      }
+    };
     if (k0 < k1) {
       pr.settle();
-      fetch(k0);
+      fetch(k0, begin);
       here[0] = here[2];
+      if constexpr (BOTH)
+        second();
     }
     if (wave == 0)
       Sched(p, st).get(st.unit[turn ^ 1]);
@@ -878,11 +913,9 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
     typename P::Acc acc = {};
     typename P::Scores s;
     if (k0 < k1) {
-      convert(0);
-      if (k0 + 1 < k1) {
-        fetch(k0 + 1);
-        here[1] = here[2];
-      }
+      convert(0, begin);
+      if constexpr (!BOTH)
+        second();
     }
     __syncthreads();
     auto iter = [&](int k, auto slot_c) __attribute__((always_inline)) {
@@ -890,7 +923,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       const int n0 = k * BN;
       const bool on = live(k);
       if (k + 1 < k1)
-        convert(1 - SL);
+        convert(1 - SL, next);
       if (on) {
         typename P::KF kf;
         A::read_k(here_only(bs.k[0]), SL * P::TILE, kf);
@@ -900,7 +933,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       }
       __builtin_amdgcn_sched_barrier(0); // (the codes' registers are K's fragments' before)
       if (k + 2 < k1)
-        fetch(k + 2);
+        fetch(k + 2, next);
       if (on) {
         constexpr int VR = A::VR;
         typename P::template VF<VR> vf;
