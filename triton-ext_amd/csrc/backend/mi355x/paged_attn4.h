@@ -331,15 +331,29 @@ template <int D_, bool BF, bool NV_, int RT_> struct Paged4Split {
   __device__ __forceinline__ static int quad_at(int row, int qd) {
     return (row >> 4) * P16::QUADS * 64 + P16::quad_at(row & 15, qd);
   }
-  // V fragments of dim blocks b0 .. b0 + VN - 1 as P16 reads them, from the first one's address: the others
-  // differ in bits that it has not set.
+  // V's tile: 16-byte chunk c of row r lies at c ^ swz(r).  A transposed read takes 32 bytes of each of 8
+  // rows: P16's swizzle puts these pairs of chunks on different banks, and bit 0 (which chunk of a pair is
+  // first) those that the lanes of 4 keys write together.
+  static constexpr int ROW = P16::ROW;
+  __device__ __forceinline__ static int swz(int r) { return P16::vswz(r) ^ ((r >> 1) & 1); }
+  // V fragments of dim blocks b0 .. b0 + VN - 1 as P16 reads them: the address of the first, from which the
+  // others' differ in bits that it has not set.
   static constexpr int VN = D == 256 ? 4 : P16::VN;
-  __device__ __forceinline__ static void read_v(const typename P16::Bases &bs, int b0, i32x4_t (&vf)[VN]) {
+  struct Bases {
+    uint32_t v[D == 256 ? 1 : P16::NV]; // (heads of 256: 15 registers less; of 128 forming them costs 4%)
+  };
+  __device__ __forceinline__ static void bases(uint32_t v_lds, Bases &bs) {
+    const int lane = threadIdx.x & 63, r = lane & 15, key = 4 * (lane >> 4) + (r >> 2), d = 4 * (r & 3);
+    const uint32_t v = v_lds + key * ROW + (((d >> 3) ^ swz(key)) << 4) + (d & 7) * 2;
+#pragma unroll
+    for (int bd = 0; bd < (D == 256 ? 1 : P16::NV); ++bd)
+      bs.v[bd] = v ^ (32 * bd);
+  }
+  __device__ __forceinline__ static void read_v(const Bases &bs, int b0, i32x4_t (&vf)[VN]) {
     const uint32_t v = here_only(bs.v[0]);
 #pragma unroll
     for (int bd = 0; bd < VN; ++bd) {
-      // (heads of 256: 15 registers less; of 128 it costs 4%)
-      const uint32_t a = D == 256 ? v ^ (32 * (b0 + bd)) : bs.v[b0 + bd];
+      const uint32_t a = D == 256 ? v ^ (32 * (b0 + bd)) : bs.v[D == 256 ? 0 : b0 + bd];
       const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)a);
       const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)(a + 16 * P16::ROW));
       vf[bd] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -527,11 +541,11 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
   __syncthreads();
 
   const uint32_t v_lds = lds_addr(smem[wave]);
-  typename P16::Bases bs;
-  P16::bases(v_lds, v_lds, bs);
+  typename A::Bases bs;
+  A::bases(v_lds, bs);
   const int km = lane & 15, kg = lane >> 4, vm = lane >> 2, vg = lane & 3;
   // where the lane's first 8 dims of V go in the tile (16 rows on: 16 * ROW; dword c: at ^ Piece::at(c))
-  const uint32_t vw = v_lds + vm * P16::ROW + (((Piece::dim(0, vg) / 8) ^ P16::vswz(vm)) << 4);
+  const uint32_t vw = v_lds + vm * P16::ROW + (((Piece::dim(0, vg) / 8) ^ A::swz(vm)) << 4);
 
   for (int turn = 0;; turn ^= 1) {
     const Paged4Args &p4 = paged4_args();
@@ -746,8 +760,17 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
 #ifndef VRX
 #define VRX 4
 #endif
+  // V's tile: P's swizzle puts the 64 bytes of 4 rows that a transposed read takes on different banks, and
+  // the same bits again those within 64 that the lanes of 4 keys write together (without: a quarter of
+  // the LDS's time).
+  __device__ __forceinline__ static int swz(int r) { return 5 * (P::vswz(r) / 4); }
   // Fragments as P reads them, from one address each of K and V: those of the other chunks and dim blocks
   // differ in bits that the first has not set.
+  __device__ __forceinline__ static uint32_t v_base(uint32_t v_lds) {
+    const int lane = threadIdx.x & 63, L = lane & 15, key = 4 * (lane >> 5) + (L >> 2);
+    const int d = 16 * ((lane >> 4) & 1) + 4 * (L & 3);
+    return v_lds + key * P::ROW + (((d >> 3) ^ swz(key)) << 4) + (d & 7) * 2;
+  }
   __device__ __forceinline__ static void read_k(uint32_t k, int at, typename P::KF &kf) {
     typedef __attribute__((address_space(3))) i32x4_t lds_i32x4;
 #pragma unroll
@@ -798,9 +821,10 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
   const uint32_t k_lds = lds_addr(smem), v_lds = k_lds + 2 * P::TILE;
   typename P::Bases bs;
   P::bases(k_lds, v_lds, bs);
+  bs.v[0] = A::v_base(v_lds);
   const int em = lane >> 2, eg = lane & 3, er = 16 * wave + em; // the key of a block that the lane converts
   const uint32_t kw = k_lds + er * P::ROW + (((Piece::dim(0, eg) / 8) ^ P::kswz(er)) << 4);
-  const uint32_t vw = v_lds + er * P::ROW + (((Piece::dim(0, eg) / 8) ^ P::vswz(er)) << 4);
+  const uint32_t vw = v_lds + er * P::ROW + (((Piece::dim(0, eg) / 8) ^ A::swz(er)) << 4);
 
   for (int turn = 0;; turn ^= 1) {
     const Paged4Args &p4 = paged4_args();
