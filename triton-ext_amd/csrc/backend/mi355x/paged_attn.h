@@ -319,100 +319,6 @@ __global__ void __launch_bounds__(256, paged_split_groups<A>()) paged_attn_split
 // Many rows: the waves of a workgroup share the keys
 // ---------------------------------------------------------------------------
 
-// A unit's end: its rows (32 a wave) are written out as T, or left as one part of several, which the
-// last workgroup to arrive joins.
-template <class A, class T>
-__device__ __forceinline__ void paged_rows_end(const PagedUnit &unit, typename A::Acc &acc, float m,
-                                               float l, int *flag) {
-  constexpr int D = A::D;
-  typedef T T4 __attribute__((ext_vector_type(4)));
-  const int lane = threadIdx.x & 63, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  l = A::X::xsum(l);
-  const PagedAttnArgs &pe = paged_args();
-  const PagedUnit ue = paged_unit(unit);
-  __syncthreads(); // (the first wave will write the unit after the next there)
-  const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
-  const int r_e = 32 * wave + (lane & 31), rr_e = ue.r0 + (r_e < ue.rows ? r_e : 0);
-  const bool busy_e = ue.rows > 32 * wave;
-  const int of_e = paged_token(pe, rr_e), head_e = ue.hk * pe.G + rr_e - of_e * pe.G;
-  const int64_t tok_e = ue.t0 + of_e;
-  const int64_t part_bytes = 128 * (D + 2) * 4;
-  constexpr int kSC1 = 16;
-  if (ue.parts > 1) {
-    // (lane order: quads of a wave side by side)
-    const uint64_t slot = 2ull * (ue.w0 + ue.part) + (ue.part == 0 ? ue.slot0 : 0);
-    const auto mine = __builtin_amdgcn_make_buffer_rsrc(pe.parts + slot * part_bytes, 0,
-                                                        (int)part_bytes, 0x00020000);
-    if (busy_e) {
-#pragma unroll
-      for (int q = 0; q < D / 8; ++q)
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(i32x4_t, f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
-                                               acc[q / 4][4 * (q % 4) + 2],
-                                               acc[q / 4][4 * (q % 4) + 3]}),
-            mine, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1);
-      if (g == 0) {
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(m), mine, (128 * D + r_e) * 4, 0, kSC1);
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(l), mine, (128 * D + 128 + r_e) * 4, 0,
-                                              kSC1);
-      }
-    }
-    if (!paged_arrive(&pe.counters[ue.w0], ue.parts, flag))
-      return;
-    if (busy_e) {
-      m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int bd = 0; bd < D / 32; ++bd)
-        acc[bd] = typename A::f16v{};
-      for (uint32_t j = 0; j < ue.parts; ++j) {
-        const uint64_t from = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
-        const auto part = __builtin_amdgcn_make_buffer_rsrc(pe.parts + from * part_bytes, 0,
-                                                            (int)part_bytes, 0x00020000);
-        i32x4_t x[D / 8];
-#pragma unroll
-        for (int q = 0; q < D / 8; ++q)
-          x[q] = __builtin_bit_cast(
-              i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                           part, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1));
-        const float m1 = __int_as_float(
-            __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + r_e) * 4, 0, kSC1));
-        const float l1 = __int_as_float(
-            __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + 128 + r_e) * 4, 0, kSC1));
-        if (l1 == 0.f)
-          continue;
-        const float to = fmaxf(m, m1);
-        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
-        const float a1 = __builtin_amdgcn_exp2f(m1 - to);
-        l = l * a + l1 * a1;
-        m = to;
-#pragma unroll
-        for (int q = 0; q < D / 8; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[q / 4][4 * (q % 4) + e] =
-                acc[q / 4][4 * (q % 4) + e] * a + __int_as_float(x[q][e]) * a1;
-      }
-    }
-  }
-  if (r_e < ue.rows) {
-    const float f = l == 0.f ? 0.f : vs / l;
-    T *const orow = static_cast<T *>(pe.o) + tok_e * pe.o_st + head_e * pe.o_sh;
-#pragma unroll
-    for (int q = 0; q < D / 8; ++q) {
-      const int d = 32 * (q / 4) + 8 * (q % 4) + 4 * g;
-      T4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        y[e] = (T)(acc[q / 4][4 * (q % 4) + e] * f);
-      if (d < pe.head_dim)
-        *reinterpret_cast<T4 *>(orow + d) = y;
-    }
-    if (g == 0 && pe.lse)
-      pe.lse[tok_e * pe.Hq + head_e] = l == 0.f ? -INFINITY : m + __builtin_log2f(l);
-  }
-}
-
 // 128 rows a unit, 32 a wave (chunks of a prompt).  K and V have two LDS slots each.  A block has
 // two barriers: after the first K_k is whole (and V_{k-1}'s slot free, for V_{k+1}), after the second
 // V_k is (and K_k's slot free, for K_{k+2}), so that loads have about two blocks' time to land.  All
@@ -585,7 +491,89 @@ __global__ void __launch_bounds__(256, paged_rows_groups<A>()) paged_attn_rows_k
         iter(k++, std::integral_constant<int, 1>());
     }
 
-    paged_rows_end<A, elt>(st.unit[turn], acc, m, l, &flag);
+    l = A::X::xsum(l);
+    const PagedAttnArgs &pe = paged_args();
+    const PagedUnit ue = paged_unit(st.unit[turn]);
+    __syncthreads(); // (the first wave will write the unit after the next there)
+    const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
+    const int r_e = 32 * wave + (lane & 31), rr_e = ue.r0 + (r_e < ue.rows ? r_e : 0);
+    const bool busy_e = ue.rows > 32 * wave;
+    const int of_e = paged_token(pe, rr_e), head_e = ue.hk * pe.G + rr_e - of_e * pe.G;
+    const int64_t tok_e = ue.t0 + of_e;
+    const int64_t part_bytes = 128 * (D + 2) * 4;
+    constexpr int kSC1 = 16;
+    if (ue.parts > 1) {
+      // (lane order: quads of a wave side by side)
+      const uint64_t slot = 2ull * (ue.w0 + ue.part) + (ue.part == 0 ? ue.slot0 : 0);
+      const auto mine = __builtin_amdgcn_make_buffer_rsrc(pe.parts + slot * part_bytes, 0,
+                                                          (int)part_bytes, 0x00020000);
+      if (busy_e) {
+#pragma unroll
+        for (int q = 0; q < D / 8; ++q)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(i32x4_t, f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
+                                                 acc[q / 4][4 * (q % 4) + 2],
+                                                 acc[q / 4][4 * (q % 4) + 3]}),
+              mine, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1);
+        if (g == 0) {
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(m), mine, (128 * D + r_e) * 4, 0, kSC1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(l), mine, (128 * D + 128 + r_e) * 4, 0,
+                                                kSC1);
+        }
+      }
+      if (!paged_arrive(&pe.counters[ue.w0], ue.parts, &flag))
+        continue;
+      if (busy_e) {
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int bd = 0; bd < D / 32; ++bd)
+          acc[bd] = typename A::f16v{};
+        for (uint32_t j = 0; j < ue.parts; ++j) {
+          const uint64_t from = 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0);
+          const auto part = __builtin_amdgcn_make_buffer_rsrc(pe.parts + from * part_bytes, 0,
+                                                              (int)part_bytes, 0x00020000);
+          i32x4_t x[D / 8];
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+            x[q] = __builtin_bit_cast(
+                i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                             part, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1));
+          const float m1 = __int_as_float(
+              __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + r_e) * 4, 0, kSC1));
+          const float l1 = __int_as_float(
+              __builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + 128 + r_e) * 4, 0, kSC1));
+          if (l1 == 0.f)
+            continue;
+          const float to = fmaxf(m, m1);
+          const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+          const float a1 = __builtin_amdgcn_exp2f(m1 - to);
+          l = l * a + l1 * a1;
+          m = to;
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[q / 4][4 * (q % 4) + e] =
+                  acc[q / 4][4 * (q % 4) + e] * a + __int_as_float(x[q][e]) * a1;
+        }
+      }
+    }
+    if (r_e < ue.rows) {
+      const float f = l == 0.f ? 0.f : vs / l;
+      elt *const orow = static_cast<elt *>(pe.o) + tok_e * pe.o_st + head_e * pe.o_sh;
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const int d = 32 * (q / 4) + 8 * (q % 4) + 4 * g;
+        typename A::h4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = (elt)(acc[q / 4][4 * (q % 4) + e] * f);
+        if (d < pe.head_dim)
+          *reinterpret_cast<typename A::h4 *>(orow + d) = y;
+      }
+      if (g == 0 && pe.lse)
+        pe.lse[tok_e * pe.Hq + head_e] = l == 0.f ? -INFINITY : m + __builtin_log2f(l);
+    }
   }
   paged_zero_rows<elt>(args);
 }

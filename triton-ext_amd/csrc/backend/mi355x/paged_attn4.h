@@ -793,6 +793,114 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
   }
   static constexpr int VR = D == 128 ? VRX : D < 128 ? P::NV : P::VN; // dim blocks of V read ahead of the softmax
 };
+// A unit's end: its rows (32 a wave) are written out as T, or left as one part of several, which the
+// last workgroup to arrive joins, in order; of more than kRowsSet parts in sets, as
+// paged4_split_end.  460 rows of one sequence over 14470 keys (heads of 128): 97 us part by part.
+constexpr uint32_t kRowsSet = 8;
+template <class P, class T>
+__device__ __forceinline__ void paged4_rows_end(const PagedUnit &unit, typename P::Acc &acc, float m, float l,
+                                                int *flag) {
+  constexpr int D = P::D, kSC1 = 16;
+  constexpr int64_t part_bytes = 128 * (D + 2) * 4;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  l = P::X::xsum(l);
+  const PagedAttnArgs &pe = paged_args();
+  const PagedUnit ue = paged_unit(unit);
+  __syncthreads(); // (the first wave will write the unit after the next there)
+  const float vs = pe.v_scale ? pe.v_scale[ue.hk] : 1.f;
+  const int r = 32 * wave + (lane & 31), rr = ue.r0 + (r < ue.rows ? r : 0);
+  const bool busy = ue.rows > 32 * wave;
+  if (ue.parts > 1) {
+    auto place = [&](uint64_t slot) {
+      return __builtin_amdgcn_make_buffer_rsrc(pe.parts + slot * part_bytes, 0, (int)part_bytes, 0x00020000);
+    };
+    auto part_at = [&](uint32_t j) -> uint64_t { return 2ull * (ue.w0 + j) + (j == 0 ? ue.slot0 : 0); };
+    // (lane order: quads of a wave side by side)
+    auto store = [&](uint64_t slot) __attribute__((always_inline)) {
+      if (!busy)
+        return;
+      const auto to = place(slot);
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(i32x4_t, f32x4v{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1],
+                                               acc[q / 4][4 * (q % 4) + 2], acc[q / 4][4 * (q % 4) + 3]}),
+            to, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1);
+      if (g == 0) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(m), to, (128 * D + r) * 4, 0, kSC1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(l), to, (128 * D + 128 + r) * 4, 0, kSC1);
+      }
+    };
+    constexpr uint32_t R = kRowsSet;
+    // (places and counters of sets: as in paged4_split_end)
+    const uint32_t s = ue.part / R, sets = (ue.parts + R - 1) / R;
+    auto set_at = [&](uint32_t k) -> uint64_t {
+      return k * R + 1 == ue.parts ? part_at(k * R) : 2ull * (ue.w0 + (k ? k * R : 1)) + 1;
+    };
+    bool last = ue.parts <= R; // what is joined next is all of the unit, not a set
+    uint32_t n = last ? ue.parts : ue.parts - s * R < R ? ue.parts - s * R : R;
+    uint64_t to = part_at(ue.part);
+    if (n == 1) // a set of one part: that is what it leaves
+      last = true, n = sets;
+    for (;; last = true, n = sets, to = set_at(s)) {
+      store(to);
+      if (!paged_arrive(&pe.counters[last ? ue.w0 : kSetCounters + ue.w0 + s * R], n, flag))
+        return;
+      if (busy) {
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int bd = 0; bd < D / 32; ++bd)
+          acc[bd] = typename P::f16v{};
+#pragma nounroll
+        for (uint32_t j = 0; j < n; ++j) {
+          const auto part = place(!last ? part_at(s * R + j) : ue.parts <= R ? part_at(j) : set_at(j));
+          i32x4_t x[D / 8];
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+            x[q] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   part, ((wave * (D / 8) + q) * 64 + lane) * 16, 0, kSC1));
+          const float m1 = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + r) * 4, 0, kSC1));
+          const float l1 = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(part, (128 * D + 128 + r) * 4, 0, kSC1));
+          if (l1 == 0.f) // nothing (a NaN among the scores makes it NaN)
+            continue;
+          const float up = fmaxf(m, m1);
+          const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - up);
+          const float a1 = __builtin_amdgcn_exp2f(m1 - up);
+          l = l * a + l1 * a1;
+          m = up;
+#pragma unroll
+          for (int q = 0; q < D / 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[q / 4][4 * (q % 4) + e] = acc[q / 4][4 * (q % 4) + e] * a + __int_as_float(x[q][e]) * a1;
+        }
+      }
+      if (last)
+        break;
+    }
+  }
+  if (r < ue.rows) {
+    const int of = paged_token(pe, rr), head = ue.hk * pe.G + rr - of * pe.G;
+    const int64_t tok = ue.t0 + of;
+    const float f = l == 0.f ? 0.f : vs / l;
+    T *const orow = static_cast<T *>(pe.o) + tok * pe.o_st + head * pe.o_sh;
+#pragma unroll
+    for (int q = 0; q < D / 8; ++q) {
+      const int d = 32 * (q / 4) + 8 * (q % 4) + 4 * g;
+      T4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = (T)(acc[q / 4][4 * (q % 4) + e] * f);
+      if (d < pe.head_dim)
+        *reinterpret_cast<T4 *>(orow + d) = y;
+    }
+    if (g == 0 && pe.lse)
+      pe.lse[tok * pe.Hq + head] = l == 0.f ? -INFINITY : m + __builtin_log2f(l);
+  }
+}
+
 template <class A> constexpr int paged4_rows_groups() { return A::D > 128 ? 1 : A::D > 64 ? 2 : 3; }
 
 template <class A>
@@ -998,7 +1106,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
       if (k < k1)
         iter(k++, std::integral_constant<int, 1>());
     }
-    paged_rows_end<P, elt>(st.unit[turn], acc, m, l, &flag);
+    paged4_rows_end<P, elt>(st.unit[turn], acc, m, l, &flag);
   }
   paged_zero_rows<elt>(args4.a);
 }
