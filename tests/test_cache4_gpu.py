@@ -1,6 +1,8 @@
 """The paged cache held in 4 bits against 64-bit oracles on the CPU: what append writes, what read
 gives back, the attention over it, at the sizes and contents where they can go wrong."""
 import math
+import os
+import sys
 
 import pytest
 
@@ -539,6 +541,31 @@ def test_step_in_a_graph(gpu, kind):
     want = torch.einsum("bhgl,blhd->bhgd", s.softmax(-1), vd).reshape(6, Hq, D)
     mag = torch.einsum("bhgl,blhd->bhgd", s.softmax(-1), vd.abs()).reshape(6, Hq, D)
     check(o, want, (2.0 ** -8 + 2.0 ** -12) * mag + 2.0 ** -8 * want.abs(), "o")
+
+
+@pytest.mark.parametrize("kind", ["mx", "nv"])
+def test_generation_example(gpu, kind):
+    """The example with a cache in 4 bits: it runs, its beams share pages, and what the cache holds of
+    every sequence is the same after pages were freed and moved."""
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(tx.__file__)), "..", "examples"))
+    import paged_generation as ex
+    d, fed, got = ex.generate(sequences=3, tokens=6, beams=2, cache_dtype=kind)
+    assert int(d.missing) == 0 and d.length.tolist() == [f.shape[0] for f in fed]
+    assert all(bool(torch.isfinite(x).all()) for x in got)
+    assert int((d.refs > 1).sum()) == sum((int(n) - 6) // d.page for n in d.length[:3].tolist())
+
+    def held(rows):
+        n = d.length[rows].tolist()
+        return [tx.paged_read(d.k[i], d.v[i], d.table[rows], d.length[rows], starts(n).to(gpu), tokens=sum(n),
+                              dtype=BF, k_block_scale=d.ks[i], v_block_scale=d.vs[i]) for i in range(2)]
+    d.free(torch.arange(6, device=gpu) % 2 == 1)
+    rows = torch.tensor([0, 2, 4], device=gpu)
+    before = held(rows)
+    d.compact()
+    used = int((d.refs > 0).sum())
+    assert bool((d.refs[:used] > 0).all()) and not d.refs[used:].any()
+    for (k, v), (k0, v0) in zip(held(rows), before):
+        assert torch.equal(k, k0) and torch.equal(v, v0)
 
 
 def test_graph_replayed_after_a_larger_call(gpu):

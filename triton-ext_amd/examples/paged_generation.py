@@ -1,6 +1,7 @@
 """Generation from a paged key/value cache: a few layers of attention with random weights.
 
     python triton-ext_amd/examples/paged_generation.py [--sequences 4] [--tokens 32] [--beams 2]
+                                                       [--cache bf16|e4m3|mx|nv]
 
 Prompts of different lengths go through in chunks, each of them then forks into beams that share
 its pages, and all beams take one token a step, in a HIP graph that is captured once and
@@ -19,7 +20,8 @@ import triton_ext_amd as tx  # noqa: E402
 
 
 class Decoder:
-    """`layers` layers of y = x + Wo attention(Wqkv x / rms), with a paged cache each."""
+    """`layers` layers of y = x + Wo attention(Wqkv x / rms), with a paged cache each: in `dtype`, in
+    float8_e4m3fn, or in 4 bits ("mx", "nv": e2m1 codes under scales of 32 or 16 dims)."""
 
     def __init__(self, layers=2, width=512, Hq=8, Hkv=2, D=64, pages=256, page=16, rows=16,
                  entries=64, dtype=torch.bfloat16, cache_dtype=None, device="cuda", seed=0):
@@ -32,8 +34,20 @@ class Decoder:
         self.qkv = [weight((Hq + 2 * Hkv) * D, width) for _ in range(layers)]
         self.out = [weight(width, Hq * D) for _ in range(layers)]
         kind = cache_dtype or dtype
-        self.k, self.v = ([torch.zeros(pages, page, Hkv, D, dtype=kind, device=device)
-                           for _ in range(layers)] for _ in range(2))
+        self.ks = self.vs = [None] * layers  # scales of blocks
+        if kind in ("mx", "nv"):  # a head's tokens together, and of the scales those of a block of dims
+            def codes():
+                return torch.zeros(pages, Hkv, page, D // 2, dtype=torch.uint8, device=device).permute(0, 2, 1, 3)
+
+            def scales():
+                s = torch.zeros(pages, Hkv, D // (32 if kind == "mx" else 16), page, dtype=torch.uint8, device=device)
+                return (s if kind == "mx" else s.view(torch.float8_e4m3fn)).permute(0, 3, 1, 2)
+            self.k, self.v = ([codes() for _ in range(layers)] for _ in range(2))
+            self.ks, self.vs = ([scales() for _ in range(layers)] for _ in range(2))
+        else:
+            self.k, self.v = ([torch.zeros(pages, page, Hkv, D, dtype=kind, device=device)
+                               for _ in range(layers)] for _ in range(2))
+        self.pages = [t for t in self.k + self.v + self.ks + self.vs if t is not None]
         self.scale = (torch.full((Hkv,), 1 / 64, device=device)
                       if kind == torch.float8_e4m3fn else None)
         self.inv_freq, self.rope_scale = tx.rotary_frequencies(D, device=device)
@@ -50,21 +64,23 @@ class Decoder:
         """x [T, width], the new tokens of sequences `rows` (a slice), already reserved."""
         H, G, D = self.Hq, self.Hkv, self.D
         table, length = self.table[rows], self.length[rows]
-        for qkv, out, k, v in zip(self.qkv, self.out, self.k, self.v):
+        for qkv, out, k, v, ks, vs in zip(self.qkv, self.out, self.k, self.v, self.ks, self.vs):
             h = x.float()
             h = (h * h.square().mean(-1, keepdim=True).add(1e-6).rsqrt()).to(x.dtype)
             y = (h @ qkv.t()).view(x.shape[0], H + 2 * G, D)
             q = tx.paged_append(y[:, H:H + G], y[:, H + G:], k, v, table, length, cu_q,
                                 q=y[:, :H], inv_freq=self.inv_freq, scale=self.rope_scale,
-                                k_scale=self.scale, v_scale=self.scale)
+                                k_scale=self.scale, v_scale=self.scale, k_block_scale=ks,
+                                v_block_scale=vs)
             o = tx.paged_attention(q, k, v, table, length, cu_q, sm_scale=D ** -0.5,
-                                   k_scale=self.scale, v_scale=self.scale)
+                                   k_scale=self.scale, v_scale=self.scale, k_block_scale=ks,
+                                   v_block_scale=vs)
             x = x + o.reshape(x.shape[0], H * D) @ out.t()
         return x
 
     def fork(self, parent, child):
         """Sequences `child` continue `parent`, in every layer's cache."""
-        self.missing = tx.page_fork(self.k + self.v, self.table, self.length, self.refs, parent,
+        self.missing = tx.page_fork(self.pages, self.table, self.length, self.refs, parent,
                                     child, out=(self.table, self.length, self.refs))[3]
 
     def free(self, drop):
@@ -72,7 +88,7 @@ class Decoder:
                      out=(self.table, self.length, self.refs))
 
     def compact(self):
-        return tx.page_compact(self.k + self.v, self.table, self.refs,
+        return tx.page_compact(self.pages, self.table, self.refs,
                                out=(self.table, self.refs))[2]
 
 
@@ -148,8 +164,10 @@ def main():
     ap.add_argument("--sequences", type=int, default=4)
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--beams", type=int, default=2)
+    ap.add_argument("--cache", choices=("bf16", "e4m3", "mx", "nv"), default="bf16")
     a = ap.parse_args()
-    d, fed, _ = generate(a.sequences, a.tokens, a.beams)
+    kind = {"bf16": None, "e4m3": torch.float8_e4m3fn}.get(a.cache, a.cache)
+    d, fed, _ = generate(a.sequences, a.tokens, a.beams, cache_dtype=kind)
     used = int((d.refs > 0).sum())
     print(f"{len(fed)} sequences of {min(map(len, fed))} .. {max(map(len, fed))} tokens in {used} "
           f"pages of {d.page} ({int((d.refs > 1).sum())} of them shared), {d.step_ms:.2f} ms a step")
