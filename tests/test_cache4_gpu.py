@@ -152,6 +152,34 @@ def test_append_rotated(gpu, n, lens, Hq, Hkv, D, rot, page, dtype, layout, inte
 
 
 @pytest.mark.parametrize("kind", ["mx", "nv"])
+@pytest.mark.parametrize("Hq,D,rot,interleaved,odd", [
+    (4, 64, 32, False, False), (4, 64, 64, False, False), (5, 96, 96, False, False), (16, 96, 40, False, False),
+    (4, 64, 0, False, False), (4, 64, 32, False, True), (33, 96, 96, False, True), (4, 64, 32, True, False),
+    (300, 128, 16, False, False), (2, 4128, 4128, False, False)])
+def test_append_in_place(gpu, Hq, D, rot, interleaved, odd, kind):
+    """q_out may be q: what comes back is what a tensor of its own gets."""
+    n = [3, 1, 7, 30]
+    c = Cache4(5, [9, 1, 20, 31], 4, 1, D, BF, kind)
+    T = sum(n) + 1
+    store = randn(c.g, T * (Hq + 2) * D + 1, dtype=BF)[int(odd):]
+    y = store[:T * (Hq + 2) * D].view(T, Hq + 2, D)
+    freq = tx.rotary_frequencies(rot)[0].to(gpu) if rot else None
+
+    def run(own):
+        dev = c.to(gpu)
+        d = torch.empty(T * (Hq + 2) * D + 8, dtype=BF, device=gpu)[int(odd):][:y.numel()].view(y.shape).copy_(y)
+        q = d[:, :Hq]
+        out = torch.empty(T, Hq, D, dtype=BF, device=gpu) if own else q
+        got = tx.paged_append(d[:, Hq:Hq + 1], d[:, Hq + 1:], cu_q=starts(n).to(gpu), q=q, inv_freq=freq,
+                              interleaved=interleaved, q_out=out, **books(dev))
+        assert got is out
+        return [out.clone()] + [raw(dev[x]) for x in ("k_cache", "v_cache", "k_block_scale", "v_block_scale")]
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["mx", "nv"])
 @pytest.mark.parametrize("lie", ["odd base", "odd strides", "strided last", "broadcast"])
 def test_append_views(gpu, lie, kind):
     """Tokens that are not read 16 bytes at a time, and scales in an order of their own."""

@@ -3,9 +3,13 @@
 //
 // A row of codes is 16 .. 128 bytes, a quarter of what LDS tiles of 16-bit pages are made for, so
 // they are loaded into registers, straight from the pages: of 16 keys, lane (m, g) takes the
-// g-th quarter of key m's row (of 256 dims: one 16-byte piece of each half) and its scales, one byte
-// each.  A piece is 8 bytes (heads of up to 64) or 16 (32 dims: one or two blocks), so the
-// conversion to 16 bits needs one or two factors.
+// g-th quarter of key m's row (of 256 dims: one 16-byte piece of each half).  A piece is 8 bytes
+// (heads of up to 64) or 16 (32 dims: one or two blocks), so the conversion to 16 bits needs one or
+// two factors; the scales come as dwords of four keys and reach their lanes by ds_bpermute.
+//
+// Codes become the 16-bit type that q is in, which holds every code under an e8m0 scale of its range
+// exactly; under e4m3 scales fp16, which holds all of their products exactly too and, unlike bf16, is
+// multiplied two at a time.
 //
 // K: S^T = K . Q^T does not ask in which order dims are summed.  With m = lane % 16 the lane's
 // dims are an operand of the 16x16x32 MFMAs as they stand, Q is loaded in the same order, and K
@@ -298,7 +302,7 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
 constexpr uint32_t kSplit4Overhead = 3, kRows4Overhead = 6;
 
 // Counters of sets of parts begin here in the workspace's 16384 (those of units, and of other
-// launches, before them: a launch has at most 512 workgroups).
+// launches, before them: a launch has at most 768 workgroups).
 constexpr uint32_t kSetCounters = 8192;
 
 // Which of 16 keys (four adjacent lanes each) a lane's flag is set of.
@@ -518,6 +522,13 @@ template <int N, class F> __device__ __forceinline__ void each_slot(F f) {
 // Workgroups of a CU: by LDS, and by registers where heads are long.
 template <class A> constexpr int paged4_split_groups() { return A::BYTES * 4 <= 81920 ? 2 : 1; }
 
+// A wave takes every fourth block of 32 keys by itself, NS blocks of codes under way: codes, scales and
+// page numbers are in registers before they are needed, and no barrier stands between a unit's begin
+// and its end.  Bound by how many bytes are under way.  One token for each of 32 sequences of 100 .. 16384
+// keys, 32 heads of 128 over 8: 36.5 us, 3.3 TB/s (33 us with the arithmetic taken out); 4 tokens for each of 4
+// sequences of 60000 .. 131072: 101 us, 4.5 TB/s (94); 8 sequences of 5000 .. 32768, 16 heads of 256 over 2, one
+// block under way for lack of registers: 35 us, 2.0 TB/s (31).  One token over 1500 keys: 10 us, of which the
+// launch, the table, the codes behind it and the join of the parts each wait for memory once.
 template <class A>
 __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_split_kernel(Paged4Args args4) {
   constexpr int D = A::D, BN = A::BN, RT = A::RT, ROWS = A::ROWS, NS = A::NS;
@@ -749,7 +760,14 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
 
 // 128 rows a unit, 32 a wave.  Of a block of 64 keys each wave holds the codes of 16, converts them
 // into the tiles of 16-bit rows that all four read, and loads those of the next block: K and V have
-// two tiles each, one barrier a block.
+// two tiles each, one barrier a block.  (K goes through LDS here: each wave alone would convert it
+// four times.)
+//
+// Bound by the work between the products: a block's conversions, exponentials, masks and LDS accesses
+// take about as long as its MFMAs, and two workgroups a CU (heads of 64: three), which is what registers
+// allow, overlap only part of them.  2 sequences of 2048 new tokens over up to 16384 keys, 32 heads of 128
+// over 8: 1052 us, 0.84 PFLOP/s of the 1.26 that a large product of the library reaches (1102 before
+// V's tile had its swizzle).
 template <int D_, bool BF, bool NV_> struct Paged4Rows {
   static constexpr int D = D_, BN = 64;
   static constexpr bool NV = NV_, CBF = BF && !NV;
@@ -757,9 +775,6 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
   typedef PagedFrag<D, CBF, false, BN> P;
   typedef Piece4<D, NV> Piece;
   typedef typename AttnFwd<64, BF, 32, 64>::elt elt; // of q and o
-#ifndef VRX
-#define VRX 4
-#endif
   // V's tile: P's swizzle puts the 64 bytes of 4 rows that a transposed read takes on different banks, and
   // the same bits again those within 64 that the lanes of 4 keys write together (without: a quarter of
   // the LDS's time).
@@ -791,11 +806,12 @@ template <int D_, bool BF, bool NV_> struct Paged4Rows {
         vf.v[bd][c] = __builtin_bit_cast(i32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
   }
-  static constexpr int VR = D == 128 ? VRX : D < 128 ? P::NV : P::VN; // dim blocks of V read ahead of the softmax
+  static constexpr int VR = D <= 128 ? P::NV : P::VN; // dim blocks of V read ahead of the softmax
 };
+
 // A unit's end: its rows (32 a wave) are written out as T, or left as one part of several, which the
 // last workgroup to arrive joins, in order; of more than kRowsSet parts in sets, as
-// paged4_split_end.  460 rows of one sequence over 14470 keys (heads of 128): 97 us part by part.
+// paged4_split_end.  460 rows of one sequence (heads of 128) over 14470 keys: 42 us, 97 part by part.
 constexpr uint32_t kRowsSet = 8;
 template <class P, class T>
 __device__ __forceinline__ void paged4_rows_end(const PagedUnit &unit, typename P::Acc &acc, float m, float l,
