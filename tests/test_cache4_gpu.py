@@ -361,6 +361,22 @@ def test_rows_of_a_sequence(gpu, rows, D, kind):
     attend(gpu, [n], [n + 40], 2 * G, 2, D, 16, BF, kind, window=33, scaled=True)
 
 
+@pytest.mark.parametrize("kind", ["mx", "nv"])
+@pytest.mark.parametrize("D", [32, 160, 192, 224])
+@pytest.mark.parametrize("n", [1, 20, 150])
+def test_head_dims_between(gpu, n, D, kind):
+    """Heads whose dims a form fills up with none."""
+    attend(gpu, [n, 1], [n + 300, 70], 4, 2, D, 16, HF if n == 20 else BF, kind, layout="hnd")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_parts_of_every_number(gpu, n, D):
+    """One unit (n * 3 rows) of 1, 2, .. blocks of keys: as many parts, in sets of any rest."""
+    for blocks in list(range(1, 28)) + [33, 41, 64, 65, 66]:
+        attend(gpu, [n], [max(n, blocks * (64 if n == 40 else 128) - 5)], 3, 1, D, 64, BF, "mx")
+
+
 @pytest.mark.parametrize("layout", ["nhd", "hnd"])
 @pytest.mark.parametrize("page", [1, 2, 4, 8, 16, 32, 64, 512])
 def test_attend_page_sizes(gpu, page, layout):
