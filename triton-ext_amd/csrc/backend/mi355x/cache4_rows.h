@@ -209,37 +209,20 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
           y[0][i] = y[0][i] * c[i] + elt_to_f32(x.partner.v[i]) * s[i];
     }
   };
-  // f(head, its values) of heads lane, lane + head_lanes, ..
-  auto each = [&](const T *src, int64_t sh, int heads, bool turn, auto f) __attribute__((always_inline)) {
-    const T *head = src + at.lane * sh;
-    const int64_t step = p.head_lanes * sh;
-    for (int h0 = at.lane; h0 < heads; h0 += BATCH * p.head_lanes) {
-      Loaded x[BATCH];
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k, head += step)
-        if (h0 + k * p.head_lanes < heads)
-          load(head, x[k], turn);
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int h = h0 + k * p.head_lanes;
-        if (h >= heads)
-          break;
-        float y[RUNS][8];
-        values(x[k], turn, y);
-        f(h, y);
-      }
-    }
+
+  // Heads are counted through q, k and v: a thread's are lane, lane + head_lanes, .. of them, so that
+  // loads of all three are under way together.  A token without a page: its q alone.
+  const int q_end = p.Hq, k_end = q_end + p.Hkv, end = pl.page < 0 ? q_end : k_end + p.Hkv;
+  auto head_at = [&](int h) __attribute__((always_inline)) {
+    return h < q_end   ? static_cast<const T *>(p.q) + t * p.q_st + h * p.q_sh
+           : h < k_end ? static_cast<const T *>(p.k) + t * p.k_st + (h - q_end) * p.k_sh
+                       : static_cast<const T *>(p.v) + t * p.v_st + (h - k_end) * p.v_sh;
   };
-  if (p.Hq) {
-    const T *const in = static_cast<const T *>(p.q) + t * p.q_st;
-    T *const out = static_cast<T *>(p.q_out) + t * p.o_st;
-    if constexpr (MODE != kRunAlone) {
-      each(in, p.q_sh, p.Hq, pl.mine, [&](int h, float (&y)[RUNS][8]) {
-#pragma unroll
-        for (int r = 0; r < RUNS; ++r)
-          store8<T, WHOLE>(out + h * p.o_sh + d[r], y[r]);
-      });
-    } else { // no blocks in q: a thread has whole pairs, so that q_out may be q
+  auto turns = [&](int h) { return h < q_end ? pl.mine : h < k_end; };
+  if constexpr (MODE == kRunAlone) // no blocks in q: a thread has whole pairs, so that q_out may be q
+    if (p.Hq) {
+      const T *const in = static_cast<const T *>(p.q) + t * p.q_st;
+      T *const out = static_cast<T *>(p.q_out) + t * p.o_st;
       auto sine = [&](int j) __attribute__((always_inline)) {
         return shared ? sines[mine0 + j] : turn4_of((double)pl.pos, p.inv_freq[j], p.scale);
       };
@@ -300,15 +283,35 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
         }
       }
     }
-  }
-  if (pl.page < 0) // a token without a page: its q alone
-    return;
   const int64_t slot = pl.pos & ((1 << p.page_shift) - 1);
-  auto side = [&](const T *src, int64_t sh, bool turn, const float *head_scale, uint8_t *codes, int64_t ch,
-                  const BlockScales &bs) __attribute__((always_inline)) {
-    uint8_t *const scales = bs.s + pl.page * bs.sp + slot * bs.st;
-    each(src, sh, p.Hkv, turn, [&](int h, float (&y)[RUNS][8]) {
-      const float f = head_scale ? head_scale[h] : 1.f;
+  for (int h0 = (MODE == kRunAlone ? q_end : 0) + at.lane; h0 < end; h0 += BATCH * p.head_lanes) {
+    Loaded x[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (const int h = h0 + k * p.head_lanes; h < end)
+        load(head_at(h), x[k], turns(h));
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int h = h0 + k * p.head_lanes;
+      if (h >= end)
+        break;
+      float y[RUNS][8];
+      values(x[k], turns(h), y);
+      if (MODE != kRunAlone && h < q_end) {
+        T *const out = static_cast<T *>(p.q_out) + t * p.o_st + h * p.o_sh;
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r)
+          store8<T, WHOLE>(out + d[r], y[r]);
+        continue;
+      }
+      const bool v = h >= k_end;
+      const int hk = h - (v ? k_end : q_end);
+      const BlockScales &bs = v ? args.vs : args.ks;
+      uint8_t *const codes = v ? p.vc + pl.page * p.vc_sp + slot * p.vc_st + hk * p.vc_sh
+                               : p.kc + pl.page * p.kc_sp + slot * p.kc_st + hk * p.kc_sh;
+      uint8_t *const scales = bs.s + pl.page * bs.sp + slot * bs.st + hk * bs.sh;
+      const float *const head_scale = v ? p.v_scale : p.k_scale;
+      const float f = head_scale ? head_scale[hk] : 1.f;
 #pragma unroll
       for (int r = 0; r < RUNS; ++r) {
         if (head_scale) {
@@ -317,16 +320,12 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
             y[r][i] = y[r][i] / f;
         }
         const uint32_t scale = block4_scale<NV>(block4_max<LANES>(y[r]), args.lo, args.hi);
-        *reinterpret_cast<uint32_t *>(codes + h * ch + d[r] / 2) = block4_codes<NV>(y[r], scale);
+        *reinterpret_cast<uint32_t *>(codes + d[r] / 2) = block4_codes<NV>(y[r], scale);
         if (d[r] / 8 % LANES == 0)
-          scales[h * bs.sh + d[r] / (8 * LANES) * bs.sb] = scale;
+          scales[d[r] / (8 * LANES) * bs.sb] = scale;
       }
-    });
-  };
-  side(static_cast<const T *>(p.k) + t * p.k_st, p.k_sh, true, p.k_scale, p.kc + pl.page * p.kc_sp + slot * p.kc_st,
-       p.kc_sh, args.ks);
-  side(static_cast<const T *>(p.v) + t * p.v_st, p.v_sh, false, p.v_scale,
-       p.vc + pl.page * p.vc_sp + slot * p.vc_st, p.vc_sh, args.vs);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
