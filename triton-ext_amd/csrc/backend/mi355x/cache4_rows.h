@@ -7,10 +7,10 @@
 //
 // Read: the same threads; a lane turns 8 dims into 16 or 32 bytes.
 //
-// Both are bound by memory.  Append, 9001 tokens of 32 + 2 * 8 heads of 128 in bf16, e4m3 scales: 45 us,
-// 4.4 TB/s (a copy reaches 5.07); 48 tokens: 6 us, the latency of the table, the sines and the values one
+// Both are bound by memory.  Append, 9001 tokens of 32 + 2 * 8 heads of 128 in bf16, e4m3 scales: 44 us,
+// 4.5 TB/s (a copy reaches 5.07); 48 tokens: 5 us, the latency of the table, the sines and the values one
 // after the other.  With a thread for 8 dims of one head, its sines its own, that prompt and its reading back
-// took 90 us, now 58.  Read, 156000 tokens of 2 * 8 heads of 128 into bf16: 167 us, 5.0 TB/s (so: 233).
+// took 90 us, now 56.  Read, 156000 tokens of 2 * 8 heads of 128 into bf16: 167 us, 5.0 TB/s (so: 233).
 #pragma once
 
 #include <hip/hip_runtime.h>
