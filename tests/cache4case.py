@@ -124,3 +124,16 @@ class Cache4(Cache):
                     kv_len=self.kv_len.to(device),
                     k_scale=None if self.k_scale is None else self.k_scale.to(device),
                     v_scale=None if self.v_scale is None else self.v_scale.to(device))
+
+
+# Appends whose tokens have more than 256 threads, the last workgroup of a token fewer than there are
+# rotated pairs, with a head of q or k in it: n, lens, Hq, Hkv, D, rot, page, dtype, layout, interleaved.
+MANY_THREADS = [
+    ([1, 1, 1], [5, 70, 3000], 16, 2, 256, 256, 16, torch.bfloat16, "hnd", False),
+    ([1, 1], [9, 33], 32, 2, 128, 128, 64, torch.float16, "nhd", False),
+    ([2, 1], [40, 7], 32, 1, 128, 128, 16, torch.bfloat16, "hnd", False),
+    ([1, 3], [6, 50], 16, 1, 128, 128, 16, torch.bfloat16, "hnd", True),
+    ([600], [700], 64, 8, 256, 256, 16, torch.bfloat16, "hnd", False),  # fewer threads than heads
+    ([990, 10], [990, 500], 31, 17, 256, 80, 16, torch.float16, "hnd", False),  # halves end inside a block
+    ([990, 10], [990, 500], 31, 17, 256, 76, 16, torch.bfloat16, "nhd", False),
+]

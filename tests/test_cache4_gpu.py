@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import triton_ext_amd as tx  # noqa: E402
-from cache4case import BLOCK, Cache4, nearest, quantise, scale_bytes, scale_values, values  # noqa: E402
+from cache4case import BLOCK, MANY_THREADS, Cache4, nearest, quantise, scale_bytes, scale_values, values  # noqa: E402
 from cachecase import E4M3, F, Cache, attend64, check, gen, randn, rotate64, rotate_bound, starts  # noqa: E402
 from dotcase import say  # noqa: E402
 
@@ -657,3 +657,11 @@ def test_nothing_to_do(gpu):
     assert k.shape == (2, 2, 64) and not k.any() and not v.any()
     got = tx.paged_append(q[:, :2], q[:, :2], page_table=table, kv_len=kv, q=q, **none)
     assert torch.equal(got, q)
+
+
+@pytest.mark.parametrize("kind", ["mx", "nv"])
+@pytest.mark.parametrize("n,lens,Hq,Hkv,D,rot,page,dtype,layout,interleaved", MANY_THREADS)
+def test_append_tokens_of_more_than_a_workgroup(gpu, n, lens, Hq, Hkv, D, rot, page, dtype, layout, interleaved,
+                                                kind):
+    """Heads that are rotated in a token's last workgroup, of fewer threads than there are pairs."""
+    test_append_rotated(gpu, n, lens, Hq, Hkv, D, rot, page, dtype, layout, interleaved, kind)

@@ -19,6 +19,7 @@
 
 #include "cache4.h"
 #include "rotary.h"
+#include "sine_share.h"
 
 namespace txk {
 
@@ -126,10 +127,11 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
   const int rot = p.rot, half = rot / 2;
 
   // The token's sines, a pair a thread, in LDS; heads of more pairs than that: each thread its own.
-  const int per = p.token_threads <= 256 ? p.token_threads : 256, mine0 = (int)threadIdx.x / per * half;
-  const bool shared = (256 / per) * half <= kAppendSines;
+  const SineShare mine = sine_share(threadIdx.x, p.token_threads, at.lane * p.items + at.item);
+  const int mine0 = (int)mine.token * half;
+  const bool shared = (p.token_threads <= 256 ? 256 / p.token_threads : 1) * half <= kAppendSines;
   if (shared && on)
-    for (int i = (int)threadIdx.x % per; i < half; i += per)
+    for (int i = mine.first; i < half; i += mine.step)
       sines[mine0 + i] = turn4_of((double)pl.pos, p.inv_freq[i], p.scale);
   __syncthreads();
   if (!on)
