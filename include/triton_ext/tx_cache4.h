@@ -92,7 +92,9 @@ TX_API int tx_paged_read_launch(const tx_paged_read_plan *plan, const void *k_ca
 
 /* ---- attention of new tokens over the cache ------------------------------
  * As tx_paged_attn over the values that the cache holds, which are taken in q's type (MX32:
- * exact but for what fp16 has no place for; NV16: exact, in fp16).  A row that attends to a
+ * exact but for what fp16 has no place for; NV16: exact, in fp16).  p is rounded to bf16 under
+ * MX32 with q in bf16, else to fp16, where a weight is off by 2^-32 of the row's sum or by its
+ * relative half step, whichever is more.  A row that attends to a
  * token with a scale of NaN, or an MX32 scale above 2^125 (q in fp16: 2^13), in any block of its
  * k or v is NaN as a whole; other rows are not touched by it.  c.cache_type is TX_F4E2M1,
  * c.head_dim a multiple of 32 up to 256; the caches' strides count bytes. */

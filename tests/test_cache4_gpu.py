@@ -665,3 +665,36 @@ def test_append_tokens_of_more_than_a_workgroup(gpu, n, lens, Hq, Hkv, D, rot, p
                                                 kind):
     """Heads that are rotated in a token's last workgroup, of fewer threads than there are pairs."""
     test_append_rotated(gpu, n, lens, Hq, Hkv, D, rot, page, dtype, layout, interleaved, kind)
+
+
+@pytest.mark.parametrize("kind,dtype", [("mx", BF), ("mx", HF), ("nv", BF), ("nv", HF)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 20, 150])
+def test_small_weights_add_up(gpu, n, D, kind, dtype):
+    """One key outweighs all the others, and what it holds is 0: the result is what the small weights
+    add up to.  In fp16 a weight (2^7 or more at a row's reference) is off by half its least step, 2^-25."""
+    L, less = 600, 26.3  # keys, and how far below the one the others are: a factor of 2^less
+    c = Cache4(21, [L], 16, 1, D, dtype, kind, "hnd")
+    one, two56 = (127, 135) if kind == "mx" else (0x38, 0x78)  # scales of 1 and 256
+    blocks = D // BLOCK[kind]
+    for j in range(L):
+        k = torch.zeros(1, D // 2, dtype=torch.uint8)
+        k[0, 0] = 6 if j == 0 else 0  # dim 0: 4 or 0
+        c.put("k", 0, j, k, torch.full((1, blocks), one, dtype=torch.uint8))
+        v = torch.full((1, D // 2), 0 if j == 0 else 0x66, dtype=torch.uint8)
+        c.put("v", 0, j, v, torch.full((1, blocks), two56, dtype=torch.uint8))
+    assert torch.equal(c.rows("k", 0)[0][:2, 0, 0], torch.tensor([4.0, 0.0], dtype=torch.float64))
+    assert torch.equal(c.rows("v", 0)[0][:2, 0, -1], torch.tensor([0.0, 1024.0], dtype=torch.float64))
+    q = torch.zeros(n, 1, D, dtype=dtype)
+    q[:, :, 0] = 1.0
+    o, lse = tx.paged_attention(q.to(gpu), cu_q=starts([n]).to(gpu), sm_scale=less * math.log(2.0) / 4, causal=False,
+                                return_lse=True, **books(c.to(gpu)))
+    small = (L - 1) * 2.0 ** -less
+    want = torch.full((n, 1, D), small * 1024.0 / (1 + small), dtype=torch.float64)
+    # roundings: of a weight (bf16: relative; fp16: absolute, here larger), of the result, and of the
+    # score, (D + 2) F and less * 4 F of the exponent's
+    bound = (L - 1) * 1024.0 * 2.0 ** -32 if (kind, dtype) != ("mx", BF) else 2.0 ** -8 * want
+    bound = bound + torch.finfo(dtype).eps / 2 * want + (D + 2 + 4) * less * F * want
+    check(o, want, bound, "o")
+    top = torch.full((n, 1), less, dtype=torch.float64)
+    check(lse, top + math.log2(1 + small), (D + 10) * F * top, "lse")

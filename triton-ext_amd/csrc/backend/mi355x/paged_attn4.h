@@ -298,6 +298,11 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
   }
 }
 
+// What a row's weights are raised by (PagedFrag::softmax), as an exponent: in fp16 up to 2^15, so that
+// a weight loses no more than 2^-32 of the row's sum (without, 2^-25: a row of 131072 small ones 2^-8 of what they
+// hold, as much as all of bf16's rounding).
+template <bool CBF> constexpr int kUp4 = CBF ? 0 : 7;
+
 // What a unit's beginning and end cost, in steps (paged_sched.h).
 constexpr uint32_t kSplit4Overhead = 3, kRows4Overhead = 6;
 
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
           seen &= a < 64 ? ~0ull << a : 0;
           P16::mask(s[i], seen & here[0]);
         }
-        P16::softmax(s[i], scale[i], acc[i], m[i], l[i], pf[i]);
+        P16::template softmax<kUp4<A::CBF>>(s[i], scale[i], acc[i], m[i], l[i], pf[i]);
       }
 #pragma unroll
       for (int b0 = 0; b0 < P16::NV; b0 += A::VN) {
@@ -1106,7 +1111,7 @@ __global__ void __launch_bounds__(256, paged4_rows_groups<A>()) paged_attn4_rows
           P::mask(s, seen & here[0]);
         }
         typename P::PF pf;
-        P::softmax(s, scale, acc, m, l, pf);
+        P::template softmax<kUp4<A::CBF>>(s, scale, acc, m, l, pf);
         P::pv(vf, 0, pf, acc);
 #pragma unroll
         for (int b0 = VR; b0 < P::NV; b0 += VR) {

@@ -224,7 +224,9 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
   // Updates the row's reference m (both lanes of a row hold the same), the lane's part of the sum
   // l, and acc; p as MFMA operands.  m follows the row's maximum only when that has grown past
   // it by 8, so acc is seldom rescaled; p is up to 2^8 then, in range in both types, and rounded by
-  // the same relative half step.
+  // the same relative half step.  UP: the reference lies so far below the maximum that it is set by,
+  // so that p is up to 2^(8 + UP), and fp16 has that many more places for small ones.
+  template <int UP = 0>
   __device__ __forceinline__ static void softmax(f16v (&s)[BN / 32], float qk_scale,
                                                  f16v (&acc)[D / 32], float &m, float &l,
                                                  h8 (&pf)[BN / 16]) {
@@ -235,8 +237,8 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag {
       for (int r = 0; r < 16; ++r)
         mx = fmaxf(mx, s[b][r]);
     mx = X::xmax(mx) * qk_scale;
-    if (__builtin_expect(__any(mx > m + 8.f), 0)) {
-      const float to = mx > m + 8.f ? mx : m;
+    if (__builtin_expect(__any(mx > m + (8.f + UP)), 0)) {
+      const float to = mx > m + (8.f + UP) ? mx - UP : m;
       const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
       l *= alpha;
 #pragma unroll
@@ -445,6 +447,7 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag16 {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
   // As PagedFrag's.
+  template <int UP = 0>
   __device__ __forceinline__ static void softmax(Scores &s, float qk_scale, Acc &acc, float &m,
                                                  float &l, PF &pf) {
     float mx = s[0][0];
@@ -454,8 +457,8 @@ template <int D_, bool BF, bool F8_, int BN_> struct PagedFrag16 {
       for (int r = 0; r < 4; ++r)
         mx = fmaxf(mx, s[b][r]);
     mx = row_max(mx) * qk_scale;
-    if (__builtin_expect(__any(mx > m + 8.f), 0)) {
-      const float to = mx > m + 8.f ? mx : m;
+    if (__builtin_expect(__any(mx > m + (8.f + UP)), 0)) {
+      const float to = mx > m + (8.f + UP) ? mx - UP : m;
       const float alpha = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
       l *= alpha;
 #pragma unroll
