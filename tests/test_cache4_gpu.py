@@ -698,3 +698,28 @@ def test_small_weights_add_up(gpu, n, D, kind, dtype):
     check(o, want, bound, "o")
     top = torch.full((n, 1), less, dtype=torch.float64)
     check(lse, top + math.log2(1 + small), (D + 10) * F * top, "lse")
+
+
+@pytest.mark.parametrize("kind", ["mx", "nv"])
+@pytest.mark.parametrize("n", [2, 20, 150])
+def test_infinite_query(gpu, n, kind):
+    """A row of q with an infinity and finite dims past fp16's range: every score is the infinity's, here
+    -infinity, so that the row attends to nothing; other rows stay as they are."""
+    D = 128
+    c = Cache4(23, [200], 16, 1, D, BF, kind, "hnd").fill()
+    for j in range(200):  # dims 0 and 1: -1 and 1
+        page, slot = c.place(0, j)
+        c.k[page, slot, 0, 0] = 0x2a
+        c.kb[page, slot, 0, 0] = 127 if kind == "mx" else 0x38
+    q = randn(c.g, n, 1, D, dtype=BF)
+    dev, cu = c.to(gpu), starts([n]).to(gpu)
+    o, lse = tx.paged_attention(q.to(gpu), cu_q=cu, sm_scale=0.1, causal=False, return_lse=True, **books(dev))
+    assert bool(torch.isfinite(o).all())
+    q[1, 0, 0], q[1, 0, 1] = math.inf, 1e30
+    o2, lse2 = tx.paged_attention(q.to(gpu), cu_q=cu, sm_scale=0.1, causal=False, return_lse=True, **books(dev))
+    rest = torch.arange(n) != 1
+    assert torch.equal(o2[rest], o[rest]) and torch.equal(lse2[rest], lse[rest])
+    assert not o2[1].any() and bool((lse2[1] == -math.inf).all())
+    q[1, 0, 0] = -math.inf  # every score is infinity: no numbers
+    o2, lse2 = tx.paged_attention(q.to(gpu), cu_q=cu, sm_scale=0.1, causal=False, return_lse=True, **books(dev))
+    assert torch.equal(o2[rest], o[rest]) and bool(o2[1].isnan().all())

@@ -266,7 +266,8 @@ template <int D, bool NV, int KEYS, bool ALIKE> struct Scales4 {
 
 // Q in the type that codes are computed in.  bf16 rows under e4m3 scales become fp16, times the
 // power of two that takes the row's largest magnitude to [2^7, 2^8): exact but for what is below
-// 2^-31 of that.  Returns what the row's scores are to be multiplied by.
+// 2^-31 of that.  Returns what the row's scores are to be multiplied by.  A row with an infinity: its
+// scores are infinite or no numbers whatever its other dims are, which have to stay finite.
 // x: the lane's dims of a row; the lanes of a row: those that `row_max` goes over.
 template <bool BF, int N, class F>
 __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
@@ -283,8 +284,7 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
       }
     mx = row_max(mx);
     const int e = (__float_as_uint(mx) >> 23) & 255;
-    // (0, infinity: as it is)
-    const int up = e == 0 || e == 255 ? 0 : 134 - e < 127 ? 134 - e : 127;
+    const int up = e == 0 ? 0 : e == 255 ? -120 : 134 - e < 127 ? 134 - e : 127;
     const float f = __builtin_amdgcn_ldexpf(1.f, up);
 #pragma unroll
     for (int c = 0; c < N; ++c)
@@ -294,7 +294,7 @@ __device__ __forceinline__ float q4_to_f16(u32x4 (&x)[N], F row_max) {
                            (_Float16)(__uint_as_float((uint32_t)x[c][i] & 0xffff0000u) * f)};
         x[c][i] = __builtin_bit_cast(uint32_t, h);
       }
-    return __builtin_amdgcn_ldexpf(1.f, -up);
+    return e == 255 ? 1.f : __builtin_amdgcn_ldexpf(1.f, -up);
   }
 }
 
