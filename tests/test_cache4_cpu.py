@@ -7,7 +7,7 @@ import pytest
 
 import triton_ext_amd as tx
 from cache4case import BLOCK, LEVELS, quantise, scale_values, values
-from triton_ext_amd import capi
+from triton_ext_amd import cache4 as cache4_module, capi
 
 torch = pytest.importorskip("torch")
 BF, HF, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
@@ -124,6 +124,18 @@ def test_read_refusals():
     with pytest.raises(tx.TxError) as e:  # rows that overlap are not written
         read(k_out=rows[:1].expand(2, 2, 64))
     assert e.value.code == tx.ERR_INVALID
+
+
+def test_no_number_of_rows_stands_for_none(monkeypatch):
+    """A negative `tokens` is refused also after a call that gives none (whose form is known then)."""
+    if tx.load().tx_device_available():
+        pytest.skip("there is a GPU")
+    monkeypatch.setattr(cache4_module, "_current_stream", lambda device: 0)
+    with pytest.raises(tx.TxError) as e:
+        read(stream=0)
+    assert e.value.code == tx.ERR_NO_DEVICE
+    with pytest.raises(ValueError):
+        read(stream=0, tokens=-1)
 
 
 def test_calls_without_a_gpu():

@@ -176,7 +176,7 @@ def paged_read(k_cache, v_cache, page_table, kv_len, cu_q=None, *, tokens=None, 
     import torch
     native = cache._native or _calls()
     form = native.form("read", k_cache, v_cache, page_table, kv_len, cu_q,
-                       -1 if tokens is None else cache.index(tokens), str(dtype), k_scale, v_scale,
+                       None if tokens is None else cache.index(tokens), str(dtype), k_scale, v_scale,
                        k_block_scale, v_block_scale, k_out, v_out)
     found = _forms.get(form)
     if found is None:
