@@ -299,6 +299,26 @@ def test_read_every_code_and_scale(gpu, kind):
         assert bool(same.all()), (out, torch.nonzero(~same)[:4])
 
 
+@pytest.mark.parametrize("kind", ["mx", "nv"])
+def test_read_every_code_and_scale_of_both(gpu, kind):
+    """As before, with codes and scales of their own in K and V, and every one of both compared."""
+    B = 32 // BLOCK[kind]
+    codes = torch.arange(16, dtype=torch.uint8).repeat(2)
+    kc = (codes[0::2] | codes[1::2] << 4).expand(256, 1, 1, 16).contiguous()
+    vc = kc.flip(-1).contiguous()
+    ks = torch.arange(256, dtype=torch.uint8).view(256, 1, 1, 1).expand(256, 1, 1, B).contiguous()
+    vs = ks.flip(0).contiguous()
+    table, length = torch.arange(256, dtype=torch.int32).view(256, 1), torch.ones(256, dtype=torch.int32)
+    byte = torch.uint8 if kind == "mx" else E4M3
+    for out in (torch.float32, BF, HF):
+        got = tx.paged_read(kc.to(gpu), vc.to(gpu), table.to(gpu), length.to(gpu), dtype=out,
+                            k_block_scale=ks.to(gpu).view(byte), v_block_scale=vs.to(gpu).view(byte))
+        for x, c, s in zip(got, (kc, vc), (ks, vs)):
+            ref = values(c, s, kind).view(256, 1, 32).float().to(out)
+            same = (x.cpu() == ref) | (x.cpu().isnan() & ref.isnan())
+            assert bool(same.all()), (out, torch.nonzero(~same)[:4])
+
+
 # ---- attention over the cache -----------------------------------------------
 
 def small_weights(c, n, bo):
