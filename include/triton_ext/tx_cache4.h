@@ -8,7 +8,7 @@
  * Block scales are bytes at (page, token, head, block) by any strides:
  *   TX_SCALE_MX32   e8m0 of 32 dims: value = code * 2^(byte - 127), 255 is NaN
  *   TX_SCALE_NV16   e4m3 of 16 dims: value = code * scale
- * and k_scale, v_scale (fp32 [Hkv], NULL: 1) multiply all of a head.  A call takes 128 + 4
+ * and k_scale, v_scale (fp32 [Hkv], NULL: 1) multiply all of a head.  A cache takes 128 + 8
  * bits of 32 dims (MX32) or 128 + 16 (NV16) where 16-bit caches take 512.
  */
 #ifndef TRITON_EXT_AMD_TX_CACHE4_H
@@ -33,7 +33,8 @@ typedef struct tx_block_scales {
  *   MX32  e = the least integer with a <= 7 * 2^e, within [-125, 125] (bf16 tokens) or
  *         [-23, 13] (fp16); the scale is e + 127, a code the nearest to y / 2^e
  *   NV16  the scale is a / 6 in e4m3, to nearest even, within [2^-9, 448]; a code the nearest
- *         to y / scale
+ *         to y / scale.  Blocks with a below 0.1 have scales among e4m3's subnormals, whose few
+ *         bits cost up to a third of a value: k_scale below 1 lifts them
  * Codes go to nearest, ties to the even one, saturated at 6, with y's sign.  A block with a NaN
  * or an infinity gets a scale of NaN and codes of 0.
  * c.cache_type is TX_F4E2M1; c.head_dim a multiple of 32; the caches' strides count bytes and are

@@ -402,7 +402,9 @@ extern "C" TX_API int tx_paged_attn4_plan_create(const tx_paged_attn4_desc *desc
   // nothing; past a form's rows its units convert the same keys again, which the form of 128 does once
   // for all of its waves.  16 sequences of 16384 keys, heads of 128: 16 rows each 68 us in the form of 16,
   // 82 in that of 32; 32 rows 89, and 146 in that of 128; 64 rows 160 and 175.  Heads of 64: 32 rows 67
-  // and 90, 64 rows 118 and 106.  8 sequences, heads of 256: 64 rows 131 and 170.
+  // and 90, 64 rows 118 and 106.  8 sequences, heads of 256: 64 rows 131 and 170.  The average decides for all
+  // of a call: one chunk of 2048 tokens beside 47 single ones, 8192 keys each, 32 heads of 128 over 8, takes 538
+  // us, and 397 in two calls, the chunk by itself.
   const int D = attnDims(d.head_dim);
   const int64_t G = d.Hq / d.Hkv, rows = d.T * G;
   plan->variant = rows <= 16 * d.B ? 0 : rows <= (D > 64 ? 64 : 32) * d.B ? 1 : 2;

@@ -1,4 +1,5 @@
-// Table of the attention over a 4-bit paged cache, up to 32 rows a sequence (paged_attn4.h).
+// Table of the attention over a 4-bit paged cache, up to 32 rows a sequence on average, heads of more than 64
+// dims 64 (paged_attn4.h).
 
 #include "paged_attn4.h"
 

@@ -527,9 +527,9 @@ template <int N, class F> __device__ __forceinline__ void each_slot(F f) {
 // Workgroups of a CU: by LDS, and by registers where heads are long.
 template <class A> constexpr int paged4_split_groups() { return A::BYTES * 4 <= 81920 ? 2 : 1; }
 
-// A wave takes every fourth block of 32 keys by itself, NS blocks of codes under way: codes, scales and
-// page numbers are in registers before they are needed, and no barrier stands between a unit's begin
-// and its end.  Bound by how many bytes are under way.  One token for each of 32 sequences of 100 .. 16384
+// A wave takes a quarter of a unit's blocks of 32 keys, one after the other and by itself, NS blocks of codes
+// under way: codes, scales and page numbers are in registers before they are needed, and no barrier stands
+// between a unit's begin and its end.  Bound by how many bytes are under way.  One token for each of 32 sequences of 100 .. 16384
 // keys, 32 heads of 128 over 8: 36.5 us, 3.3 TB/s (33 us with the arithmetic taken out); 4 tokens for each of 4
 // sequences of 60000 .. 131072: 101 us, 4.5 TB/s (94); 8 sequences of 5000 .. 32768, 16 heads of 256 over 2, one
 // block under way for lack of registers: 35 us, 2.0 TB/s (31).  One token over 1500 keys: 10 us, of which the
@@ -772,7 +772,9 @@ __global__ void __launch_bounds__(256, paged4_split_groups<A>()) paged_attn4_spl
 // take about as long as its MFMAs, and two workgroups a CU (heads of 64: three), which is what registers
 // allow, overlap only part of them.  2 sequences of 2048 new tokens over up to 16384 keys, 32 heads of 128
 // over 8: 1052 us, 0.84 PFLOP/s of the 1.26 that a large product of the library reaches (1102 before
-// V's tile had its swizzle).
+// V's tile had its swizzle; the 16-bit cache's form, which converts nothing, takes 970).  24 sequences of 1 ..
+// 300 tokens, 16 heads of 64, window 1024: 42 us with a head's tokens together, 48 to 50 with a token's heads
+// together, where four heads share a line that each workgroup fetches by itself.
 template <int D_, bool BF, bool NV_> struct Paged4Rows {
   static constexpr int D = D_, BN = 64;
   static constexpr bool NV = NV_, CBF = BF && !NV;

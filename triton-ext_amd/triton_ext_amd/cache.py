@@ -322,8 +322,10 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_len, cu_q=None, *, q=Non
     Hkv, D / 2] of e2m1 codes (D a multiple of 32, the even dim in the low four bits), quantised as they
     are written.  The block scales, in any strides, are uint8 [pages, page_size, Hkv, D / 32] (e8m0: the
     least power of two 2^e with max |x| <= 7 * 2^e over 32 dims, e within [-125, 125] for bf16 and
-    [-23, 13] for fp16) or float8_e4m3fn [.., D / 16] (max |x| / 6, within [2^-9, 448]); codes go to
-    nearest, ties to even, saturated at 6; a block with a NaN or an infinity becomes NaN.  The fast
+    [-23, 13] for fp16) or float8_e4m3fn [.., D / 16] (max |x| / 6, within [2^-9, 448]; where blocks
+    stay below 0.1, k_scale and v_scale below 1 lift them out of e4m3's subnormals, whose few bits cost
+    up to a third of a value); codes go to nearest, ties to even, saturated at 6; a block with a NaN or
+    an infinity becomes NaN.  The fast
     order in memory has a head's tokens together, torch.empty(pages, Hkv, page_size, D // 2).permute(0,
     2, 1, 3), and of the scales those of one block of dims, torch.empty(pages, Hkv, D // 32,
     page_size).permute(0, 3, 1, 2); pages of these are what page_copy and its kin move."""
@@ -422,8 +424,10 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_len, cu_q=None, *, sm_sc
     where nothing is attended to).  cu_q as for paged_append.
 
     With k_block_scale and v_block_scale: over a cache held in 4 bits (see paged_append; D a multiple
-    of 32 up to 256), whose values are taken in q's type.  A row that attends to a token with a block
-    scale of NaN (or e8m0 above 2^125, fp16 q: 2^13) is NaN."""
+    of 32 up to 256), whose values are taken in q's type (e4m3 scales: exactly, in fp16).  A row that
+    attends to a token with a block scale of NaN (or e8m0 above 2^125, fp16 q: 2^13) is NaN.  The form is
+    chosen by the call's average of new tokens a sequence: long chunks and decoding sequences are
+    faster in two calls."""
     if stream is not None and stream != _current_stream(q.device):
         return _there(q.device, stream, paged_attention, q, k_cache, v_cache, page_table, kv_len, cu_q,
                       sm_scale=sm_scale, causal=causal, window=window, k_scale=k_scale,
