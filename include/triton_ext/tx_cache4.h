@@ -28,7 +28,8 @@ typedef struct tx_block_scales {
 } tx_block_scales;
 
 /* ---- new tokens into the cache -------------------------------------------
- * As tx_paged_append, but k (after its rotation) and v are quantised.  Of the block y = x /
+ * As tx_paged_append, but k (after its rotation: sines rounded once to fp32, then two products and their
+ * sum) and v are quantised.  Of the block y = x /
  * k_scale[head] with the largest magnitude a:
  *   MX32  e = the least integer with a <= 7 * 2^e, within [-125, 125] (bf16 tokens) or
  *         [-23, 13] (fp16); the scale is e + 127, a code the nearest to y / 2^e

@@ -152,6 +152,34 @@ def test_append_rotated(gpu, n, lens, Hq, Hkv, D, rot, page, dtype, layout, inte
 
 
 @pytest.mark.parametrize("kind", ["mx", "nv"])
+@pytest.mark.parametrize("Hq,Hkv,D,rot,interleaved", [(8, 2, 128, 128, False), (8, 2, 64, 32, True),
+                                                      (12, 3, 96, 40, False), (6, 2, 128, 76, False)])
+def test_append_rotates_step_by_step(gpu, Hq, Hkv, D, rot, interleaved, kind):
+    """Sines rounded once to fp32, products and their sum each rounded to fp32: keys at a border of two
+    codes go where these steps lead.  (An angle off by 2^-51 changes a sine's rounding once in 2^26, and that
+    a value's once in 2^12: of 2 million values none.)"""
+    n, lens = [1500, 1, 500], [30000, 7, 3000]
+    c = Cache4(31, lens, 16, Hkv, D, HF, kind, "hnd")
+    qkv = randn(c.g, sum(n), Hq + 2 * Hkv, D, dtype=HF)
+    inv_freq, scale = tx.rotary_frequencies(rot)
+    assert scale == 1.0
+    dev, d = c.to(gpu), qkv.to(gpu)
+    got = tx.paged_append(d[:, Hq:Hq + Hkv], d[:, Hq + Hkv:], cu_q=starts(n).to(gpu), q=d[:, :Hq],
+                          inv_freq=inv_freq.to(gpu), interleaved=interleaved, **books(dev))
+    pos = torch.cat([torch.arange(lens[b] - k, lens[b]) for b, k in enumerate(n)])
+    angle = pos.double()[:, None] * inv_freq.double()
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+    y = qkv[:, :Hq + Hkv].float()
+    i, j = ((slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot)))
+    a, z = y[..., i].clone(), y[..., j].clone()
+    y[..., i], y[..., j] = a * cos - z * sin, z * cos + a * sin
+    assert torch.equal(got.cpu(), y[:, :Hq].to(HF))
+    codes, sb = quantise(y[:, Hq:].double(), kind, HF)
+    k, _ = tx.paged_read(cu_q=starts(n).to(gpu), tokens=sum(n), dtype=torch.float32, **books(dev))
+    assert torch.equal(k.cpu().double(), values(codes, sb, kind))
+
+
+@pytest.mark.parametrize("kind", ["mx", "nv"])
 @pytest.mark.parametrize("Hq,D,rot,interleaved,odd", [
     (4, 64, 32, False, False), (4, 64, 64, False, False), (5, 96, 96, False, False), (16, 96, 40, False, False),
     (4, 64, 0, False, False), (4, 64, 32, False, True), (33, 96, 96, False, True), (4, 64, 32, True, False),

@@ -96,15 +96,21 @@ __device__ __forceinline__ void store8(T *p, const float (&y)[8]) {
   }
 }
 
-// cos and sin of position * f, times scale: turn_of (rotary.h) with the turn's rounding to fp32 made good to
-// first order, since a key is quantised after it.
+// cos and sin of position * f, times scale, in 64 bits and rounded once: a key is quantised after its
+// rotation, and one that lies at a border of two codes goes to either by the last bit of its sines.  (The
+// second constant is what the first leaves of 1 / 2 pi: the turn is off by less than 2^-53 then.)
 __device__ __forceinline__ float2_t turn4_of(double pos, float f, float scale) {
-  double t = pos * (double)f * 0.15915494309189535; // turns
-  t -= rint(t);
-  const float turn = (float)t, rest = 6.2831853f * (float)(t - (double)turn);
-  float s, c;
-  sincospif(2.0f * turn, &s, &c);
-  return float2_t{(c - s * rest) * scale, (s + c * rest) * scale};
+  const double a = pos * (double)f, n = rint(a * 0.15915494309189535);
+  const double turn = fma(a, -9.839338337591243e-18, fma(a, 0.15915494309189535, -n));
+  double s, c;
+  sincospi(2.0 * turn, &s, &c);
+  return float2_t{(float)(c * scale), (float)(s * scale)};
+}
+// A rotated dim, x c + z s with its partner z: both products and their sum rounded to fp32 (not
+// contracted, so that both dims of a pair, of every form, are rounded alike).
+__device__ __forceinline__ float turned4(float x, float c, float z, float s) {
+#pragma clang fp contract(off)
+  return x * c + z * s;
 }
 
 // How a thread has the dims of a head: 8 adjacent ones whose partners are elsewhere (any rot_dim), 8 of
@@ -195,20 +201,20 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float a = y[0][i], b = y[RUNS - 1][i];
-        y[0][i] = a * c[i] - b * s[i], y[RUNS - 1][i] = b * c[i] + a * s[i];
+        y[0][i] = turned4(a, c[i], b, -s[i]), y[RUNS - 1][i] = turned4(b, c[i], a, s[i]);
       }
     } else if constexpr (MODE == kRunPairs) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const float a = y[0][2 * i], b = y[0][2 * i + 1];
         if (d[0] + 2 * i < rot)
-          y[0][2 * i] = a * c[i] - b * s[i], y[0][2 * i + 1] = b * c[i] + a * s[i];
+          y[0][2 * i] = turned4(a, c[i], b, -s[i]), y[0][2 * i + 1] = turned4(b, c[i], a, s[i]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (d[0] + i < rot)
-          y[0][i] = y[0][i] * c[i] + elt_to_f32(x.partner.v[i]) * s[i];
+          y[0][i] = turned4(y[0][i], c[i], elt_to_f32(x.partner.v[i]), s[i]);
     }
   };
 
@@ -260,7 +266,7 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const float u = elt_to_f32(x[k].v[i]), w = pair ? elt_to_f32(z[k].v[i]) : 0.f;
-                y[0][i] = turn ? u * qc[i] - w * qs[i] : u, y[1][i] = turn ? w * qc[i] + u * qs[i] : w;
+                y[0][i] = turn ? turned4(u, qc[i], w, -qs[i]) : u, y[1][i] = turn ? turned4(w, qc[i], u, qs[i]) : w;
               }
               store8<T, true>(out + h * p.o_sh + a, y[0]);
               if (pair)
@@ -278,9 +284,9 @@ __global__ void __launch_bounds__(256) paged_append4_kernel(Append4Args args) {
             T *const to = out + h * p.o_sh + a;
             const T x = from[0], z = from[pair ? half : 0];
             const float u = elt_to_f32(x), w = elt_to_f32(z);
-            to[0] = turn ? (T)(u * cs[0] - w * cs[1]) : x;
+            to[0] = turn ? (T)turned4(u, cs[0], w, -cs[1]) : x;
             if (pair)
-              to[half] = turn ? (T)(w * cs[0] + u * cs[1]) : z;
+              to[half] = turn ? (T)turned4(w, cs[0], u, cs[1]) : z;
           }
         }
       }
